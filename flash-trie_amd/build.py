@@ -111,6 +111,10 @@ def build(verbose=False):
         "tbs_kernel.hip": os.path.join(OBJ, "tbs_kernel.o"),
         "sort_rows.hip": os.path.join(OBJ, "sort_rows.o"),
         "ft_runtime.cpp": os.path.join(OBJ, "ft_runtime.o"),
+        "adapter_logits.hip": os.path.join(OBJ, "adapter_logits.o"),
+        "propose.hip": os.path.join(OBJ, "propose.o"),
+        "key_loss.hip": os.path.join(OBJ, "key_loss.o"),
+        "operators.cpp": os.path.join(OBJ, "operators.o"),
     }
     host_objs = {
         "marisa_trie.cc": os.path.join(OBJ, "marisa_trie.o"),
@@ -120,7 +124,10 @@ def build(verbose=False):
         "synth.cc": os.path.join(OBJ, "synth.o"),
         "synth_trie.cc": os.path.join(OBJ, "synth_trie.o"),
     }
-    bind_obj = os.path.join(OBJ, "bindings.o")
+    bind_objs = {
+        "bindings.cc": os.path.join(OBJ, "bindings.o"),
+        "bind_operators.cc": os.path.join(OBJ, "bind_operators.o"),
+    }
     jobs = []
     for src, obj in hip_objs.items():
         lang = ["-x", "hip"] if src.endswith(".hip") else []
@@ -131,9 +138,9 @@ def build(verbose=False):
                                                "-o", obj])
     jobs.append([HIPCC] + HIP_FLAGS + ["-x", "hip", os.path.join(CSRC, "copy_calib.hip"),
                                        "-o", COPY_CALIB])
-    jobs.append([CXX] + CXX_FLAGS + bid + _pybind_includes() +
-                ["-fvisibility=hidden", "-c", os.path.join(CSRC, "bindings.cc"),
-                 "-o", bind_obj])
+    for src, obj in bind_objs.items():
+        jobs.append([CXX] + CXX_FLAGS + bid + _pybind_includes() +
+                    ["-fvisibility=hidden", "-c", os.path.join(CSRC, src), "-o", obj])
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 4)) as ex:
         outs = list(ex.map(_run, jobs))
     if verbose:
@@ -149,8 +156,9 @@ def build(verbose=False):
     _run([CXX] + CXX_FLAGS + [os.path.join(CSRC, "ft_beam_search.cc"), "-o", BEAM_CLI,
                               "-L" + HERE, "-lmarisa_amd", "-lflashtrie_amd",
                               "-Wl,-rpath,$ORIGIN"])
-    _run([CXX, "-shared", "-fPIC", "-fopenmp", "-o", PYMOD, bind_obj,
-          "-L" + HERE, "-lmarisa_amd", "-lflashtrie_amd",
+    _run([CXX, "-shared", "-fPIC", "-fopenmp", "-o", PYMOD]
+         + list(bind_objs.values()) +
+         ["-L" + HERE, "-lmarisa_amd", "-lflashtrie_amd",
           "-Wl,-rpath,$ORIGIN"])
     return [LIB_AMD, LIB_MARISA, PYMOD, COPY_CALIB, BEAM_CLI]
 

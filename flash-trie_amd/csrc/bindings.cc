@@ -25,6 +25,7 @@
 #include <thread>
 
 #include "../../include/flashtrie_amd.h"
+#include "bind_operators.h"
 #include "image_builder.h"
 #include "marisa_format.h"
 #include "marisa.h"
@@ -205,6 +206,8 @@ PYBIND11_MODULE(flashtrie, m) {
     return std::string(ft_build_id());
   });
   py::register_exception<marisa::Exception>(m, "MarisaError", PyExc_RuntimeError);
+
+  bind_operators(m);
 
   py::class_<Trie>(m, "Trie")
       .def(py::init<>())

@@ -25,6 +25,7 @@
 #include <vector>
 
 #include "../../include/flashtrie_amd.h"
+#include "operators.h"
 #include "tbs_kernel.h"
 
 using namespace ftk;
@@ -646,6 +647,15 @@ static int build_root_dir(ft_ctx* c, const uint8_t* image) {
     return hip_fail(e, "hipStreamSynchronize(root directory)");
   c->root_n = n;
   return FT_OK;
+}
+
+int ftk::set_error(int code, const char* msg) noexcept {
+  try {
+    g_err = msg;
+  } catch (...) {  // no memory for the text: the code says it
+    g_err.clear();
+  }
+  return code;
 }
 
 #ifndef FT_BUILD_ID

@@ -1,0 +1,607 @@
+// key_loss.hip -- the losses on the keys of a search, and their gradient with
+// respect to the logits that scored them.
+//
+// With lp = x[tok] - lse(x) for each token and g = dloss/dlp,
+//   dloss/dx[v] = sum over the row's tokens of (tok = v ? g : 0) - p[v] g
+//               = (sum of the g's of v) - p[v] G,  p[v] = exp(x[v] - lse),
+// so a row needs its lse, G and a short list of (token, summed g); many keys
+// share a token at the first positions of a trie.  The sums are made in a
+// fixed order: the list is sorted by (token, key) and summed by a segmented
+// scan, with no atomics.
+//
+//   key_stats    (row, chunk): (max, sum of exponentials) of the chunk
+//   key_policy   row: token scores, the loss's terms and g
+//   key_scores   16 lanes a key: token scores and the key's margin
+//   key_pairs    64 keys a workgroup: dloss/ds over all pairs, loss's terms
+//   key_lists    row: the list of (token, summed g), and G   (keys > 1)
+//   key_gradient (row, chunk): the gradient; block 0 also adds up the loss
+#include "op_device.h"
+#include "operators.h"
+
+namespace fto {
+namespace {
+
+constexpr int kStatT = 256;
+constexpr int kStatU = 4;   // vectors in flight a thread
+constexpr int kListT = 1024;
+
+struct Args {
+  const void* logits;
+  int64_t stride[2];
+  void* dlogits;
+  int64_t dstride[2];
+  uint32_t batch, steps, vocab, keys, rows, chunks, chunk_vecs;
+  const int32_t* tokens;
+  const int32_t* lengths;
+  float* logp;
+  float* loss;
+  const float* old_logp;
+  const float* ref_logp;
+  const float* advantage;
+  const float* weight;
+  float low, high, kl;  // clip bounds, KL coefficient
+  uint64_t pairs;
+  const int32_t* pair;
+  float beta, smoothing;
+  // workspace
+  MaxSum* part;      // [rows, chunks]
+  float* g;          // [rows, keys]: dloss/dlp of the row's tokens (policy)
+  float* margin;     // [batch * keys] (preference)
+  float* gkey;       // [batch * keys]: dloss/ds (preference)
+  float* total;      // [rows]: G
+  float* terms;      // [nterms]: parts of the loss
+  uint32_t nterms;
+  uint32_t* listed;  // [rows]: entries of the row's list
+  uint32_t* ltok;    // [rows, keys]
+  float* lg;         // [rows, keys]
+};
+
+template <typename T>
+__device__ __forceinline__ const T* row_of(const Args& a, uint32_t row) {
+  const uint32_t r = row / a.steps, t = row - r * a.steps;
+  return (const T*)a.logits + (int64_t)r * a.stride[0] + (int64_t)t * a.stride[1];
+}
+
+__device__ __forceinline__ uint32_t length_of(const Args& a, uint32_t key) {
+  const int32_t n = a.lengths[key];
+  return n < 0 ? 0u : min((uint32_t)n, a.steps);
+}
+
+// Whether row (r, t) scores any token; every thread of the block.
+__device__ __forceinline__ bool row_used(const Args& a, uint32_t row) {
+  const uint32_t r = row / a.steps, t = row - r * a.steps;
+  bool any = false;
+  for (uint32_t c = threadIdx.x; c < a.keys; c += blockDim.x)
+    any = any || length_of(a, r * a.keys + c) > t;
+  return __syncthreads_or(any);
+}
+
+template <typename T>
+__device__ __forceinline__ u32x4 load_row(const T* p, uint32_t vec, uint32_t vocab, T fill) {
+  const uint32_t e = vec * kVec<T>;
+  if (e + kVec<T> <= vocab) return load_vec(p + e);
+  return load_part(p + (e < vocab ? e : 0u), e < vocab ? (int)(vocab - e) : 0, fill);
+}
+
+// Block (row, chunk).  Rows without a token are not read.
+template <typename T>
+__global__ void __launch_bounds__(kStatT) key_stats(Args a) {
+  const uint32_t row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks;
+  const uint32_t tid = threadIdx.x;
+  if (!row_used(a, row)) return;
+  const T* p = row_of<T>(a, row);
+  const uint32_t vecs = (a.vocab + kVec<T> - 1) / kVec<T>;
+  const uint32_t v0 = chunk * a.chunk_vecs, v1 = min(v0 + a.chunk_vecs, vecs);
+  MaxSum ms{-INFINITY, 0.0f};
+  for (uint32_t v = v0; v < v1; v += kStatU * kStatT) {
+    u32x4 raw[kStatU];
+#pragma unroll
+    for (int u = 0; u < kStatU; ++u)
+      raw[u] = load_row(p, v + u * kStatT + tid, a.vocab, (T)-INFINITY);
+#pragma unroll
+    for (int u = 0; u < kStatU; ++u) {
+      float x[kVec<T>];
+      to_float<T>(raw[u], x);
+      add_terms(ms, x);
+    }
+  }
+  ms = wave_merge(ms);
+  __shared__ MaxSum waves[kStatT / 64];
+  if ((tid & 63) == 0) waves[tid >> 6] = ms;
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < kStatT / 64; ++w) ms = merge(ms, waves[w]);
+    a.part[(uint64_t)row * a.chunks + chunk] = ms;
+  }
+}
+
+// The row's (max, sum) from its chunks' parts, in their order.
+__device__ __forceinline__ MaxSum row_sum(const Args& a, uint32_t row) {
+  MaxSum ms = a.part[(uint64_t)row * a.chunks];
+  for (uint32_t i = 1; i < a.chunks; ++i) ms = merge(ms, a.part[(uint64_t)row * a.chunks + i]);
+  return ms;
+}
+
+// A token's log-probability; NaN for one out of range.
+template <typename T>
+__device__ __forceinline__ float score(const T* p, int32_t tok, uint32_t vocab, float m, float ls) {
+  if ((uint32_t)tok >= vocab) return NAN;
+  const float x = (float)p[tok];
+  return x == -INFINITY && ls == ls ? x : (x - m) - ls;
+}
+
+// The policy loss of one token, and its derivative by lp.
+__device__ __forceinline__ float policy_term(const Args& a, uint64_t at, float lp, float adv,
+                                             float w, float* g) {
+  const float ratio = expf(lp - a.old_logp[at]);
+  const float clipped = fminf(fmaxf(ratio, a.low), a.high);
+  const float u = ratio * adv, v = clipped * adv;
+  const bool moves = !(u > v);  // (NaN too: the loss and gradient show it)
+  float each = moves ? -u : -v, d = moves ? -u : 0.0f;
+  if (a.kl != 0.0f) {
+    const float r = a.ref_logp[at] - lp, e = expm1f(r);
+    each += a.kl * (r == INFINITY ? r : e - r);  // (a token whose logit is -infinity)
+    d -= a.kl * e;
+  }
+  *g = w * d;
+  return w * each;
+}
+
+__device__ __forceinline__ float block_sum(float v, float* waves) {
+  v = wave_sum(v);
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0.0f;
+  for (uint32_t w = 0; w < blockDim.x / 64; ++w) v += waves[w];
+  __syncthreads();
+  return v;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) key_policy(Args a) {
+  __shared__ float waves[4];
+  const uint32_t row = blockIdx.x, r = row / a.steps, t = row - r * a.steps;
+  const bool used = row_used(a, row);
+  const T* p = row_of<T>(a, row);
+  MaxSum ms{0.0f, 1.0f};
+  if (used) ms = row_sum(a, row);
+  const float m = exp_base(ms.m), ls = logf(ms.s);
+  float loss = 0.0f, total = 0.0f;
+  for (uint32_t c = threadIdx.x; c < a.keys; c += 256) {
+    const uint32_t key = r * a.keys + c;
+    const uint64_t at = (uint64_t)key * a.steps + t;
+    float lp = 0.0f, g = 0.0f;
+    if (length_of(a, key) > t) {
+      lp = score(p, a.tokens[at], a.vocab, m, ls);
+      loss += policy_term(a, at, lp, a.advantage[key], a.weight[key], &g);
+    }
+    a.logp[at] = lp;
+    a.g[(uint64_t)row * a.keys + c] = g;
+    total += g;
+  }
+  loss = block_sum(loss, waves);
+  total = block_sum(total, waves);
+  if (threadIdx.x == 0) {
+    a.terms[row] = loss;
+    a.total[row] = total;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) key_scores(Args a) {
+  const uint32_t key = blockIdx.x * 16 + (threadIdx.x >> 4), lane = threadIdx.x & 15;
+  if (key >= a.batch * a.keys) return;
+  const uint32_t r = key / a.keys, len = length_of(a, key);
+  float sum = 0.0f;
+  for (uint32_t t = lane; t < a.steps; t += 16) {
+    const uint64_t at = (uint64_t)key * a.steps + t;
+    float lp = 0.0f;
+    if (t < len) {
+      const MaxSum ms = row_sum(a, r * a.steps + t);
+      lp = score(row_of<T>(a, r * a.steps + t), a.tokens[at], a.vocab, exp_base(ms.m), logf(ms.s));
+    }
+    a.logp[at] = lp;
+    sum += lp;
+  }
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) sum += __shfl_xor(sum, d, 64);
+  if (lane == 0) a.margin[key] = sum - a.ref_logp[key];
+}
+
+// Wave w of a workgroup takes the pairs of its share in their order, one at
+// a time for its 64 keys, a key a lane; the waves' sums are added in order.
+__global__ void __launch_bounds__(1024) key_pairs(Args a) {
+  __shared__ float sums[16][64];
+  __shared__ float waves[16];
+  const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const uint32_t keys = a.batch * a.keys, key = blockIdx.x * 64 + lane;
+  const uint64_t each = (a.pairs + 15) / 16;
+  const uint64_t p0 = wave * each, p1 = min(p0 + each, a.pairs);
+  float g = 0.0f, loss = 0.0f;
+  for (uint64_t q = p0; q < p1; q += 64) {
+    // a pair a lane: its derivative
+    uint32_t ka = ~0u, kb = ~0u;
+    float d = 0.0f;
+    if (q + lane < p1) {
+      ka = (uint32_t)a.pair[2 * (q + lane)];
+      kb = (uint32_t)a.pair[2 * (q + lane) + 1];
+      const float w = a.weight[q + lane];
+      const float h =
+          ka < keys && kb < keys ? a.beta * (a.margin[ka] - a.margin[kb]) : NAN;
+      // sigmoid(h) and softplus(-h), softplus(h) without overflow
+      const float e = expf(-fabsf(h)), tail = log1pf(e);
+      const float sig = (h >= 0.0f ? 1.0f : e) / (1.0f + e);
+      d = w * a.beta * (sig - (1.0f - a.smoothing));
+      const float won = tail + (h < 0.0f ? -h : 0.0f), lost = tail + (h > 0.0f ? h : 0.0f);
+      loss += w * ((1.0f - a.smoothing) * won + a.smoothing * lost);
+    }
+    const uint32_t n = (uint32_t)min((uint64_t)64, p1 - q);
+    for (uint32_t i = 0; i < n; ++i) {
+      const uint32_t pa = (uint32_t)__builtin_amdgcn_readlane((int)ka, (int)i);
+      const uint32_t pb = (uint32_t)__builtin_amdgcn_readlane((int)kb, (int)i);
+      const float pd = __uint_as_float(
+          (uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(d), (int)i));
+      if (pa == key) g += pd;
+      if (pb == key) g -= pd;
+    }
+  }
+  sums[wave][lane] = g;
+  __syncthreads();
+  if (wave == 0) {
+    g = 0.0f;
+    for (int w = 0; w < 16; ++w) g += sums[w][lane];
+    if (key < keys) a.gkey[key] = g;
+  }
+  if (blockIdx.x == 0) {
+    loss = block_sum(loss, waves);
+    if (tid == 0) a.terms[0] = loss;
+  }
+}
+
+// dloss/dlp of the row's token of key c
+template <bool kPolicy>
+__device__ __forceinline__ float slope(const Args& a, uint32_t row, uint32_t c) {
+  return kPolicy ? a.g[(uint64_t)row * a.keys + c] : a.gkey[row / a.steps * a.keys + c];
+}
+
+// The row's tokens sorted by (token, key), their slopes summed by token.
+// kP: pairs a thread.
+template <bool kPolicy, int kP>
+__global__ void __launch_bounds__(kListT) key_lists(Args a) {
+  __shared__ uint64_t keys[kListT * kP];
+  __shared__ float gs[kListT * kP];
+  __shared__ float wsum[kListT / 64];
+  __shared__ uint32_t wtok[kListT / 64], wcount[kListT / 64];
+  const uint32_t row = blockIdx.x, r = row / a.steps, t = row - r * a.steps, tid = threadIdx.x;
+  const uint32_t wave = tid >> 6, lane = tid & 63;
+  uint32_t n = kListT * kP;  // the next power of two, at least a wave
+  while (n > 64 && n / 2 >= a.keys) n >>= 1;
+  float total = 0.0f;
+  for (uint32_t c = tid; c < n; c += kListT) {
+    uint64_t k = ~0ull;
+    float g = 0.0f;
+    if (c < a.keys) {
+      const uint32_t key = r * a.keys + c;
+      if (length_of(a, key) > t) {
+        g = slope<kPolicy>(a, row, c);
+        const uint32_t tok = (uint32_t)a.tokens[(uint64_t)key * a.steps + t];
+        if (tok < a.vocab) k = ((uint64_t)tok << 32) | c;
+      }
+    }
+    keys[c] = k;
+    gs[c] = g;
+    total += g;
+  }
+  if (!kPolicy) {
+    total = block_sum(total, wsum);
+    if (tid == 0) a.total[row] = total;
+  }
+  __syncthreads();
+  for (uint32_t k = 2; k <= n; k <<= 1) {
+    for (uint32_t j = k >> 1; j > 0; j >>= 1) {
+      for (uint32_t i = tid; i < n / 2; i += kListT) {
+        const uint32_t lo = 2 * i - (i & (j - 1)), hi = lo + j;
+        const uint64_t x = keys[lo], y = keys[hi];
+        if ((x > y) == ((lo & k) == 0)) {
+          keys[lo] = y;
+          keys[hi] = x;
+        }
+      }
+      __syncthreads();
+    }
+  }
+  // segmented sums, kListT pairs at a time; the last entry of a token's run
+  // holds its sum
+  uint32_t listed = 0;  // entries so far
+  uint32_t ctok = ~0u;  // the run that goes on from the pairs before
+  float csum = 0.0f;
+  for (uint32_t b = 0; b < n; b += kListT) {
+    const uint32_t i = b + tid;
+    uint32_t tok = ~0u;
+    float g = 0.0f;
+    if (i < n) {
+      tok = (uint32_t)(keys[i] >> 32);
+      if (tok != ~0u) g = gs[(uint32_t)keys[i]];
+    }
+    const uint32_t next = i + 1 < n ? (uint32_t)(keys[i + 1] >> 32) : ~0u;
+    const uint32_t tok0 = (uint32_t)__shfl((int)tok, 0, 64);  // (by the whole wave)
+    float s = g;
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d <<= 1) {
+      const float o = __shfl_up(s, d, 64);
+      const uint32_t ot = (uint32_t)__shfl_up((int)tok, d, 64);
+      if (lane >= d && ot == tok) s += o;
+    }
+    if (lane == 63) {
+      wsum[wave] = s;
+      wtok[wave] = tok;
+    }
+    __syncthreads();
+    // what the run of this wave's first token holds in front of the wave
+    float front = 0.0f;
+    uint32_t first = wave;
+    while (first > 0 && wtok[first - 1] == tok0) {
+      --first;
+      if ((uint32_t)(keys[b + first * 64] >> 32) != tok0) break;
+    }
+    if (tok0 != ~0u) {
+      if (first == 0 && ctok == tok0) front = csum;
+      for (uint32_t w = first; w < wave; ++w) front += wsum[w];
+    }
+    if (tok == tok0) s += front;
+    const bool last = tok != ~0u && next != tok;
+    const uint64_t ends = __ballot(last);
+    if (lane == 0) wcount[wave] = (uint32_t)__popcll(ends);
+    __syncthreads();
+    uint32_t at = listed;
+    for (uint32_t w = 0; w < wave; ++w) at += wcount[w];
+    at += (uint32_t)__popcll(ends & ((1ull << lane) - 1));
+    if (last) {
+      a.ltok[(uint64_t)row * a.keys + at] = tok;
+      a.lg[(uint64_t)row * a.keys + at] = s;
+    }
+    for (uint32_t w = 0; w < kListT / 64; ++w) listed += wcount[w];
+    __syncthreads();
+    if (tid == kListT - 1) {
+      wsum[0] = s;
+      wtok[0] = tok;
+    }
+    __syncthreads();
+    csum = wsum[0];
+    ctok = wtok[0];
+    __syncthreads();
+  }
+  if (tid == 0) a.listed[row] = listed;
+}
+
+__device__ __forceinline__ void add_loss(const Args& a, float* waves) {
+  float v = 0.0f;
+  for (uint32_t i = threadIdx.x; i < a.nterms; i += blockDim.x) v += a.terms[i];
+  v = block_sum(v, waves);
+  if (threadIdx.x == 0) *a.loss = v;
+}
+
+__global__ void __launch_bounds__(256) key_loss(Args a) {
+  __shared__ float waves[4];
+  add_loss(a, waves);
+}
+
+// Block (row, chunk): kU vectors a thread, in one go.
+template <typename T, bool kPolicy>
+__global__ void __launch_bounds__(kStatT) key_gradient(Args a) {
+  constexpr uint32_t kSpan = kStatU * kStatT * kVec<T>;
+  __shared__ float adds[kSpan];
+  __shared__ float waves[kStatT / 64];
+  const uint32_t vecs = (a.vocab + kVec<T> - 1) / kVec<T>;
+  const uint32_t spans = (vecs + kStatU * kStatT - 1) / (kStatU * kStatT);
+  const uint32_t row = blockIdx.x / spans, span = blockIdx.x - row * spans, tid = threadIdx.x;
+  const uint32_t r = row / a.steps, t = row - r * a.steps;
+  if (blockIdx.x == 0) add_loss(a, waves);
+  T* out = (T*)a.dlogits + (int64_t)r * a.dstride[0] + (int64_t)t * a.dstride[1];
+  const uint32_t v0 = span * kStatU * kStatT, e0 = v0 * kVec<T>;
+  const bool used = row_used(a, row);
+  u32x4 raw[kStatU];
+  float base = 0.0f, scale = 0.0f;
+  bool any = false;
+  if (used) {
+    const T* p = row_of<T>(a, row);
+#pragma unroll
+    for (int u = 0; u < kStatU; ++u)
+      raw[u] = load_row(p, v0 + u * kStatT + tid, a.vocab, (T)-INFINITY);
+    uint32_t l0 = 0, l1;
+    const uint32_t* ltok = a.ltok + (uint64_t)row * a.keys;
+    if (a.keys == 1) {
+      const uint32_t tok = (uint32_t)a.tokens[row];
+      l1 = tok < a.vocab && tok >= e0 && tok - e0 < kSpan;
+    } else {
+      // the entries of [e0, e0 + kSpan)
+      const uint32_t n = a.listed[row];
+      uint32_t b = n;
+      while (l0 < b) {
+        const uint32_t mid = (l0 + b) >> 1;
+        if (ltok[mid] < e0) l0 = mid + 1;
+        else b = mid;
+      }
+      l1 = l0;
+      b = n;
+      while (l1 < b) {
+        const uint32_t mid = (l1 + b) >> 1;
+        if (ltok[mid] < e0 + kSpan) l1 = mid + 1;
+        else b = mid;
+      }
+    }
+    const MaxSum ms = row_sum(a, row);
+    base = exp_base(ms.m);
+    const float total = a.keys == 1 ? slope<kPolicy>(a, row, 0) : a.total[row];
+    scale = total / ms.s;
+    any = l1 > l0;
+    if (any) {
+#pragma unroll
+      for (uint32_t i = 0; i < kSpan / kStatT; ++i) adds[i * kStatT + tid] = 0.0f;
+      __syncthreads();
+      if (a.keys == 1) {
+        if (tid == 0) adds[(uint32_t)a.tokens[row] - e0] = total;
+      } else {
+        for (uint32_t i = l0 + tid; i < l1; i += kStatT)
+          adds[ltok[i] - e0] = a.lg[(uint64_t)row * a.keys + i];
+      }
+      __syncthreads();
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kStatU; ++u) {
+    const uint32_t vec = v0 + u * kStatT + tid, e = vec * kVec<T>;
+    if (vec >= vecs) continue;
+    float x[kVec<T>];
+    if (used) {
+      to_float<T>(raw[u], x);
+#pragma unroll
+      for (int i = 0; i < kVec<T>; ++i) {
+        x[i] = -scale * exp_term(x[i], base);
+        if (any) x[i] += adds[e - e0 + i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVec<T>; ++i) x[i] = 0.0f;
+    }
+    const u32x4 o = from_float<T>(x);
+    if (e + kVec<T> <= a.vocab) store_vec(out + e, o);
+    else store_part(out + e, (int)(a.vocab - e), o);
+  }
+}
+
+struct Plan {
+  uint32_t vecs, chunks, chunk_vecs;
+  uint64_t part, g, margin, gkey, total, terms, listed, ltok, lg, bytes;
+};
+
+Plan plan(const ft_keys& k, bool policy) {
+  Plan p{};
+  const uint64_t rows = k.batch * k.steps, keys = k.batch * k.keys;
+  const uint32_t vec = k.dtype == FT_F32 ? 4 : 8;
+  p.vecs = (k.vocab + vec - 1) / vec;
+  // about 4096 workgroups, in whole turns of their loads
+  uint64_t each = rows ? (p.vecs * rows + 4095) / 4096 : 1;
+  p.chunk_vecs = (uint32_t)round_up(each ? each : 1, kStatU * kStatT);
+  p.chunks = (p.vecs + p.chunk_vecs - 1) / p.chunk_vecs;
+  Arena ar;
+  p.part = ar.take(rows * p.chunks * sizeof(MaxSum));
+  if (policy) p.g = ar.take(rows * k.keys * 4);
+  else {
+    p.margin = ar.take(keys * 4);
+    p.gkey = ar.take(keys * 4);
+  }
+  p.total = ar.take(rows * 4);
+  p.terms = ar.take((policy ? rows : 1) * 4);
+  p.listed = ar.take(rows * 4);
+  if (k.keys > 1) {
+    p.ltok = ar.take(rows * k.keys * 4);
+    p.lg = ar.take(rows * k.keys * 4);
+  }
+  p.bytes = ar.used;
+  return p;
+}
+
+Args base_args(const ft_keys& k, const Plan& p, uint8_t* ws) {
+  Args a{};
+  a.logits = k.logits;
+  a.dlogits = k.dlogits;
+  for (int i = 0; i < 2; ++i) {
+    a.stride[i] = k.stride[i];
+    a.dstride[i] = k.dstride[i];
+  }
+  a.batch = (uint32_t)k.batch;
+  a.steps = (uint32_t)k.steps;
+  a.vocab = k.vocab;
+  a.keys = k.keys;
+  a.rows = (uint32_t)(k.batch * k.steps);
+  a.chunks = p.chunks;
+  a.chunk_vecs = p.chunk_vecs;
+  a.tokens = k.tokens;
+  a.lengths = k.lengths;
+  a.logp = k.logp;
+  a.loss = k.loss;
+  a.part = (MaxSum*)(ws + p.part);
+  a.g = (float*)(ws + p.g);
+  a.margin = (float*)(ws + p.margin);
+  a.gkey = (float*)(ws + p.gkey);
+  a.total = (float*)(ws + p.total);
+  a.terms = (float*)(ws + p.terms);
+  a.listed = (uint32_t*)(ws + p.listed);
+  a.ltok = (uint32_t*)(ws + p.ltok);
+  a.lg = (float*)(ws + p.lg);
+  return a;
+}
+
+template <typename T, bool kPolicy>
+hipError_t launch(const Args& a, const Plan& p, hipStream_t s) {
+  if (a.rows) {
+    hipLaunchKernelGGL((key_stats<T>), dim3(a.rows * a.chunks), dim3(kStatT), 0, s, a);
+    if (kPolicy) {
+      hipLaunchKernelGGL((key_policy<T>), dim3(a.rows), dim3(256), 0, s, a);
+    } else {
+      const uint32_t keys = a.batch * a.keys;
+      hipLaunchKernelGGL((key_scores<T>), dim3((keys + 15) / 16), dim3(256), 0, s, a);
+      hipLaunchKernelGGL(key_pairs, dim3((keys + 63) / 64), dim3(1024), 0, s, a);
+    }
+  }
+  if (!a.dlogits || !a.rows) {
+    hipLaunchKernelGGL(key_loss, dim3(1), dim3(256), 0, s, a);
+    return hipGetLastError();
+  }
+  if (a.keys > 1) {
+    if (a.keys <= kListT)
+      hipLaunchKernelGGL((key_lists<kPolicy, 1>), dim3(a.rows), dim3(kListT), 0, s, a);
+    else
+      hipLaunchKernelGGL((key_lists<kPolicy, 4>), dim3(a.rows), dim3(kListT), 0, s, a);
+  }
+  const uint32_t spans = (p.vecs + kStatU * kStatT - 1) / (kStatU * kStatT);
+  hipLaunchKernelGGL((key_gradient<T, kPolicy>), dim3(a.rows * spans), dim3(kStatT), 0, s, a);
+  return hipGetLastError();
+}
+
+template <bool kPolicy>
+hipError_t launch_typed(int dtype, const Args& a, const Plan& p, hipStream_t s) {
+  switch (dtype) {
+    case FT_F32: return launch<float, kPolicy>(a, p, s);
+    case FT_F16: return launch<_Float16, kPolicy>(a, p, s);
+    default: return launch<__bf16, kPolicy>(a, p, s);
+  }
+}
+
+}  // namespace
+
+uint64_t policy_loss_workspace(const ft_policy_loss_args& q) { return plan(q.k, true).bytes; }
+
+hipError_t launch_policy_loss(const ft_policy_loss_args& q, uint8_t* ws, hipStream_t s) {
+  const Plan p = plan(q.k, true);
+  Args a = base_args(q.k, p, ws);
+  a.old_logp = q.old_logp;
+  a.ref_logp = q.ref_logp;
+  a.advantage = q.advantage;
+  a.weight = q.weight;
+  a.low = 1.0f - q.clip_low;
+  a.high = 1.0f + q.clip_high;
+  a.kl = q.kl_coef;
+  a.nterms = a.rows;
+  return launch_typed<true>(q.k.dtype, a, p, s);
+}
+
+uint64_t preference_loss_workspace(const ft_preference_loss_args& q) {
+  return plan(q.k, false).bytes;
+}
+
+hipError_t launch_preference_loss(const ft_preference_loss_args& q, uint8_t* ws, hipStream_t s) {
+  const Plan p = plan(q.k, false);
+  Args a = base_args(q.k, p, ws);
+  a.pairs = q.pairs;
+  a.pair = q.pair;
+  a.ref_logp = q.ref_logp;
+  a.weight = q.weight;
+  a.beta = q.beta;
+  a.smoothing = q.smoothing;
+  a.nterms = a.rows ? 1 : 0;
+  return launch_typed<false>(q.k.dtype, a, p, s);
+}
+
+}  // namespace fto

@@ -1,0 +1,157 @@
+// op_device.h -- what the model head's kernels share on the device: number
+// types, 16-byte loads of rows at any alignment, and sums of exponentials.
+#ifndef FTAMD_OP_DEVICE_H_
+#define FTAMD_OP_DEVICE_H_
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace fto {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// A row of V elements starts at any element of memory (V may be odd), so
+// vectors are loaded and stored with the element's alignment: the hardware
+// takes it, and a wave's 1 KB touches one more line.
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Vec16 {
+  u32x4 v;
+};
+
+template <typename T>
+constexpr int kVec = 16 / (int)sizeof(T);  // elements of a vector
+
+template <typename T>
+__device__ __forceinline__ u32x4 load_vec(const T* p) {
+  return ((const Vec16<T>*)p)->v;
+}
+template <typename T>
+__device__ __forceinline__ void store_vec(T* p, u32x4 v) {
+  ((Vec16<T>*)p)->v = v;
+}
+
+// The first n elements of a vector, the others `fill`.
+template <typename T>
+__device__ __forceinline__ u32x4 load_part(const T* p, int n, T fill) {
+  union {
+    u32x4 v;
+    T e[kVec<T>];
+  } u;
+#pragma unroll
+  for (int i = 0; i < kVec<T>; ++i) u.e[i] = i < n ? p[i] : fill;
+  return u.v;
+}
+template <typename T>
+__device__ __forceinline__ void store_part(T* p, int n, u32x4 v) {
+  union {
+    u32x4 v;
+    T e[kVec<T>];
+  } u;
+  u.v = v;
+#pragma unroll
+  for (int i = 0; i < kVec<T>; ++i)
+    if (i < n) p[i] = u.e[i];
+}
+
+template <typename T>
+__device__ __forceinline__ void to_float(u32x4 v, float (&f)[kVec<T>]) {
+  union {
+    u32x4 v;
+    T e[kVec<T>];
+  } u;
+  u.v = v;
+#pragma unroll
+  for (int i = 0; i < kVec<T>; ++i) f[i] = (float)u.e[i];
+}
+// rounded to nearest even, once
+template <typename T>
+__device__ __forceinline__ u32x4 from_float(const float (&f)[kVec<T>]) {
+  union {
+    u32x4 v;
+    T e[kVec<T>];
+  } u;
+#pragma unroll
+  for (int i = 0; i < kVec<T>; ++i) u.e[i] = (T)f[i];
+  return u.v;
+}
+
+// --- sums of exponentials ---------------------------------------------------
+// A part of a row is summed up as (m, s): its maximum (NaN left out) and
+// s = sum of exp(x - m), in 32 bits, relative to 0 where m is -infinity.
+// Terms are 2^((x - m) log2 e): the difference first, so that logits of any
+// size keep their own precision (a mask of the type's lowest value among
+// them).  A NaN, or an infinity (inf - inf), makes s NaN, as the formula
+// does.
+constexpr float kLog2e = 1.44269504088896340736f;
+
+__device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float exp_base(float m) { return m == -INFINITY ? 0.0f : m; }
+__device__ __forceinline__ float exp_term(float x, float base) {
+  return exp2_raw((x - base) * kLog2e);
+}
+
+struct MaxSum {
+  float m, s;
+};
+__device__ __forceinline__ MaxSum merge(MaxSum a, MaxSum b) {
+  MaxSum r;
+  r.m = fmaxf(a.m, b.m);
+  const float base = exp_base(r.m);
+  r.s = a.s * exp_term(a.m, base) + b.s * exp_term(b.m, base);
+  return r;
+}
+template <int kN>
+__device__ __forceinline__ void add_terms(MaxSum& a, const float (&x)[kN]) {
+  float v = x[0];
+#pragma unroll
+  for (int i = 1; i < kN; ++i) v = fmaxf(v, x[i]);
+  if (v > a.m) {
+    a.s *= exp_term(a.m, v);
+    a.m = v;
+  }
+  const float base = exp_base(a.m);
+#pragma unroll
+  for (int i = 0; i < kN; ++i) a.s += exp_term(x[i], base);
+}
+
+__device__ __forceinline__ MaxSum wave_merge(MaxSum a) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    MaxSum b{__shfl_xor(a.m, d, 64), __shfl_xor(a.s, d, 64)};
+    a = merge(a, b);
+  }
+  return a;
+}
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
+  return v;
+}
+
+// exclusive sum over the lanes in front
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t lane, uint32_t* total) {
+  uint32_t s = v;
+#pragma unroll
+  for (uint32_t d = 1; d < 64; d <<= 1) {
+    const uint32_t o = (uint32_t)__shfl_up((int)s, d, 64);
+    if (lane >= d) s += o;
+  }
+  *total = (uint32_t)__shfl((int)s, 63, 64);
+  return s - v;
+}
+
+// unsigned order of the floats; NaN as -infinity, -0 as 0
+__device__ __forceinline__ uint32_t order_key(float x) {
+  x = x == x ? x + 0.0f : -INFINITY;
+  const uint32_t b = __float_as_uint(x);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+}
+
+}  // namespace fto
+
+#endif  // FTAMD_OP_DEVICE_H_

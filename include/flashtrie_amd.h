@@ -276,6 +276,145 @@ const char* ft_last_error(void);
 int ft_device_info(ft_ctx* ctx, int* num_cus, int* lds_per_block,
                    int* wall_clock_khz, char* name, size_t name_len);
 
+/* ---------------------------------------------------------------------------
+ * The model head: what a generative retrieval model computes around the
+ * search, on device memory.  No counterpart in the reference, whose requests
+ * begin at finished proposal rows.
+ *
+ *   ft_adapter_logits   hidden states -> logits over the vocabulary, each row
+ *                       with its request's low-rank adapter
+ *   ft_propose          logits -> proposal rows as the search takes them
+ *   ft_policy_loss      a clipped policy loss with a KL term on the keys that
+ *                       the search returned, and the logits' gradient
+ *   ft_preference_loss  a loss on pairs of such keys, and the gradient
+ *
+ * Every pointer is device memory of `device` (or memory mapped for it).  A
+ * call checks its arguments, launches on `stream` (a hipStream_t of that
+ * device, null for its default stream) and returns; it allocates nothing,
+ * does not synchronise and can be recorded into a HIP graph.  `workspace` is
+ * device memory of at least the size that the *_workspace function names for
+ * the same arguments (0 for invalid ones), 256-byte aligned, free for other
+ * use once the launches have run; its contents do not matter.  Values that
+ * lie on the device cannot be checked before the launch: an adapter, token
+ * or pair out of range makes the results that depend on it NaN and reads
+ * nothing out of bounds.  Strides are in elements; innermost dimensions are
+ * contiguous.  Outputs overlap no input.  Results are the same from call to
+ * call, bit for bit.
+ * ------------------------------------------------------------------------- */
+#define FT_F32 0
+#define FT_F16 1
+#define FT_BF16 2
+
+#define FT_MAX_RANK 256            /* rank of an adapter */
+#define FT_MAX_HEAD_VOCAB (1 << 24) /* vocabulary of the head's operators */
+#define FT_MAX_PROPOSALS 4096      /* topk of ft_propose */
+#define FT_MAX_KEYS 4096           /* keys of a request in the losses */
+
+/* out[t, v] = sum_h x[t, h] weight[v, h]
+ *           + scale[g] sum_j up[g, v, j] sum_h down[g, j, h] x[t, h],
+ * g = adapter[t]; a negative g is a row without an adapter.  Sums in 32
+ * bits; the rank-wide intermediate keeps 22 or more bits. */
+typedef struct ft_adapter_logits_args {
+  int device;
+  int dtype;                  /* of x, weight, down, up: FT_F16 or FT_BF16 */
+  int out_dtype;              /* FT_F32, or the inputs' type */
+  uint64_t rows;
+  uint32_t hidden, vocab;
+  uint32_t adapters, rank;    /* adapters may be 0 (down, up, scale unread) */
+  const void* x;              /* [rows, hidden] */
+  int64_t x_stride;
+  const void* weight;         /* [vocab, hidden] */
+  int64_t weight_stride;
+  const void* down;           /* [adapters, rank, hidden] */
+  int64_t down_stride[2];     /* of an adapter, of a rank */
+  const void* up;             /* [adapters, vocab, rank] */
+  int64_t up_stride[2];       /* of an adapter, of a token */
+  const int32_t* adapter;     /* [rows] */
+  const float* scale;         /* [adapters] */
+  void* out;                  /* [rows, vocab] */
+  int64_t out_stride;
+} ft_adapter_logits_args;
+
+size_t ft_adapter_logits_workspace(const ft_adapter_logits_args* args);
+int ft_adapter_logits(const ft_adapter_logits_args* args, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* For each row the topk tokens of the largest logits (ties: the lowest ids;
+ * NaN counts as -infinity here) in ascending token order, and their
+ * log-probabilities under the row's whole softmax.  A logit of -infinity
+ * has log-probability -infinity, also where a row holds nothing else; a NaN
+ * or +infinity in a row makes its log-probabilities NaN. */
+typedef struct ft_propose_args {
+  int device;
+  int dtype;                  /* FT_F32, FT_F16 or FT_BF16 */
+  uint64_t batch, steps;      /* rows are (request, step) */
+  uint32_t vocab, topk;       /* 1 <= topk <= min(vocab, FT_MAX_PROPOSALS) */
+  const void* logits;         /* [batch, steps, vocab] */
+  int64_t stride[2];          /* of a request, of a step */
+  int32_t* ids;               /* [batch, steps, topk] */
+  float* logp;                /* [batch, steps, topk] */
+} ft_propose_args;
+
+size_t ft_propose_workspace(const ft_propose_args* args);
+int ft_propose(const ft_propose_args* args, void* workspace,
+               size_t workspace_bytes, void* stream);
+
+/* Keys and the logits that score them: token t of key (r, c) is scored by
+ * row (r, t) of the logits, so a request's keys share its rows, as the
+ * search's results do; with keys = 1 every key has rows of its own.  Tokens
+ * at t >= lengths[r, c] are not read as tokens and count nothing. */
+typedef struct ft_keys {
+  int device;
+  int dtype;                  /* of logits and dlogits */
+  uint64_t batch, steps;
+  uint32_t vocab, keys;       /* keys <= FT_MAX_KEYS */
+  const void* logits;         /* [batch, steps, vocab] */
+  int64_t stride[2];          /* of a request, of a step */
+  const int32_t* tokens;      /* [batch, keys, steps] */
+  const int32_t* lengths;     /* [batch, keys]; above steps: steps, < 0: 0 */
+  float* logp;                /* out [batch, keys, steps]: the tokens'
+                                 log-probabilities, 0 past a key's end */
+  float* loss;                /* out [1] */
+  void* dlogits;              /* out [batch, steps, vocab]: dloss/dlogits,
+                                 zero in rows that score no token; null: not
+                                 wanted */
+  int64_t dstride[2];
+} ft_keys;
+
+/* loss = sum over keys of weight * sum over their tokens of
+ *   -min(ratio A, clamp(ratio, 1 - clip_low, 1 + clip_high) A)
+ *   + kl_coef (exp(ref - logp) - (ref - logp) - 1),
+ * ratio = exp(logp - old_logp), A the key's advantage. */
+typedef struct ft_policy_loss_args {
+  ft_keys k;
+  const float* old_logp;      /* [batch, keys, steps] */
+  const float* ref_logp;      /* likewise; may be null when kl_coef is 0 */
+  const float* advantage;     /* [batch, keys] */
+  const float* weight;        /* [batch, keys] */
+  float clip_low, clip_high, kl_coef;
+} ft_policy_loss_args;
+
+size_t ft_policy_loss_workspace(const ft_policy_loss_args* args);
+int ft_policy_loss(const ft_policy_loss_args* args, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/* loss = sum over pairs (a, b) of weight *
+ *   ((1 - smoothing) softplus(-h) + smoothing softplus(h)),
+ * h = beta ((s_a - ref_a) - (s_b - ref_b)), s a key's summed logp; a and b
+ * index batch * keys. */
+typedef struct ft_preference_loss_args {
+  ft_keys k;
+  uint64_t pairs;
+  const int32_t* pair;        /* [pairs, 2]: the preferred key, the other */
+  const float* ref_logp;      /* [batch, keys]: of whole keys */
+  const float* weight;        /* [pairs] */
+  float beta, smoothing;
+} ft_preference_loss_args;
+
+size_t ft_preference_loss_workspace(const ft_preference_loss_args* args);
+int ft_preference_loss(const ft_preference_loss_args* args, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
