@@ -54,6 +54,10 @@ __device__ __forceinline__ void store_part(T* p, int n, u32x4 v) {
     if (i < n) p[i] = u.e[i];
 }
 
+// Hides where a vector came from, so that its elements are unpacked again at
+// each use instead of being kept: registers hold the packed row.
+__device__ __forceinline__ void repack(u32x4& v) { asm volatile("" : "+v"(v)); }
+
 template <typename T>
 __device__ __forceinline__ void to_float(u32x4 v, float (&f)[kVec<T>]) {
   union {

@@ -12,6 +12,8 @@
 // Selections are by counting: the largest key that at least topk keys reach
 // is bisected with ballots over keys in registers, with no atomics and no
 // sort, and rows are written by ordered compaction, ascending as they are.
+#include <type_traits>
+
 #include "op_device.h"
 #include "operators.h"
 
@@ -22,7 +24,8 @@ constexpr int kScanT = 256;     // threads of a scanning workgroup
 constexpr int kScanU = 4;       // vectors in flight a thread
 constexpr int kFinT = 1024;     // of a finishing one
 constexpr int kFinWaves = kFinT / 64;
-constexpr uint32_t kMaxGroups = 65536;  // of a row: 64 keys a thread
+constexpr uint32_t kMaxGroups = 65536;  // of a row
+constexpr uint32_t kRowVecs = 16384;    // of a row that one workgroup scans
 constexpr uint32_t kCap = 8192;         // candidates held in LDS
 
 struct ScanPlan {
@@ -124,296 +127,408 @@ __global__ void __launch_bounds__(kScanT) propose_scan(Args a) {
   }
 }
 
-// Keys are the type's own order: the float's, without the bits that are
-// the same for every value of the type.
+// Keys are the type's own order, as unsigned numbers of its size: NaN as
+// -infinity, -0 as 0.
 template <typename T>
-constexpr int kShift = sizeof(T) == 4 ? 0 : 13;
-template <>
-constexpr int kShift<__bf16> = 16;
+using Half = std::conditional_t<sizeof(T) == 2, T, _Float16>;
+template <typename T>
+using Key = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
 
 template <typename T>
 __device__ __forceinline__ uint32_t key_of(float x) {
-  return order_key(x) >> kShift<T>;
+  if (sizeof(T) == 4) return order_key(x);
+  x = x == x ? x + 0.0f : -INFINITY;
+  const uint32_t b = __builtin_bit_cast(uint16_t, (T)x);
+  return b & 0x8000u ? b ^ 0xFFFFu : b | 0x8000u;
+}
+template <>
+__device__ __forceinline__ uint32_t key_of<float>(float x) {
+  return order_key(x);
 }
 template <typename T>
 __device__ __forceinline__ float value_of(uint32_t k) {
-  // (a negative value's dropped bits are ones)
-  k <<= kShift<T>;
-  if (!(k & 0x80000000u)) k |= (1u << kShift<T>) - 1u;
+  return (float)__builtin_bit_cast(T, (uint16_t)(k & 0x8000u ? k & 0x7FFFu : k ^ 0xFFFFu));
+}
+template <>
+__device__ __forceinline__ float value_of<float>(uint32_t k) {
   return key_value(k);
 }
 
-struct FinShared {
-  uint32_t count[2][3][kFinWaves];
+// The kernels that end a row are bound by latencies: a workgroup walks once
+// through some thousand instructions, with barriers, and every line of them
+// comes from L2.  So their loops are short and rolled, over keys in LDS, and
+// selections are by histograms of 11 bits.
+constexpr uint32_t kKeyBytes = 72u << 10;  // LDS for a row's group keys
+constexpr uint32_t kBins = 2 * kFinT;
+
+struct Shared {
+  uint32_t hist[kBins];
+  uint32_t found[2];
   uint32_t scan[2][kFinWaves];
+  MaxSum ms[kFinWaves];
   float lse, m;
+  uint32_t ckey[kCap], cid[kCap];  // candidates, ascending ids
 };
 
-// The largest key that at least `need` of all keys reach (0 if fewer reach
-// any): count(t1, t2, t3, out) adds up how many of this wave's keys reach
-// each bound; three bounds a round, so two bits.
-template <typename F>
-__device__ __forceinline__ uint32_t nth_largest(FinShared& sh, uint32_t need, uint32_t top,
-                                                F&& count) {
-  const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  uint32_t lo = 0, hi = top;  // reached by enough; not
-  for (int round = 0; hi - lo > 1; ++round) {
-    const uint32_t d = hi - lo, q = d >> 2;
-    const uint32_t t2 = lo + (d >> 1), t1 = q ? lo + q : t2, t3 = q ? t2 + q : t2;
-    uint32_t n[3] = {0, 0, 0};
-    count(t1, t2, t3, n);
-    if (lane == 0)
-      for (int i = 0; i < 3; ++i) sh.count[round & 1][i][wave] = n[i];
-    __syncthreads();
-    uint32_t s[3];
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      s[i] = lane < kFinWaves ? sh.count[round & 1][i][lane] : 0;
-#pragma unroll
-      for (int k = 1; k < kFinWaves; k <<= 1) s[i] += (uint32_t)__shfl_xor((int)s[i], k, 64);
-      s[i] = (uint32_t)__builtin_amdgcn_readfirstlane((int)s[i]);
-    }
-    if (s[2] >= need) lo = t3;
-    else if (s[1] >= need) lo = t2, hi = t3;
-    else if (s[0] >= need) lo = t1, hi = t2;
-    else hi = t1;
+// The highest bin that `need` keys reach, and how many reach it; the
+// histogram is filled (before a barrier) and holds at least as many.
+__device__ __forceinline__ uint32_t pick_bin(Shared& sh, uint32_t need, uint32_t* reach) {
+  const uint32_t tid = threadIdx.x, wave = tid >> 6, top = kBins - 1 - 2 * tid;
+  const uint32_t a = sh.hist[top], own = a + sh.hist[top - 1];
+  uint32_t total, front = wave_scan(own, tid & 63, &total);
+  if ((tid & 63) == 0) sh.scan[0][wave] = total;
+  __syncthreads();
+#pragma unroll 4
+  for (uint32_t w = 0; w < kFinWaves; ++w) front += w < wave ? sh.scan[0][w] : 0;
+  if (front < need && need <= front + own) {
+    const bool first = need <= front + a;
+    sh.found[0] = first ? top : top - 1;
+    sh.found[1] = first ? front + a : front + own;
   }
   __syncthreads();
+  *reach = sh.found[1];
+  return sh.found[0];
+}
+
+// A key that at least `need` of all keys reach, and how many do (n): the
+// largest such key, or the first one found that at most `enough` keys reach.
+// n keys reach lo, at least `need`; over of them, fewer, reach hi.  key(i),
+// i < size, are the keys.
+template <typename F>
+__device__ __forceinline__ uint32_t largest_reached(Shared& sh, uint32_t need, uint32_t enough,
+                                                    uint32_t lo, uint32_t hi, uint32_t over,
+                                                    uint32_t size, uint32_t* n, F&& key) {
+  const uint32_t tid = threadIdx.x;
+  while (hi - lo > 1 && *n > enough) {
+    const int bits = 32 - __clz((int)(hi - lo - 1)), shift = bits > 11 ? bits - 11 : 0;
+    sh.hist[tid] = sh.hist[tid + kFinT] = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (uint32_t i = tid; i < size; i += kFinT) {
+      const uint32_t k = key(i);
+      if (k >= lo && k < hi) atomicAdd(&sh.hist[(k - lo) >> shift], 1u);
+    }
+    __syncthreads();
+    uint32_t reach;
+    const uint32_t bin = pick_bin(sh, need - over, &reach);
+    *n = over + reach;
+    over = *n - sh.hist[bin];
+    lo += bin << shift;
+    hi = min(hi - lo, 1u << shift) + lo;
+    __syncthreads();
+  }
   return lo;
 }
 
-// Sums over the threads in front of (a, b); every thread of the block.
-__device__ __forceinline__ void block_scan2(FinShared& sh, uint32_t& a, uint32_t& b,
-                                            uint32_t* total_a) {
+// Sums over the threads in front of (a, b), and all's in *ta, *tb; every
+// thread of the block.
+__device__ __forceinline__ void block_scan2(Shared& sh, uint32_t& a, uint32_t& b, uint32_t* ta,
+                                            uint32_t* tb) {
   const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  uint32_t ta, tb;
-  a = wave_scan(a, lane, &ta);
-  b = wave_scan(b, lane, &tb);
-  if (lane == 0) {
-    sh.scan[0][wave] = ta;
-    sh.scan[1][wave] = tb;
+  uint64_t v = (uint64_t)a << 32 | b, s = v;
+#pragma unroll
+  for (uint32_t d = 1; d < 64; d <<= 1) {
+    const uint64_t o = (uint64_t)__shfl_up((long long)s, d, 64);
+    if (lane >= d) s += o;
   }
+  if (lane == 63) {
+    sh.scan[0][wave] = (uint32_t)(s >> 32);
+    sh.scan[1][wave] = (uint32_t)s;
+  }
+  s -= v;
+  a = (uint32_t)(s >> 32);
+  b = (uint32_t)s;
   __syncthreads();
-  uint32_t all = 0;
+  uint32_t all_a = 0, all_b = 0;
+#pragma unroll 4
   for (uint32_t w = 0; w < kFinWaves; ++w) {
     const uint32_t wa = sh.scan[0][w], wb = sh.scan[1][w];
-    all += wa;
-    if (w < wave) {
-      a += wa;
-      b += wb;
-    }
+    all_a += wa;
+    all_b += wb;
+    a += w < wave ? wa : 0;
+    b += w < wave ? wb : 0;
   }
-  *total_a = all;
+  *ta = all_a;
+  *tb = all_b;
   __syncthreads();
 }
 
-// A row's end: kK group keys a thread.
-template <typename T, int kK>
-__global__ void __launch_bounds__(kFinT) propose_finish(Args a) {
-  __shared__ FinShared sh;
-  __shared__ uint32_t list[FT_MAX_PROPOSALS];
-  __shared__ uint32_t ckey[kCap], cid[kCap];
-  const uint64_t row = blockIdx.x;
+// How many groups may reach the bound T: it need not be the very K-th
+// largest group maximum, each round that is saved is worth an eighth more
+// groups.
+__device__ __forceinline__ uint32_t enough_groups(uint32_t K) { return K + K / 8 + 32; }
+constexpr uint32_t kMaxListed = FT_MAX_PROPOSALS + FT_MAX_PROPOSALS / 8 + 32;
+
+// Writes a row's proposals; sh.m and sh.lse are there, gkey(g) is group g's
+// key.
+template <typename T, typename G>
+__device__ __forceinline__ void finish_row(Shared& sh, uint16_t* list, const Args& a, uint64_t row,
+                                           uint32_t groups, uint32_t lg, G&& gkey) {
   const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, K = a.topk;
   const T* p = row_of<T>(a, row);
-  const T* gmax = (const T*)a.gmax + row * a.groups;
-
-  // the groups' keys, kK neighbours a thread
-  uint32_t gk[kK];
-#pragma unroll
-  for (int i = 0; i < kK; ++i) {
-    const uint32_t g = tid * kK + i;
-    gk[i] = g < a.groups ? key_of<T>((float)gmax[g]) : 0u;
-  }
-  // the row's sum
-  if (wave == 0) {
-    MaxSum ms{-INFINITY, 0.0f};
-    for (uint32_t i = lane; i < a.chunks; i += 64) ms = merge(ms, a.part[row * a.chunks + i]);
-    ms = wave_merge(ms);
-    if (lane == 0) {
-      sh.m = exp_base(ms.m);
-      sh.lse = logf(ms.s);
-    }
-  }
-  __syncthreads();
-
-  const uint32_t top = key_of<T>(INFINITY) + 1;
-  uint32_t bound = 0;  // T
-  if (a.groups > K)
-    bound = nth_largest(sh, K, top, [&](uint32_t t1, uint32_t t2, uint32_t t3, uint32_t (&n)[3]) {
-#pragma unroll
-      for (int i = 0; i < kK; ++i) {
-        n[0] += (uint32_t)__popcll(__ballot(gk[i] >= t1));
-        n[1] += (uint32_t)__popcll(__ballot(gk[i] >= t2));
-        n[2] += (uint32_t)__popcll(__ballot(gk[i] >= t3));
-      }
-    });
-  // the groups to read again, ascending
-  uint32_t above = 0, tied = 0, sel;
-#pragma unroll
-  for (int i = 0; i < kK; ++i) {
-    const uint32_t g = tid * kK + i;
-    above += g < a.groups && gk[i] > bound;
-    tied += g < a.groups && gk[i] == bound;
-  }
-  block_scan2(sh, above, tied, &sel);
-  {
-    const uint32_t ties = K - sel;  // (sel < K, or every group is wanted)
-#pragma unroll
-    for (int i = 0; i < kK; ++i) {
-      const uint32_t g = tid * kK + i;
-      if (g >= a.groups) continue;
-      const bool t = gk[i] == bound;
-      if (gk[i] > bound || (t && tied < ties)) list[above + min(tied, ties)] = g;
-      above += gk[i] > bound;
-      tied += t;
-    }
-    sel = min(K, a.groups);
-  }
-  __syncthreads();
-
-  // the logits of those groups that reach the bound, in order: each wave
-  // takes a run of vectors, counts, then writes
-  const uint32_t lg = a.lanes_log2, vecs = sel << lg;
-  const uint32_t run = (uint32_t)(((uint64_t)vecs + kFinT - 1) / kFinT) * 64;
-  const uint32_t r0 = min(wave * run, vecs), r1 = min(r0 + run, vecs);
-  auto load = [&](uint32_t i, float (&x)[kVec<T>]) -> uint32_t {  // logits there, their id
-    const uint32_t vec = (list[i >> lg] << lg) + (i & ((1u << lg) - 1));
-    to_float<T>(load_row(p, vec, a.vocab), x);
-    return vec * kVec<T>;
-  };
-  uint32_t mine = 0, zero = 0, n;
-  for (uint32_t i = r0 + lane; i < r1; i += 64) {
-    float x[kVec<T>];
-    const uint32_t id = load(i, x);
-#pragma unroll
-    for (int e = 0; e < kVec<T>; ++e) mine += id + e < a.vocab && key_of<T>(x[e]) >= bound;
-  }
-  block_scan2(sh, mine, zero, &n);
-  const bool held = n <= kCap;
-  if (held) {
-    // (a thread's logits are not neighbours: the order is by vector, so the
-    // wave's offset advances vector row by vector row)
-    uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)mine);  // lane 0: the waves in front
-    for (uint32_t i0 = r0; i0 < r1; i0 += 64) {
-      const uint32_t i = i0 + lane;
-      float x[kVec<T>];
-      uint32_t id = 0, c = 0, t;
-      if (i < r1) {
-        id = load(i, x);
-#pragma unroll
-        for (int e = 0; e < kVec<T>; ++e) c += id + e < a.vocab && key_of<T>(x[e]) >= bound;
-      }
-      uint32_t w = at + wave_scan(c, lane, &t);
-      if (c) {
-#pragma unroll
-        for (int e = 0; e < kVec<T>; ++e)
-          if (id + e < a.vocab && key_of<T>(x[e]) >= bound) {
-            ckey[w] = key_of<T>(x[e]);
-            cid[w++] = id + e;
-          }
-      }
-      at += t;
-    }
-  }
-  __syncthreads();
-
+  // The bound T: first by a histogram of the groups' distance from the row's
+  // maximum, 2047 steps of 1/64 (differences of logits are of that order,
+  // whatever their size); then, where too many groups reach its bin, by
+  // their keys.  (A row of -infinity has m = 0, above its keys too.)
+  constexpr float kSteps = 64.0f;
   const float m = sh.m, lse = sh.lse;
+  const auto bin_of = [&](float x) {  // (x = m may be infinity)
+    return kBins - 1 - (x == m ? 0u : (uint32_t)fminf((m - x) * kSteps, (float)(kBins - 1)));
+  };
+  const uint32_t top = key_of<T>(m) + 1, enough = enough_groups(K);
+  uint32_t bound = 0, reached = groups;
+  if (groups > K) {
+    sh.hist[tid] = sh.hist[tid + kFinT] = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (uint32_t g = tid; g < groups; g += kFinT)
+      atomicAdd(&sh.hist[bin_of(value_of<T>(gkey(g)))], 1u);
+    __syncthreads();
+    const uint32_t bin = pick_bin(sh, K, &reached);
+    const uint32_t over = reached - sh.hist[bin];
+    // the smallest key whose bin is at least b: 64 guesses a round
+    const auto first_key = [&](uint32_t b) {
+      uint32_t lo = 0, hi = top - 1;  // too small; large enough
+      while (hi - lo > 1) {
+        const uint32_t step = (hi - lo - 1) / 64 + 1;
+        const uint32_t k = (uint32_t)min((uint64_t)hi, (uint64_t)lo + (uint64_t)(lane + 1) * step);
+        const uint64_t yes = __ballot(bin_of(value_of<T>(k)) >= b);
+        const uint32_t f = (uint32_t)__ffsll((unsigned long long)yes) - 1u;
+        hi = (uint32_t)min((uint64_t)hi, (uint64_t)lo + (uint64_t)(f + 1) * step);
+        lo += f * step;
+      }
+      return hi;
+    };
+    const uint32_t above = bin < kBins - 1 ? first_key(bin + 1) : top;
+    bound = bin > 0 ? first_key(bin) : 0u;
+    __syncthreads();
+    bound = largest_reached(sh, K, enough, bound, above, over, groups, &reached, gkey);
+  }
+  // The groups to read again, ascending: those above the bound and the first
+  // of those at it, as many as reach it or, where too many do, up to K.  A
+  // wave takes a run of groups, counts them, then lists them.
+  const uint32_t most = reached <= enough ? reached : K;
+  {
+    const uint32_t run = (groups + kFinT - 1) / kFinT * 64;
+    const uint32_t g0 = min(wave * run, groups), g1 = min(g0 + run, groups);
+    uint32_t above = 0, tied = 0;
+#pragma unroll 4
+    for (uint32_t g = g0 + lane; g < g1; g += 64) {
+      const uint32_t k = gkey(g);
+      above += k > bound;
+      tied += k == bound;
+    }
+    uint32_t sum, ties;
+    block_scan2(sh, above, tied, &sum, &ties);
+    ties = most - sum;
+    // (lane 0 has the sums over the waves in front)
+    above = (uint32_t)__builtin_amdgcn_readfirstlane((int)above);
+    tied = (uint32_t)__builtin_amdgcn_readfirstlane((int)tied);
+    const uint64_t before = (1ull << lane) - 1;
+#pragma unroll 2
+    for (uint32_t i = g0; i < g1; i += 64) {
+      const uint32_t g = i + lane, k = g < g1 ? gkey(g) : 0u;
+      const uint64_t ma = __ballot(g < g1 && k > bound), mt = __ballot(g < g1 && k == bound);
+      const uint32_t pa = above + (uint32_t)__popcll(ma & before);
+      const uint32_t pt = tied + (uint32_t)__popcll(mt & before);
+      if (g < g1 && (k > bound || (k == bound && pt < ties))) list[pa + min(pt, ties)] = (uint16_t)g;
+      above += (uint32_t)__popcll(ma);
+      tied += (uint32_t)__popcll(mt);
+    }
+  }
+  __syncthreads();
+  const uint32_t vecs = most << lg, beyond = (a.vocab + kVec<T> - 1) / kVec<T>;
+  const auto place = [&](uint32_t i) {  // where vector i of the listed groups is
+    return i < vecs ? ((uint32_t)list[i >> lg] << lg) + (i & ((1u << lg) - 1)) : beyond;
+  };
+
+  // The logits there that reach the bound, in order; those past kCap are
+  // counted only.  NaN is -infinity here; a bound at or below that lets all
+  // through.
+  const bool all = bound <= key_of<T>(-INFINITY);
+  const float least_value = value_of<T>(bound);
+  uint32_t n = 0;
+  constexpr uint32_t kRun = 4;  // neighbouring vectors a thread
+  u32x4 ahead[kRun];
+  const auto fetch = [&](uint32_t i0) {
+#pragma unroll
+    for (uint32_t u = 0; u < kRun; ++u)
+      ahead[u] = load_row(p, place(i0 + tid * kRun + u), a.vocab);
+  };
+  fetch(0);
+  for (uint32_t i0 = 0; i0 < vecs; i0 += kRun * kFinT) {
+    u32x4 raw[kRun];
+#pragma unroll
+    for (uint32_t u = 0; u < kRun; ++u) raw[u] = ahead[u];
+    if (i0 + kRun * kFinT < vecs) fetch(i0 + kRun * kFinT);
+    uint32_t hits = 0;
+#pragma unroll
+    for (uint32_t u = 0; u < kRun; ++u) {
+      const uint32_t id = place(i0 + tid * kRun + u) * kVec<T>;
+      float x[kVec<T>];
+      to_float<T>(raw[u], x);
+      uint32_t h = 0;
+#pragma unroll
+      for (int e = 0; e < kVec<T>; ++e) h |= (all || x[e] >= least_value ? 1u : 0u) << e;
+      if (id + kVec<T> > a.vocab) h &= id < a.vocab ? (1u << (a.vocab - id)) - 1u : 0u;
+      hits |= h << (u * kVec<T>);
+    }
+    uint32_t at = (uint32_t)__popc(hits), none = 0, total, zero;
+    block_scan2(sh, at, none, &total, &zero);
+    at += n;
+    n += total;
+    while (hits) {
+      const uint32_t bit = (uint32_t)__ffs(hits) - 1u, u = bit / kVec<T>, e = bit % kVec<T>;
+      hits &= hits - 1;
+      if (at < kCap) {
+        const u32x4 v = u < 2 ? (u == 0 ? raw[0] : raw[1]) : u == 2 ? raw[2] : raw[3];
+        const uint32_t w = e * sizeof(T) / 4;
+        const uint32_t word = w < 2 ? (w == 0 ? v.x : v.y) : w == 2 ? v.z : v.w;
+        float x;
+        if (sizeof(T) == 4) x = __uint_as_float(word);
+        else x = (float)__builtin_bit_cast(Half<T>, (uint16_t)(word >> (e & 1) * 16));
+        sh.ckey[at] = key_of<T>(x);
+        sh.cid[at] = place(i0 + tid * kRun + u) * kVec<T> + e;
+      }
+      ++at;
+    }
+  }
+  __syncthreads();
+
   const auto put = [&](uint32_t at, uint32_t id, uint32_t key) {
     const float x = value_of<T>(key);
     a.ids[row * K + at] = (int32_t)id;
     a.logp[row * K + at] = x == -INFINITY && lse == lse ? x : (x - m) - lse;
   };
-  if (held) {
-    // up to 8 neighbouring candidates a thread
+  reached = n;
+  if (n <= kCap) {
+    const uint32_t least = largest_reached(sh, K, K, bound, top, 0, n, &reached,
+                                           [&](uint32_t i) { return sh.ckey[i]; });
+    // neighbouring candidates a thread
     const uint32_t each = (n + kFinT - 1) / kFinT, c0 = min(tid * each, n), c1 = min(c0 + each, n);
-    uint32_t k[kCap / kFinT];
-#pragma unroll
-    for (uint32_t i = 0; i < kCap / kFinT; ++i) k[i] = c0 + i < c1 ? ckey[c0 + i] : 0u;
-    const uint32_t least =
-        nth_largest(sh, K, top, [&](uint32_t t1, uint32_t t2, uint32_t t3, uint32_t (&cnt)[3]) {
-#pragma unroll
-          for (uint32_t i = 0; i < kCap / kFinT; ++i) {
-            if (i >= each) break;
-            cnt[0] += (uint32_t)__popcll(__ballot(k[i] >= t1));
-            cnt[1] += (uint32_t)__popcll(__ballot(k[i] >= t2));
-            cnt[2] += (uint32_t)__popcll(__ballot(k[i] >= t3));
-          }
-        });
-    uint32_t gt = 0, eq = 0, all;
-    for (uint32_t i = 0; c0 + i < c1; ++i) {
-      gt += ckey[c0 + i] > least;
-      eq += ckey[c0 + i] == least;
-    }
-    block_scan2(sh, gt, eq, &all);
-    const uint32_t ties = K - all;
+    uint32_t gt = 0, eq = 0, above, ties;
     for (uint32_t i = c0; i < c1; ++i) {
-      const uint32_t key = ckey[i];
-      const bool t = key == least;
-      if (key > least || (t && eq < ties)) put(gt + min(eq, ties), cid[i], key);
-      gt += key > least;
+      const uint32_t k = sh.ckey[i];
+      gt += k > least;
+      eq += k == least;
+    }
+    block_scan2(sh, gt, eq, &above, &ties);
+    ties = K - above;
+    for (uint32_t i = c0; i < c1; ++i) {
+      const uint32_t k = sh.ckey[i];
+      const bool t = k == least;
+      if (k > least || (t && eq < ties)) put(gt + min(eq, ties), sh.cid[i], k);
+      gt += k > least;
       eq += t;
     }
     return;
   }
-  // More than kCap logits reach the bound (rows in order, or of few values):
-  // the same on the groups in memory.
-  const uint32_t least =
-      nth_largest(sh, K, top, [&](uint32_t t1, uint32_t t2, uint32_t t3, uint32_t (&cnt)[3]) {
-        for (uint32_t i0 = r0; i0 < r1; i0 += 64) {
-          const uint32_t i = i0 + lane;
-          float x[kVec<T>];
-          uint32_t id = a.vocab;
-          if (i < r1) id = load(i, x);
+  // More logits reach the bound than are held (rows in order, or of few
+  // values): the same on the logits in memory.
+  const uint32_t size = vecs * kVec<T>;
+  const auto logit = [&](uint32_t i, uint32_t* id) -> uint32_t {  // its key; 0: none
+    *id = place(i / kVec<T>) * kVec<T> + i % kVec<T>;
+    return *id < a.vocab ? key_of<T>((float)p[*id]) : 0u;
+  };
+  const uint32_t least = largest_reached(sh, K, K, bound, top, 0, size, &reached, [&](uint32_t i) {
+    uint32_t id;
+    return logit(i, &id);
+  });
+  uint32_t ties = K;
+  for (int pass = 0; pass < 2; ++pass) {  // counts, then writes
+    uint32_t gt = 0, eq = 0;
+    for (uint32_t i0 = 0; i0 < size; i0 += kFinT) {
+      uint32_t id = 0;
+      const uint32_t k = i0 + tid < size ? logit(i0 + tid, &id) : 0u;
+      uint32_t g = k > least, q = k != 0 && k == least, all_g, all_q;
+      const bool any = g || q;
+      block_scan2(sh, g, q, &all_g, &all_q);
+      g += gt;
+      q += eq;
+      if (pass && any && (k > least || q < ties)) put(g + min(q, ties), id, k);
+      gt += all_g;
+      eq += all_q;
+    }
+    ties = K - gt;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void set_row_sum(Shared& sh, MaxSum ms) {
+  ms = wave_merge(ms);
+  if ((threadIdx.x & 63) == 0) {
+    sh.m = exp_base(ms.m);
+    sh.lse = logf(ms.s);
+  }
+}
+
+// A row's end.  kLds: the groups' keys fit there.
+template <typename T, bool kLds>
+__global__ void __launch_bounds__(kFinT) propose_finish(Args a) {
+  __shared__ Shared sh;
+  __shared__ uint16_t list[kMaxListed];
+  __shared__ Key<T> keys[kLds ? kKeyBytes / sizeof(T) : 1];
+  const uint64_t row = blockIdx.x;
+  const T* gmax = (const T*)a.gmax + row * a.groups;
+  if (kLds) {
+    const uint32_t vecs = (a.groups + kVec<T> - 1) / kVec<T>;
+    for (uint32_t v = threadIdx.x; v < vecs; v += kFinT) {
+      const uint32_t g = v * kVec<T>;
+      const u32x4 raw = g + kVec<T> <= a.groups ? load_vec(gmax + g)
+                                                : load_part(gmax + g, (int)(a.groups - g), (T)0.0f);
+      float x[kVec<T>];
+      to_float<T>(raw, x);
 #pragma unroll
-          for (int e = 0; e < kVec<T>; ++e) {
-            const uint32_t key = i < r1 && id + e < a.vocab ? key_of<T>(x[e]) : 0u;
-            cnt[0] += (uint32_t)__popcll(__ballot(key >= t1));
-            cnt[1] += (uint32_t)__popcll(__ballot(key >= t2));
-            cnt[2] += (uint32_t)__popcll(__ballot(key >= t3));
-          }
-        }
-      });
-  uint32_t gt = 0, eq = 0, all;
-  for (uint32_t i = r0 + lane; i < r1; i += 64) {
-    float x[kVec<T>];
-    const uint32_t id = load(i, x);
-#pragma unroll
-    for (int e = 0; e < kVec<T>; ++e) {
-      const uint32_t key = id + e < a.vocab ? key_of<T>(x[e]) : 0u;
-      gt += key > least;
-      eq += id + e < a.vocab && key == least;
+      for (int e = 0; e < kVec<T>; ++e) keys[g + e] = (Key<T>)key_of<T>(x[e]);
     }
   }
-  block_scan2(sh, gt, eq, &all);
-  const uint32_t ties = K - all;
-  uint32_t gat = (uint32_t)__builtin_amdgcn_readfirstlane((int)gt);
-  uint32_t eat = (uint32_t)__builtin_amdgcn_readfirstlane((int)eq);
-  for (uint32_t i0 = r0; i0 < r1; i0 += 64) {
-    const uint32_t i = i0 + lane;
-    float x[kVec<T>];
-    uint32_t id = a.vocab, cg = 0, ce = 0, tg, te;
-    if (i < r1) id = load(i, x);
+  if (threadIdx.x < 64) {
+    MaxSum ms{-INFINITY, 0.0f};
+    for (uint32_t i = threadIdx.x; i < a.chunks; i += 64)
+      ms = merge(ms, a.part[row * a.chunks + i]);
+    set_row_sum<T>(sh, ms);
+  }
+  __syncthreads();
+  finish_row<T>(sh, list, a, row, a.groups, a.lanes_log2, [&](uint32_t g) -> uint32_t {
+    return kLds ? (uint32_t)keys[g] : key_of<T>((float)gmax[g]);
+  });
+}
+
+// A whole row in one workgroup; the groups are its vectors.
+template <typename T>
+__global__ void __launch_bounds__(kFinT) propose_row(Args a) {
+  __shared__ Shared sh;
+  __shared__ uint16_t list[kMaxListed];
+  __shared__ Key<T> keys[kRowVecs];
+  const uint64_t row = blockIdx.x;
+  const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const T* p = row_of<T>(a, row);
+  const uint32_t vecs = (a.vocab + kVec<T> - 1) / kVec<T>;
+  MaxSum ms{-INFINITY, 0.0f};
+  for (uint32_t v = tid; v < vecs; v += kScanU * kFinT) {
+    u32x4 raw[kScanU];
 #pragma unroll
-    for (int e = 0; e < kVec<T>; ++e) {
-      const bool in = i < r1 && id + e < a.vocab;
-      const uint32_t key = in ? key_of<T>(x[e]) : 0u;
-      cg += in && key > least;
-      ce += in && key == least;
-    }
-    uint32_t g = gat + wave_scan(cg, lane, &tg), q = eat + wave_scan(ce, lane, &te);
-    gat += tg;
-    eat += te;
+    for (int u = 0; u < kScanU; ++u) raw[u] = load_row(p, v + u * kFinT, a.vocab);
 #pragma unroll
-    for (int e = 0; e < kVec<T>; ++e) {
-      if (!(i < r1 && id + e < a.vocab)) continue;
-      const uint32_t key = key_of<T>(x[e]);
-      const bool t = key == least;
-      if (key > least || (t && q < ties)) put(g + min(q, ties), id + e, key);
-      g += key > least;
-      q += t;
+    for (int u = 0; u < kScanU; ++u) {
+      float x[kVec<T>];
+      to_float<T>(raw[u], x);
+      float g = x[0];
+#pragma unroll
+      for (int e = 1; e < kVec<T>; ++e) g = fmaxf(g, x[e]);
+      if (v + u * kFinT < vecs) keys[v + u * kFinT] = (Key<T>)key_of<T>(g);
+      add_terms(ms, x);
     }
   }
+  ms = wave_merge(ms);
+  if (lane == 0) sh.ms[wave] = ms;
+  __syncthreads();
+  if (wave == 0) {
+    ms = lane < kFinWaves ? sh.ms[lane] : MaxSum{-INFINITY, 0.0f};
+    set_row_sum<T>(sh, ms);
+  }
+  __syncthreads();
+  finish_row<T>(sh, list, a, row, vecs, 0, [&](uint32_t g) -> uint32_t { return keys[g]; });
 }
 
 template <typename T>
@@ -435,15 +550,17 @@ hipError_t launch(const ft_propose_args& a, uint8_t* ws, hipStream_t s) {
   k.ids = a.ids;
   k.logp = a.logp;
   const uint32_t rows = (uint32_t)(a.batch * a.steps);
+  if ((a.vocab + kVec<T> - 1) / kVec<T> <= kRowVecs) {
+    hipLaunchKernelGGL((propose_row<T>), dim3(rows), dim3(kFinT), 0, s, k);
+    return hipGetLastError();
+  }
   hipLaunchKernelGGL((propose_scan<T>), dim3(rows * p.chunks), dim3(kScanT), 0, s, k);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  if (p.groups <= 4 * kFinT)
-    hipLaunchKernelGGL((propose_finish<T, 4>), dim3(rows), dim3(kFinT), 0, s, k);
-  else if (p.groups <= 16 * kFinT)
-    hipLaunchKernelGGL((propose_finish<T, 16>), dim3(rows), dim3(kFinT), 0, s, k);
+  if (p.groups <= kKeyBytes / sizeof(T))
+    hipLaunchKernelGGL((propose_finish<T, true>), dim3(rows), dim3(kFinT), 0, s, k);
   else
-    hipLaunchKernelGGL((propose_finish<T, 64>), dim3(rows), dim3(kFinT), 0, s, k);
+    hipLaunchKernelGGL((propose_finish<T, false>), dim3(rows), dim3(kFinT), 0, s, k);
   return hipGetLastError();
 }
 
