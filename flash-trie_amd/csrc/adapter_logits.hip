@@ -53,6 +53,7 @@ struct Args {
   int32_t* sorted;    // [rows]: their adapters (-1: none)
   float* zscale;      // [rows]: power of two that z was divided by
   uint16_t* z;        // [rows to whole 16s][kParts][rank32]
+  uint32_t* zeros;  // 16 bytes of zeros
   uint32_t row_tiles;
 };
 
@@ -68,6 +69,7 @@ __global__ void __launch_bounds__(1024) logits_order(Args a) {
   __shared__ uint32_t at[kMaxBins + 2];
   __shared__ uint32_t waves[16];
   const uint32_t tid = threadIdx.x, bins = a.adapters + 2;
+  if (tid < 4) a.zeros[tid] = 0;
   const auto bin = [&](int32_t g) {
     return g < 0 ? 0u : (uint32_t)g < a.adapters ? (uint32_t)g + 1 : bins - 1;
   };
@@ -161,10 +163,59 @@ __global__ void __launch_bounds__(256) logits_shrink(Args a) {
   }
 }
 
-constexpr int kBM = 64, kBN = 128, kBK = 64, kThreads = 256;
+// The rows of a tile by their adapters: each run's product of z by its
+// adapter's up is added to the rows that have it (not to the others in a
+// 16-row tile: their product may hold a NaN of an adapter that is not
+// theirs).  The wave's tokens are v0 ... v0 + 16 kN - 1, its rows the
+// subtiles s0 ... s0 + kM - 1 of the tile.
+template <typename T, int kN, int kM>
+__device__ __forceinline__ void add_adapters(const Args& a, const int32_t* ad, const float* zsc,
+                                             uint32_t m0, uint32_t rows, uint32_t v0, uint32_t s0,
+                                             f32x4 (&acc)[kN][kM]) {
+  const uint32_t lane = threadIdx.x & 63, col = lane & 15, q = lane >> 4;
+  const uint32_t end = min((s0 + kM) * 16, rows);
+  for (uint32_t i = s0 * 16; i < end;) {
+    const int32_t g = __builtin_amdgcn_readfirstlane(ad[i]);
+    uint32_t j = i + 1;
+    while (j < end && __builtin_amdgcn_readfirstlane(ad[j]) == g) ++j;
+    if (g >= 0 && (uint32_t)g < a.adapters) {
+      for (uint32_t k0 = 0; k0 < a.rank32; k0 += 32) {
+        u32x4 uf[kN];
+#pragma unroll
+        for (int v = 0; v < kN; ++v) {
+          const uint32_t tok = min(v0 + v * 16 + col, a.vocab - 1);
+          uf[v] = load_k((const T*)a.up + (int64_t)g * a.up_stride[0] + (int64_t)tok * a.up_stride[1],
+                         k0 + q * 8, a.rank);
+        }
+#pragma unroll
+        for (int s = 0; s < kM; ++s) {
+          const uint32_t r0 = (s0 + s) * 16, row = r0 + col;
+          if (r0 + 16 <= i || r0 >= j) continue;
+          const T* z = (const T*)a.z + (uint64_t)(m0 + row) * kParts<T> * a.rank32 + k0 + q * 8;
+          f32x4 d[kN] = {};
+#pragma unroll
+          for (int part = 0; part < kParts<T>; ++part) {
+            const u32x4 zf = load_vec(z + part * a.rank32);
+#pragma unroll
+            for (int v = 0; v < kN; ++v) d[v] = mfma(uf[v], zf, d[v], T{});
+          }
+          if (row >= i && row < j) {
+            const float f = zsc[row];
+#pragma unroll
+            for (int v = 0; v < kN; ++v) acc[v][s] += d[v] * f;
+          }
+        }
+      }
+    }
+    i = j;
+  }
+}
 
-// Block: rows [kBM m, ...) of the order by tokens [kBN n, ...); wave w has
-// tokens 32 w ... 32 w + 31 of them, and all rows.
+constexpr int kBK = 64;  // hidden columns of a step: a line of a row
+
+// Any alignment.  Block: rows [64 m, ...) of the order by tokens [128 n,
+// ...); wave w has tokens 32 w ... 32 w + 31 of them, and all rows.
+constexpr int kBM = 64, kBN = 128, kThreads = 256;
 template <typename T, typename O>
 __global__ void __launch_bounds__(kThreads) logits_product(Args a) {
   __shared__ u32x4 ws[kBN][kBK / 8];  // columns by 8, exchanged within a row
@@ -220,46 +271,7 @@ __global__ void __launch_bounds__(kThreads) logits_product(Args a) {
         for (int j = 0; j < kBM / 16; ++j) acc[i][j] = mfma(wf[i], xf[j], acc[i][j], T{});
     }
   }
-  // the adapters of the tile's rows, each for the rows that have it
-  for (uint32_t i = 0; i < rows;) {
-    const int32_t g = ad[i];
-    uint32_t j = i + 1;
-    while (j < rows && ad[j] == g) ++j;
-    if (g >= 0 && (uint32_t)g < a.adapters) {
-      const uint32_t s0 = i / 16, s1 = (j + 15) / 16;
-      f32x4 d[2][kBM / 16] = {};
-      for (uint32_t k0 = 0; k0 < a.rank32; k0 += 32) {
-        u32x4 uf[2];
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          const uint32_t tok = min(n0 + wave * 32 + v * 16 + col, a.vocab - 1);
-          uf[v] = load_k((const T*)a.up + (int64_t)g * a.up_stride[0] + (int64_t)tok * a.up_stride[1],
-                         k0 + q * 8, a.rank);
-        }
-#pragma unroll
-        for (int s = 0; s < kBM / 16; ++s) {
-          if ((uint32_t)s < s0 || (uint32_t)s >= s1) continue;
-          const T* z = (const T*)a.z + (uint64_t)(m0 + s * 16 + col) * kParts<T> * a.rank32 + k0 + q * 8;
-#pragma unroll
-          for (int part = 0; part < kParts<T>; ++part) {
-            const u32x4 zf = load_vec(z + part * a.rank32);
-#pragma unroll
-            for (int v = 0; v < 2; ++v) d[v][s] = mfma(uf[v], zf, d[v][s], T{});
-          }
-        }
-      }
-#pragma unroll
-      for (int s = 0; s < kBM / 16; ++s) {
-        const uint32_t row = s * 16 + col;
-        if (row >= i && row < j) {
-          const float f = zsc[row];
-#pragma unroll
-          for (int v = 0; v < 2; ++v) acc[v][s] += d[v][s] * f;
-        }
-      }
-    }
-    i = j;
-  }
+  add_adapters<T, 2, kBM / 16>(a, ad, zsc, m0, rows, n0 + wave * 32, 0, acc);
 #pragma unroll
   for (int s = 0; s < kBM / 16; ++s) {
     const uint32_t row = s * 16 + col;
@@ -276,8 +288,177 @@ __global__ void __launch_bounds__(kThreads) logits_product(Args a) {
   }
 }
 
+// Inputs whose rows start at multiples of 16 bytes.  Block: rows [16 kBMs m,
+// ...) by tokens [16 kBNs n, ...), as kWM x kWN waves.  Steps of kBK hidden
+// columns are copied straight to LDS, kStages - 1 of them ahead; a row is a
+// line of eight 16-byte columns, exchanged by the row's number so that the
+// matrix operands are read without bank conflicts.  Columns past the end are
+// copied from a line of zeros.
+template <int kBMs, int kBNs, int kWM, int kWN, int kStages>
+struct Shape {
+  static constexpr int BM = 16 * kBMs, BN = 16 * kBNs, Threads = 64 * kWM * kWN;
+  static constexpr int M = kBMs / kWM, N = kBNs / kWN;  // subtiles of a wave
+  static constexpr int WM = kWM, WN = kWN, Stages = kStages;
+  // 16-byte copies of a thread and step: tokens', rows'
+  static constexpr int CW = BN * 8 / Threads, CX = (BM * 8 + Threads - 1) / Threads;
+  static constexpr int XLanes = BM * 8 / CX / (kWM * kWN);  // lanes of a wave in the rows' copies
+};
+
+__device__ __forceinline__ void copy_to_lds(const void* from, void* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)from,
+                                   (__attribute__((address_space(3))) uint32_t*)to, 16, 0, 0);
+}
+
+// All LDS reads of the wave are done, and all its copies but the last n.
+template <int n>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("" ::: "memory");
+  // vmcnt n, lgkmcnt 0, the third counter free
+  __builtin_amdgcn_s_waitcnt((n & 15) | (n >> 4) << 14 | 7 << 4);
+}
+
+template <typename T, typename O, typename S>
+__global__ void __launch_bounds__(S::Threads) logits_staged(Args a) {
+  // (an array a stage: the compiler tells their copies and reads apart)
+  __shared__ u32x4 st0[(S::BM + S::BN) * 8], st1[(S::BM + S::BN) * 8];
+  __shared__ u32x4 st2[S::Stages > 2 ? (S::BM + S::BN) * 8 : 1];
+  __shared__ u32x4 st3[S::Stages > 3 ? (S::BM + S::BN) * 8 : 1];
+  __shared__ int32_t ad[S::BM], to[S::BM];
+  __shared__ float zsc[S::BM];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 15, q = lane >> 4;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+  const uint32_t wm = wave % S::WM, wn = wave / S::WM;
+  // Consecutive workgroups go to the XCDs in turn: each XCD takes a run of
+  // tiles, the row tiles of a few token tiles together, so that its L2
+  // serves the shared operands.
+  const uint32_t n = gridDim.x, run = n / 8;
+  const uint32_t tile = blockIdx.x < run * 8 ? (blockIdx.x % 8) * run + blockIdx.x / 8 : blockIdx.x;
+  const uint32_t m0 = tile % a.row_tiles * S::BM, n0 = tile / a.row_tiles * S::BN;
+  const uint32_t rows = min((uint32_t)S::BM, a.rows - m0);
+  for (uint32_t i = tid; i < (uint32_t)S::BM; i += S::Threads) {
+    const uint32_t m = m0 + min(i, rows - 1);
+    to[i] = a.perm[m];
+    ad[i] = i < rows ? a.sorted[m] : -1;
+    zsc[i] = a.zscale[m];
+  }
+  __syncthreads();
+
+  // this thread's part of each copy: a row and one of its columns
+  const T* wp[S::CW];
+  const T* xp[S::CX];
+  uint32_t wk[S::CW], xk[S::CX];
+#pragma unroll
+  for (int i = 0; i < S::CW; ++i) {
+    const uint32_t at = i * S::Threads + tid, r = at / 8;
+    wk[i] = ((at & 7) ^ (r & 7)) * 8;
+    wp[i] = (const T*)a.weight + (int64_t)min(n0 + r, a.vocab - 1) * a.weight_stride;
+  }
+#pragma unroll
+  for (int i = 0; i < S::CX; ++i) {
+    const uint32_t at = (i * S::WM * S::WN + wave) * S::XLanes + lane, r = min(at / 8, S::BM - 1u);
+    xk[i] = ((at & 7) ^ (r & 7)) * 8;
+    xp[i] = (const T*)a.x + (int64_t)to[r] * a.x_stride;
+  }
+  const auto copy = [&](u32x4* st, uint32_t k0) {
+#pragma unroll
+    for (int i = 0; i < S::CW; ++i) {
+      const uint32_t k = k0 + wk[i];
+      copy_to_lds(k < a.hidden ? (const void*)(wp[i] + k) : (const void*)a.zeros,
+                  st + i * S::Threads + wave * 64);
+    }
+#pragma unroll
+    for (int i = 0; i < S::CX; ++i) {
+      const uint32_t k = k0 + xk[i];
+      if (S::XLanes == 64 || lane < (uint32_t)S::XLanes)
+        copy_to_lds(k < a.hidden ? (const void*)(xp[i] + k) : (const void*)a.zeros,
+                    st + S::BN * 8 + (i * S::WM * S::WN + wave) * S::XLanes);
+    }
+  };
+  f32x4 acc[S::N][S::M] = {};
+  const auto multiply = [&](const u32x4* st) {
+    const u32x4* ws = st + (wn * S::N * 16 + col) * 8;
+    const u32x4* xs = st + S::BN * 8 + (wm * S::M * 16 + col) * 8;
+#pragma unroll
+    for (int kk = 0; kk < kBK / 32; ++kk) {
+      const uint32_t c = (kk * 4 + q) ^ (col & 7);
+      u32x4 wf[S::N], xf[S::M];
+#pragma unroll
+      for (int i = 0; i < S::N; ++i) wf[i] = ws[i * 128 + c];
+#pragma unroll
+      for (int j = 0; j < S::M; ++j) xf[j] = xs[j * 128 + c];
+#pragma unroll
+      for (int j = 0; j < S::M; ++j)
+#pragma unroll
+        for (int i = 0; i < S::N; ++i) acc[i][j] = mfma(wf[i], xf[j], acc[i][j], T{});
+    }
+  };
+  // One barrier a step: past it, every wave's copies of this step are in LDS
+  // and every wave has read the step before, whose place the next copy
+  // takes.  Copies complete in order, so those of later steps may be left.
+  constexpr int kCopies = S::CW + S::CX;
+  const uint32_t steps = (a.hidden + kBK - 1) / kBK;
+  const auto step = [&](uint32_t i, const u32x4* st, u32x4* next) {
+    if (i + S::Stages - 1 <= steps) wait_copies<kCopies * (S::Stages - 2)>();
+    else wait_copies<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (i + S::Stages - 1 < steps) copy(next, (i + S::Stages - 1) * kBK);
+    multiply(st);
+  };
+  copy(st0, 0);
+  if (S::Stages > 2 && steps > 1) copy(st1, kBK);
+  if (S::Stages > 3 && steps > 2) copy(st2, 2 * kBK);
+  for (uint32_t i = 0; i < steps; i += S::Stages) {
+    if (S::Stages == 2) {
+      step(i, st0, st1);
+      if (i + 1 < steps) step(i + 1, st1, st0);
+    } else if (S::Stages == 3) {
+      step(i, st0, st2);
+      if (i + 1 < steps) step(i + 1, st1, st0);
+      if (i + 2 < steps) step(i + 2, st2, st1);
+    } else {
+      step(i, st0, st3);
+      if (i + 1 < steps) step(i + 1, st1, st0);
+      if (i + 2 < steps) step(i + 2, st2, st1);
+      if (i + 3 < steps) step(i + 3, st3, st2);
+    }
+  }
+  add_adapters<T, S::N, S::M>(a, ad, zsc, m0, rows, n0 + wn * S::N * 16, wm * S::M, acc);
+  // 16 rows at a time through LDS (a part of it for each wave), so that a
+  // row's tokens are stored side by side
+  __syncthreads();
+  constexpr int kRow = S::N * 16 + 4;  // floats; shifted by four banks a row
+  static_assert(kRow * 16 * 4 * S::WM * S::WN <= (S::BM + S::BN) * 128 * 2, "fits two stages");
+  constexpr int kHalf = S::WM * S::WN / 2;
+  float* const mine = (float*)(wave < (uint32_t)kHalf ? st0 : st1) +
+                      (wave < (uint32_t)kHalf ? wave : wave - kHalf) * (kRow * 16);
+  constexpr int kE = 16 / (int)sizeof(O), kPer = S::N * 16 / kE;  // elements, pieces of a row
+#pragma unroll
+  for (int s = 0; s < S::M; ++s) {
+#pragma unroll
+    for (int i = 0; i < S::N; ++i) *(f32x4*)(mine + col * kRow + i * 16 + q * 4) = acc[i][s];
+    asm volatile("" ::: "memory");  // (a wave's LDS accesses are in order)
+#pragma unroll
+    for (int p = 0; p < 16 * kPer / 64; ++p) {
+      const uint32_t at = p * 64 + lane, r = at / kPer, c = at % kPer * kE;
+      const uint32_t row = (wm * S::M + s) * 16 + r, tok = n0 + wn * S::N * 16 + c;
+      if (row < rows && tok < a.vocab) {
+        const bool bad = ad[row] >= 0 && (uint32_t)ad[row] >= a.adapters;
+        float y[kE];
+#pragma unroll
+        for (int e = 0; e < kE; ++e) y[e] = bad ? NAN : mine[r * kRow + c + e];
+        O* out = (O*)a.out + (int64_t)to[row] * a.out_stride + tok;
+        const u32x4 o = from_float<O>(y);
+        if (tok + kE <= a.vocab) store_vec(out, o);
+        else store_part(out, (int)(a.vocab - tok), o);
+      }
+    }
+    asm volatile("" ::: "memory");
+  }
+}
+
 struct Plan {
-  uint64_t perm, sorted, zscale, z, bytes;
+  uint64_t perm, sorted, zscale, zeros, z, bytes;
 };
 
 Plan plan(const ft_adapter_logits_args& a) {
@@ -287,16 +468,38 @@ Plan plan(const ft_adapter_logits_args& a) {
   p.perm = ar.take(a.rows * 4);
   p.sorted = ar.take(a.rows * 4);
   p.zscale = ar.take(a.rows * 4);
-  // (whole tiles of rows are read)
-  p.z = ar.take(round_up(a.rows, kBM) * parts * round_up(a.rank, 32) * 2);
+  p.zeros = ar.take(16);
+  p.z = ar.take(round_up(a.rows, 16) * parts * round_up(a.rank, 32) * 2);
   p.bytes = ar.used;
   return p;
 }
 
+template <typename T, typename O, typename S>
+hipError_t launch_staged(Args a, hipStream_t s) {
+  a.row_tiles = (a.rows + S::BM - 1) / S::BM;
+  const uint32_t tiles = (a.vocab + S::BN - 1) / S::BN;
+  hipLaunchKernelGGL((logits_staged<T, O, S>), dim3(tiles * a.row_tiles), dim3(S::Threads), 0, s, a);
+  return hipGetLastError();
+}
+
+bool whole_vectors(const void* p, int64_t stride) {
+  return (uintptr_t)p % 16 == 0 && stride % 8 == 0;
+}
+
 template <typename T, typename O>
-hipError_t launch(const ft_adapter_logits_args& q, const Args& a, hipStream_t s) {
+hipError_t launch(Args a, hipStream_t s) {
   hipLaunchKernelGGL(logits_order, dim3(1), dim3(1024), 0, s, a);
   hipLaunchKernelGGL((logits_shrink<T>), dim3((a.rows + 15) / 16), dim3(256), 0, s, a);
+  if (a.hidden % 8 == 0 && whole_vectors(a.x, a.x_stride) &&
+      whole_vectors(a.weight, a.weight_stride)) {
+    if (a.rows <= 16) return launch_staged<T, O, Shape<1, 8, 1, 4, 4>>(a, s);
+    if (a.rows <= 32) return launch_staged<T, O, Shape<2, 8, 1, 4, 3>>(a, s);
+    if (a.rows <= 64) return launch_staged<T, O, Shape<4, 8, 1, 4, 3>>(a, s);
+    if (a.rows <= 96) return launch_staged<T, O, Shape<6, 16, 1, 8, 3>>(a, s);
+    if (a.rows <= 128) return launch_staged<T, O, Shape<8, 16, 1, 8, 3>>(a, s);
+    return launch_staged<T, O, Shape<16, 16, 2, 4, 2>>(a, s);
+  }
+  a.row_tiles = (a.rows + kBM - 1) / kBM;
   const uint32_t tiles = (a.vocab + kBN - 1) / kBN;
   hipLaunchKernelGGL((logits_product<T, O>), dim3(tiles * a.row_tiles), dim3(kThreads), 0, s, a);
   return hipGetLastError();
@@ -334,11 +537,11 @@ hipError_t launch_adapter_logits(const ft_adapter_logits_args& q, uint8_t* ws, h
   a.sorted = (int32_t*)(ws + p.sorted);
   a.zscale = (float*)(ws + p.zscale);
   a.z = (uint16_t*)(ws + p.z);
-  a.row_tiles = (a.rows + kBM - 1) / kBM;
+  a.zeros = (uint32_t*)(ws + p.zeros);
   if (q.dtype == FT_BF16)
-    return q.out_dtype == FT_F32 ? launch<__bf16, float>(q, a, s) : launch<__bf16, __bf16>(q, a, s);
-  return q.out_dtype == FT_F32 ? launch<_Float16, float>(q, a, s)
-                               : launch<_Float16, _Float16>(q, a, s);
+    return q.out_dtype == FT_F32 ? launch<__bf16, float>(a, s) : launch<__bf16, __bf16>(a, s);
+  return q.out_dtype == FT_F32 ? launch<_Float16, float>(a, s)
+                               : launch<_Float16, _Float16>(a, s);
 }
 
 }  // namespace fto

@@ -31,7 +31,7 @@ __device__ __forceinline__ void store_vec(T* p, u32x4 v) {
   ((Vec16<T>*)p)->v = v;
 }
 
-// The first n elements of a vector, the others `fill`.
+// The first n elements of a vector, the others `fill`; p[0] is there.
 template <typename T>
 __device__ __forceinline__ u32x4 load_part(const T* p, int n, T fill) {
   union {
@@ -39,7 +39,10 @@ __device__ __forceinline__ u32x4 load_part(const T* p, int n, T fill) {
     T e[kVec<T>];
   } u;
 #pragma unroll
-  for (int i = 0; i < kVec<T>; ++i) u.e[i] = i < n ? p[i] : fill;
+  for (int i = 0; i < kVec<T>; ++i) {
+    const T e = p[max(min(i, n - 1), 0)];
+    u.e[i] = i < n ? e : fill;
+  }
   return u.v;
 }
 template <typename T>
