@@ -454,8 +454,9 @@ __device__ __forceinline__ void store_lines(const Args& a, const Rows<kBM>& tile
     for (int i = 0; i < kN; ++i) *(f32x4*)(mine + col * kRow + i * 16 + q * 4) = acc[i][s];
     asm volatile("" ::: "memory");  // (a wave's LDS accesses are in order)
 #pragma unroll 1
-    for (int p = 0; p < 16 * kPer / 64; ++p) {
+    for (int p = 0; p < (16 * kPer + 63) / 64; ++p) {
       const uint32_t at = p * 64 + lane, r = at / kPer, c = at % kPer * kE;
+      if (16 * kPer < 64 && at >= 16 * kPer) break;
       const uint32_t row = (s0 + s) * 16 + r, tok = v0 + c;
       if (row < rows && tok < a.vocab) {
         const bool bad = tile.ad[row] >= 0 && (uint32_t)tile.ad[row] >= a.adapters;
@@ -625,31 +626,32 @@ __global__ void __launch_bounds__(S::Threads) logits_staged(Args a) {
     load_ups<T, S::BM, S::BN, S::Threads>(a, r, n0, tid, 0, min(r.runs, kUp * (S::Stages - 1)), 0, 0,
                                           ahead);
   // this thread's part of each copy: a row and one of its columns
-  const T* wp[S::CW];
-  const T* xp[S::CX];
-  uint32_t wk[S::CW], xk[S::CX];
+  const auto exchanged = [](uint32_t row) { return row & 7; };
+  const T* wp[8W];
+  const T* xp[8X];
+  uint32_t wk[8W], xk[8X];
 #pragma unroll
-  for (int i = 0; i < S::CW; ++i) {
+  for (int i = 0; i < 8W; ++i) {
     const uint32_t at = i * S::Threads + tid, row = at / 8;
-    wk[i] = ((at & 7) ^ (row & 7)) * 8;
+    wk[i] = ((at % 8) ^ exchanged(row)) * 8;
     wp[i] = (const T*)a.weight + (int64_t)min(n0 + row, a.vocab - 1) * a.weight_stride;
   }
 #pragma unroll
-  for (int i = 0; i < S::CX; ++i) {
+  for (int i = 0; i < 8X; ++i) {
     const uint32_t at = (i * S::WM * S::WN + wave) * S::XLanes + lane;
     const uint32_t row = min(at / 8, S::BM - 1u);
-    xk[i] = ((at & 7) ^ (row & 7)) * 8;
+    xk[i] = ((at % 8) ^ exchanged(row)) * 8;
     xp[i] = (const T*)a.x + (int64_t)r.to[row] * a.x_stride;
   }
   const auto copy = [&](u32x4* st, uint32_t k0) {
 #pragma unroll
-    for (int i = 0; i < S::CW; ++i) {
+    for (int i = 0; i < 8W; ++i) {
       const uint32_t k = k0 + wk[i];
       copy_to_lds(k < a.hidden ? (const void*)(wp[i] + k) : (const void*)a.zeros,
                   st + i * S::Threads + wave * 64);
     }
 #pragma unroll
-    for (int i = 0; i < S::CX; ++i) {
+    for (int i = 0; i < 8X; ++i) {
       const uint32_t k = k0 + xk[i];
       if (S::XLanes == 64 || lane < (uint32_t)S::XLanes)
         copy_to_lds(k < a.hidden ? (const void*)(xp[i] + k) : (const void*)a.zeros,
@@ -662,12 +664,12 @@ __global__ void __launch_bounds__(S::Threads) logits_staged(Args a) {
     const u32x4* xs = st + S::BN * 8 + (wm * S::M * 16 + col) * 8;
 #pragma unroll
     for (int kk = 0; kk < kBK / 32; ++kk) {
-      const uint32_t c = (kk * 4 + q) ^ (col & 7);
+      const uint32_t c = (kk * 4 + q) ^ exchanged(col);
       u32x4 wf[S::N], xf[S::M];
 #pragma unroll
-      for (int i = 0; i < S::N; ++i) wf[i] = ws[i * 128 + c];
+      for (int i = 0; i < S::N; ++i) wf[i] = ws[i * 16 * 8 + c];
 #pragma unroll
-      for (int j = 0; j < S::M; ++j) xf[j] = xs[j * 128 + c];
+      for (int j = 0; j < S::M; ++j) xf[j] = xs[j * 16 * 8 + c];
 #pragma unroll
       for (int j = 0; j < S::M; ++j)
 #pragma unroll
@@ -677,7 +679,7 @@ __global__ void __launch_bounds__(S::Threads) logits_staged(Args a) {
   // One barrier a step: past it, every wave's copies of this step are in LDS
   // and every wave has read the step before, whose place the next copy
   // takes.  Copies complete in order, so those of later steps may be left.
-  constexpr int kCopies = S::CW + S::CX;
+  constexpr int kCopies = 8W + 8X;
   const uint32_t steps = (a.hidden + kBK - 1) / kBK;
   const auto step = [&](uint32_t i, const u32x4* st, u32x4* next) {
     if (i + S::Stages - 1 <= steps) wait_copies<kCopies * (S::Stages - 2)>();
@@ -712,10 +714,10 @@ __global__ void __launch_bounds__(S::Threads) logits_staged(Args a) {
     store_rows<T, O, S::N, S::M>(a, r, rows, n0 + wn * S::N * 16, wm * S::M, acc);
   } else {
     __syncthreads();
-    constexpr uint32_t kHeld = (S::BM + S::BN) * 128 / (stored_floats<S::N>() * 4);
-    static_assert(S::WM * S::WN <= 2 * kHeld, "fits two stages");
+    constexpr uint32_t kHeld = (S::BM + S::BN) * 8 * 16 / (stored_floats<S::N>() * 4);
+    static_assert(S::WM * S::WN <= S::Stages * kHeld, "fits the stages");
     store_lines<T, O, S::N, S::M>(a, r, rows, n0 + wn * S::N * 16, wm * S::M, tid, acc,
-                                  (float*)(wave < kHeld ? st0 : st1) +
+                                  (float*)(wave < kHeld ? st0 : wave < 2 * kHeld ? st1 : wave < 3 * kHeld ? st2 : st3) +
                                       wave % kHeld * stored_floats<S::N>());
   }
 }
@@ -751,9 +753,9 @@ __global__ void __launch_bounds__(S::Threads) logits_tile(Args a) {
   const uint32_t kc = ((tid & 7) ^ (tid >> 3 & 7)) * 8;
   const uint32_t woff = (tid / 8 * (uint32_t)a.weight_stride + kc) * 2;
   const uint32_t wnext = S::Threads / 8 * 2 * (uint32_t)a.weight_stride;  // to the next copy's row
-  uint32_t xoff[S::CX];
+  uint32_t xoff[8X];
 #pragma unroll
-  for (int i = 0; i < S::CX; ++i)
+  for (int i = 0; i < 8X; ++i)
     xoff[i] = ((uint32_t)r.to[(i * S::Threads + tid) / 8] * (uint32_t)a.x_stride + kc) * 2;
   const __amdgpu_buffer_rsrc_t wb = whole_buffer((const T*)a.weight + (int64_t)n0 * a.weight_stride);
   const __amdgpu_buffer_rsrc_t xb = whole_buffer(a.x);
@@ -761,10 +763,10 @@ __global__ void __launch_bounds__(S::Threads) logits_tile(Args a) {
   const auto copy = [&](u32x4* st, uint32_t i) {
     const uint32_t k = min(i, steps - 1) * (kBK * 2);  // (past the end: again, unused)
 #pragma unroll
-    for (int c = 0; c < S::CW; ++c)
+    for (int c = 0; c < 8W; ++c)
       copy_to_lds(wb, woff, k + c * wnext, st + c * S::Threads + wave * 64);
 #pragma unroll
-    for (int c = 0; c < S::CX; ++c)
+    for (int c = 0; c < 8X; ++c)
       copy_to_lds(xb, xoff[c], k, st + S::BN * 8 + c * S::Threads + wave * 64);
   };
   // byte addresses in a stage, of either half (hidden from the compiler, so
@@ -776,7 +778,7 @@ __global__ void __launch_bounds__(S::Threads) logits_tile(Args a) {
     return *(const u32x4*)((const char*)st + bytes + more);
   };
   f32x4 acc[S::N][S::M] = {};
-  constexpr int kCopies = S::CW + S::CX;
+  constexpr int kCopies = 8W + 8X;
   // Half a step: the products of w and x, while w and `ahead` take the next
   // half's operands, at `wat` and `xat` of the stage `next`.  A token operand's
   // register is free when its products are issued; the rows' have two sets.
@@ -892,17 +894,24 @@ hipError_t launch(Args a, hipStream_t s) {
   hipLaunchKernelGGL((logits_shrink<T>), dim3((a.rows + 15) / 16), dim3(kShrinkT), 0, s, a);
   if (a.hidden % 8 == 0 && whole_vectors(a.x, a.x_stride) &&
       whole_vectors(a.weight, a.weight_stride)) {
+    // Up to 96 rows the weights' stream is the bound: two workgroups of 8
+    // waves on a CU, one in its adapters' turns while the other streams (84 x
+    // 262144 x 1024, 6 adapters of rank 12: 174 us; with tiles of 256 tokens
+    // and three stages, one workgroup on a CU: 187).  Up to 16 rows, smaller
+    // tiles where the larger make too few workgroups (8 x 32768 x 512: 7.8
+    // us to 9.0; 16 x 2.2M x 512: 511 to 502).
+    if (a.rows <= 16 && a.vocab < 128 * 1024) return launch_staged<T, O, Shape<1, 4, 1, 4, 4>>(a, s);
     if (a.rows <= 16) return launch_staged<T, O, Shape<1, 8, 1, 4, 4>>(a, s);
-    if (a.rows <= 32) return launch_staged<T, O, Shape<2, 8, 1, 4, 3>>(a, s);
-    if (a.rows <= 64) return launch_staged<T, O, Shape<4, 8, 1, 4, 3>>(a, s);
-    if (a.rows <= 96) return launch_staged<T, O, Shape<6, 16, 1, 8, 3>>(a, s);
+    if (a.rows <= 32) return launch_staged<T, O, Shape<2, 8, 1, 8, 2>>(a, s);
+    if (a.rows <= 64) return launch_staged<T, O, Shape<4, 8, 1, 8, 2>>(a, s);
+    if (a.rows <= 96) return launch_staged<T, O, Shape<6, 8, 1, 8, 2>>(a, s);
     if (a.rows <= 128) return launch_staged<T, O, Shape<8, 16, 1, 8, 3>>(a, s);
     // (32-bit offsets within the rows and within a tile's tokens)
     if (a.rows > 128 && a.hidden % 64 == 0 && a.x_stride >= 0 && a.weight_stride >= 0 &&
         a.rows * (uint64_t)a.x_stride < 1ull << 31 && a.weight_stride < 1ll << 22 &&
         a.vocab >= 256)
       return launch_tile<T, O, TileShape<16, 16, 2, 4>>(a, s);
-    return launch_staged<T, O, Shape<16, 16, 2, 4, 2>>(a, s);
+    return launch_staged<T, O, Shape<16, 8, 2, 8, 2>>(a, s);
   }
   a.row_tiles = (a.rows + kBM - 1) / kBM;
   const uint32_t tiles = (a.vocab + kBN - 1) / kBN;
