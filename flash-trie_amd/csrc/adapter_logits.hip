@@ -626,32 +626,31 @@ __global__ void __launch_bounds__(S::Threads) logits_staged(Args a) {
     load_ups<T, S::BM, S::BN, S::Threads>(a, r, n0, tid, 0, min(r.runs, kUp * (S::Stages - 1)), 0, 0,
                                           ahead);
   // this thread's part of each copy: a row and one of its columns
-  const auto exchanged = [](uint32_t row) { return row & 7; };
-  const T* wp[8W];
-  const T* xp[8X];
-  uint32_t wk[8W], xk[8X];
+  const T* wp[S::CW];
+  const T* xp[S::CX];
+  uint32_t wk[S::CW], xk[S::CX];
 #pragma unroll
-  for (int i = 0; i < 8W; ++i) {
+  for (int i = 0; i < S::CW; ++i) {
     const uint32_t at = i * S::Threads + tid, row = at / 8;
-    wk[i] = ((at % 8) ^ exchanged(row)) * 8;
+    wk[i] = ((at ^ row) & 7) * 8;
     wp[i] = (const T*)a.weight + (int64_t)min(n0 + row, a.vocab - 1) * a.weight_stride;
   }
 #pragma unroll
-  for (int i = 0; i < 8X; ++i) {
+  for (int i = 0; i < S::CX; ++i) {
     const uint32_t at = (i * S::WM * S::WN + wave) * S::XLanes + lane;
     const uint32_t row = min(at / 8, S::BM - 1u);
-    xk[i] = ((at % 8) ^ exchanged(row)) * 8;
+    xk[i] = ((at ^ row) & 7) * 8;
     xp[i] = (const T*)a.x + (int64_t)r.to[row] * a.x_stride;
   }
   const auto copy = [&](u32x4* st, uint32_t k0) {
 #pragma unroll
-    for (int i = 0; i < 8W; ++i) {
+    for (int i = 0; i < S::CW; ++i) {
       const uint32_t k = k0 + wk[i];
       copy_to_lds(k < a.hidden ? (const void*)(wp[i] + k) : (const void*)a.zeros,
                   st + i * S::Threads + wave * 64);
     }
 #pragma unroll
-    for (int i = 0; i < 8X; ++i) {
+    for (int i = 0; i < S::CX; ++i) {
       const uint32_t k = k0 + xk[i];
       if (S::XLanes == 64 || lane < (uint32_t)S::XLanes)
         copy_to_lds(k < a.hidden ? (const void*)(xp[i] + k) : (const void*)a.zeros,
@@ -664,7 +663,7 @@ __global__ void __launch_bounds__(S::Threads) logits_staged(Args a) {
     const u32x4* xs = st + S::BN * 8 + (wm * S::M * 16 + col) * 8;
 #pragma unroll
     for (int kk = 0; kk < kBK / 32; ++kk) {
-      const uint32_t c = (kk * 4 + q) ^ exchanged(col);
+      const uint32_t c = (kk * 4 + q) ^ (col & 7);
       u32x4 wf[S::N], xf[S::M];
 #pragma unroll
       for (int i = 0; i < S::N; ++i) wf[i] = ws[i * 16 * 8 + c];
@@ -679,7 +678,7 @@ __global__ void __launch_bounds__(S::Threads) logits_staged(Args a) {
   // One barrier a step: past it, every wave's copies of this step are in LDS
   // and every wave has read the step before, whose place the next copy
   // takes.  Copies complete in order, so those of later steps may be left.
-  constexpr int kCopies = 8W + 8X;
+  constexpr int kCopies = S::CW + S::CX;
   const uint32_t steps = (a.hidden + kBK - 1) / kBK;
   const auto step = [&](uint32_t i, const u32x4* st, u32x4* next) {
     if (i + S::Stages - 1 <= steps) wait_copies<kCopies * (S::Stages - 2)>();
@@ -753,9 +752,9 @@ __global__ void __launch_bounds__(S::Threads) logits_tile(Args a) {
   const uint32_t kc = ((tid & 7) ^ (tid >> 3 & 7)) * 8;
   const uint32_t woff = (tid / 8 * (uint32_t)a.weight_stride + kc) * 2;
   const uint32_t wnext = S::Threads / 8 * 2 * (uint32_t)a.weight_stride;  // to the next copy's row
-  uint32_t xoff[8X];
+  uint32_t xoff[S::CX];
 #pragma unroll
-  for (int i = 0; i < 8X; ++i)
+  for (int i = 0; i < S::CX; ++i)
     xoff[i] = ((uint32_t)r.to[(i * S::Threads + tid) / 8] * (uint32_t)a.x_stride + kc) * 2;
   const __amdgpu_buffer_rsrc_t wb = whole_buffer((const T*)a.weight + (int64_t)n0 * a.weight_stride);
   const __amdgpu_buffer_rsrc_t xb = whole_buffer(a.x);
@@ -763,10 +762,10 @@ __global__ void __launch_bounds__(S::Threads) logits_tile(Args a) {
   const auto copy = [&](u32x4* st, uint32_t i) {
     const uint32_t k = min(i, steps - 1) * (kBK * 2);  // (past the end: again, unused)
 #pragma unroll
-    for (int c = 0; c < 8W; ++c)
+    for (int c = 0; c < S::CW; ++c)
       copy_to_lds(wb, woff, k + c * wnext, st + c * S::Threads + wave * 64);
 #pragma unroll
-    for (int c = 0; c < 8X; ++c)
+    for (int c = 0; c < S::CX; ++c)
       copy_to_lds(xb, xoff[c], k, st + S::BN * 8 + c * S::Threads + wave * 64);
   };
   // byte addresses in a stage, of either half (hidden from the compiler, so
@@ -778,7 +777,7 @@ __global__ void __launch_bounds__(S::Threads) logits_tile(Args a) {
     return *(const u32x4*)((const char*)st + bytes + more);
   };
   f32x4 acc[S::N][S::M] = {};
-  constexpr int kCopies = 8W + 8X;
+  constexpr int kCopies = S::CW + S::CX;
   // Half a step: the products of w and x, while w and `ahead` take the next
   // half's operands, at `wat` and `xat` of the stage `next`.  A token operand's
   // register is free when its products are issued; the rows' have two sets.
