@@ -10,11 +10,15 @@
 // scan, with no atomics.
 //
 //   key_stats    (row, chunk): (max, sum of exponentials) of the chunk
-//   key_policy   row: token scores, the loss's terms and g
-//   key_scores   16 lanes a key: token scores and the key's margin
+//   key_scores   16 lanes a key: token scores and the key's margin (preference)
 //   key_pairs    64 keys a workgroup: dloss/ds over all pairs, loss's terms
-//   key_lists    row: the list of (token, summed g), and G   (keys > 1)
-//   key_gradient (row, chunk): the gradient; block 0 also adds up the loss
+//   key_rows     row: token scores, the loss's terms and g (policy); the list
+//                of (token, summed g), and what key_gradient needs of the row
+//   key_gradient (row, span): the gradient; block 0 also adds up the loss
+//   key_whole    row: all of the policy loss in one workgroup, for rows that
+//                fit its registers: the logits are read once
+// The gradient is stored as -p G first; then, past a barrier, the list's
+// tokens are stored over it.
 #include "op_device.h"
 #include "operators.h"
 
@@ -25,6 +29,13 @@ constexpr int kStatT = 256;
 constexpr int kStatU = 4;   // vectors in flight a thread
 constexpr int kListT = 1024;
 
+// logits of a workgroup of key_gradient
+template <typename T>
+constexpr uint32_t span_of() {
+  return kStatU * kStatT * kVec<T>;
+}
+
+struct RowInfo;
 struct Args {
   const void* logits;
   int64_t stride[2];
@@ -45,15 +56,22 @@ struct Args {
   float beta, smoothing;
   // workspace
   MaxSum* part;      // [rows, chunks]
-  float* g;          // [rows, keys]: dloss/dlp of the row's tokens (policy)
+  float* g;          // [rows]: dloss/dlp of the row's token (policy, keys = 1)
   float* margin;     // [batch * keys] (preference)
   float* gkey;       // [batch * keys]: dloss/ds (preference)
-  float* total;      // [rows]: G
   float* terms;      // [nterms]: parts of the loss
   uint32_t nterms;
-  uint32_t* listed;  // [rows]: entries of the row's list
+  RowInfo* info;      // [rows] (keys > 1)
   uint32_t* ltok;    // [rows, keys]
   float* lg;         // [rows, keys]
+  uint32_t* from;    // [rows, spans + 1]: the list's entries of each span
+  uint32_t spans;
+};
+
+// What key_gradient needs of a row: p G = scale exp(x - base).
+struct RowInfo {
+  float base, scale;
+  uint32_t used;
 };
 
 template <typename T>
@@ -158,36 +176,6 @@ __device__ __forceinline__ float block_sum(float v, float* waves) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) key_policy(Args a) {
-  __shared__ float waves[4];
-  const uint32_t row = blockIdx.x, r = row / a.steps, t = row - r * a.steps;
-  const bool used = row_used(a, row);
-  const T* p = row_of<T>(a, row);
-  MaxSum ms{0.0f, 1.0f};
-  if (used) ms = row_sum(a, row);
-  const float m = exp_base(ms.m), ls = logf(ms.s);
-  float loss = 0.0f, total = 0.0f;
-  for (uint32_t c = threadIdx.x; c < a.keys; c += 256) {
-    const uint32_t key = r * a.keys + c;
-    const uint64_t at = (uint64_t)key * a.steps + t;
-    float lp = 0.0f, g = 0.0f;
-    if (length_of(a, key) > t) {
-      lp = score(p, a.tokens[at], a.vocab, m, ls);
-      loss += policy_term(a, at, lp, a.advantage[key], a.weight[key], &g);
-    }
-    a.logp[at] = lp;
-    a.g[(uint64_t)row * a.keys + c] = g;
-    total += g;
-  }
-  loss = block_sum(loss, waves);
-  total = block_sum(total, waves);
-  if (threadIdx.x == 0) {
-    a.terms[row] = loss;
-    a.total[row] = total;
-  }
-}
-
-template <typename T>
 __global__ void __launch_bounds__(256) key_scores(Args a) {
   const uint32_t key = blockIdx.x * 16 + (threadIdx.x >> 4), lane = threadIdx.x & 15;
   if (key >= a.batch * a.keys) return;
@@ -258,58 +246,76 @@ __global__ void __launch_bounds__(1024) key_pairs(Args a) {
   }
 }
 
-// dloss/dlp of the row's token of key c
-template <bool kPolicy>
-__device__ __forceinline__ float slope(const Args& a, uint32_t row, uint32_t c) {
-  return kPolicy ? a.g[(uint64_t)row * a.keys + c] : a.gkey[row / a.steps * a.keys + c];
-}
+// LDS of a row's list: kP keys a thread.
+template <int kP>
+struct ListShared {
+  uint64_t keys[kListT * kP];
+  float gs[kListT * kP];
+  float wsum[kListT / 64];
+  uint32_t wtok[kListT / 64], wcount[kListT / 64];
+};
 
-// The row's tokens sorted by (token, key), their slopes summed by token.
-// kP: pairs a thread.
-template <bool kPolicy, int kP>
-__global__ void __launch_bounds__(kListT) key_lists(Args a) {
-  __shared__ uint64_t keys[kListT * kP];
-  __shared__ float gs[kListT * kP];
-  __shared__ float wsum[kListT / 64];
-  __shared__ uint32_t wtok[kListT / 64], wcount[kListT / 64];
-  const uint32_t row = blockIdx.x, r = row / a.steps, t = row - r * a.steps, tid = threadIdx.x;
+// The keys' scores and slopes of row (r, t), the loss's terms (policy); then
+// the row's tokens sorted by (token, key), their slopes summed by token:
+// entries ltok, lg.  Returns their number; *total = G, *loss the row's terms.
+template <typename T, bool kPolicy, int kP>
+__device__ __forceinline__ uint32_t row_list(const Args& a, ListShared<kP>& sh, uint32_t row, float m,
+                                             float ls, uint32_t* ltok, float* lg, float* total,
+                                             float* loss) {
+  const uint32_t r = row / a.steps, t = row - r * a.steps, tid = threadIdx.x;
   const uint32_t wave = tid >> 6, lane = tid & 63;
+  const T* p = row_of<T>(a, row);
   uint32_t n = kListT * kP;  // the next power of two, at least a wave
   while (n > 64 && n / 2 >= a.keys) n >>= 1;
-  float total = 0.0f;
+  float sum = 0.0f, terms = 0.0f;
   for (uint32_t c = tid; c < n; c += kListT) {
     uint64_t k = ~0ull;
     float g = 0.0f;
     if (c < a.keys) {
       const uint32_t key = r * a.keys + c;
-      if (length_of(a, key) > t) {
-        g = slope<kPolicy>(a, row, c);
-        const uint32_t tok = (uint32_t)a.tokens[(uint64_t)key * a.steps + t];
-        if (tok < a.vocab) k = ((uint64_t)tok << 32) | c;
+      const uint64_t at = (uint64_t)key * a.steps + t;
+      // (read before the length is known: the arrays hold it)
+      const int32_t tok = a.tokens[at];
+      const bool in = length_of(a, key) > t;
+      float lp = 0.0f;
+      if (kPolicy) {
+        if (in) {
+          lp = score(p, tok, a.vocab, m, ls);
+          terms += policy_term(a, at, lp, a.advantage[key], a.weight[key], &g);
+        }
+        a.logp[at] = lp;
+      } else if (in) {
+        g = a.gkey[key];
       }
+      if (in && (uint32_t)tok < a.vocab) k = ((uint64_t)(uint32_t)tok << 32) | c;
     }
-    keys[c] = k;
-    gs[c] = g;
-    total += g;
+    sh.keys[c] = k;
+    sh.gs[c] = g;
+    sum += g;
   }
-  if (!kPolicy) {
-    total = block_sum(total, wsum);
-    if (tid == 0) a.total[row] = total;
-  }
-  __syncthreads();
+  *total = block_sum(sum, sh.wsum);
+  if (kPolicy) *loss = block_sum(terms, sh.wsum);
+  if (!a.dlogits) return 0;
+  // (block_sum ends with a barrier)
+#pragma unroll 1
   for (uint32_t k = 2; k <= n; k <<= 1) {
+#pragma unroll 1
     for (uint32_t j = k >> 1; j > 0; j >>= 1) {
       for (uint32_t i = tid; i < n / 2; i += kListT) {
         const uint32_t lo = 2 * i - (i & (j - 1)), hi = lo + j;
-        const uint64_t x = keys[lo], y = keys[hi];
+        const uint64_t x = sh.keys[lo], y = sh.keys[hi];
         if ((x > y) == ((lo & k) == 0)) {
-          keys[lo] = y;
-          keys[hi] = x;
+          sh.keys[lo] = y;
+          sh.keys[hi] = x;
         }
       }
-      __syncthreads();
+      // At distances up to 64 a wave has 128 places to itself; then only the
+      // next exchange decides.
+      if (kP > 1 || j > 64 || (j == 1 && k > 64)) __syncthreads();
+      else __builtin_amdgcn_wave_barrier();
     }
   }
+  __syncthreads();
   // segmented sums, kListT pairs at a time; the last entry of a token's run
   // holds its sum
   uint32_t listed = 0;  // entries so far
@@ -320,10 +326,10 @@ __global__ void __launch_bounds__(kListT) key_lists(Args a) {
     uint32_t tok = ~0u;
     float g = 0.0f;
     if (i < n) {
-      tok = (uint32_t)(keys[i] >> 32);
-      if (tok != ~0u) g = gs[(uint32_t)keys[i]];
+      tok = (uint32_t)(sh.keys[i] >> 32);
+      if (tok != ~0u) g = sh.gs[(uint32_t)sh.keys[i]];
     }
-    const uint32_t next = i + 1 < n ? (uint32_t)(keys[i + 1] >> 32) : ~0u;
+    const uint32_t next = i + 1 < n ? (uint32_t)(sh.keys[i + 1] >> 32) : ~0u;
     const uint32_t tok0 = (uint32_t)__shfl((int)tok, 0, 64);  // (by the whole wave)
     float s = g;
 #pragma unroll
@@ -333,45 +339,95 @@ __global__ void __launch_bounds__(kListT) key_lists(Args a) {
       if (lane >= d && ot == tok) s += o;
     }
     if (lane == 63) {
-      wsum[wave] = s;
-      wtok[wave] = tok;
+      sh.wsum[wave] = s;
+      sh.wtok[wave] = tok;
     }
     __syncthreads();
     // what the run of this wave's first token holds in front of the wave
     float front = 0.0f;
     uint32_t first = wave;
-    while (first > 0 && wtok[first - 1] == tok0) {
+    while (first > 0 && sh.wtok[first - 1] == tok0) {
       --first;
-      if ((uint32_t)(keys[b + first * 64] >> 32) != tok0) break;
+      if ((uint32_t)(sh.keys[b + first * 64] >> 32) != tok0) break;
     }
     if (tok0 != ~0u) {
       if (first == 0 && ctok == tok0) front = csum;
-      for (uint32_t w = first; w < wave; ++w) front += wsum[w];
+      for (uint32_t w = first; w < wave; ++w) front += sh.wsum[w];
     }
     if (tok == tok0) s += front;
     const bool last = tok != ~0u && next != tok;
     const uint64_t ends = __ballot(last);
-    if (lane == 0) wcount[wave] = (uint32_t)__popcll(ends);
+    if (lane == 0) sh.wcount[wave] = (uint32_t)__popcll(ends);
     __syncthreads();
     uint32_t at = listed;
-    for (uint32_t w = 0; w < wave; ++w) at += wcount[w];
+    for (uint32_t w = 0; w < wave; ++w) at += sh.wcount[w];
     at += (uint32_t)__popcll(ends & ((1ull << lane) - 1));
     if (last) {
-      a.ltok[(uint64_t)row * a.keys + at] = tok;
-      a.lg[(uint64_t)row * a.keys + at] = s;
+      ltok[at] = tok;
+      lg[at] = s;
     }
-    for (uint32_t w = 0; w < kListT / 64; ++w) listed += wcount[w];
+    for (uint32_t w = 0; w < kListT / 64; ++w) listed += sh.wcount[w];
     __syncthreads();
     if (tid == kListT - 1) {
-      wsum[0] = s;
-      wtok[0] = tok;
+      sh.wsum[0] = s;
+      sh.wtok[0] = tok;
     }
     __syncthreads();
-    csum = wsum[0];
-    ctok = wtok[0];
+    csum = sh.wsum[0];
+    ctok = sh.wtok[0];
     __syncthreads();
   }
-  if (tid == 0) a.listed[row] = listed;
+  return listed;
+}
+
+// A row of a request's keys.
+template <typename T, bool kPolicy, int kP>
+__global__ void __launch_bounds__(kListT) key_rows(Args a) {
+  __shared__ ListShared<kP> sh;
+  const uint32_t row = blockIdx.x, tid = threadIdx.x;
+  const bool used = row_used(a, row);
+  MaxSum ms{0.0f, 1.0f};
+  if (used) ms = row_sum(a, row);
+  const float base = exp_base(ms.m);
+  uint32_t* ltok = a.ltok + (uint64_t)row * a.keys;
+  float total, loss = 0.0f;
+  const uint32_t n = row_list<T, kPolicy, kP>(a, sh, row, base, logf(ms.s), ltok,
+                                              a.lg + (uint64_t)row * a.keys, &total, &loss);
+  if (tid == 0) {
+    if (kPolicy) a.terms[row] = loss;
+    a.info[row] = RowInfo{base, total / ms.s, used};
+  }
+  if (!a.dlogits) return;
+  // the list's entries of each span
+  __threadfence_block();
+  __syncthreads();
+  const uint32_t span = span_of<T>();
+  for (uint32_t s = tid; s <= a.spans; s += kListT) {
+    uint32_t lo = 0, hi = n;
+    while (lo < hi) {
+      const uint32_t mid = (lo + hi) >> 1;
+      if ((uint64_t)ltok[mid] < (uint64_t)s * span) lo = mid + 1;
+      else hi = mid;
+    }
+    a.from[(uint64_t)row * (a.spans + 1) + s] = lo;
+  }
+}
+
+// Policy, one key a request: a row a thread.
+template <typename T>
+__global__ void __launch_bounds__(256) key_single(Args a) {
+  const uint32_t row = blockIdx.x * 256 + threadIdx.x;
+  if (row >= a.rows) return;
+  const uint32_t r = row / a.steps, t = row - r * a.steps;
+  float lp = 0.0f, g = 0.0f, term = 0.0f;
+  if (length_of(a, r) > t) {
+    const MaxSum ms = row_sum(a, row);
+    lp = score(row_of<T>(a, row), a.tokens[row], a.vocab, exp_base(ms.m), logf(ms.s));
+    term = policy_term(a, row, lp, a.advantage[r], a.weight[r], &g);
+  }
+  a.logp[row] = lp;
+  a.g[row] = g;
+  a.terms[row] = term;
 }
 
 __device__ __forceinline__ void add_loss(const Args& a, float* waves) {
@@ -386,93 +442,150 @@ __global__ void __launch_bounds__(256) key_loss(Args a) {
   add_loss(a, waves);
 }
 
-// Block (row, chunk): kU vectors a thread, in one go.
-template <typename T, bool kPolicy>
-__global__ void __launch_bounds__(kStatT) key_gradient(Args a) {
-  constexpr uint32_t kSpan = kStatU * kStatT * kVec<T>;
-  __shared__ float adds[kSpan];
-  __shared__ float waves[kStatT / 64];
-  const uint32_t vecs = (a.vocab + kVec<T> - 1) / kVec<T>;
-  const uint32_t spans = (vecs + kStatU * kStatT - 1) / (kStatU * kStatT);
-  const uint32_t row = blockIdx.x / spans, span = blockIdx.x - row * spans, tid = threadIdx.x;
-  const uint32_t r = row / a.steps, t = row - r * a.steps;
-  if (blockIdx.x == 0) add_loss(a, waves);
-  T* out = (T*)a.dlogits + (int64_t)r * a.dstride[0] + (int64_t)t * a.dstride[1];
-  const uint32_t v0 = span * kStatU * kStatT, e0 = v0 * kVec<T>;
-  const bool used = row_used(a, row);
-  u32x4 raw[kStatU];
-  float base = 0.0f, scale = 0.0f;
-  bool any = false;
-  if (used) {
-    const T* p = row_of<T>(a, row);
+// A vector of -p G.
+template <typename T>
+__device__ __forceinline__ void store_plain(T* out, uint32_t vec, uint32_t vocab, const RowInfo& info,
+                                            u32x4 raw) {
+  const uint32_t e = vec * kVec<T>;
+  float x[kVec<T>];
+  to_float<T>(raw, x);
 #pragma unroll
-    for (int u = 0; u < kStatU; ++u)
-      raw[u] = load_row(p, v0 + u * kStatT + tid, a.vocab, (T)-INFINITY);
-    uint32_t l0 = 0, l1;
-    const uint32_t* ltok = a.ltok + (uint64_t)row * a.keys;
-    if (a.keys == 1) {
-      const uint32_t tok = (uint32_t)a.tokens[row];
-      l1 = tok < a.vocab && tok >= e0 && tok - e0 < kSpan;
-    } else {
-      // the entries of [e0, e0 + kSpan)
-      const uint32_t n = a.listed[row];
-      uint32_t b = n;
-      while (l0 < b) {
-        const uint32_t mid = (l0 + b) >> 1;
-        if (ltok[mid] < e0) l0 = mid + 1;
-        else b = mid;
-      }
-      l1 = l0;
-      b = n;
-      while (l1 < b) {
-        const uint32_t mid = (l1 + b) >> 1;
-        if (ltok[mid] < e0 + kSpan) l1 = mid + 1;
-        else b = mid;
-      }
-    }
-    const MaxSum ms = row_sum(a, row);
-    base = exp_base(ms.m);
-    const float total = a.keys == 1 ? slope<kPolicy>(a, row, 0) : a.total[row];
-    scale = total / ms.s;
-    any = l1 > l0;
-    if (any) {
-#pragma unroll
-      for (uint32_t i = 0; i < kSpan / kStatT; ++i) adds[i * kStatT + tid] = 0.0f;
-      __syncthreads();
-      if (a.keys == 1) {
-        if (tid == 0) adds[(uint32_t)a.tokens[row] - e0] = total;
-      } else {
-        for (uint32_t i = l0 + tid; i < l1; i += kStatT)
-          adds[ltok[i] - e0] = a.lg[(uint64_t)row * a.keys + i];
-      }
-      __syncthreads();
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < kStatU; ++u) {
-    const uint32_t vec = v0 + u * kStatT + tid, e = vec * kVec<T>;
-    if (vec >= vecs) continue;
-    float x[kVec<T>];
-    if (used) {
-      to_float<T>(raw[u], x);
-#pragma unroll
-      for (int i = 0; i < kVec<T>; ++i) {
-        x[i] = -scale * exp_term(x[i], base);
-        if (any) x[i] += adds[e - e0 + i];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kVec<T>; ++i) x[i] = 0.0f;
-    }
-    const u32x4 o = from_float<T>(x);
-    if (e + kVec<T> <= a.vocab) store_vec(out + e, o);
-    else store_part(out + e, (int)(a.vocab - e), o);
+  for (int i = 0; i < kVec<T>; ++i) x[i] = info.used ? -info.scale * exp_term(x[i], info.base) : 0.0f;
+  const u32x4 o = from_float<T>(x);
+  if (e + kVec<T> <= vocab) store_vec(out + e, o);
+  else store_part(out + e, (int)(vocab - e), o);
+}
+
+// Stores the list's entries [l0, l1) over -p G, in whose place other threads
+// have stored: their stores are waited for.
+template <typename T>
+__device__ __forceinline__ void store_listed(const T* p, T* out, const uint32_t* ltok, const float* lg,
+                                             uint32_t l0, uint32_t l1, float base, float scale) {
+  __builtin_amdgcn_s_waitcnt(0);
+  __threadfence_block();
+  __syncthreads();
+  for (uint32_t i = l0 + threadIdx.x; i < l1; i += blockDim.x) {
+    const uint32_t tok = ltok[i];
+    out[tok] = (T)(lg[i] - scale * exp_term((float)p[tok], base));
   }
 }
 
+// Block (row, span): kStatU vectors a thread, in one go.
+template <typename T, bool kPolicy>
+__global__ void __launch_bounds__(kStatT) key_gradient(Args a) {
+  __shared__ float waves[kStatT / 64];
+  const uint32_t row = blockIdx.x / a.spans, span = blockIdx.x - row * a.spans, tid = threadIdx.x;
+  const uint32_t r = row / a.steps, t = row - r * a.steps;
+  if (blockIdx.x == 0) add_loss(a, waves);
+  const T* p = row_of<T>(a, row);
+  T* out = (T*)a.dlogits + (int64_t)r * a.dstride[0] + (int64_t)t * a.dstride[1];
+  const uint32_t vecs = (a.vocab + kVec<T> - 1) / kVec<T>;
+  const uint32_t v0 = span * kStatU * kStatT, e0 = v0 * kVec<T>;
+  RowInfo info;
+  const uint32_t* ltok = a.ltok + (uint64_t)row * a.keys;
+  const float* lg = a.lg + (uint64_t)row * a.keys;
+  uint32_t l0 = 0, l1 = 0;
+  if (a.keys == 1) {
+    info = RowInfo{0.0f, 0.0f, length_of(a, r) > t};
+    if (info.used) {
+      const MaxSum ms = row_sum(a, row);
+      info.base = exp_base(ms.m);
+      lg = kPolicy ? a.g + row : a.gkey + r;
+      info.scale = *lg / ms.s;
+      ltok = (const uint32_t*)a.tokens + row;
+      const uint32_t tok = *ltok;
+      l1 = tok < a.vocab && tok >= e0 && tok - e0 < span_of<T>();
+    }
+  } else {
+    info = a.info[row];
+    const uint32_t* from = a.from + (uint64_t)row * (a.spans + 1) + span;
+    l0 = from[0];
+    l1 = from[1];
+  }
+  u32x4 raw[kStatU];
+  if (info.used) {
+#pragma unroll
+    for (int u = 0; u < kStatU; ++u) raw[u] = load_row(p, v0 + u * kStatT + tid, a.vocab, (T)-INFINITY);
+  }
+#pragma unroll
+  for (int u = 0; u < kStatU; ++u) {
+    const uint32_t vec = v0 + u * kStatT + tid;
+    if (vec < vecs) store_plain(out, vec, a.vocab, info, raw[u]);
+  }
+  if (l1 > l0) store_listed(p, out, ltok, lg, l0, l1, info.base, info.scale);
+}
+
+// The policy loss of a row, kU vectors of it a thread.
+template <typename T, int kU>
+__global__ void __launch_bounds__(kListT) key_whole(Args a) {
+  __shared__ ListShared<1> sh;
+  __shared__ MaxSum waves[kListT / 64];
+  __shared__ uint32_t ltok[kListT];
+  __shared__ float lg[kListT];
+  const uint32_t row = blockIdx.x, r = row / a.steps, t = row - r * a.steps, tid = threadIdx.x;
+  const T* p = row_of<T>(a, row);
+  T* out = (T*)a.dlogits + (int64_t)r * a.dstride[0] + (int64_t)t * a.dstride[1];
+  const uint32_t vecs = (a.vocab + kVec<T> - 1) / kVec<T>;
+  const bool used = row_used(a, row);
+  u32x4 raw[kU];
+  MaxSum ms{-INFINITY, 0.0f};
+  if (used) {
+#pragma unroll
+    for (int u = 0; u < kU; ++u) raw[u] = load_row(p, u * kListT + tid, a.vocab, (T)-INFINITY);
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      float x[kVec<T>];
+      repack(raw[u]);
+      to_float<T>(raw[u], x);
+      add_terms(ms, x);
+    }
+    ms = wave_merge(ms);
+    if ((tid & 63) == 0) waves[tid >> 6] = ms;
+    __syncthreads();
+    ms = waves[0];
+#pragma unroll 1
+    for (uint32_t w = 1; w < kListT / 64; ++w) ms = merge(ms, waves[w]);
+  } else {
+    ms = MaxSum{0.0f, 1.0f};
+  }
+  const float base = exp_base(ms.m);
+  float total, loss;
+  uint32_t n;
+  if (a.keys == 1) {
+    // (every thread for itself)
+    n = 0;
+    float lp = 0.0f, g = 0.0f;
+    loss = 0.0f;
+    if (used) {
+      const int32_t tok = a.tokens[row];
+      lp = score(p, tok, a.vocab, base, logf(ms.s));
+      loss = policy_term(a, row, lp, a.advantage[r], a.weight[r], &g);
+      if ((uint32_t)tok < a.vocab) {
+        n = 1;
+        ltok[0] = (uint32_t)tok;
+        lg[0] = g;
+      }
+    }
+    if (tid == 0) a.logp[row] = lp;
+    total = g;
+  } else {
+    n = row_list<T, true, 1>(a, sh, row, base, logf(ms.s), ltok, lg, &total, &loss);
+  }
+  if (tid == 0) a.terms[row] = loss;
+  if (!a.dlogits) return;
+  const RowInfo info{base, total / ms.s, used};
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    const uint32_t vec = u * kListT + tid;
+    repack(raw[u]);
+    if (vec < vecs) store_plain(out, vec, a.vocab, info, raw[u]);
+  }
+  if (n) store_listed(p, out, ltok, lg, 0, n, info.base, info.scale);
+}
+
 struct Plan {
-  uint32_t vecs, chunks, chunk_vecs;
-  uint64_t part, g, margin, gkey, total, terms, listed, ltok, lg, bytes;
+  uint32_t vecs, chunks, chunk_vecs, spans;
+  uint64_t part, g, margin, gkey, terms, info, ltok, lg, from, bytes;
 };
 
 Plan plan(const ft_keys& k, bool policy) {
@@ -486,15 +599,16 @@ Plan plan(const ft_keys& k, bool policy) {
   p.chunks = (p.vecs + p.chunk_vecs - 1) / p.chunk_vecs;
   Arena ar;
   p.part = ar.take(rows * p.chunks * sizeof(MaxSum));
-  if (policy) p.g = ar.take(rows * k.keys * 4);
+  p.spans = (p.vecs + kStatU * kStatT - 1) / (kStatU * kStatT);
+  if (policy) p.g = ar.take(rows * 4);
   else {
     p.margin = ar.take(keys * 4);
     p.gkey = ar.take(keys * 4);
   }
-  p.total = ar.take(rows * 4);
   p.terms = ar.take((policy ? rows : 1) * 4);
-  p.listed = ar.take(rows * 4);
   if (k.keys > 1) {
+    p.info = ar.take(rows * sizeof(RowInfo));
+    p.from = ar.take(rows * (p.spans + 1) * 4);
     p.ltok = ar.take(rows * k.keys * 4);
     p.lg = ar.take(rows * k.keys * 4);
   }
@@ -525,9 +639,10 @@ Args base_args(const ft_keys& k, const Plan& p, uint8_t* ws) {
   a.g = (float*)(ws + p.g);
   a.margin = (float*)(ws + p.margin);
   a.gkey = (float*)(ws + p.gkey);
-  a.total = (float*)(ws + p.total);
   a.terms = (float*)(ws + p.terms);
-  a.listed = (uint32_t*)(ws + p.listed);
+  a.info = (RowInfo*)(ws + p.info);
+  a.from = (uint32_t*)(ws + p.from);
+  a.spans = p.spans;
   a.ltok = (uint32_t*)(ws + p.ltok);
   a.lg = (float*)(ws + p.lg);
   return a;
@@ -535,28 +650,34 @@ Args base_args(const ft_keys& k, const Plan& p, uint8_t* ws) {
 
 template <typename T, bool kPolicy>
 hipError_t launch(const Args& a, const Plan& p, hipStream_t s) {
-  if (a.rows) {
-    hipLaunchKernelGGL((key_stats<T>), dim3(a.rows * a.chunks), dim3(kStatT), 0, s, a);
-    if (kPolicy) {
-      hipLaunchKernelGGL((key_policy<T>), dim3(a.rows), dim3(256), 0, s, a);
-    } else {
-      const uint32_t keys = a.batch * a.keys;
-      hipLaunchKernelGGL((key_scores<T>), dim3((keys + 15) / 16), dim3(256), 0, s, a);
-      hipLaunchKernelGGL(key_pairs, dim3((keys + 63) / 64), dim3(1024), 0, s, a);
-    }
-  }
-  if (!a.dlogits || !a.rows) {
+  if (a.rows == 0) {
     hipLaunchKernelGGL(key_loss, dim3(1), dim3(256), 0, s, a);
     return hipGetLastError();
   }
-  if (a.keys > 1) {
-    if (a.keys <= kListT)
-      hipLaunchKernelGGL((key_lists<kPolicy, 1>), dim3(a.rows), dim3(kListT), 0, s, a);
+  if (kPolicy && p.vecs <= 8 * kListT && a.keys <= (uint32_t)kListT) {
+    if (p.vecs <= 4 * kListT)
+      hipLaunchKernelGGL((key_whole<T, 4>), dim3(a.rows), dim3(kListT), 0, s, a);
     else
-      hipLaunchKernelGGL((key_lists<kPolicy, 4>), dim3(a.rows), dim3(kListT), 0, s, a);
+      hipLaunchKernelGGL((key_whole<T, 8>), dim3(a.rows), dim3(kListT), 0, s, a);
+    hipLaunchKernelGGL(key_loss, dim3(1), dim3(256), 0, s, a);
+    return hipGetLastError();
   }
-  const uint32_t spans = (p.vecs + kStatU * kStatT - 1) / (kStatU * kStatT);
-  hipLaunchKernelGGL((key_gradient<T, kPolicy>), dim3(a.rows * spans), dim3(kStatT), 0, s, a);
+  hipLaunchKernelGGL((key_stats<T>), dim3(a.rows * a.chunks), dim3(kStatT), 0, s, a);
+  if (!kPolicy) {
+    const uint32_t keys = a.batch * a.keys;
+    hipLaunchKernelGGL((key_scores<T>), dim3((keys + 15) / 16), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(key_pairs, dim3((keys + 63) / 64), dim3(1024), 0, s, a);
+  }
+  if (a.keys > (uint32_t)kListT)
+    hipLaunchKernelGGL((key_rows<T, kPolicy, 4>), dim3(a.rows), dim3(kListT), 0, s, a);
+  else if (a.keys > 1)
+    hipLaunchKernelGGL((key_rows<T, kPolicy, 1>), dim3(a.rows), dim3(kListT), 0, s, a);
+  else if (kPolicy)
+    hipLaunchKernelGGL((key_single<T>), dim3((a.rows + 255) / 256), dim3(256), 0, s, a);
+  if (a.dlogits)
+    hipLaunchKernelGGL((key_gradient<T, kPolicy>), dim3(a.rows * a.spans), dim3(kStatT), 0, s, a);
+  else
+    hipLaunchKernelGGL(key_loss, dim3(1), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
