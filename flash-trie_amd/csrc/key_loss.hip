@@ -5,9 +5,9 @@
 //   dloss/dx[v] = sum over the row's tokens of (tok = v ? g : 0) - p[v] g
 //               = (sum of the g's of v) - p[v] G,  p[v] = exp(x[v] - lse),
 // so a row needs its lse, G and a short list of (token, summed g); many keys
-// share a token at the first positions of a trie.  The sums are made in a
-// fixed order: the list is sorted by (token, key) and summed by a segmented
-// scan, with no atomics.
+// share a token at the first positions of a trie.  Results do not depend on
+// the order in which threads run: sums are made in a fixed order, or of whole
+// numbers.
 //
 //   key_stats    (row, chunk): (max, sum of exponentials) of the chunk
 //   key_scores   16 lanes a key: token scores and the key's margin (preference)
@@ -19,6 +19,8 @@
 //                fit its registers: the logits are read once
 // The gradient is stored as -p G first; then, past a barrier, the list's
 // tokens are stored over it.
+#include <type_traits>
+
 #include "op_device.h"
 #include "operators.h"
 
@@ -175,6 +177,18 @@ __device__ __forceinline__ float block_sum(float v, float* waves) {
   return v;
 }
 
+// (block_sum's barriers are between the uses of `waves`)
+__device__ __forceinline__ float block_max(float v, float* waves) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v = fmaxf(v, __shfl_xor(v, d, 64));
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0.0f;
+  for (uint32_t w = 0; w < blockDim.x / 64; ++w) v = fmaxf(v, waves[w]);
+  __syncthreads();
+  return v;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) key_scores(Args a) {
   const uint32_t key = blockIdx.x * 16 + (threadIdx.x >> 4), lane = threadIdx.x & 15;
@@ -246,31 +260,38 @@ __global__ void __launch_bounds__(1024) key_pairs(Args a) {
   }
 }
 
-// LDS of a row's list: kP keys a thread.
+// A row's tokens and the sums of their slopes: a hash table.  Sums are whole
+// numbers of 2^-52 of the row's largest slope (kP * 1024 of them fit 63
+// bits), so that they do not depend on the order of the atomics and are finer
+// than a 32-bit sum's roundings.
 template <int kP>
-struct ListShared {
-  uint64_t keys[kListT * kP];
-  float gs[kListT * kP];
+struct Table {
+  static constexpr uint32_t kSlots = 2 * kListT * kP;
+  uint32_t tok[kSlots];  // ~0: free
+  unsigned long long sum[kSlots];
   float wsum[kListT / 64];
-  uint32_t wtok[kListT / 64], wcount[kListT / 64];
 };
 
-// The keys' scores and slopes of row (r, t), the loss's terms (policy); then
-// the row's tokens sorted by (token, key), their slopes summed by token:
-// entries ltok, lg.  Returns their number; *total = G, *loss the row's terms.
+// The keys' scores and slopes of row (r, t) and the loss's terms (policy),
+// and the table of its tokens, whose sums count *unit each.  *total = G,
+// *loss the row's terms.
 template <typename T, bool kPolicy, int kP>
-__device__ __forceinline__ uint32_t row_list(const Args& a, ListShared<kP>& sh, uint32_t row, float m,
-                                             float ls, uint32_t* ltok, float* lg, float* total,
-                                             float* loss) {
+__device__ __forceinline__ void row_table(const Args& a, Table<kP>& sh, uint32_t row, float m, float ls,
+                                          float* total, float* loss, double* unit) {
   const uint32_t r = row / a.steps, t = row - r * a.steps, tid = threadIdx.x;
-  const uint32_t wave = tid >> 6, lane = tid & 63;
   const T* p = row_of<T>(a, row);
-  uint32_t n = kListT * kP;  // the next power of two, at least a wave
-  while (n > 64 && n / 2 >= a.keys) n >>= 1;
-  float sum = 0.0f, terms = 0.0f;
-  for (uint32_t c = tid; c < n; c += kListT) {
-    uint64_t k = ~0ull;
-    float g = 0.0f;
+  if (a.dlogits)
+    for (uint32_t i = tid; i < Table<kP>::kSlots; i += kListT) {
+      sh.tok[i] = ~0u;
+      sh.sum[i] = 0;
+    }
+  float sum = 0.0f, terms = 0.0f, most = 0.0f, gs[kP];
+  uint32_t toks[kP];
+#pragma unroll
+  for (int i = 0; i < kP; ++i) {
+    const uint32_t c = i * kListT + tid;
+    gs[i] = 0.0f;
+    toks[i] = ~0u;
     if (c < a.keys) {
       const uint32_t key = r * a.keys + c;
       const uint64_t at = (uint64_t)key * a.steps + t;
@@ -281,136 +302,88 @@ __device__ __forceinline__ uint32_t row_list(const Args& a, ListShared<kP>& sh, 
       if (kPolicy) {
         if (in) {
           lp = score(p, tok, a.vocab, m, ls);
-          terms += policy_term(a, at, lp, a.advantage[key], a.weight[key], &g);
+          terms += policy_term(a, at, lp, a.advantage[key], a.weight[key], &gs[i]);
         }
         a.logp[at] = lp;
       } else if (in) {
-        g = a.gkey[key];
+        gs[i] = a.gkey[key];
       }
-      if (in && (uint32_t)tok < a.vocab) k = ((uint64_t)(uint32_t)tok << 32) | c;
+      if (in && (uint32_t)tok < a.vocab) toks[i] = (uint32_t)tok;
+      sum += gs[i];
+      most = fmaxf(most, fabsf(gs[i]));
     }
-    sh.keys[c] = k;
-    sh.gs[c] = g;
-    sum += g;
   }
   *total = block_sum(sum, sh.wsum);
   if (kPolicy) *loss = block_sum(terms, sh.wsum);
-  if (!a.dlogits) return 0;
-  // (block_sum ends with a barrier)
-#pragma unroll 1
-  for (uint32_t k = 2; k <= n; k <<= 1) {
-#pragma unroll 1
-    for (uint32_t j = k >> 1; j > 0; j >>= 1) {
-      for (uint32_t i = tid; i < n / 2; i += kListT) {
-        const uint32_t lo = 2 * i - (i & (j - 1)), hi = lo + j;
-        const uint64_t x = sh.keys[lo], y = sh.keys[hi];
-        if ((x > y) == ((lo & k) == 0)) {
-          sh.keys[lo] = y;
-          sh.keys[hi] = x;
-        }
-      }
-      // At distances up to 64 a wave has 128 places to itself; then only the
-      // next exchange decides.
-      if (kP > 1 || j > 64 || (j == 1 && k > 64)) __syncthreads();
-      else __builtin_amdgcn_wave_barrier();
+  if (!a.dlogits) return;
+  most = block_max(most, sh.wsum);
+  // (a slope that is not finite makes the sums NaN)
+  const bool finite = fabsf(*total) < INFINITY && most < INFINITY;
+  const double scale = most > 0.0f ? 0x1p52 / (double)most : 0.0;
+  *unit = finite ? (double)most * 0x1p-52 : (double)NAN;
+#pragma unroll
+  for (int i = 0; i < kP; ++i) {
+    if (toks[i] == ~0u) continue;
+    uint32_t h = toks[i] * 2654435761u % Table<kP>::kSlots;
+    for (;;) {  // (half the slots stay free)
+      const uint32_t old = atomicCAS(&sh.tok[h], ~0u, toks[i]);
+      if (old == ~0u || old == toks[i]) break;
+      h = (h + 1) % Table<kP>::kSlots;
     }
+    if (finite) atomicAdd(&sh.sum[h], (unsigned long long)(long long)rint((double)gs[i] * scale));
   }
   __syncthreads();
-  // segmented sums, kListT pairs at a time; the last entry of a token's run
-  // holds its sum
-  uint32_t listed = 0;  // entries so far
-  uint32_t ctok = ~0u;  // the run that goes on from the pairs before
-  float csum = 0.0f;
-  for (uint32_t b = 0; b < n; b += kListT) {
-    const uint32_t i = b + tid;
-    uint32_t tok = ~0u;
-    float g = 0.0f;
-    if (i < n) {
-      tok = (uint32_t)(sh.keys[i] >> 32);
-      if (tok != ~0u) g = sh.gs[(uint32_t)sh.keys[i]];
-    }
-    const uint32_t next = i + 1 < n ? (uint32_t)(sh.keys[i + 1] >> 32) : ~0u;
-    const uint32_t tok0 = (uint32_t)__shfl((int)tok, 0, 64);  // (by the whole wave)
-    float s = g;
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d <<= 1) {
-      const float o = __shfl_up(s, d, 64);
-      const uint32_t ot = (uint32_t)__shfl_up((int)tok, d, 64);
-      if (lane >= d && ot == tok) s += o;
-    }
-    if (lane == 63) {
-      sh.wsum[wave] = s;
-      sh.wtok[wave] = tok;
-    }
-    __syncthreads();
-    // what the run of this wave's first token holds in front of the wave
-    float front = 0.0f;
-    uint32_t first = wave;
-    while (first > 0 && sh.wtok[first - 1] == tok0) {
-      --first;
-      if ((uint32_t)(sh.keys[b + first * 64] >> 32) != tok0) break;
-    }
-    if (tok0 != ~0u) {
-      if (first == 0 && ctok == tok0) front = csum;
-      for (uint32_t w = first; w < wave; ++w) front += sh.wsum[w];
-    }
-    if (tok == tok0) s += front;
-    const bool last = tok != ~0u && next != tok;
-    const uint64_t ends = __ballot(last);
-    if (lane == 0) sh.wcount[wave] = (uint32_t)__popcll(ends);
-    __syncthreads();
-    uint32_t at = listed;
-    for (uint32_t w = 0; w < wave; ++w) at += sh.wcount[w];
-    at += (uint32_t)__popcll(ends & ((1ull << lane) - 1));
-    if (last) {
-      ltok[at] = tok;
-      lg[at] = s;
-    }
-    for (uint32_t w = 0; w < kListT / 64; ++w) listed += sh.wcount[w];
-    __syncthreads();
-    if (tid == kListT - 1) {
-      sh.wsum[0] = s;
-      sh.wtok[0] = tok;
-    }
-    __syncthreads();
-    csum = sh.wsum[0];
-    ctok = sh.wtok[0];
-    __syncthreads();
-  }
-  return listed;
 }
 
-// A row of a request's keys.
+// A row of a request's keys: the table's entries by span.
+constexpr uint32_t kMaxSpans = 4096;  // of 2^24 logits
+
 template <typename T, bool kPolicy, int kP>
 __global__ void __launch_bounds__(kListT) key_rows(Args a) {
-  __shared__ ListShared<kP> sh;
+  static_assert((1u << 24) / span_of<T>() <= kMaxSpans, "counters of the spans");
+  __shared__ Table<kP> sh;
+  __shared__ uint32_t count[kMaxSpans], waves[kListT / 64];
   const uint32_t row = blockIdx.x, tid = threadIdx.x;
   const bool used = row_used(a, row);
   MaxSum ms{0.0f, 1.0f};
   if (used) ms = row_sum(a, row);
   const float base = exp_base(ms.m);
-  uint32_t* ltok = a.ltok + (uint64_t)row * a.keys;
   float total, loss = 0.0f;
-  const uint32_t n = row_list<T, kPolicy, kP>(a, sh, row, base, logf(ms.s), ltok,
-                                              a.lg + (uint64_t)row * a.keys, &total, &loss);
+  double unit = 0.0;
+  for (uint32_t i = tid; i < a.spans; i += kListT) count[i] = 0;
+  row_table<T, kPolicy, kP>(a, sh, row, base, logf(ms.s), &total, &loss, &unit);
   if (tid == 0) {
     if (kPolicy) a.terms[row] = loss;
     a.info[row] = RowInfo{base, total / ms.s, used};
   }
   if (!a.dlogits) return;
-  // the list's entries of each span
-  __threadfence_block();
+  for (uint32_t i = tid; i < Table<kP>::kSlots; i += kListT)
+    if (sh.tok[i] != ~0u) atomicAdd(&count[sh.tok[i] / span_of<T>()], 1u);
   __syncthreads();
-  const uint32_t span = span_of<T>();
-  for (uint32_t s = tid; s <= a.spans; s += kListT) {
-    uint32_t lo = 0, hi = n;
-    while (lo < hi) {
-      const uint32_t mid = (lo + hi) >> 1;
-      if ((uint64_t)ltok[mid] < (uint64_t)s * span) lo = mid + 1;
-      else hi = mid;
-    }
-    a.from[(uint64_t)row * (a.spans + 1) + s] = lo;
+  // exclusive sums over the spans, neighbours a thread
+  uint32_t* from = a.from + (uint64_t)row * (a.spans + 1);
+  const uint32_t each = (a.spans + kListT - 1) / kListT;
+  const uint32_t s0 = min(tid * each, a.spans), s1 = min(s0 + each, a.spans);
+  uint32_t sum = 0, all;
+  for (uint32_t i = s0; i < s1; ++i) sum += count[i];
+  uint32_t front = wave_scan(sum, tid & 63, &all);
+  if ((tid & 63) == 0) waves[tid >> 6] = all;
+  __syncthreads();
+#pragma unroll 1
+  for (uint32_t w = 0; w < tid >> 6; ++w) front += waves[w];
+  for (uint32_t i = s0; i < s1; ++i) {
+    const uint32_t n = count[i];
+    count[i] = from[i] = front;
+    front += n;
   }
+  if (tid == kListT - 1) from[a.spans] = front;
+  __syncthreads();
+  for (uint32_t i = tid; i < Table<kP>::kSlots; i += kListT)
+    if (sh.tok[i] != ~0u) {
+      const uint32_t at = atomicAdd(&count[sh.tok[i] / span_of<T>()], 1u);
+      a.ltok[(uint64_t)row * a.keys + at] = sh.tok[i];
+      a.lg[(uint64_t)row * a.keys + at] = (float)((double)(long long)sh.sum[i] * unit);
+    }
 }
 
 // Policy, one key a request: a row a thread.
@@ -456,18 +429,17 @@ __device__ __forceinline__ void store_plain(T* out, uint32_t vec, uint32_t vocab
   else store_part(out + e, (int)(vocab - e), o);
 }
 
-// Stores the list's entries [l0, l1) over -p G, in whose place other threads
-// have stored: their stores are waited for.
-template <typename T>
-__device__ __forceinline__ void store_listed(const T* p, T* out, const uint32_t* ltok, const float* lg,
-                                             uint32_t l0, uint32_t l1, float base, float scale) {
+// Past this, the block's stores are in memory's order before its later ones.
+__device__ __forceinline__ void stores_done() {
   __builtin_amdgcn_s_waitcnt(0);
   __threadfence_block();
   __syncthreads();
-  for (uint32_t i = l0 + threadIdx.x; i < l1; i += blockDim.x) {
-    const uint32_t tok = ltok[i];
-    out[tok] = (T)(lg[i] - scale * exp_term((float)p[tok], base));
-  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_token(const T* p, T* out, uint32_t tok, float g,
+                                            const RowInfo& info) {
+  out[tok] = (T)(g - info.scale * exp_term((float)p[tok], info.base));
 }
 
 // Block (row, span): kStatU vectors a thread, in one go.
@@ -512,26 +484,28 @@ __global__ void __launch_bounds__(kStatT) key_gradient(Args a) {
     const uint32_t vec = v0 + u * kStatT + tid;
     if (vec < vecs) store_plain(out, vec, a.vocab, info, raw[u]);
   }
-  if (l1 > l0) store_listed(p, out, ltok, lg, l0, l1, info.base, info.scale);
+  if (l1 > l0) {
+    stores_done();
+    for (uint32_t i = l0 + tid; i < l1; i += kStatT) store_token(p, out, ltok[i], lg[i], info);
+  }
 }
 
-// The policy loss of a row, kU vectors of it a thread.
-template <typename T, int kU>
-__global__ void __launch_bounds__(kListT) key_whole(Args a) {
-  __shared__ ListShared<1> sh;
-  __shared__ MaxSum waves[kListT / 64];
-  __shared__ uint32_t ltok[kListT];
-  __shared__ float lg[kListT];
+// The policy loss of a row, kU vectors of it a thread of kT.  kMany: several
+// keys (kT = kListT).
+template <typename T, bool kMany, int kT, int kU>
+__global__ void __launch_bounds__(kT) key_whole(Args a) {
+  __shared__ std::conditional_t<kMany, Table<1>, int> sh;
+  __shared__ MaxSum waves[kT / 64];
   const uint32_t row = blockIdx.x, r = row / a.steps, t = row - r * a.steps, tid = threadIdx.x;
   const T* p = row_of<T>(a, row);
   T* out = (T*)a.dlogits + (int64_t)r * a.dstride[0] + (int64_t)t * a.dstride[1];
   const uint32_t vecs = (a.vocab + kVec<T> - 1) / kVec<T>;
-  const bool used = row_used(a, row);
+  const bool used = kMany ? row_used(a, row) : length_of(a, r) > t;
   u32x4 raw[kU];
   MaxSum ms{-INFINITY, 0.0f};
   if (used) {
 #pragma unroll
-    for (int u = 0; u < kU; ++u) raw[u] = load_row(p, u * kListT + tid, a.vocab, (T)-INFINITY);
+    for (int u = 0; u < kU; ++u) raw[u] = load_row(p, u * kT + tid, a.vocab, (T)-INFINITY);
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       float x[kVec<T>];
@@ -544,43 +518,43 @@ __global__ void __launch_bounds__(kListT) key_whole(Args a) {
     __syncthreads();
     ms = waves[0];
 #pragma unroll 1
-    for (uint32_t w = 1; w < kListT / 64; ++w) ms = merge(ms, waves[w]);
+    for (uint32_t w = 1; w < kT / 64; ++w) ms = merge(ms, waves[w]);
   } else {
     ms = MaxSum{0.0f, 1.0f};
   }
-  const float base = exp_base(ms.m);
-  float total, loss;
-  uint32_t n;
-  if (a.keys == 1) {
-    // (every thread for itself)
-    n = 0;
-    float lp = 0.0f, g = 0.0f;
-    loss = 0.0f;
+  const float base = exp_base(ms.m), ls = logf(ms.s);
+  float total = 0.0f, loss = 0.0f;
+  double unit = 0.0;
+  int32_t tok = -1;
+  if constexpr (kMany) {
+    row_table<T, true, 1>(a, sh, row, base, ls, &total, &loss, &unit);
+  } else {  // every thread for itself
+    float lp = 0.0f;
     if (used) {
-      const int32_t tok = a.tokens[row];
-      lp = score(p, tok, a.vocab, base, logf(ms.s));
-      loss = policy_term(a, row, lp, a.advantage[r], a.weight[r], &g);
-      if ((uint32_t)tok < a.vocab) {
-        n = 1;
-        ltok[0] = (uint32_t)tok;
-        lg[0] = g;
-      }
+      tok = a.tokens[row];
+      lp = score(p, tok, a.vocab, base, ls);
+      loss = policy_term(a, row, lp, a.advantage[r], a.weight[r], &total);
     }
     if (tid == 0) a.logp[row] = lp;
-    total = g;
-  } else {
-    n = row_list<T, true, 1>(a, sh, row, base, logf(ms.s), ltok, lg, &total, &loss);
   }
   if (tid == 0) a.terms[row] = loss;
   if (!a.dlogits) return;
   const RowInfo info{base, total / ms.s, used};
 #pragma unroll
   for (int u = 0; u < kU; ++u) {
-    const uint32_t vec = u * kListT + tid;
+    const uint32_t vec = u * kT + tid;
     repack(raw[u]);
     if (vec < vecs) store_plain(out, vec, a.vocab, info, raw[u]);
   }
-  if (n) store_listed(p, out, ltok, lg, 0, n, info.base, info.scale);
+  if (!used) return;
+  stores_done();
+  if constexpr (kMany) {
+    for (uint32_t i = tid; i < Table<1>::kSlots; i += kT)
+      if (sh.tok[i] != ~0u)
+        store_token(p, out, sh.tok[i], (float)((double)(long long)sh.sum[i] * unit), info);
+  } else if (tid == 0 && (uint32_t)tok < a.vocab) {
+    store_token(p, out, (uint32_t)tok, total, info);
+  }
 }
 
 struct Plan {
@@ -655,10 +629,17 @@ hipError_t launch(const Args& a, const Plan& p, hipStream_t s) {
     return hipGetLastError();
   }
   if (kPolicy && p.vecs <= 8 * kListT && a.keys <= (uint32_t)kListT) {
-    if (p.vecs <= 4 * kListT)
-      hipLaunchKernelGGL((key_whole<T, 4>), dim3(a.rows), dim3(kListT), 0, s, a);
-    else
-      hipLaunchKernelGGL((key_whole<T, 8>), dim3(a.rows), dim3(kListT), 0, s, a);
+    const dim3 g(a.rows);
+    if (a.keys > 1) {
+      if (p.vecs <= 4 * kListT)
+        hipLaunchKernelGGL((key_whole<T, true, kListT, 4>), g, dim3(kListT), 0, s, a);
+      else
+        hipLaunchKernelGGL((key_whole<T, true, kListT, 8>), g, dim3(kListT), 0, s, a);
+    } else if (p.vecs <= 8 * 512) {
+      hipLaunchKernelGGL((key_whole<T, false, 512, 8>), g, dim3(512), 0, s, a);
+    } else {
+      hipLaunchKernelGGL((key_whole<T, false, 1024, 8>), g, dim3(1024), 0, s, a);
+    }
     hipLaunchKernelGGL(key_loss, dim3(1), dim3(256), 0, s, a);
     return hipGetLastError();
   }
