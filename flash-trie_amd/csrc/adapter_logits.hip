@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(1024) logits_order(Args a) {
   const uint32_t b0 = min(tid * each, cells), b1 = min(b0 + each, cells);
   uint32_t sum = 0, t;
   for (uint32_t i = b0; i < b1; ++i) sum += (&at[0][0])[i];
-  uint32_t front = wave_scan(sum, lane, &t);
+  uint32_t front = wave_scan(sum, &t);
   if (lane == 0) waves[wave] = t;
   __syncthreads();
   for (uint32_t w = 0; w < wave; ++w) front += waves[w];
@@ -205,8 +205,7 @@ __global__ void __launch_bounds__(kShrinkT) logits_shrink(Args a) {
   const uint32_t row = wave;
   float big = 0.0f;
   for (uint32_t k = lane; k < a.rank; k += 64) big = fmaxf(big, fabsf(zs[row][k]));
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) big = fmaxf(big, __shfl_xor(big, d, 64));
+  big = wave_max(big);
   int e = 0;
   // f16: its largest to [1, 2); bf16 has the range of z
   if (kParts<T> == 2 && big > 0.0f && big < INFINITY) (void)frexpf(big, &e), e -= 1;

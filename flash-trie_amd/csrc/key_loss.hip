@@ -179,8 +179,7 @@ __device__ __forceinline__ float block_sum(float v, float* waves) {
 
 // (block_sum's barriers are between the uses of `waves`)
 __device__ __forceinline__ float block_max(float v, float* waves) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v = fmaxf(v, __shfl_xor(v, d, 64));
+  v = wave_max(v);
   if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
   __syncthreads();
   v = 0.0f;
@@ -366,7 +365,7 @@ __global__ void __launch_bounds__(kListT) key_rows(Args a) {
   const uint32_t s0 = min(tid * each, a.spans), s1 = min(s0 + each, a.spans);
   uint32_t sum = 0, all;
   for (uint32_t i = s0; i < s1; ++i) sum += count[i];
-  uint32_t front = wave_scan(sum, tid & 63, &all);
+  uint32_t front = wave_scan(sum, &all);
   if ((tid & 63) == 0) waves[tid >> 6] = all;
   __syncthreads();
 #pragma unroll 1
@@ -516,9 +515,7 @@ __global__ void __launch_bounds__(kT) key_whole(Args a) {
     ms = wave_merge(ms);
     if ((tid & 63) == 0) waves[tid >> 6] = ms;
     __syncthreads();
-    ms = waves[0];
-#pragma unroll 1
-    for (uint32_t w = 1; w < kT / 64; ++w) ms = merge(ms, waves[w]);
+    ms = wave_merge(tid % 64 < kT / 64 ? waves[tid % 64] : MaxSum{-INFINITY, 0.0f});
   } else {
     ms = MaxSum{0.0f, 1.0f};
   }

@@ -122,31 +122,52 @@ __device__ __forceinline__ void add_terms(MaxSum& a, const float (&x)[kN]) {
   for (int i = 0; i < kN; ++i) a.s += exp_term(x[i], base);
 }
 
-__device__ __forceinline__ MaxSum wave_merge(MaxSum a) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    MaxSum b{__shfl_xor(a.m, d, 64), __shfl_xor(a.s, d, 64)};
-    a = merge(a, b);
-  }
-  return a;
+// --- a wave's sums ----------------------------------------------------------
+// By the lanes' own paths (shifts within 16 lanes, then broadcasts of lanes 15
+// and 31 to the rows behind): some ten cycles a step, where a shuffle by way of
+// LDS takes a hundred.  Lane 63 ends with the whole.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ uint32_t dpp(uint32_t fill, uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)fill, (int)v, kCtrl, kRows, 0xF, false);
 }
-
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
+template <typename F>
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t v, uint32_t fill, F&& op) {
+  v = op(v, dpp<0x111, 0xF>(fill, v));  // one lane down, then 2, 4, 8
+  v = op(v, dpp<0x112, 0xF>(fill, v));
+  v = op(v, dpp<0x114, 0xF>(fill, v));
+  v = op(v, dpp<0x118, 0xF>(fill, v));
+  v = op(v, dpp<0x142, 0xA>(fill, v));  // lane 15 to the second and fourth row
+  v = op(v, dpp<0x143, 0xC>(fill, v));  // lane 31 to the last two
   return v;
 }
+__device__ __forceinline__ uint32_t last_lane(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
 
+__device__ __forceinline__ float wave_max(float v) {  // NaN left out
+  const uint32_t r = wave_prefix(__float_as_uint(v), 0xFF800000u, [](uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  });
+  return __uint_as_float(last_lane(r));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  const uint32_t r = wave_prefix(__float_as_uint(v), 0u, [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  });
+  return __uint_as_float(last_lane(r));
+}
+__device__ __forceinline__ uint32_t wave_add(uint32_t v) {
+  return last_lane(wave_prefix(v, 0u, [](uint32_t a, uint32_t b) { return a + b; }));
+}
 // exclusive sum over the lanes in front
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t lane, uint32_t* total) {
-  uint32_t s = v;
-#pragma unroll
-  for (uint32_t d = 1; d < 64; d <<= 1) {
-    const uint32_t o = (uint32_t)__shfl_up((int)s, d, 64);
-    if (lane >= d) s += o;
-  }
-  *total = (uint32_t)__shfl((int)s, 63, 64);
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t* total) {
+  const uint32_t s = wave_prefix(v, 0u, [](uint32_t a, uint32_t b) { return a + b; });
+  *total = last_lane(s);
   return s - v;
+}
+__device__ __forceinline__ MaxSum wave_merge(MaxSum a) {
+  const float m = wave_max(a.m);
+  return MaxSum{m, wave_sum(a.s * exp_term(a.m, exp_base(m)))};
 }
 
 // unsigned order of the floats; NaN as -infinity, -0 as 0

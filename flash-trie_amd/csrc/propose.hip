@@ -164,18 +164,22 @@ constexpr uint32_t kBins = 2 * kFinT;
 struct Shared {
   uint32_t hist[kBins];
   uint32_t found[2];
-  uint32_t scan[2][kFinWaves];
+  uint32_t scan[2][kFinWaves], least[kFinWaves];
   MaxSum ms[kFinWaves];
   float lse, m;
   uint32_t ckey[kCap], cid[kCap];  // candidates, ascending ids
 };
+
+__device__ __forceinline__ uint32_t wave_prefix_max(uint32_t v) {  // of the whole wave
+  return last_lane(wave_prefix(v, 0u, [](uint32_t a, uint32_t b) { return max(a, b); }));
+}
 
 // The highest bin that `need` keys reach, and how many reach it; the
 // histogram is filled (before a barrier) and holds at least as many.
 __device__ __forceinline__ uint32_t pick_bin(Shared& sh, uint32_t need, uint32_t* reach) {
   const uint32_t tid = threadIdx.x, wave = tid >> 6, top = kBins - 1 - 2 * tid;
   const uint32_t a = sh.hist[top], own = a + sh.hist[top - 1];
-  uint32_t total, front = wave_scan(own, tid & 63, &total);
+  uint32_t total, front = wave_scan(own, &total);
   if ((tid & 63) == 0) sh.scan[0][wave] = total;
   __syncthreads();
 #pragma unroll 4
@@ -225,19 +229,13 @@ __device__ __forceinline__ uint32_t largest_reached(Shared& sh, uint32_t need, u
 __device__ __forceinline__ void block_scan2(Shared& sh, uint32_t& a, uint32_t& b, uint32_t* ta,
                                             uint32_t* tb) {
   const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  uint64_t v = (uint64_t)a << 32 | b, s = v;
-#pragma unroll
-  for (uint32_t d = 1; d < 64; d <<= 1) {
-    const uint64_t o = (uint64_t)__shfl_up((long long)s, d, 64);
-    if (lane >= d) s += o;
+  uint32_t wave_a, wave_b;
+  a = wave_scan(a, &wave_a);
+  b = wave_scan(b, &wave_b);
+  if (lane == 0) {
+    sh.scan[0][wave] = wave_a;
+    sh.scan[1][wave] = wave_b;
   }
-  if (lane == 63) {
-    sh.scan[0][wave] = (uint32_t)(s >> 32);
-    sh.scan[1][wave] = (uint32_t)s;
-  }
-  s -= v;
-  a = (uint32_t)(s >> 32);
-  b = (uint32_t)s;
   __syncthreads();
   uint32_t all_a = 0, all_b = 0;
 #pragma unroll 4
@@ -276,7 +274,7 @@ __device__ __forceinline__ void finish_row(Shared& sh, uint16_t* list, const Arg
     return kBins - 1 - (x == m ? 0u : (uint32_t)fminf((m - x) * kSteps, (float)(kBins - 1)));
   };
   const uint32_t top = key_of<T>(m) + 1, enough = enough_groups(K);
-  uint32_t bound = 0, reached = groups;
+  uint32_t bound = 0, reached = groups, least_bin = 0;
   if (groups > K) {
     sh.hist[tid] = sh.hist[tid + kFinT] = 0;
     __syncthreads();
@@ -284,54 +282,81 @@ __device__ __forceinline__ void finish_row(Shared& sh, uint16_t* list, const Arg
     for (uint32_t g = tid; g < groups; g += kFinT)
       atomicAdd(&sh.hist[bin_of(value_of<T>(gkey(g)))], 1u);
     __syncthreads();
-    const uint32_t bin = pick_bin(sh, K, &reached);
-    const uint32_t over = reached - sh.hist[bin];
-    // the smallest key whose bin is at least b: 64 guesses a round
-    const auto first_key = [&](uint32_t b) {
-      uint32_t lo = 0, hi = top - 1;  // too small; large enough
-      while (hi - lo > 1) {
-        const uint32_t step = (hi - lo - 1) / 64 + 1;
-        const uint32_t k = (uint32_t)min((uint64_t)hi, (uint64_t)lo + (uint64_t)(lane + 1) * step);
-        const uint64_t yes = __ballot(bin_of(value_of<T>(k)) >= b);
-        const uint32_t f = (uint32_t)__ffsll((unsigned long long)yes) - 1u;
-        hi = (uint32_t)min((uint64_t)hi, (uint64_t)lo + (uint64_t)(f + 1) * step);
-        lo += f * step;
-      }
-      return hi;
-    };
-    const uint32_t above = bin < kBins - 1 ? first_key(bin + 1) : top;
-    bound = bin > 0 ? first_key(bin) : 0u;
-    __syncthreads();
-    bound = largest_reached(sh, K, enough, bound, above, over, groups, &reached, gkey);
+    least_bin = pick_bin(sh, K, &reached);
+    const uint32_t over = reached - sh.hist[least_bin];
+    // (the bins of the groups' keys decide, or the keys themselves)
+    if (reached > enough) {
+      // the smallest key whose bin is at least b: 64 guesses a round
+      const auto first_key = [&](uint32_t b) {
+        uint32_t lo = 0, hi = top - 1;  // too small; large enough
+        while (hi - lo > 1) {
+          const uint32_t step = (hi - lo - 1) / 64 + 1;
+          const uint32_t k = (uint32_t)min((uint64_t)hi, (uint64_t)lo + (uint64_t)(lane + 1) * step);
+          const uint64_t yes = __ballot(bin_of(value_of<T>(k)) >= b);
+          const uint32_t f = (uint32_t)__ffsll((unsigned long long)yes) - 1u;
+          hi = (uint32_t)min((uint64_t)hi, (uint64_t)lo + (uint64_t)(f + 1) * step);
+          lo += f * step;
+        }
+        return hi;
+      };
+      const uint32_t above = least_bin < kBins - 1 ? first_key(least_bin + 1) : top;
+      bound = least_bin > 0 ? first_key(least_bin) : 0u;
+      least_bin = 0;
+      __syncthreads();
+      bound = largest_reached(sh, K, enough, bound, above, over, groups, &reached, gkey);
+    }
   }
-  // The groups to read again, ascending: those above the bound and the first
-  // of those at it, as many as reach it or, where too many do, up to K.  A
-  // wave takes a run of groups, counts them, then lists them.
-  const uint32_t most = reached <= enough ? reached : K;
+  // The groups to read again, ascending: those that reach the bound, or,
+  // where too many do, those above it and the first of those at it, up to K.
+  // A wave takes a run of groups, counts them, then lists them; the bound is
+  // the least of their keys where a bin was it.
+  const bool cut = reached > enough;
+  const uint32_t most = cut ? K : reached;
   {
     const uint32_t run = (groups + kFinT - 1) / kFinT * 64;
     const uint32_t g0 = min(wave * run, groups), g1 = min(g0 + run, groups);
-    uint32_t above = 0, tied = 0;
+    uint32_t above = 0, tied = 0, least = ~0u;
+    const auto look = [&](uint32_t g, uint32_t* k) {  // 2: above, 1: tied
+      *k = g < g1 ? gkey(g) : 0u;
+      if (g >= g1) return 0;
+      if (cut) return *k > bound ? 2 : *k == bound ? 1 : 0;
+      return *k >= bound && (least_bin == 0 || bin_of(value_of<T>(*k)) >= least_bin) ? 2 : 0;
+    };
 #pragma unroll 4
-    for (uint32_t g = g0 + lane; g < g1; g += 64) {
-      const uint32_t k = gkey(g);
-      above += k > bound;
-      tied += k == bound;
+    for (uint32_t i = g0; i < g1; i += 64) {
+      uint32_t k;
+      const int is = look(i + lane, &k);
+      above += (uint32_t)__popcll(__ballot(is == 2));
+      tied += (uint32_t)__popcll(__ballot(is == 1));
+      if (is == 2) least = min(least, k);
     }
-    uint32_t sum, ties;
-    block_scan2(sh, above, tied, &sum, &ties);
-    ties = most - sum;
-    // (lane 0 has the sums over the waves in front)
-    above = (uint32_t)__builtin_amdgcn_readfirstlane((int)above);
-    tied = (uint32_t)__builtin_amdgcn_readfirstlane((int)tied);
+    least = ~wave_prefix_max(~least);
+    if (lane == 0) {
+      sh.scan[0][wave] = above;
+      sh.scan[1][wave] = tied;
+      sh.least[wave] = least;
+    }
+    __syncthreads();
+    // of the waves in front, and of all
+    const bool there = lane < kFinWaves;
+    const uint32_t va = there ? sh.scan[0][lane] : 0u, vt = there ? sh.scan[1][lane] : 0u;
+    uint32_t sum, none;
+    const uint32_t fa = wave_scan(va, &sum), ft = wave_scan(vt, &none);
+    const uint32_t all_least = ~wave_prefix_max(there ? ~sh.least[lane] : 0u);
+    above = (uint32_t)__builtin_amdgcn_readlane((int)fa, (int)wave);
+    tied = (uint32_t)__builtin_amdgcn_readlane((int)ft, (int)wave);
+    if (!cut && groups > K) bound = all_least;
+    const uint32_t ties = most - sum;
     const uint64_t before = (1ull << lane) - 1;
 #pragma unroll 2
     for (uint32_t i = g0; i < g1; i += 64) {
-      const uint32_t g = i + lane, k = g < g1 ? gkey(g) : 0u;
-      const uint64_t ma = __ballot(g < g1 && k > bound), mt = __ballot(g < g1 && k == bound);
+      uint32_t k;
+      const int is = cut ? look(i + lane, &k)
+                         : (i + lane < g1 && gkey(i + lane) >= bound ? 2 : 0);
+      const uint64_t ma = __ballot(is == 2), mt = __ballot(is == 1);
       const uint32_t pa = above + (uint32_t)__popcll(ma & before);
       const uint32_t pt = tied + (uint32_t)__popcll(mt & before);
-      if (g < g1 && (k > bound || (k == bound && pt < ties))) list[pa + min(pt, ties)] = (uint16_t)g;
+      if (is == 2 || (is == 1 && pt < ties)) list[pa + min(pt, ties)] = (uint16_t)(i + lane);
       above += (uint32_t)__popcll(ma);
       tied += (uint32_t)__popcll(mt);
     }
