@@ -61,16 +61,7 @@ struct Args {
 // Eight elements of a row of n from column k on, zero past its end.
 template <typename T>
 __device__ __forceinline__ u32x4 load_k(const T* row, uint32_t k, uint32_t n) {
-  if (k + 8 <= n) return load_vec(row + k);
-  if (k >= n) return u32x4{};
-  if (n < 8) return load_part(row + k, (int)(n - k), (T)0.0f);
-  // the row's last eight, less those in front of k
-  const u32x4 v = load_vec(row + n - 8);
-  const uint32_t drop = (k + 8 - n) * 16;  // bits, 16 to 112
-  uint64_t lo = (uint64_t)v.y << 32 | v.x, hi = (uint64_t)v.w << 32 | v.z;
-  lo = drop < 64 ? lo >> drop | hi << (64 - drop) : hi >> (drop - 64);
-  hi = drop < 64 ? hi >> drop : 0;
-  return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+  return load_row_vec(row, k, n, (T)0.0f);
 }
 
 // Rows of an adapter stay in their order, so that a row's place, and with it

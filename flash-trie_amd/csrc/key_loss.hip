@@ -96,13 +96,6 @@ __device__ __forceinline__ bool row_used(const Args& a, uint32_t row) {
   return __syncthreads_or(any);
 }
 
-template <typename T>
-__device__ __forceinline__ u32x4 load_row(const T* p, uint32_t vec, uint32_t vocab, T fill) {
-  const uint32_t e = vec * kVec<T>;
-  if (e + kVec<T> <= vocab) return load_vec(p + e);
-  return load_part(p + (e < vocab ? e : 0u), e < vocab ? (int)(vocab - e) : 0, fill);
-}
-
 // Block (row, chunk).  Rows without a token are not read.
 template <typename T>
 __global__ void __launch_bounds__(kStatT) key_stats(Args a) {
@@ -115,9 +108,8 @@ __global__ void __launch_bounds__(kStatT) key_stats(Args a) {
   MaxSum ms{-INFINITY, 0.0f};
   for (uint32_t v = v0; v < v1; v += kStatU * kStatT) {
     u32x4 raw[kStatU];
-#pragma unroll
-    for (int u = 0; u < kStatU; ++u)
-      raw[u] = load_row(p, v + u * kStatT + tid, a.vocab, (T)-INFINITY);
+    load_run<kStatU>(raw, p, v + tid, kStatT, a.vocab, (T)-INFINITY,
+                     (v + kStatU * kStatT) * kVec<T> <= a.vocab);
 #pragma unroll
     for (int u = 0; u < kStatU; ++u) {
       float x[kVec<T>];
@@ -417,14 +409,14 @@ __global__ void __launch_bounds__(256) key_loss(Args a) {
 // A vector of -p G.
 template <typename T>
 __device__ __forceinline__ void store_plain(T* out, uint32_t vec, uint32_t vocab, const RowInfo& info,
-                                            u32x4 raw) {
+                                            u32x4 raw, bool whole) {
   const uint32_t e = vec * kVec<T>;
   float x[kVec<T>];
   to_float<T>(raw, x);
 #pragma unroll
   for (int i = 0; i < kVec<T>; ++i) x[i] = info.used ? -info.scale * exp_term(x[i], info.base) : 0.0f;
   const u32x4 o = from_float<T>(x);
-  if (e + kVec<T> <= vocab) store_vec(out + e, o);
+  if (whole || e + kVec<T> <= vocab) store_vec(out + e, o);
   else store_part(out + e, (int)(vocab - e), o);
 }
 
@@ -474,14 +466,12 @@ __global__ void __launch_bounds__(kStatT) key_gradient(Args a) {
     l1 = from[1];
   }
   u32x4 raw[kStatU];
-  if (info.used) {
-#pragma unroll
-    for (int u = 0; u < kStatU; ++u) raw[u] = load_row(p, v0 + u * kStatT + tid, a.vocab, (T)-INFINITY);
-  }
+  const bool whole = (v0 + kStatU * kStatT) * kVec<T> <= a.vocab;
+  if (info.used) load_run<kStatU>(raw, p, v0 + tid, kStatT, a.vocab, (T)-INFINITY, whole);
 #pragma unroll
   for (int u = 0; u < kStatU; ++u) {
     const uint32_t vec = v0 + u * kStatT + tid;
-    if (vec < vecs) store_plain(out, vec, a.vocab, info, raw[u]);
+    if (whole || vec < vecs) store_plain(out, vec, a.vocab, info, raw[u], whole);
   }
   if (l1 > l0) {
     stores_done();
@@ -500,11 +490,11 @@ __global__ void __launch_bounds__(kT) key_whole(Args a) {
   T* out = (T*)a.dlogits + (int64_t)r * a.dstride[0] + (int64_t)t * a.dstride[1];
   const uint32_t vecs = (a.vocab + kVec<T> - 1) / kVec<T>;
   const bool used = kMany ? row_used(a, row) : length_of(a, r) > t;
+  const bool whole = (uint32_t)(kU * kT * kVec<T>) <= a.vocab;
   u32x4 raw[kU];
   MaxSum ms{-INFINITY, 0.0f};
   if (used) {
-#pragma unroll
-    for (int u = 0; u < kU; ++u) raw[u] = load_row(p, u * kT + tid, a.vocab, (T)-INFINITY);
+    load_run<kU>(raw, p, tid, kT, a.vocab, (T)-INFINITY, whole);
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       float x[kVec<T>];
@@ -541,7 +531,7 @@ __global__ void __launch_bounds__(kT) key_whole(Args a) {
   for (int u = 0; u < kU; ++u) {
     const uint32_t vec = u * kT + tid;
     repack(raw[u]);
-    if (vec < vecs) store_plain(out, vec, a.vocab, info, raw[u]);
+    if (whole || vec < vecs) store_plain(out, vec, a.vocab, info, raw[u], whole);
   }
   if (!used) return;
   stores_done();

@@ -45,6 +45,57 @@ __device__ __forceinline__ u32x4 load_part(const T* p, int n, T fill) {
   }
   return u.v;
 }
+// Elements e ... of a row of `size`, `fill` past its end: one load also for
+// the vector that the row ends in (its last whole vector, shifted), none past
+// it.
+template <typename T>
+__device__ __forceinline__ u32x4 load_row_vec(const T* row, uint32_t e, uint32_t size, T fill) {
+  if (e + kVec<T> <= size) return load_vec(row + e);
+  union {
+    u32x4 v;
+    uint64_t q[2];
+    T e[kVec<T>];
+  } f;
+#pragma unroll
+  for (int i = 0; i < kVec<T>; ++i) f.e[i] = fill;
+  if (e >= size) return f.v;
+  if (size < (uint32_t)kVec<T>) return load_part(row + e, (int)(size - e), fill);
+  union {
+    u32x4 v;
+    uint64_t q[2];
+  } u;
+  u.v = load_vec(row + size - kVec<T>);
+  const uint32_t drop = (e + kVec<T> - size) * (uint32_t)sizeof(T) * 8;  // bits, 1 to 127
+  const uint32_t keep = 128 - drop;
+  union {
+    u32x4 v;
+    uint64_t q[2];
+  } o;
+  o.q[0] = drop < 64 ? u.q[0] >> drop | u.q[1] << (64 - drop) : u.q[1] >> (drop - 64);
+  o.q[1] = drop < 64 ? u.q[1] >> drop : 0;
+  if (keep < 64) {
+    o.q[0] |= f.q[0] << keep;
+    o.q[1] = f.q[1];
+  } else {
+    o.q[1] |= keep == 64 ? f.q[1] : f.q[1] << (keep - 64);
+  }
+  return o.v;
+}
+
+// kU vectors of a row, kStep apart from vector v on; `whole` says that all
+// threads' are inside it.
+template <int kU, typename T>
+__device__ __forceinline__ void load_run(u32x4 (&raw)[kU], const T* row, uint32_t v, uint32_t step,
+                                         uint32_t size, T fill, bool whole) {
+  if (whole) {
+#pragma unroll
+    for (int u = 0; u < kU; ++u) raw[u] = load_vec(row + (v + u * step) * kVec<T>);
+  } else {
+#pragma unroll
+    for (int u = 0; u < kU; ++u) raw[u] = load_row_vec(row, (v + u * step) * kVec<T>, size, fill);
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ void store_part(T* p, int n, u32x4 v) {
   union {

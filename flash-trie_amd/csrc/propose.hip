@@ -85,9 +85,7 @@ __device__ __forceinline__ const T* row_of(const Args& a, uint64_t row) {
 
 template <typename T>
 __device__ __forceinline__ u32x4 load_row(const T* p, uint32_t vec, uint32_t vocab) {
-  const uint32_t e = vec * kVec<T>;
-  if (e + kVec<T> <= vocab) return load_vec(p + e);
-  return load_part(p + (e < vocab ? e : 0u), e < vocab ? (int)(vocab - e) : 0, (T)-INFINITY);
+  return load_row_vec(p, vec * kVec<T>, vocab, (T)-INFINITY);
 }
 
 // Block (row, chunk).
@@ -102,8 +100,8 @@ __global__ void __launch_bounds__(kScanT) propose_scan(Args a) {
   MaxSum ms{-INFINITY, 0.0f};
   for (uint32_t v = v0; v < v1; v += kScanU * kScanT) {
     u32x4 raw[kScanU];
-#pragma unroll
-    for (int u = 0; u < kScanU; ++u) raw[u] = load_row(p, v + u * kScanT + tid, a.vocab);
+    load_run<kScanU>(raw, p, v + tid, kScanT, a.vocab, (T)-INFINITY,
+                     (v + kScanU * kScanT) * kVec<T> <= a.vocab);
 #pragma unroll
     for (int u = 0; u < kScanU; ++u) {
       const uint32_t at = v + u * kScanT + tid;
@@ -164,14 +162,30 @@ constexpr uint32_t kBins = 2 * kFinT;
 struct Shared {
   uint32_t hist[kBins];
   uint32_t found[2];
-  uint32_t scan[2][kFinWaves], least[kFinWaves];
+  uint32_t scan[2][kFinWaves];
+  uint32_t cells[8][kFinWaves], all_cells;  // sums of a turn and wave
   MaxSum ms[kFinWaves];
   float lse, m;
   uint32_t ckey[kCap], cid[kCap];  // candidates, ascending ids
 };
 
-__device__ __forceinline__ uint32_t wave_prefix_max(uint32_t v) {  // of the whole wave
-  return last_lane(wave_prefix(v, 0u, [](uint32_t a, uint32_t b) { return max(a, b); }));
+// The cells' first `turns` rows to the sums of all cells in front; the whole
+// sum is all_cells.  Between barriers.
+__device__ __forceinline__ void scan_cells(Shared& sh, uint32_t turns) {
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    uint32_t front = 0;
+    for (uint32_t i = threadIdx.x; i - threadIdx.x < turns * kFinWaves; i += 64) {
+      uint32_t* c = &sh.cells[0][0] + i;
+      const uint32_t v = i < turns * kFinWaves ? *c : 0u;
+      uint32_t total;
+      const uint32_t f = wave_scan(v, &total);
+      if (i < turns * kFinWaves) *c = front + f;
+      front += total;
+    }
+    if (threadIdx.x == 0) sh.all_cells = front;
+  }
+  __syncthreads();
 }
 
 // The highest bin that `need` keys reach, and how many reach it; the
@@ -252,111 +266,143 @@ __device__ __forceinline__ void block_scan2(Shared& sh, uint32_t& a, uint32_t& b
 }
 
 // How many groups may reach the bound T: it need not be the very K-th
-// largest group maximum, each round that is saved is worth an eighth more
-// groups.
-__device__ __forceinline__ uint32_t enough_groups(uint32_t K) { return K + K / 8 + 32; }
-constexpr uint32_t kMaxListed = FT_MAX_PROPOSALS + FT_MAX_PROPOSALS / 8 + 32;
+// largest group maximum (that of vectors of eight groups' keys lets through
+// an eighth more in random rows), and a turn saved is worth more than that.
+__device__ __forceinline__ uint32_t enough_groups(uint32_t K) { return K + K / 4 + 32; }
+constexpr uint32_t kListTurns = 5;  // turns of vectors of the keys that LDS holds
+constexpr uint32_t kMaxListed = FT_MAX_PROPOSALS + FT_MAX_PROPOSALS / 4 + 32;
 
 // Writes a row's proposals; sh.m and sh.lse are there, gkey(g) is group g's
-// key.
-template <typename T, typename G>
+// key (kLds: keys[g]).
+template <typename T, bool kLds, typename G>
 __device__ __forceinline__ void finish_row(Shared& sh, uint16_t* list, const Args& a, uint64_t row,
-                                           uint32_t groups, uint32_t lg, G&& gkey) {
+                                           uint32_t groups, uint32_t lg, const Key<T>* keys,
+                                           G&& gkey) {
   const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, K = a.topk;
   const T* p = row_of<T>(a, row);
-  // The bound T: first by a histogram of the groups' distance from the row's
-  // maximum, 2047 steps of 1/64 (differences of logits are of that order,
-  // whatever their size); then, where too many groups reach its bin, by
-  // their keys.  (A row of -infinity has m = 0, above its keys too.)
+  // The bound T: first by a histogram of distances from the row's maximum,
+  // 2047 steps of 1/64 (differences of logits are of that order, whatever
+  // their size), of the groups or, where there are enough of them, of vectors
+  // of their keys, whose maxima bound as well; then, where too many groups
+  // reach its bin, by the groups' keys.  (A row of -infinity has m = 0, above
+  // its keys too.)
   constexpr float kSteps = 64.0f;
   const float m = sh.m, lse = sh.lse;
   const auto bin_of = [&](float x) {  // (x = m may be infinity)
     return kBins - 1 - (x == m ? 0u : (uint32_t)fminf((m - x) * kSteps, (float)(kBins - 1)));
   };
   const uint32_t top = key_of<T>(m) + 1, enough = enough_groups(K);
-  uint32_t bound = 0, reached = groups, least_bin = 0;
+  constexpr uint32_t kKeys = kLds ? 16 / sizeof(Key<T>) : 1;  // of a vector
+  const uint32_t kvecs = (groups + kKeys - 1) / kKeys;
+  const auto keys_of = [&](uint32_t v, uint32_t (&k)[kKeys]) {
+    if constexpr (kLds) {
+      const u32x4 raw = *(const u32x4*)(keys + v * kKeys);
+#pragma unroll
+      for (uint32_t e = 0; e < kKeys; ++e) {
+        const uint32_t w = raw[e * sizeof(Key<T>) / 4];
+        k[e] = sizeof(Key<T>) == 4 ? w : e & 1 ? w >> 16 : w & 0xFFFFu;
+        if (v * kKeys + e >= groups) k[e] = 0;
+      }
+    } else {
+      k[0] = gkey(v);
+    }
+  };
+  uint32_t bound = 0, reached = groups;
   if (groups > K) {
+    const bool by_vector = kKeys > 1 && kvecs >= 2 * K;
     sh.hist[tid] = sh.hist[tid + kFinT] = 0;
     __syncthreads();
-#pragma unroll 4
-    for (uint32_t g = tid; g < groups; g += kFinT)
-      atomicAdd(&sh.hist[bin_of(value_of<T>(gkey(g)))], 1u);
-    __syncthreads();
-    least_bin = pick_bin(sh, K, &reached);
-    const uint32_t over = reached - sh.hist[least_bin];
-    // (the bins of the groups' keys decide, or the keys themselves)
-    if (reached > enough) {
-      // the smallest key whose bin is at least b: 64 guesses a round
-      const auto first_key = [&](uint32_t b) {
-        uint32_t lo = 0, hi = top - 1;  // too small; large enough
-        while (hi - lo > 1) {
-          const uint32_t step = (hi - lo - 1) / 64 + 1;
-          const uint32_t k = (uint32_t)min((uint64_t)hi, (uint64_t)lo + (uint64_t)(lane + 1) * step);
-          const uint64_t yes = __ballot(bin_of(value_of<T>(k)) >= b);
-          const uint32_t f = (uint32_t)__ffsll((unsigned long long)yes) - 1u;
-          hi = (uint32_t)min((uint64_t)hi, (uint64_t)lo + (uint64_t)(f + 1) * step);
-          lo += f * step;
-        }
-        return hi;
-      };
-      const uint32_t above = least_bin < kBins - 1 ? first_key(least_bin + 1) : top;
-      bound = least_bin > 0 ? first_key(least_bin) : 0u;
-      least_bin = 0;
-      __syncthreads();
-      bound = largest_reached(sh, K, enough, bound, above, over, groups, &reached, gkey);
+    if (by_vector) {
+#pragma unroll 1
+      for (uint32_t v = tid; v < kvecs; v += kFinT) {
+        uint32_t k[kKeys], most = 0;
+        keys_of(v, k);
+#pragma unroll
+        for (uint32_t e = 0; e < kKeys; ++e) most = max(most, k[e]);
+        atomicAdd(&sh.hist[bin_of(value_of<T>(most))], 1u);
+      }
+    } else {
+#pragma unroll 2
+      for (uint32_t g = tid; g < groups; g += kFinT)
+        atomicAdd(&sh.hist[bin_of(value_of<T>(gkey(g)))], 1u);
     }
+    __syncthreads();
+    const uint32_t bin = pick_bin(sh, K, &reached);
+    // the smallest key whose bin is at least b: 64 guesses a round
+    uint32_t lo = 0, hi = top - 1;  // too small; large enough
+    while (bin > 0 && hi - lo > 1) {
+      const uint32_t step = (hi - lo - 1) / 64 + 1;
+      const uint32_t k = (uint32_t)min((uint64_t)hi, (uint64_t)lo + (uint64_t)(lane + 1) * step);
+      const uint64_t yes = __ballot(bin_of(value_of<T>(k)) >= bin);
+      const uint32_t f = (uint32_t)__ffsll((unsigned long long)yes) - 1u;
+      hi = (uint32_t)min((uint64_t)hi, (uint64_t)lo + (uint64_t)(f + 1) * step);
+      lo += f * step;
+    }
+    bound = bin > 0 ? hi : 0u;
   }
-  // The groups to read again, ascending: those that reach the bound, or,
-  // where too many do, those above it and the first of those at it, up to K.
-  // A wave takes a run of groups, counts them, then lists them; the bound is
-  // the least of their keys where a bin was it.
-  const bool cut = reached > enough;
-  const uint32_t most = cut ? K : reached;
-  {
+  // The groups to read again, ascending: those that reach the bound.
+  uint32_t most = 0;
+  const auto list_turns = [&](uint32_t v0, uint32_t most, bool write) {
+    // vectors of keys v0 ... of up to kListTurns turns: counted, or listed
+    uint32_t hits[kListTurns];
+#pragma unroll
+    for (uint32_t t = 0; t < kListTurns; ++t) {
+      const uint32_t v = v0 + t * kFinT + tid;
+      uint32_t k[kKeys], h = 0;
+      if (v < kvecs) {
+        keys_of(v, k);
+#pragma unroll
+        for (uint32_t e = 0; e < kKeys; ++e) h |= (k[e] >= max(bound, 1u) ? 1u : 0u) << e;
+      }
+      hits[t] = h;
+      uint32_t total = wave_add((uint32_t)__popc(h));
+      if (lane == 0) sh.cells[t][wave] = total;
+    }
+    scan_cells(sh, kListTurns);
+    const uint32_t n = sh.all_cells;
+    if (write && most + n <= kMaxListed) {
+#pragma unroll
+      for (uint32_t t = 0; t < kListTurns; ++t) {
+        uint32_t h = hits[t], none;
+        uint32_t at = most + sh.cells[t][wave] + wave_scan((uint32_t)__popc(h), &none);
+        while (h) {
+          const uint32_t e = (uint32_t)__ffs(h) - 1u;
+          h &= h - 1;
+          list[at++] = (uint16_t)((v0 + t * kFinT + tid) * kKeys + e);
+        }
+      }
+    }
+    __syncthreads();
+    return n;
+  };
+  for (uint32_t v0 = 0; v0 < kvecs; v0 += kListTurns * kFinT) most += list_turns(v0, most, true);
+  if (groups > K && most > enough) {
+    // Too many: the bound by the keys, as exact as it takes; where ties are
+    // too many still, those above it and the first of those at it, up to K.
+    reached = most;
+    bound = largest_reached(sh, K, enough, bound, top, 0, groups, &reached, gkey);
+    const bool cut = reached > enough;
+    most = cut ? K : reached;
     const uint32_t run = (groups + kFinT - 1) / kFinT * 64;
     const uint32_t g0 = min(wave * run, groups), g1 = min(g0 + run, groups);
-    uint32_t above = 0, tied = 0, least = ~0u;
-    const auto look = [&](uint32_t g, uint32_t* k) {  // 2: above, 1: tied
-      *k = g < g1 ? gkey(g) : 0u;
-      if (g >= g1) return 0;
-      if (cut) return *k > bound ? 2 : *k == bound ? 1 : 0;
-      return *k >= bound && (least_bin == 0 || bin_of(value_of<T>(*k)) >= least_bin) ? 2 : 0;
-    };
-#pragma unroll 4
-    for (uint32_t i = g0; i < g1; i += 64) {
-      uint32_t k;
-      const int is = look(i + lane, &k);
-      above += (uint32_t)__popcll(__ballot(is == 2));
-      tied += (uint32_t)__popcll(__ballot(is == 1));
-      if (is == 2) least = min(least, k);
+    uint32_t above = 0, tied = 0, sum, ties;
+    for (uint32_t g = g0 + lane; g < g1; g += 64) {
+      above += gkey(g) > bound;
+      tied += gkey(g) == bound;
     }
-    least = ~wave_prefix_max(~least);
-    if (lane == 0) {
-      sh.scan[0][wave] = above;
-      sh.scan[1][wave] = tied;
-      sh.least[wave] = least;
-    }
-    __syncthreads();
-    // of the waves in front, and of all
-    const bool there = lane < kFinWaves;
-    const uint32_t va = there ? sh.scan[0][lane] : 0u, vt = there ? sh.scan[1][lane] : 0u;
-    uint32_t sum, none;
-    const uint32_t fa = wave_scan(va, &sum), ft = wave_scan(vt, &none);
-    const uint32_t all_least = ~wave_prefix_max(there ? ~sh.least[lane] : 0u);
-    above = (uint32_t)__builtin_amdgcn_readlane((int)fa, (int)wave);
-    tied = (uint32_t)__builtin_amdgcn_readlane((int)ft, (int)wave);
-    if (!cut && groups > K) bound = all_least;
-    const uint32_t ties = most - sum;
+    block_scan2(sh, above, tied, &sum, &ties);
+    ties = most - sum;
+    // (lane 0 has the sums over the waves in front)
+    above = (uint32_t)__builtin_amdgcn_readfirstlane((int)above);
+    tied = (uint32_t)__builtin_amdgcn_readfirstlane((int)tied);
     const uint64_t before = (1ull << lane) - 1;
-#pragma unroll 2
+#pragma unroll 1
     for (uint32_t i = g0; i < g1; i += 64) {
-      uint32_t k;
-      const int is = cut ? look(i + lane, &k)
-                         : (i + lane < g1 && gkey(i + lane) >= bound ? 2 : 0);
-      const uint64_t ma = __ballot(is == 2), mt = __ballot(is == 1);
+      const uint32_t g = i + lane, k = g < g1 ? gkey(g) : 0u;
+      const uint64_t ma = __ballot(g < g1 && k > bound), mt = __ballot(g < g1 && k == bound);
       const uint32_t pa = above + (uint32_t)__popcll(ma & before);
       const uint32_t pt = tied + (uint32_t)__popcll(mt & before);
-      if (is == 2 || (is == 1 && pt < ties)) list[pa + min(pt, ties)] = (uint16_t)(i + lane);
+      if (g < g1 && (k > bound || (k == bound && pt < ties))) list[pa + min(pt, ties)] = (uint16_t)g;
       above += (uint32_t)__popcll(ma);
       tied += (uint32_t)__popcll(mt);
     }
@@ -373,52 +419,60 @@ __device__ __forceinline__ void finish_row(Shared& sh, uint16_t* list, const Arg
   const bool all = bound <= key_of<T>(-INFINITY);
   const float least_value = value_of<T>(bound);
   uint32_t n = 0;
-  constexpr uint32_t kRun = 4;  // neighbouring vectors a thread
-  u32x4 ahead[kRun];
-  const auto fetch = [&](uint32_t i0) {
+  constexpr uint32_t kRun = 4;    // neighbouring vectors a thread and turn
+  constexpr uint32_t kTurns = 3;  // loaded together
+  for (uint32_t i0 = 0; i0 < vecs; i0 += kTurns * kRun * kFinT) {
+    u32x4 raw[kTurns][kRun];
+    uint32_t hits[kTurns];
 #pragma unroll
-    for (uint32_t u = 0; u < kRun; ++u)
-      ahead[u] = load_row(p, place(i0 + tid * kRun + u), a.vocab);
-  };
-  fetch(0);
-  for (uint32_t i0 = 0; i0 < vecs; i0 += kRun * kFinT) {
-    u32x4 raw[kRun];
+    for (uint32_t t = 0; t < kTurns; ++t)
+      if (i0 + t * kRun * kFinT < vecs) {
 #pragma unroll
-    for (uint32_t u = 0; u < kRun; ++u) raw[u] = ahead[u];
-    if (i0 + kRun * kFinT < vecs) fetch(i0 + kRun * kFinT);
-    uint32_t hits = 0;
-#pragma unroll
-    for (uint32_t u = 0; u < kRun; ++u) {
-      const uint32_t id = place(i0 + tid * kRun + u) * kVec<T>;
-      float x[kVec<T>];
-      to_float<T>(raw[u], x);
-      uint32_t h = 0;
-#pragma unroll
-      for (int e = 0; e < kVec<T>; ++e) h |= (all || x[e] >= least_value ? 1u : 0u) << e;
-      if (id + kVec<T> > a.vocab) h &= id < a.vocab ? (1u << (a.vocab - id)) - 1u : 0u;
-      hits |= h << (u * kVec<T>);
-    }
-    uint32_t at = (uint32_t)__popc(hits), none = 0, total, zero;
-    block_scan2(sh, at, none, &total, &zero);
-    at += n;
-    n += total;
-    while (hits) {
-      const uint32_t bit = (uint32_t)__ffs(hits) - 1u, u = bit / kVec<T>, e = bit % kVec<T>;
-      hits &= hits - 1;
-      if (at < kCap) {
-        const u32x4 v = u < 2 ? (u == 0 ? raw[0] : raw[1]) : u == 2 ? raw[2] : raw[3];
-        const uint32_t w = e * sizeof(T) / 4;
-        const uint32_t word = w < 2 ? (w == 0 ? v.x : v.y) : w == 2 ? v.z : v.w;
-        float x;
-        if (sizeof(T) == 4) x = __uint_as_float(word);
-        else x = (float)__builtin_bit_cast(Half<T>, (uint16_t)(word >> (e & 1) * 16));
-        sh.ckey[at] = key_of<T>(x);
-        sh.cid[at] = place(i0 + tid * kRun + u) * kVec<T> + e;
+        for (uint32_t u = 0; u < kRun; ++u)
+          raw[t][u] = load_row(p, place(i0 + (t * kFinT + tid) * kRun + u), a.vocab);
       }
-      ++at;
+#pragma unroll
+    for (uint32_t t = 0; t < kTurns; ++t) {
+      hits[t] = 0;
+      if (i0 + t * kRun * kFinT < vecs) {
+#pragma unroll
+        for (uint32_t u = 0; u < kRun; ++u) {
+          const uint32_t id = place(i0 + (t * kFinT + tid) * kRun + u) * kVec<T>;
+          float x[kVec<T>];
+          to_float<T>(raw[t][u], x);
+          uint32_t h = 0;
+#pragma unroll
+          for (int e = 0; e < kVec<T>; ++e) h |= (all || x[e] >= least_value ? 1u : 0u) << e;
+          if (id + kVec<T> > a.vocab) h &= id < a.vocab ? (1u << (a.vocab - id)) - 1u : 0u;
+          hits[t] |= h << (u * kVec<T>);
+        }
+      }
+      const uint32_t total = wave_add((uint32_t)__popc(hits[t]));
+      if (lane == 0) sh.cells[t][wave] = total;
     }
+    scan_cells(sh, kTurns);
+#pragma unroll
+    for (uint32_t t = 0; t < kTurns; ++t) {
+      uint32_t none, at = n + sh.cells[t][wave] + wave_scan((uint32_t)__popc(hits[t]), &none);
+      while (hits[t]) {
+        const uint32_t bit = (uint32_t)__ffs(hits[t]) - 1u, u = bit / kVec<T>, e = bit % kVec<T>;
+        hits[t] &= hits[t] - 1;
+        if (at < kCap) {
+          const u32x4 v = u < 2 ? (u == 0 ? raw[t][0] : raw[t][1]) : u == 2 ? raw[t][2] : raw[t][3];
+          const uint32_t w = e * sizeof(T) / 4;
+          const uint32_t word = w < 2 ? (w == 0 ? v.x : v.y) : w == 2 ? v.z : v.w;
+          float x;
+          if (sizeof(T) == 4) x = __uint_as_float(word);
+          else x = (float)__builtin_bit_cast(Half<T>, (uint16_t)(word >> (e & 1) * 16));
+          sh.ckey[at] = key_of<T>(x);
+          sh.cid[at] = place(i0 + (t * kFinT + tid) * kRun + u) * kVec<T> + e;
+        }
+        ++at;
+      }
+    }
+    n += sh.all_cells;
+    __syncthreads();
   }
-  __syncthreads();
 
   const auto put = [&](uint32_t at, uint32_t id, uint32_t key) {
     const float x = value_of<T>(key);
@@ -492,7 +546,7 @@ template <typename T, bool kLds>
 __global__ void __launch_bounds__(kFinT) propose_finish(Args a) {
   __shared__ Shared sh;
   __shared__ uint16_t list[kMaxListed];
-  __shared__ Key<T> keys[kLds ? kKeyBytes / sizeof(T) : 1];
+  __shared__ __attribute__((aligned(16))) Key<T> keys[kLds ? kKeyBytes / sizeof(T) : 1];
   const uint64_t row = blockIdx.x;
   const T* gmax = (const T*)a.gmax + row * a.groups;
   if (kLds) {
@@ -514,7 +568,7 @@ __global__ void __launch_bounds__(kFinT) propose_finish(Args a) {
     set_row_sum<T>(sh, ms);
   }
   __syncthreads();
-  finish_row<T>(sh, list, a, row, a.groups, a.lanes_log2, [&](uint32_t g) -> uint32_t {
+  finish_row<T, kLds>(sh, list, a, row, a.groups, a.lanes_log2, keys, [&](uint32_t g) -> uint32_t {
     return kLds ? (uint32_t)keys[g] : key_of<T>((float)gmax[g]);
   });
 }
@@ -524,7 +578,7 @@ template <typename T>
 __global__ void __launch_bounds__(kFinT) propose_row(Args a) {
   __shared__ Shared sh;
   __shared__ uint16_t list[kMaxListed];
-  __shared__ Key<T> keys[kRowVecs];
+  __shared__ __attribute__((aligned(16))) Key<T> keys[kRowVecs];
   const uint64_t row = blockIdx.x;
   const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const T* p = row_of<T>(a, row);
@@ -532,8 +586,8 @@ __global__ void __launch_bounds__(kFinT) propose_row(Args a) {
   MaxSum ms{-INFINITY, 0.0f};
   for (uint32_t v = tid; v < vecs; v += kScanU * kFinT) {
     u32x4 raw[kScanU];
-#pragma unroll
-    for (int u = 0; u < kScanU; ++u) raw[u] = load_row(p, v + u * kFinT, a.vocab);
+    load_run<kScanU>(raw, p, v, kFinT, a.vocab, (T)-INFINITY,
+                     (v - tid + kScanU * kFinT) * kVec<T> <= a.vocab);
 #pragma unroll
     for (int u = 0; u < kScanU; ++u) {
       float x[kVec<T>];
@@ -553,7 +607,7 @@ __global__ void __launch_bounds__(kFinT) propose_row(Args a) {
     set_row_sum<T>(sh, ms);
   }
   __syncthreads();
-  finish_row<T>(sh, list, a, row, vecs, 0, [&](uint32_t g) -> uint32_t { return keys[g]; });
+  finish_row<T, true>(sh, list, a, row, vecs, 0, keys, [&](uint32_t g) -> uint32_t { return keys[g]; });
 }
 
 template <typename T>
