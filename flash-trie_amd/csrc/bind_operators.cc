@@ -5,6 +5,8 @@
 // is ordered, freed and captured as torch's own operators are.
 #include "bind_operators.h"
 
+#include <dlfcn.h>
+
 #include <cstring>
 #include <initializer_list>
 #include <string>
@@ -23,6 +25,19 @@ namespace {
   throw py::value_error(call + ": " + what);
 }
 
+// torch brings a HIP runtime of its own.  Imported first, it is this module's
+// too; imported after this module, there are two, and neither knows the
+// other's streams.
+bool shares_runtime(const py::module_& torch) {
+  const std::string init = py::cast<std::string>(torch.attr("__file__"));
+  const std::string lib = init.substr(0, init.find_last_of('/') + 1) + "lib/libc10_hip.so";
+  void* h = dlopen(lib.c_str(), RTLD_LAZY | RTLD_NOLOAD);
+  if (!h) return true;  // a torch without GPUs: its tensors are refused
+  const void* theirs = dlsym(h, "hipGetDevice");
+  dlclose(h);
+  return !theirs || theirs == ft_hip_runtime();
+}
+
 // What the calls use of torch, looked up once.
 struct Torch {
   py::object tensor, dtypes[3], int32, uint8, raw_stream, current_stream;
@@ -34,8 +49,12 @@ const Torch& torch() {
   // another thread in, which then makes its own)
   static const Torch* t = nullptr;
   if (!t) {
-    auto* n = new Torch();
     py::module_ m = py::module_::import("torch");
+    if (!shares_runtime(m))
+      throw marisa::Exception(MARISA_STATE_ERROR,
+                              "torch was imported after flashtrie and runs on a HIP runtime of "
+                              "its own: import torch first");
+    auto* n = new Torch();
     n->tensor = m.attr("Tensor");
     n->dtypes[FT_F32] = m.attr("float32");
     n->dtypes[FT_F16] = m.attr("float16");

@@ -176,6 +176,8 @@ int run(const A* a, void* ws, size_t ws_bytes, void* stream, const char* call,
 
 extern "C" {
 
+const void* ft_hip_runtime(void) { return (const void*)&hipGetDevice; }
+
 size_t ft_adapter_logits_workspace(const ft_adapter_logits_args* a) {
   return workspace(a, fto::adapter_logits_workspace);
 }

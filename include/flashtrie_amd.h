@@ -301,6 +301,12 @@ int ft_device_info(ft_ctx* ctx, int* num_cus, int* lds_per_block,
  * contiguous.  Outputs overlap no input.  Results are the same from call to
  * call, bit for bit.
  * ------------------------------------------------------------------------- */
+/* An address inside the HIP runtime that this library calls.  A process can
+ * hold two runtimes (an application that brings its own copy); streams and
+ * graphs belong to one of them.  A caller that has streams from elsewhere
+ * compares this with its own hipGetDevice before it hands them over. */
+const void* ft_hip_runtime(void);
+
 #define FT_F32 0
 #define FT_F16 1
 #define FT_BF16 2
