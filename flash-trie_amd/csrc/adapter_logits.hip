@@ -128,28 +128,44 @@ __global__ void __launch_bounds__(1024) logits_order(Args a) {
 // Block b: rows [16 b, 16 b + 16) of the order, 64 ranks at a time; the 16
 // waves share the hidden columns, a run of steps each with its loads
 // together, and add up in LDS.  Bound by latency: one way to memory for each
-// run of rows with the same adapter.  With at most 16 rows there is no order
-// to make: the block writes what logits_order would.
+// run of rows with the same adapter.  At most 16 rows are put in order here, as
+// logits_order would (16 rows of 4 adapters in turn, 262144 x 1024: 126 us to
+// 144 in their own order).
 constexpr int kShrinkT = 1024;
 
 template <typename T>
 __global__ void __launch_bounds__(kShrinkT) logits_shrink(Args a) {
   __shared__ float part[16][64][16 + 1];     // wave, rank, row
   __shared__ float zs[16][FT_MAX_RANK + 1];  // row, rank
+  __shared__ uint32_t order[16];
   const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const uint32_t r0 = blockIdx.x * 16, n = min(16u, a.rows - r0), col = lane & 15, q = lane >> 4;
   const bool alone = a.rows <= 16;
   for (uint32_t i = tid; i < 16 * a.rank32; i += kShrinkT) zs[i / a.rank32][i % a.rank32] = 0.0f;
   const uint32_t mine = r0 + min(col, n - 1);
-  const uint32_t at = alone ? mine : (uint32_t)a.perm[mine];
+  uint32_t at = mine;
   // the adapters of the 16 rows, a row a lane
-  const int32_t own = max(alone ? a.adapter[mine] : a.sorted[mine], -1);
-  if (alone && tid < n) {
-    a.perm[tid] = (int32_t)tid;
-    a.sorted[tid] = own;
+  int32_t own;
+  if (alone) {
+    own = max(a.adapter[mine], -1);
+    uint32_t rank = 0;  // of this lane's row
+    for (uint32_t j = 0; j < n; ++j) {
+      const int32_t g = __builtin_amdgcn_readlane(own, (int)j);
+      rank += g < own || (g == own && j < mine);
+    }
+    if (tid < n) order[rank] = tid;
+    __syncthreads();
+    at = order[mine];
+    own = __shfl(own, (int)at, 64);
+    if (tid < n) {
+      a.perm[tid] = (int32_t)at;
+      a.sorted[tid] = own;
+    }
     if (tid < 4) a.zeros[tid] = 0;
+  } else {
+    at = (uint32_t)a.perm[mine];
+    own = max(a.sorted[mine], -1);
   }
-  if (alone && tid >= n && tid < 4) a.zeros[tid] = 0;
   const T* x = (const T*)a.x + (int64_t)at * a.x_stride;
   __syncthreads();
   for (uint32_t i = 0; i < n;) {
@@ -883,20 +899,20 @@ hipError_t launch(Args a, hipStream_t s) {
   hipLaunchKernelGGL((logits_shrink<T>), dim3((a.rows + 15) / 16), dim3(kShrinkT), 0, s, a);
   if (a.hidden % 8 == 0 && whole_vectors(a.x, a.x_stride) &&
       whole_vectors(a.weight, a.weight_stride)) {
-    // Up to 96 rows the weights' stream is the bound: two workgroups of 8
-    // waves on a CU, one in its adapters' turns while the other streams (84 x
-    // 262144 x 1024, 6 adapters of rank 12: 174 us; with tiles of 256 tokens
-    // and three stages, one workgroup on a CU: 187).  Up to 16 rows, smaller
-    // tiles where the larger make too few workgroups (8 x 32768 x 512: 7.8
-    // us to 9.0; 16 x 2.2M x 512: 511 to 502).
-    if (a.rows <= 16 && a.vocab < 128 * 1024) return launch_staged<T, O, Shape<1, 4, 1, 4, 4>>(a, s);
-    if (a.rows <= 16) return launch_staged<T, O, Shape<1, 8, 1, 4, 4>>(a, s);
+    // Up to 96 rows the weights' stream is the bound: two or more workgroups
+    // on a CU, some in their adapters' turns while others stream (84 x 262144
+    // x 1024, 6 adapters of rank 12: 174 us; with tiles of 256 tokens and
+    // three stages, one workgroup on a CU: 196).  Up to 16 rows, tiles of 64
+    // tokens where those make one round of them, three a CU (8 x 49152 x 512:
+    // 24.9 us to 27.3 with 128 tokens; 8 x 65536 x 512: 38.6 to 34.6).
+    if (a.rows <= 16 && a.vocab <= 48 * 1024) return launch_staged<T, O, Shape<1, 4, 1, 4, 4>>(a, s);
+    if (a.rows <= 16) return launch_staged<T, O, Shape<1, 8, 1, 4, 2>>(a, s);
     if (a.rows <= 32) return launch_staged<T, O, Shape<2, 8, 1, 8, 2>>(a, s);
     if (a.rows <= 64) return launch_staged<T, O, Shape<4, 8, 1, 8, 2>>(a, s);
     if (a.rows <= 96) return launch_staged<T, O, Shape<6, 8, 1, 8, 2>>(a, s);
     if (a.rows <= 128) return launch_staged<T, O, Shape<8, 16, 1, 8, 3>>(a, s);
     // (32-bit offsets within the rows and within a tile's tokens)
-    if (a.rows > 128 && a.hidden % 64 == 0 && a.x_stride >= 0 && a.weight_stride >= 0 &&
+    if (a.hidden % 64 == 0 && a.x_stride >= 0 && a.weight_stride >= 0 &&
         a.rows * (uint64_t)a.x_stride < 1ull << 31 && a.weight_stride < 1ll << 22 &&
         a.vocab >= 256)
       return launch_tile<T, O, TileShape<16, 16, 2, 4>>(a, s);

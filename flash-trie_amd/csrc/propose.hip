@@ -634,7 +634,12 @@ hipError_t launch(const ft_propose_args& a, uint8_t* ws, hipStream_t s) {
   k.ids = a.ids;
   k.logp = a.logp;
   const uint32_t rows = (uint32_t)(a.batch * a.steps);
-  if ((a.vocab + kVec<T> - 1) / kVec<T> <= kRowVecs) {
+  // One launch, a row a workgroup, up to 8192 vectors a row (128 rows of
+  // 32,768 bf16, 1000 each: 16.6 us, in two launches 18.5; 8 of 32,768 f32:
+  // 14.5, 15.5), and up to 16384 where the rows fill the chip (256 of 100,003
+  // f16: 22.9, 26.2; but 39 of them: 20.5, 18.8).
+  const uint32_t vecs = (a.vocab + kVec<T> - 1) / kVec<T>;
+  if (vecs <= (rows >= 256 ? kRowVecs : kRowVecs / 2)) {
     hipLaunchKernelGGL((propose_row<T>), dim3(rows), dim3(kFinT), 0, s, k);
     return hipGetLastError();
   }
