@@ -127,11 +127,23 @@ __global__ void __launch_bounds__(kStatT) key_stats(Args a) {
   }
 }
 
-// The row's (max, sum) from its chunks' parts, in their order.
+// The row's (max, sum) from its chunks' parts: by a thread, loads and
+// exponentials side by side, or by a wave.
 __device__ __forceinline__ MaxSum row_sum(const Args& a, uint32_t row) {
-  MaxSum ms = a.part[(uint64_t)row * a.chunks];
-  for (uint32_t i = 1; i < a.chunks; ++i) ms = merge(ms, a.part[(uint64_t)row * a.chunks + i]);
+  const MaxSum* part = a.part + (uint64_t)row * a.chunks;
+  MaxSum ms{-INFINITY, 0.0f};
+#pragma unroll 8
+  for (uint32_t i = 0; i < a.chunks; ++i) ms.m = fmaxf(ms.m, part[i].m);
+  const float base = exp_base(ms.m);
+#pragma unroll 8
+  for (uint32_t i = 0; i < a.chunks; ++i) ms.s += part[i].s * exp_term(part[i].m, base);
   return ms;
+}
+__device__ __forceinline__ MaxSum row_sum_wave(const Args& a, uint32_t row) {
+  const MaxSum* part = a.part + (uint64_t)row * a.chunks;
+  MaxSum ms{-INFINITY, 0.0f};
+  for (uint32_t i = threadIdx.x & 63; i < a.chunks; i += 64) ms = merge(ms, part[i]);
+  return wave_merge(ms);
 }
 
 // A token's log-probability; NaN for one out of range.
@@ -169,15 +181,24 @@ __device__ __forceinline__ float block_sum(float v, float* waves) {
   return v;
 }
 
-// (block_sum's barriers are between the uses of `waves`)
-__device__ __forceinline__ float block_max(float v, float* waves) {
-  v = wave_max(v);
-  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
+// The block's sums of a and b and its largest c.
+__device__ __forceinline__ void block_sums(float& a, float& b, float& c, float (*waves)[3]) {
+  a = wave_sum(a);
+  b = wave_sum(b);
+  c = wave_max(c);
+  if ((threadIdx.x & 63) == 0) {
+    float* w = waves[threadIdx.x >> 6];
+    w[0] = a;
+    w[1] = b;
+    w[2] = c;
+  }
   __syncthreads();
-  v = 0.0f;
-  for (uint32_t w = 0; w < blockDim.x / 64; ++w) v = fmaxf(v, waves[w]);
-  __syncthreads();
-  return v;
+  a = b = c = 0.0f;
+  for (uint32_t w = 0; w < blockDim.x / 64; ++w) {
+    a += waves[w][0];
+    b += waves[w][1];
+    c = fmaxf(c, waves[w][2]);
+  }
 }
 
 template <typename T>
@@ -260,7 +281,7 @@ struct Table {
   static constexpr uint32_t kSlots = 2 * kListT * kP;
   uint32_t tok[kSlots];  // ~0: free
   unsigned long long sum[kSlots];
-  float wsum[kListT / 64];
+  float waves[kListT / 64][3];
 };
 
 // The keys' scores and slopes of row (r, t) and the loss's terms (policy),
@@ -304,10 +325,10 @@ __device__ __forceinline__ void row_table(const Args& a, Table<kP>& sh, uint32_t
       most = fmaxf(most, fabsf(gs[i]));
     }
   }
-  *total = block_sum(sum, sh.wsum);
-  if (kPolicy) *loss = block_sum(terms, sh.wsum);
+  block_sums(sum, terms, most, sh.waves);
+  *total = sum;
+  *loss = terms;
   if (!a.dlogits) return;
-  most = block_max(most, sh.wsum);
   // (a slope that is not finite makes the sums NaN)
   const bool finite = fabsf(*total) < INFINITY && most < INFINITY;
   const double scale = most > 0.0f ? 0x1p52 / (double)most : 0.0;
@@ -337,7 +358,7 @@ __global__ void __launch_bounds__(kListT) key_rows(Args a) {
   const uint32_t row = blockIdx.x, tid = threadIdx.x;
   const bool used = row_used(a, row);
   MaxSum ms{0.0f, 1.0f};
-  if (used) ms = row_sum(a, row);
+  if (used) ms = row_sum_wave(a, row);
   const float base = exp_base(ms.m);
   float total, loss = 0.0f;
   double unit = 0.0;
@@ -451,7 +472,7 @@ __global__ void __launch_bounds__(kStatT) key_gradient(Args a) {
   if (a.keys == 1) {
     info = RowInfo{0.0f, 0.0f, length_of(a, r) > t};
     if (info.used) {
-      const MaxSum ms = row_sum(a, row);
+      const MaxSum ms = row_sum_wave(a, row);
       info.base = exp_base(ms.m);
       lg = kPolicy ? a.g + row : a.gkey + r;
       info.scale = *lg / ms.s;
