@@ -19,6 +19,13 @@
 //                fit its registers: the logits are read once
 // The gradient is stored as -p G first; then, past a barrier, the list's
 // tokens are stored over it.
+//
+// Bound by the logits: read twice (the second time mostly from the last
+// level's cache) and the gradient written, 128 rows x 262,144 bf16 with 1000
+// keys a request: 52 us, of them 17 the statistics at 3.9 TB/s, 12 the rows'
+// tables and 23 the gradient at 5.9 TB/s; or read once by key_whole, 2048
+// rows x 32,768 bf16: 44 us, 6.0 TB/s.  Few rows are bound by latency: 8 rows
+// x 32,768 f32, 10 keys: 17 us for 2 MB.
 #include <type_traits>
 
 #include "op_device.h"
@@ -636,6 +643,10 @@ hipError_t launch(const Args& a, const Plan& p, hipStream_t s) {
     hipLaunchKernelGGL(key_loss, dim3(1), dim3(256), 0, s, a);
     return hipGetLastError();
   }
+  // Rows that fit a workgroup's registers in one kernel: 512 rows x 32,768
+  // bf16, 64 keys a request: 22 us, in parts 31 (1024 threads of four vectors;
+  // of eight: 25); 2048 rows of a key each: 51, in parts 69 (512 threads of
+  // eight vectors; 1024: 65); 8 rows x 32,768 f32: 15.6, in parts 18.1.
   if (kPolicy && p.vecs <= 8 * kListT && a.keys <= (uint32_t)kListT) {
     const dim3 g(a.rows);
     if (a.keys > 1) {
