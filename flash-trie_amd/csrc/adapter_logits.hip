@@ -19,6 +19,8 @@
 // no order: 175 us, 3.5 TB/s, with the adapters' turns (no adapters: 132).
 // Above, the matrix cores do: 4096 rows, 32,768 x 1024 f16, 16 adapters of
 // rank 64: 384 us, 0.76 PFLOP/s counting the adapters' products once.
+#include <algorithm>
+
 #include "op_device.h"
 #include "operators.h"
 
@@ -28,6 +30,7 @@ namespace {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
+constexpr uint32_t kCUs = 256;
 constexpr int kMaxBins = 510;  // adapters that logits_order sorts by
 
 __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c, __bf16) {
@@ -63,6 +66,7 @@ struct Args {
   uint16_t* z;        // [rows to whole 16s][kParts][rank32]
   uint32_t* zeros;  // 16 bytes of zeros
   uint32_t row_tiles;
+  uint32_t shares;  // of logits_shrink's blocks
   bool whole_up;  // up's rows are whole vectors at multiples of 16 bytes
 };
 
@@ -133,10 +137,12 @@ __global__ void __launch_bounds__(1024) logits_order(Args a) {
   }
 }
 
-// Block b: rows [16 b, 16 b + 16) of the order, 64 ranks at a time; the 16
+// Rows [16 b, 16 b + 16) of the order by `shares` blocks, which take their
+// runs of rows with the same adapter in turn; 64 ranks at a time; the 16
 // waves share the hidden columns, a run of steps each with its loads
 // together, and add up in LDS.  Bound by latency: one way to memory for each
-// run of rows with the same adapter.  At most 16 rows are put in order here, as
+// run, so there are as many blocks as CUs (16 rows of an adapter each, rank 8,
+// 1024 columns, and a vocabulary of 32768: 66 us by one block, 34 by 16).  At most 16 rows are put in order here, as
 // logits_order would (16 rows of 4 adapters in turn, 262144 x 1024: 126 us to
 // 144 in their own order).
 constexpr int kShrinkT = 1024;
@@ -147,7 +153,8 @@ __global__ void __launch_bounds__(kShrinkT) logits_shrink(Args a) {
   __shared__ float zs[16][FT_MAX_RANK + 1];  // row, rank
   __shared__ uint32_t order[16];
   const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const uint32_t r0 = blockIdx.x * 16, n = min(16u, a.rows - r0), col = lane & 15, q = lane >> 4;
+  const uint32_t share = blockIdx.x % a.shares;
+  const uint32_t r0 = blockIdx.x / a.shares * 16, n = min(16u, a.rows - r0), col = lane & 15, q = lane >> 4;
   const bool alone = a.rows <= 16;
   for (uint32_t i = tid; i < 16 * a.rank32; i += kShrinkT) zs[i / a.rank32][i % a.rank32] = 0.0f;
   const uint32_t mine = r0 + min(col, n - 1);
@@ -165,22 +172,28 @@ __global__ void __launch_bounds__(kShrinkT) logits_shrink(Args a) {
     __syncthreads();
     at = order[mine];
     own = __shfl(own, (int)at, 64);
-    if (tid < n) {
+    if (share == 0 && tid < n) {
       a.perm[tid] = (int32_t)at;
       a.sorted[tid] = own;
     }
-    if (tid < 4) a.zeros[tid] = 0;
+    if (share == 0 && tid < 4) a.zeros[tid] = 0;
   } else {
     at = (uint32_t)a.perm[mine];
     own = max(a.sorted[mine], -1);
   }
   const T* x = (const T*)a.x + (int64_t)at * a.x_stride;
   __syncthreads();
-  for (uint32_t i = 0; i < n;) {
+  uint32_t run = 0, written = share == 0 ? ~0u << n : 0u;  // rows that this block writes
+  for (uint32_t i = 0; i < n; ++run) {
     const int32_t g = __builtin_amdgcn_readlane(own, (int)i);
     // rows from i on with the same adapter
     const uint64_t other = __ballot(own != g) & 0xFFFFu & ~((2u << i) - 1u);
     const uint32_t j = min(n, other ? (uint32_t)__ffsll((unsigned long long)other) - 1u : 16u);
+    if (run % a.shares != share) {
+      i = j;
+      continue;
+    }
+    written |= (1u << j) - (1u << i);
     if (g >= 0 && (uint32_t)g < a.adapters) {
       const T* down = (const T*)a.down + (int64_t)g * a.down_stride[0];
       const float scale = a.scale[g];
@@ -218,6 +231,7 @@ __global__ void __launch_bounds__(kShrinkT) logits_shrink(Args a) {
   }
   // a wave a row: its power of two, then the parts
   const uint32_t row = wave;
+  if (!(written >> row & 1)) return;
   float big = 0.0f;
   for (uint32_t k = lane; k < a.rank; k += 64) big = fmaxf(big, fabsf(zs[row][k]));
   big = wave_max(big);
@@ -908,7 +922,9 @@ bool whole_vectors(const void* p, int64_t stride) {
 template <typename T, typename O>
 hipError_t launch(Args a, hipStream_t s) {
   if (a.rows > 16) hipLaunchKernelGGL(logits_order, dim3(1), dim3(1024), 0, s, a);
-  hipLaunchKernelGGL((logits_shrink<T>), dim3((a.rows + 15) / 16), dim3(kShrinkT), 0, s, a);
+  const uint32_t blocks = (a.rows + 15) / 16;
+  a.shares = std::min(16u, std::max(1u, kCUs / blocks));
+  hipLaunchKernelGGL((logits_shrink<T>), dim3(blocks * a.shares), dim3(kShrinkT), 0, s, a);
   if (a.hidden % 8 == 0 && whole_vectors(a.x, a.x_stride) &&
       whole_vectors(a.weight, a.weight_stride)) {
     // Up to 96 rows the weights' stream is the bound: two or more workgroups
