@@ -141,10 +141,10 @@ __global__ void __launch_bounds__(1024) logits_order(Args a) {
 // runs of rows with the same adapter in turn; 64 ranks at a time; the 16
 // waves share the hidden columns, a run of steps each with its loads
 // together, and add up in LDS.  Bound by latency: one way to memory for each
-// run, so there are as many blocks as CUs (16 rows of an adapter each, rank 8,
-// 1024 columns, and a vocabulary of 32768: 66 us by one block, 34 by 16).  At most 16 rows are put in order here, as
-// logits_order would (16 rows of 4 adapters in turn, 262144 x 1024: 126 us to
-// 144 in their own order).
+// run, so there are as many blocks as CUs (16 rows of an adapter each, 32768
+// x 1024, rank 8: 66 us with one block, 34 with 16).  At most 16 rows are put
+// in order here, as logits_order would (16 rows of 4 adapters in turn, 262144
+// x 1024: 126 us, in their own order 144).
 constexpr int kShrinkT = 1024;
 
 template <typename T>
