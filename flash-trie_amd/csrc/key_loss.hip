@@ -280,12 +280,16 @@ __global__ void __launch_bounds__(1024) key_pairs(Args a) {
 }
 
 // A row's tokens and the sums of their slopes: a hash table.  Sums are whole
-// numbers of 2^-52 of the row's largest slope (kP * 1024 of them fit 63
-// bits), so that they do not depend on the order of the atomics and are finer
-// than a 32-bit sum's roundings.
+// numbers of 2^-kBits of the row's largest slope, so that they do not depend
+// on the order of the atomics and are finer than a 32-bit sum's roundings.
+// All of a row's slopes may be the largest, of one sign and of one token
+// (keys of a prefix, an advantage for all): kP * 1024 times 2^kBits is 2^62.
 template <int kP>
 struct Table {
   static constexpr uint32_t kSlots = 2 * kListT * kP;
+  static constexpr int kBits = kP == 1 ? 52 : 50;
+  static_assert((uint64_t)kListT * kP << kBits <= 1ull << 62, "a row's slopes fit a sum");
+  static constexpr double kOne = (double)(1ull << kBits);
   uint32_t tok[kSlots];  // ~0: free
   unsigned long long sum[kSlots];
   float waves[kListT / 64][3];
@@ -338,8 +342,8 @@ __device__ __forceinline__ void row_table(const Args& a, Table<kP>& sh, uint32_t
   if (!a.dlogits) return;
   // (a slope that is not finite makes the sums NaN)
   const bool finite = fabsf(*total) < INFINITY && most < INFINITY;
-  const double scale = most > 0.0f ? 0x1p52 / (double)most : 0.0;
-  *unit = finite ? (double)most * 0x1p-52 : (double)NAN;
+  const double scale = most > 0.0f ? Table<kP>::kOne / (double)most : 0.0;
+  *unit = finite ? (double)most / Table<kP>::kOne : (double)NAN;
 #pragma unroll
   for (int i = 0; i < kP; ++i) {
     if (toks[i] == ~0u) continue;

@@ -397,3 +397,26 @@ def test_refusals(ft):
     z = torch.zeros(1, 4097, device="cuda")
     with pytest.raises(ft.MarisaError, match="4096"):
         ft.policy_loss(x, t, t[..., 0], z[..., None], z, z)
+
+
+# requests up to the most keys whose slopes are of one size and sign: the
+# whole-number sums of the row's table are as large as they get
+@pytest.mark.parametrize("distinct", [1, 2])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("C", [1024, 1025, 2047, 2048, 2049, 3000, 4095, 4096])
+def test_equal_slopes(ft, C, sign, distinct):
+    x, tokens, lengths, _ = keys(2, 1, 5003, C, F32, 19, distinct=distinct, full=True)
+    lp = ref.scores(x.double(), tokens, lengths)
+    # keys on the policy that made them, one advantage for all
+    a = dict(logits=x, tokens=tokens, lengths=lengths, old_logp=lp.float(),
+             ref_logp=(lp + 0.3 * sign).float(), advantage=torch.full((2, C), sign),
+             weight=torch.full((2, C), 1.0 / (2 * C)))
+    check_policy(ft, a, kl=0.0, what="one advantage")
+    # the KL term alone
+    check_policy(ft, {**a, "advantage": torch.zeros(2, C)}, kl=0.05, what="KL")
+    # every key of a request against one of the other
+    i = torch.arange(C, dtype=torch.int32)
+    pairs = torch.stack([i, i + C] if sign > 0 else [i + C, i], 1)
+    check_preference(ft, dict(logits=x, tokens=tokens, lengths=lengths, pairs=pairs,
+                              ref_logp=lp.sum(-1).float(), weight=torch.full((C,), 1.0 / C)),
+                     what="pairs across requests")
