@@ -313,6 +313,14 @@ __device__ __forceinline__ void copy_to_lds(const void* from, void* to) {
                                    (__attribute__((address_space(3))) uint32_t*)to, 16, 0, 0);
 }
 
+// All LDS reads of the wave are done, and all its copies but the last n.
+template <int n>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("" ::: "memory");
+  // vmcnt n, lgkmcnt 0, the third counter free
+  __builtin_amdgcn_s_waitcnt((n & 15) | (n >> 4) << 14 | 7 << 4);
+}
+
 // This thread's vectors of the ups of runs b ... b + n - 1, ranks k0 ... k0 +
 // 31, those numbered t0 ... t0 + kF - 1 of its share.
 template <typename T, int kBM, int kBN, uint32_t kT, uint32_t kF>
@@ -396,6 +404,7 @@ __device__ __forceinline__ void add_adapters(const Args& a, const Rows<kBM>& r, 
           __builtin_amdgcn_sched_barrier(0);
         }
       }
+      wait_copies<0>();  // (a barrier alone does not wait for them)
       __syncthreads();
       for (uint32_t k = 0; k < n; ++k) {
         const uint32_t i = (uint32_t)__builtin_amdgcn_readfirstlane((int)r.run_i[b + k]);
@@ -614,14 +623,6 @@ struct Shape {
   static constexpr int XLanes = BM * 8 / CX / (kWM * kWN);  // lanes of a wave in the rows' copies
   static constexpr bool Ahead = M * N < 16;  // registers for ups loaded before the product
 };
-
-// All LDS reads of the wave are done, and all its copies but the last n.
-template <int n>
-__device__ __forceinline__ void wait_copies() {
-  asm volatile("" ::: "memory");
-  // vmcnt n, lgkmcnt 0, the third counter free
-  __builtin_amdgcn_s_waitcnt((n & 15) | (n >> 4) << 14 | 7 << 4);
-}
 
 // The same from a 32-bit offset (a lane's and the wave's) of a buffer.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t whole_buffer(const void* p) {
