@@ -254,7 +254,10 @@ __global__ void __launch_bounds__(1024) key_pairs(Args a) {
       const float sig = (h >= 0.0f ? 1.0f : e) / (1.0f + e);
       d = w * a.beta * (sig - (1.0f - a.smoothing));
       const float won = tail + (h < 0.0f ? -h : 0.0f), lost = tail + (h > 0.0f ? h : 0.0f);
-      loss += w * ((1.0f - a.smoothing) * won + a.smoothing * lost);
+      // (one of the two is infinite where h is, and counts only with a share)
+      const float kept = 1.0f - a.smoothing;
+      loss += w * ((kept > 0.0f ? kept * won : 0.0f) +
+                   (a.smoothing > 0.0f ? a.smoothing * lost : 0.0f));
     }
     const uint32_t n = (uint32_t)min((uint64_t)64, p1 - q);
     for (uint32_t i = 0; i < n; ++i) {

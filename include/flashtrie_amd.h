@@ -407,7 +407,9 @@ int ft_policy_loss(const ft_policy_loss_args* args, void* workspace,
 /* loss = sum over pairs (a, b) of weight *
  *   ((1 - smoothing) softplus(-h) + smoothing softplus(h)),
  * h = beta ((s_a - ref_a) - (s_b - ref_b)), s a key's summed logp; a and b
- * index batch * keys. */
+ * index batch * keys.  A term whose factor is 0 counts nothing, also where
+ * its softplus is infinite (a key with a token of logit -infinity); two such
+ * keys in a pair make h NaN. */
 typedef struct ft_preference_loss_args {
   ft_keys k;
   uint64_t pairs;

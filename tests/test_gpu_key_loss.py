@@ -420,3 +420,50 @@ def test_equal_slopes(ft, C, sign, distinct):
     check_preference(ft, dict(logits=x, tokens=tokens, lengths=lengths, pairs=pairs,
                               ref_logp=lp.sum(-1).float(), weight=torch.full((C,), 1.0 / C)),
                      what="pairs across requests")
+
+
+@pytest.mark.parametrize("smoothing", [0.0, 0.25, 1.0])
+def test_a_masked_token_in_a_pair(ft, smoothing):
+    """A pair whose one key holds a token of logit -infinity has h of -+
+    infinity: a softplus of it is 0 or infinite, counts only where its share
+    of the smoothing is above 0, and the derivative is finite.  Of two such
+    keys h is NaN."""
+    beta = 0.3
+    a = preference_case(1, 2, 50, 4, 2, F32, 20, full=True)
+    a["tokens"][0, :, 0] = torch.tensor([3, 4, 5, 6], dtype=torch.int32)
+    a["logits"][0, 0, 3] = -math.inf
+    w, rf = a["weight"].double(), a["ref_logp"].double()
+    lp = ref.scores(a["logits"].double(), a["tokens"], a["lengths"])
+    m = lp.sum(-1)[0] - rf[0]
+    h = beta * (m[2] - m[3])
+    other = w[1] * ((1 - smoothing) * torch.nn.functional.softplus(-h)
+                    + smoothing * torch.nn.functional.softplus(h))
+    d1 = w[1] * beta * (torch.sigmoid(h) - (1 - smoothing))
+    for pair, sig, finite in (((0, 1), 0.0, smoothing == 1.0), ((1, 0), 1.0, smoothing == 0.0)):
+        a["pairs"] = torch.tensor([pair, (2, 3)], dtype=torch.int32)
+        loss, logp, d = ft.preference_loss(**{k: v.cuda() for k, v in a.items()}, beta=beta,
+                                           smoothing=smoothing)
+        assert logp[0, 0, 0] == -math.inf and not logp.isnan().any()
+        if finite:
+            # scores good to LSE and a few units of at most 40, slope at most 1
+            assert abs(loss.item() - other) <= w[1] * beta * 4 * (ref.LSE + 200 * ref.U)
+        else:
+            assert loss == math.inf
+        d0 = w[0] * beta * (sig - (1 - smoothing))
+        gkey = torch.zeros(4).double()
+        gkey[pair[0]] += d0
+        gkey[pair[1]] -= d0
+        gkey[2] += d1
+        gkey[3] -= d1
+        g = gkey[None, :, None].expand(1, 4, 2)
+        p = torch.softmax(a["logits"].double(), -1)
+        want = -p * g.sum(1)[..., None]
+        want.scatter_add_(2, a["tokens"].long().transpose(1, 2), g.transpose(1, 2).contiguous())
+        gerr = (w.sum() * beta * (4 * beta * (ref.LSE + 200 * ref.U) + 16 * ref.U)).expand(1, 4, 2)
+        check_gradient(d, want, ref.gradient_bound(a["logits"].double(), a["tokens"], a["lengths"],
+                                                   g, gerr), (pair, smoothing))
+    a["tokens"][0, 1, 0] = 3
+    a["pairs"] = torch.tensor([(0, 1), (2, 3)], dtype=torch.int32)
+    loss, _, d = ft.preference_loss(**{k: v.cuda() for k, v in a.items()}, beta=beta,
+                                    smoothing=smoothing)
+    assert loss.isnan() and d.isnan().any()
