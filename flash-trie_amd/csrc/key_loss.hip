@@ -83,6 +83,11 @@ struct RowInfo {
   uint32_t used;
 };
 
+// A row of nothing but -infinity has s = 0 and probability nowhere.
+__device__ __forceinline__ float row_scale(float total, float s) {
+  return s == 0.0f ? total * 0.0f : total / s;
+}
+
 template <typename T>
 __device__ __forceinline__ const T* row_of(const Args& a, uint32_t row) {
   const uint32_t r = row / a.steps, t = row - r * a.steps;
@@ -380,7 +385,7 @@ __global__ void __launch_bounds__(kListT) key_rows(Args a) {
   row_table<T, kPolicy, kP>(a, sh, row, base, logf(ms.s), &total, &loss, &unit);
   if (tid == 0) {
     if (kPolicy) a.terms[row] = loss;
-    a.info[row] = RowInfo{base, total / ms.s, used};
+    a.info[row] = RowInfo{base, row_scale(total, ms.s), used};
   }
   if (!a.dlogits) return;
   for (uint32_t i = tid; i < Table<kP>::kSlots; i += kListT)
@@ -489,7 +494,7 @@ __global__ void __launch_bounds__(kStatT) key_gradient(Args a) {
       const MaxSum ms = row_sum_wave(a, row);
       info.base = exp_base(ms.m);
       lg = kPolicy ? a.g + row : a.gkey + r;
-      info.scale = *lg / ms.s;
+      info.scale = row_scale(*lg, ms.s);
       ltok = (const uint32_t*)a.tokens + row;
       const uint32_t tok = *ltok;
       l1 = tok < a.vocab && tok >= e0 && tok - e0 < span_of<T>();
@@ -561,7 +566,7 @@ __global__ void __launch_bounds__(kT) key_whole(Args a) {
   }
   if (tid == 0) a.terms[row] = loss;
   if (!a.dlogits) return;
-  const RowInfo info{base, total / ms.s, used};
+  const RowInfo info{base, row_scale(total, ms.s), used};
 #pragma unroll
   for (int u = 0; u < kU; ++u) {
     const uint32_t vec = u * kT + tid;

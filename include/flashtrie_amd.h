@@ -368,7 +368,9 @@ int ft_propose(const ft_propose_args* args, void* workspace,
 /* Keys and the logits that score them: token t of key (r, c) is scored by
  * row (r, t) of the logits, so a request's keys share its rows, as the
  * search's results do; with keys = 1 every key has rows of its own.  Tokens
- * at t >= lengths[r, c] are not read as tokens and count nothing. */
+ * at t >= lengths[r, c] are not read as tokens and count nothing.  A token
+ * whose logit is -infinity has log-probability -infinity, also in a row of
+ * nothing else, where no token has any probability. */
 typedef struct ft_keys {
   int device;
   int dtype;                  /* of logits and dlogits */

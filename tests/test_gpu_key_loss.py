@@ -467,3 +467,36 @@ def test_a_masked_token_in_a_pair(ft, smoothing):
     loss, _, d = ft.preference_loss(**{k: v.cuda() for k, v in a.items()}, beta=beta,
                                     smoothing=smoothing)
     assert loss.isnan() and d.isnan().any()
+
+
+# rows in a workgroup's registers, and in parts
+@pytest.mark.parametrize("C", [1, 3, 1100])
+@pytest.mark.parametrize("V", [60, 40001])
+def test_a_row_of_nothing(ft, C, V):
+    """A row whose mask leaves nothing: scores of -infinity, no probability
+    anywhere; its gradient is its tokens' own slopes, 0 for the policy loss
+    without the KL term (the ratio is 0)."""
+    a = policy_case(2, 3, V, C, F32, 21, full=True)
+    gpu = {k: v.cuda() for k, v in a.items()}
+    whole = ft.policy_loss(**gpu)
+    a["logits"][1, 1] = -math.inf
+    a["old_logp"][1, :, 1] = -2.0
+    gpu = {k: v.cuda() for k, v in a.items()}
+    loss, logp, d = ft.policy_loss(**gpu)
+    assert loss.isfinite() and (logp[1, :, 1] == -math.inf).all()
+    assert (d[1, 1] == 0).all()
+    rest = torch.ones(2, 3, dtype=torch.bool)
+    rest[1, 1] = False
+    assert torch.equal(d[rest.cuda()], whole[2][rest.cuda()])
+    # preferred keys of the other request: h is infinite, and the keys of the
+    # masked row have slopes of -weight beta smoothing
+    i = torch.arange(C, dtype=torch.int32, device="cuda")
+    w = torch.full((C,), 1.0 / C, device="cuda")
+    loss, logp, d = ft.preference_loss(gpu["logits"], gpu["tokens"], gpu["lengths"],
+                                       torch.stack([i, i + C], 1), torch.zeros(2, C, device="cuda"),
+                                       w, beta=0.5, smoothing=0.25)
+    assert (logp[1, :, 1] == -math.inf).all() and d.isfinite().all()
+    want = torch.zeros(V).double()
+    want.index_add_(0, a["tokens"][1, :, 1].long(), torch.full((C,), -0.5 * 0.25 / C).double())
+    # a pair's slope rounds a few times, up to C of them are summed
+    assert ((d[1, 1].double().cpu() - want).abs() <= (C + 8) * ref.U * want.abs()).all()
