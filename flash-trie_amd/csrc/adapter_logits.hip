@@ -904,16 +904,14 @@ template <typename T, typename O, typename S>
 hipError_t launch_tile(Args a, hipStream_t s) {
   a.row_tiles = (a.rows + S::BM - 1) / S::BM;
   const uint32_t tiles = (a.vocab + S::BN - 1) / S::BN;
-  hipLaunchKernelGGL((logits_tile<T, O, S>), dim3(tiles * a.row_tiles), dim3(S::Threads), 0, s, a);
-  return hipGetLastError();
+  return start(logits_tile<T, O, S>, tiles * a.row_tiles, S::Threads, s, a);
 }
 
 template <typename T, typename O, typename S>
 hipError_t launch_staged(Args a, hipStream_t s) {
   a.row_tiles = (a.rows + S::BM - 1) / S::BM;
   const uint32_t tiles = (a.vocab + S::BN - 1) / S::BN;
-  hipLaunchKernelGGL((logits_staged<T, O, S>), dim3(tiles * a.row_tiles), dim3(S::Threads), 0, s, a);
-  return hipGetLastError();
+  return start(logits_staged<T, O, S>, tiles * a.row_tiles, S::Threads, s, a);
 }
 
 bool whole_vectors(const void* p, int64_t stride) {
@@ -922,10 +920,12 @@ bool whole_vectors(const void* p, int64_t stride) {
 
 template <typename T, typename O>
 hipError_t launch(Args a, hipStream_t s) {
-  if (a.rows > 16) hipLaunchKernelGGL(logits_order, dim3(1), dim3(1024), 0, s, a);
+  hipError_t e = a.rows > 16 ? start(logits_order, 1, 1024, s, a) : hipSuccess;
+  if (e != hipSuccess) return e;
   const uint32_t blocks = (a.rows + 15) / 16;
   a.shares = std::min(16u, std::max(1u, kCUs / blocks));
-  hipLaunchKernelGGL((logits_shrink<T>), dim3(blocks * a.shares), dim3(kShrinkT), 0, s, a);
+  e = start(logits_shrink<T>, blocks * a.shares, kShrinkT, s, a);
+  if (e != hipSuccess) return e;
   if (a.hidden % 8 == 0 && whole_vectors(a.x, a.x_stride) &&
       whole_vectors(a.weight, a.weight_stride)) {
     // Up to 96 rows the weights' stream is the bound: two or more workgroups
@@ -951,8 +951,7 @@ hipError_t launch(Args a, hipStream_t s) {
   }
   a.row_tiles = (a.rows + kBM - 1) / kBM;
   const uint32_t tiles = (a.vocab + kBN - 1) / kBN;
-  hipLaunchKernelGGL((logits_product<T, O>), dim3(tiles * a.row_tiles), dim3(kThreads), 0, s, a);
-  return hipGetLastError();
+  return start(logits_product<T, O>, tiles * a.row_tiles, kThreads, s, a);
 }
 
 }  // namespace

@@ -651,46 +651,40 @@ Args base_args(const ft_keys& k, const Plan& p, uint8_t* ws) {
 
 template <typename T, bool kPolicy>
 hipError_t launch(const Args& a, const Plan& p, hipStream_t s) {
-  if (a.rows == 0) {
-    hipLaunchKernelGGL(key_loss, dim3(1), dim3(256), 0, s, a);
-    return hipGetLastError();
-  }
+  if (a.rows == 0) return start(key_loss, 1, 256, s, a);
+  hipError_t e;
   // Rows that fit a workgroup's registers in one kernel: 512 rows x 32,768
   // bf16, 64 keys a request: 22 us, in parts 31 (1024 threads of four vectors;
   // of eight: 25); 2048 rows of a key each: 51, in parts 69 (512 threads of
   // eight vectors; 1024: 65); 8 rows x 32,768 f32: 15.6, in parts 18.1.
   if (kPolicy && p.vecs <= 8 * kListT && a.keys <= (uint32_t)kListT) {
-    const dim3 g(a.rows);
-    if (a.keys > 1) {
-      if (p.vecs <= 4 * kListT)
-        hipLaunchKernelGGL((key_whole<T, true, kListT, 4>), g, dim3(kListT), 0, s, a);
-      else
-        hipLaunchKernelGGL((key_whole<T, true, kListT, 8>), g, dim3(kListT), 0, s, a);
-    } else if (p.vecs <= 8 * 512) {
-      hipLaunchKernelGGL((key_whole<T, false, 512, 8>), g, dim3(512), 0, s, a);
-    } else {
-      hipLaunchKernelGGL((key_whole<T, false, 1024, 8>), g, dim3(1024), 0, s, a);
-    }
-    hipLaunchKernelGGL(key_loss, dim3(1), dim3(256), 0, s, a);
-    return hipGetLastError();
+    if (a.keys > 1 && p.vecs <= 4 * kListT)
+      e = start(key_whole<T, true, kListT, 4>, a.rows, kListT, s, a);
+    else if (a.keys > 1)
+      e = start(key_whole<T, true, kListT, 8>, a.rows, kListT, s, a);
+    else if (p.vecs <= 8 * 512)
+      e = start(key_whole<T, false, 512, 8>, a.rows, 512, s, a);
+    else
+      e = start(key_whole<T, false, 1024, 8>, a.rows, 1024, s, a);
+    return e == hipSuccess ? start(key_loss, 1, 256, s, a) : e;
   }
-  hipLaunchKernelGGL((key_stats<T>), dim3(a.rows * a.chunks), dim3(kStatT), 0, s, a);
+  e = start(key_stats<T>, (uint64_t)a.rows * a.chunks, kStatT, s, a);
   if (!kPolicy) {
     const uint32_t keys = a.batch * a.keys;
-    hipLaunchKernelGGL((key_scores<T>), dim3((keys + 15) / 16), dim3(256), 0, s, a);
-    hipLaunchKernelGGL(key_pairs, dim3((keys + 63) / 64), dim3(1024), 0, s, a);
+    if (e == hipSuccess) e = start(key_scores<T>, (keys + 15) / 16, 256, s, a);
+    if (e == hipSuccess) e = start(key_pairs, (keys + 63) / 64, 1024, s, a);
   }
+  if (e != hipSuccess) return e;
   if (a.keys > (uint32_t)kListT)
-    hipLaunchKernelGGL((key_rows<T, kPolicy, 4>), dim3(a.rows), dim3(kListT), 0, s, a);
+    e = start(key_rows<T, kPolicy, 4>, a.rows, kListT, s, a);
   else if (a.keys > 1)
-    hipLaunchKernelGGL((key_rows<T, kPolicy, 1>), dim3(a.rows), dim3(kListT), 0, s, a);
+    e = start(key_rows<T, kPolicy, 1>, a.rows, kListT, s, a);
   else if (kPolicy)
-    hipLaunchKernelGGL((key_single<T>), dim3((a.rows + 255) / 256), dim3(256), 0, s, a);
+    e = start(key_single<T>, (a.rows + 255) / 256, 256, s, a);
+  if (e != hipSuccess) return e;
   if (a.dlogits)
-    hipLaunchKernelGGL((key_gradient<T, kPolicy>), dim3(a.rows * a.spans), dim3(kStatT), 0, s, a);
-  else
-    hipLaunchKernelGGL(key_loss, dim3(1), dim3(256), 0, s, a);
-  return hipGetLastError();
+    return start(key_gradient<T, kPolicy>, (uint64_t)a.rows * a.spans, kStatT, s, a);
+  return start(key_loss, 1, 256, s, a);
 }
 
 template <bool kPolicy>

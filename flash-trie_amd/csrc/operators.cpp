@@ -23,6 +23,9 @@ int hip_error(hipError_t e, const char* call) {
 
 constexpr int kMaxDevices = 64;
 constexpr uint64_t kMaxGrid = 0x7FFFFFFFull;  // workgroups of a launch
+constexpr uint64_t kMaxThreads = 0xFFFFFFFFull;
+
+constexpr uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
 // The caller's device is current during the call, and what was before after
 // it.
@@ -67,8 +70,12 @@ const char* wrong(const ft_adapter_logits_args& a, int* code) {
   if (a.adapters > 0x7FFFFFFEu || a.rank > FT_MAX_RANK) return "rank must be at most 256";
   if (a.vocab > FT_MAX_HEAD_VOCAB) return "vocab must be at most 2^24";
   if (a.hidden > (1u << 24)) return "hidden must be at most 2^24";
-  if (a.rows > kMaxGrid ||
-      ((a.vocab + 15ull) / 16) * ((a.rows + 15) / 16) > kMaxGrid) return "too many rows";
+  // (the launches: 1024 threads for 16 rows; tiles of 128 tokens by 64 rows
+  // with 256, by 256 rows with 1024)
+  if (a.rows > kMaxGrid || ceil_div(a.rows, 16) * 1024 > kMaxThreads ||
+      ceil_div(a.vocab, 128) * ceil_div(a.rows, 64) * 256 > kMaxThreads ||
+      ceil_div(a.vocab, 128) * ceil_div(a.rows, 256) * 1024 > kMaxThreads)
+    return "too many rows";
   *code = FT_E_ARG;
   if (a.rows) {
     if (!a.x || !a.weight || !a.adapter || !a.out) return "null pointer";
@@ -104,6 +111,10 @@ const char* wrong(const ft_keys& k, int* code) {
   if (k.batch > kMaxGrid || k.steps > kMaxGrid || k.batch * k.steps > kMaxGrid / 16384 ||
       k.batch * k.keys > kMaxGrid / 4)
     return "too many rows";
+  // (the gradient: 256 threads for 1024 vectors of a row)
+  if (k.dlogits && k.batch * k.steps * ceil_div(k.vocab, k.dtype == FT_F32 ? 4096 : 8192) * 256 >
+                       kMaxThreads)
+    return "too many rows";
   *code = FT_E_ARG;
   if (!k.loss) return "null pointer";
   if (k.batch) {
@@ -137,6 +148,10 @@ const char* wrong(const ft_preference_loss_args& a, int* code) {
   if (a.pairs > kMaxGrid) {
     *code = FT_E_LIMIT;
     return "too many pairs";
+  }
+  if (ceil_div(a.k.batch * a.k.keys, 64) * 1024 > kMaxThreads) {  // 1024 threads for 64 keys
+    *code = FT_E_LIMIT;
+    return "too many keys";
   }
   if (a.pairs && (!a.pair || !a.weight)) return "null pointer";
   if (a.k.batch && !a.ref_logp) return "null pointer";

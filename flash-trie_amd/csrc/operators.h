@@ -22,6 +22,17 @@ struct Arena {
   }
 };
 
+// Starts a kernel of one argument.  The launch's own status: the runtime's
+// last error may be that of another call of the application.
+template <typename A>
+hipError_t start(void (*kernel)(A), uint64_t blocks, uint32_t threads, hipStream_t s, A a) {
+  void* args[] = {&a};
+  const hipError_t e = hipLaunchKernel((const void*)kernel, dim3((uint32_t)blocks), dim3(threads),
+                                       args, 0, s);
+  if (e != hipSuccess) (void)hipGetLastError();  // it is in the caller's hands now
+  return e;
+}
+
 uint64_t adapter_logits_workspace(const ft_adapter_logits_args& a);
 hipError_t launch_adapter_logits(const ft_adapter_logits_args& a, uint8_t* ws, hipStream_t s);
 

@@ -639,18 +639,12 @@ hipError_t launch(const ft_propose_args& a, uint8_t* ws, hipStream_t s) {
   // 14.5, 15.5), and up to 16384 where the rows fill the chip (256 of 100,003
   // f16: 22.9, 26.2; but 39 of them: 20.5, 18.8).
   const uint32_t vecs = (a.vocab + kVec<T> - 1) / kVec<T>;
-  if (vecs <= (rows >= 256 ? kRowVecs : kRowVecs / 2)) {
-    hipLaunchKernelGGL((propose_row<T>), dim3(rows), dim3(kFinT), 0, s, k);
-    return hipGetLastError();
-  }
-  hipLaunchKernelGGL((propose_scan<T>), dim3(rows * p.chunks), dim3(kScanT), 0, s, k);
-  hipError_t e = hipGetLastError();
+  if (vecs <= (rows >= 256 ? kRowVecs : kRowVecs / 2))
+    return start(propose_row<T>, rows, kFinT, s, k);
+  const hipError_t e = start(propose_scan<T>, (uint64_t)rows * p.chunks, kScanT, s, k);
   if (e != hipSuccess) return e;
-  if (p.groups <= kKeyBytes / sizeof(T))
-    hipLaunchKernelGGL((propose_finish<T, true>), dim3(rows), dim3(kFinT), 0, s, k);
-  else
-    hipLaunchKernelGGL((propose_finish<T, false>), dim3(rows), dim3(kFinT), 0, s, k);
-  return hipGetLastError();
+  if (p.groups <= kKeyBytes / sizeof(T)) return start(propose_finish<T, true>, rows, kFinT, s, k);
+  return start(propose_finish<T, false>, rows, kFinT, s, k);
 }
 
 }  // namespace

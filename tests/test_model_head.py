@@ -104,3 +104,32 @@ def test_same_seed_same_rounds(ft):
     runs = [M.run(args, log=lambda *_: None) for _ in range(2)]
     assert runs[0][0]["losses"][0] == runs[1][0]["losses"][0]
     assert [x["keys"] for x in runs[0]] == [x["keys"] for x in runs[1]]
+
+
+@pytest.mark.gpu
+def test_an_error_of_another_call(ft):
+    """An error that an earlier call of the application left with the HIP
+    runtime is not taken for a launch's."""
+    import ctypes
+    with open("/proc/self/maps") as f:
+        path = next(line.split()[-1] for line in f if "libamdhip64" in line)
+    hip = ctypes.CDLL(path)
+    x = torch.randn(2, 3, 50000, device="cuda")
+    h = torch.randn(20, 64, device="cuda").bfloat16()
+    none = torch.full((20,), -1, dtype=torch.int32, device="cuda")
+    tok = torch.zeros(2, 4, 3, dtype=torch.int32, device="cuda")
+    one, old = torch.ones(2, 4, device="cuda"), torch.zeros(2, 4, 3, device="cuda")
+    length = torch.full((2, 4), 3, dtype=torch.int32, device="cuda")
+    pairs = torch.tensor([[0, 1]], dtype=torch.int32, device="cuda")
+    calls = [lambda: ft.propose(x, 5), lambda: ft.propose(x[..., :100], 5),
+             lambda: (ft.adapter_logits(h, h, h[None, :4], h[None, :, :4], none, one[0, :1]),),
+             lambda: ft.policy_loss(x, tok, length, old, one, one),
+             lambda: ft.preference_loss(x, tok, length, pairs, one, one[0, :1])]
+    for call in calls:
+        want = call()
+        assert hip.hipSetDevice(1 << 20) != 0  # no such device
+        try:
+            got = call()
+        finally:
+            hip.hipGetLastError()
+        assert all(torch.equal(p, q) for p, q in zip(got, want))

@@ -257,3 +257,28 @@ def test_kernel_resources(resources):
         assert not k.get(".uses_dynamic_stack", False), name
         assert k[".group_segment_fixed_size"] <= 160 * 1024, name
         assert k[".vgpr_spill_count"] == k[".private_segment_fixed_size"] == 0, name
+
+
+# the most that the launches' thread counts (32 bits) allow, and one more
+@pytest.mark.parametrize("name,most,more,text", [
+    ("adapter_logits", dict(rows=(1 << 26) - 16), dict(rows=(1 << 26) - 15), "rows"),
+    # 2^17 tiles of tokens by fewer than 2^5 of 256 rows
+    ("adapter_logits", dict(rows=31 * 256, vocab=1 << 24, out_stride=1 << 24),
+     dict(rows=31 * 256 + 1, vocab=1 << 24, out_stride=1 << 24), "rows"),
+    # 2^14 tiles of 64 rows by fewer than 2^10 of 128 tokens
+    ("adapter_logits", dict(rows=1 << 20, vocab=1023 * 128, out_stride=1023 * 128),
+     dict(rows=1 << 20, vocab=1023 * 128 + 1, out_stride=1 << 17), "rows"),
+    ("preference_loss", dict(batch=65535, steps=1, keys=4096),
+     dict(batch=65536, steps=1, keys=4096), "keys"),
+    *[(n, dict(batch=4095, steps=1, vocab=1 << 24, stride=[1 << 24] * 2, dstride=[1 << 24] * 2),
+       dict(batch=4096, steps=1, vocab=1 << 24, stride=[1 << 24] * 2, dstride=[1 << 24] * 2), "rows")
+      for n in ("policy_loss", "preference_loss")],
+])
+def test_launch_limits(lib, name, most, more, text):
+    need = getattr(lib, f"ft_{name}_workspace")(C.byref(CALLS[name](**most)))
+    assert need > 0
+    rc, need, message = call(lib, name, CALLS[name](**more))
+    assert (rc, need) == (E_LIMIT, 0) and text in message
+    if name == "policy_loss":  # without the gradient there is no such launch
+        a = CALLS[name](**more, dlogits=None)
+        assert getattr(lib, f"ft_{name}_workspace")(C.byref(a)) > 0
