@@ -943,9 +943,11 @@ hipError_t launch(Args a, hipStream_t s) {
     // Up to 128 rows one row tile, so that w is read once (112 x 262144 x
     // 1024: 206 us, by logits_tile 238); above, logits_tile (144 rows: 246,
     // by logits_staged 287) where 32-bit offsets reach a tile's operands.
+    // (the end of the last row counts: rows may be less than their own length
+    // apart)
     if (a.hidden % 64 == 0 && a.x_stride >= 0 && a.weight_stride >= 0 &&
-        a.rows * (uint64_t)a.x_stride < 1ull << 31 && a.weight_stride < 1ll << 22 &&
-        a.vocab >= 256)
+        (a.rows - 1) * (uint64_t)a.x_stride + a.hidden < 1ull << 31 &&
+        a.weight_stride < 1ll << 22 && a.vocab >= 256)
       return launch_tile<T, O, TileShape<16, 16, 2, 4>>(a, s);
     return launch_staged<T, O, Shape<16, 8, 2, 8, 2>>(a, s);
   }

@@ -200,3 +200,24 @@ def test_refusals(ft):
     big = inputs(4, 20, 16, 1, 257, BF16, 11)
     with pytest.raises(ft.MarisaError, match="256"):
         ft.adapter_logits(**big)
+
+
+def test_rows_that_overlap_past_32_bits(ft):
+    """Rows a little apart of hidden columns that reach further: the last
+    rows start below 2^32 bytes and end above.  Whole numbers: sums are
+    exact."""
+    stride, H, V = 65472, 131072, 256
+    T = (2 ** 31 - 1) // stride
+    assert (T - 1) * stride + 64 < 2 ** 31 < (T - 1) * stride + H
+    g = torch.Generator("cuda").manual_seed(8)
+
+    def whole(n):
+        return torch.randint(-1, 2, (n,), device="cuda", generator=g, dtype=torch.int8).to(BF16)
+
+    x = whole((T - 1) * stride + H).as_strided((T, H), (stride, 1))
+    w = whole(V * H).view(V, H)
+    y = ft.adapter_logits(x, w, w[None, :8], w[None, :, :8],
+                          torch.full((T,), -1, dtype=torch.int32, device="cuda"),
+                          torch.ones(1, device="cuda"), F32)
+    for t in (0, T // 2, T - 3, T - 2, T - 1):
+        assert torch.equal(y[t].cpu(), w.float().cpu() @ x[t].float().cpu()), t
