@@ -40,8 +40,8 @@ bool shares_runtime(const py::module_& torch) {
 
 // What the calls use of torch, looked up once.
 struct Torch {
-  py::object tensor, dtypes[3], int32, uint8, raw_stream, current_stream;
-  PyObject *get_device, *dtype, *shape, *stride, *data_ptr, *new_empty, *contiguous;
+  py::object tensor, dtypes[3], int32, uint8, raw_stream, current_stream, grad_enabled, written;
+  PyObject *get_device, *dtype, *shape, *stride, *data_ptr, *new_empty, *contiguous, *requires_grad;
 };
 
 const Torch& torch() {
@@ -64,6 +64,8 @@ const Torch& torch() {
     // the stream's handle without an object for it, where torch has that
     n->raw_stream = py::getattr(m.attr("_C"), "_cuda_getCurrentRawStream", py::none());
     n->current_stream = m.attr("cuda").attr("current_stream");
+    n->grad_enabled = m.attr("is_grad_enabled");
+    n->written = m.attr("autograd").attr("graph").attr("increment_version");
     n->get_device = PyUnicode_InternFromString("get_device");
     n->dtype = PyUnicode_InternFromString("dtype");
     n->shape = PyUnicode_InternFromString("shape");
@@ -71,6 +73,7 @@ const Torch& torch() {
     n->data_ptr = PyUnicode_InternFromString("data_ptr");
     n->new_empty = PyUnicode_InternFromString("new_empty");
     n->contiguous = PyUnicode_InternFromString("contiguous");
+    n->requires_grad = PyUnicode_InternFromString("requires_grad");
     t = n;
   }
   return *t;
@@ -265,6 +268,9 @@ py::object adapter_logits(py::object x, py::object weight, py::object down, py::
     if (to.size[0] != T || to.size[1] != V) fail_value(in.call, "out must be [rows, vocab]");
     if (!out_dtype.is_none() && !out_dtype.is(t.dtypes[odt]))
       fail_type(in.call, "out is not of out_dtype");
+    // (as torch's own out= do: no gradient passes the call)
+    if (attr(to.obj, t.requires_grad).is(py::bool_(true)) && py::cast<bool>(t.grad_enabled()))
+      fail_value(in.call, "out requires a gradient, which the call does not have");
   } else {
     if (!out_dtype.is_none()) {
       odt = -1;
@@ -298,6 +304,7 @@ py::object adapter_logits(py::object x, py::object weight, py::object down, py::
   a.scale = (const float*)ts.data;
   a.out = to.data;
   a.out_stride = to.step[0];
+  if (!out.is_none()) t.written(to.obj);  // for autograd: its values change
   launch(a, in.device, tx, "adapter_logits", ft_adapter_logits_workspace, ft_adapter_logits);
   return to.obj;
 }

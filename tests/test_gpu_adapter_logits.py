@@ -221,3 +221,19 @@ def test_rows_that_overlap_past_32_bits(ft):
                           torch.ones(1, device="cuda"), F32)
     for t in (0, T // 2, T - 3, T - 2, T - 1):
         assert torch.equal(y[t].cpu(), w.float().cpu() @ x[t].float().cpu()), t
+
+
+def test_out_and_autograd(ft):
+    """A tensor written through out= has changed for autograd too; one that
+    requires a gradient is refused there, as torch's own out= are."""
+    a = inputs(4, 20, 16, 2, 4, BF16, 13)
+    out = torch.ones(4, 20, device="cuda")
+    leaf = torch.ones(4, 20, device="cuda", requires_grad=True)
+    product = (leaf * out).sum()  # keeps `out` for its gradient
+    ft.adapter_logits(**a, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.backward()
+    with pytest.raises(ValueError, match="requires a gradient"):
+        ft.adapter_logits(**a, out=leaf)
+    with torch.no_grad():
+        assert torch.equal(ft.adapter_logits(**a, out=leaf), ft.adapter_logits(**a, out_dtype=F32))
