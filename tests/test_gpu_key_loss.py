@@ -500,3 +500,27 @@ def test_a_row_of_nothing(ft, C, V):
     want.index_add_(0, a["tokens"][1, :, 1].long(), torch.full((C,), -0.5 * 0.25 / C).double())
     # a pair's slope rounds a few times, up to C of them are summed
     assert ((d[1, 1].double().cpu() - want).abs() <= (C + 8) * ref.U * want.abs()).all()
+
+
+# rows of a key each: of a workgroup's registers, or in parts, where each
+# block decides whether the row's token is in its span
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [4097, 8193, 20001, 32769, 50021, 65537, 131073])
+def test_rows_of_a_key_each(ft, dtype, V):
+    R, S = 7, 4
+    span = 4096 if dtype == F32 else 8192  # logits of a block of the gradient
+    at = [0, span - 1, span, 2 * span - 1, 2 * span, V - 1, V - 2, (V - 1) // span * span, V // 2]
+    tokens = torch.tensor([t % V for t in at] * 4)[:R * S].view(R, 1, S).to(torch.int32)
+    a = policy_case(R, S, V, 1, dtype, V)
+    lp = ref.scores(a["logits"].double(), tokens, torch.full((R, 1), S))
+    a["tokens"] = tokens
+    a["lengths"] = torch.tensor([4, 0, 1, 4, 3, 2, 4], dtype=torch.int32)[:, None]
+    a["old_logp"], a["ref_logp"] = (lp - 0.1).float(), (lp + 0.2).float()
+    check_policy(ft, a, what="policy")
+    b = preference_case(R, S, V, 1, 9, dtype, V)
+    b.update(tokens=tokens, lengths=a["lengths"], ref_logp=lp.sum(-1).float() * 0.9)
+    check_preference(ft, b, what="preference")
+    # no gradient wanted
+    gpu = {k: v.cuda() for k, v in a.items()}
+    full, alone = (ft.policy_loss(**gpu, kl_coef=0.05, grad=g) for g in (True, False))
+    assert torch.equal(full[0], alone[0]) and torch.equal(full[1], alone[1])
