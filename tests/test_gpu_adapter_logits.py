@@ -237,3 +237,59 @@ def test_out_and_autograd(ft):
         ft.adapter_logits(**a, out=leaf)
     with torch.no_grad():
         assert torch.equal(ft.adapter_logits(**a, out=leaf), ft.adapter_logits(**a, out_dtype=F32))
+
+
+@pytest.mark.parametrize("T,V,H,G,r", [(8, 32768, 512, 4, 8), (84, 20011, 1024, 6, 12),
+                                       (16, 40000, 512, 2, 16), (600, 4099, 256, 16, 64),
+                                       (1024, 2048, 320, 40, 16)])
+@pytest.mark.parametrize("out", ["f32", "same"])
+def test_working_sizes_f16(ft, T, V, H, G, r, out):
+    a = inputs(T, V, H, G, r, F16, T)
+    check(ft, a, F32 if out == "f32" else F16, "working size")
+
+
+# few rows of a vocabulary past the tiles of 64 tokens
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,V,H,r", [(1, 49153, 512, 8), (16, 49153, 512, 11), (1, 50001, 64, 8),
+                                     (16, 50001, 1000, 16), (9, 65537, 192, 64)])
+def test_few_rows_large_vocabulary(ft, dtype, T, V, H, r):
+    check(ft, inputs(T, V, H, 3, r, dtype, T + V), F32, "few rows")
+
+
+# one row tile of three stages, from one step of 64 columns to sixteen
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T", [97, 112, 128])
+@pytest.mark.parametrize("H", [64, 128, 192, 256, 1000])
+@pytest.mark.parametrize("r", [8, 11, 40])
+def test_128_rows(ft, dtype, T, H, r):
+    check(ft, inputs(T, 777, H, 4, r, dtype, T + H), F32, "128 rows")
+
+
+# the tiles of 256 rows by 256 tokens: steps odd and even, the vocabulary's
+# last tile on the one before it, ranks of whole vectors and not
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T", [129, 300, 600])
+@pytest.mark.parametrize("V", [256, 257, 4099])
+@pytest.mark.parametrize("H,r", [(64, 8), (64, 11), (128, 11), (128, 64), (192, 8), (256, 40)])
+def test_large_tiles(ft, dtype, T, V, H, r):
+    a = inputs(T, V, H, 5, r, dtype, T + V + H)
+    check(ft, a, F32, "large tiles")
+    check(ft, a, dtype, "large tiles")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("r", [8, 11])
+def test_large_tiles_adapters(ft, dtype, r):
+    """Adapters out of range, and one of NaN and infinities, stay in their
+    rows."""
+    T, V, H = 290, 600, 128
+    adapter = torch.arange(T) % 5 - 1
+    adapter[[0, 77, 255, 256, 289]] = torch.tensor([4, 2 ** 31 - 1, 9, 4, 5])
+    a = inputs(T, V, H, 4, r, dtype, 14, adapter)
+    clean = check(ft, a, F32, "out of range")
+    a["up"][1] = math.nan
+    a["down"][2] = math.inf
+    y = ft.adapter_logits(**a, out_dtype=F32)
+    sick = ((adapter == 1) | (adapter == 2)).cuda()
+    assert y[sick].isnan().all()
+    assert torch.equal(y[~sick].nan_to_num(7.0), clean[~sick].nan_to_num(7.0))
