@@ -14,11 +14,15 @@
 //                   the product of z by its up.  Inputs of any alignment; of
 //                   whole 16-byte vectors; the same with many rows
 //
-// Up to about 250 rows one read of w bounds it: 16 rows, 2,200,000 x 512
-// bf16: 479 us, 5.1 TB/s; 84 rows, 262,144 x 1024, 6 adapters of rank 12 in
-// no order: 175 us, 3.5 TB/s, with the adapters' turns (no adapters: 132).
-// Above, the matrix cores do: 4096 rows, 32,768 x 1024 f16, 16 adapters of
-// rank 64: 384 us, 0.76 PFLOP/s counting the adapters' products once.
+// Up to 96 rows one read of w bounds it: 16 rows, 2,200,000 x 512 bf16: 481
+// us, 5.1 TB/s; 84 rows, 262,144 x 1024, 6 adapters of rank 12 in no order:
+// 172 us, 3.5 TB/s, with the adapters' turns (no adapters: 132).  From 97 to
+// 250 rows of that size neither memory (125-140 us of bytes) nor the matrix
+// cores do: 112 rows take 205 us (no adapters: 149) with one workgroup on a CU,
+// whose adapters' turns nothing hides, 144 to 250 rows 241-255 us in tiles of
+// 256 rows that are part empty.  Above, the matrix cores do: 4096 rows, 32,768
+// x 1024 f16, 16 adapters of rank 64: 378 us, 0.77 PFLOP/s counting the
+// adapters' products once.
 #include <algorithm>
 
 #include "op_device.h"
@@ -547,7 +551,9 @@ __device__ __forceinline__ void store_rows(const Args& a, const Rows<kBM>& tile,
 
 constexpr int kBK = 64;  // hidden columns of a step: a line of a row
 
-// Any alignment (4096 x 32768 x 1024: 794 us, where logits_tile takes 336).
+// Any alignment: operands pass registers on their way to LDS, by loads that
+// straddle lines, and no step is ahead (4096 x 32768 x 1024, 8 adapters of rank
+// 16: 867 us, where logits_tile takes 343).
 // Block: rows [64 m, ...) of the order by tokens [128 n,
 // ...); wave w has tokens 32 w ... 32 w + 31 of them, and all rows.
 constexpr int kBM = 64, kBN = 128, kThreads = 256;
@@ -755,8 +761,8 @@ __global__ void __launch_bounds__(S::Threads) logits_staged(Args a) {
 // kBNs tokens, steps of a line (64 hidden columns) in two LDS stages.  The
 // operands of a half step are read from LDS during the matrix instructions
 // of the half before, so that past a barrier there is work at once.  4096 x
-// 32768 x 1024 bf16, 8 adapters of rank 16: 336 us (as tiles of 256 x 128 of
-// logits_staged: 451); without adapters 302, 0.91 PFLOP/s, where the clock
+// 32768 x 1024 bf16, 8 adapters of rank 16: 343 us (as tiles of 256 x 128 of
+// logits_staged: 451); without adapters 304, 0.90 PFLOP/s, where the clock
 // under load is the bound.
 template <int kBMs, int kBNs, int kWM, int kWN>
 struct TileShape {

@@ -22,10 +22,11 @@
 //
 // Bound by the logits: read twice (the second time mostly from the last
 // level's cache) and the gradient written, 128 rows x 262,144 bf16 with 1000
-// keys a request: 52 us, of them 17 the statistics at 3.9 TB/s, 12 the rows'
-// tables and 23 the gradient at 5.9 TB/s; or read once by key_whole, 2048
-// rows x 32,768 bf16: 44 us, 6.0 TB/s.  Few rows are bound by latency: 8 rows
-// x 32,768 f32, 10 keys: 17 us for 2 MB.
+// keys a request: 56 us a call; in a trace 17 the statistics at 3.9 TB/s, 12
+// the rows' tables and 23 the gradient at 5.9 TB/s; or read once by key_whole,
+// 2048 rows x 32,768 bf16: 58 us a call on new inputs, 4.7 TB/s (in a trace,
+// with a part of the logits in the last level's cache, 44).  Few rows are bound
+// by latency: 8 rows x 32,768 f32, 10 keys: 16 us for 2 MB.
 #include <type_traits>
 
 #include "op_device.h"
@@ -236,6 +237,8 @@ __global__ void __launch_bounds__(256) key_scores(Args a) {
 
 // Wave w of a workgroup takes the pairs of its share in their order, one at
 // a time for its 64 keys, a key a lane; the waves' sums are added in order.
+// So its time goes with keys times pairs: 96 rows x 262,144 bf16, 8000 keys:
+// the whole call 57 us with 400 pairs, 84 with 4000, 304 with 32,000.
 __global__ void __launch_bounds__(1024) key_pairs(Args a) {
   __shared__ float sums[16][64];
   __shared__ float waves[16];
