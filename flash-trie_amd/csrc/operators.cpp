@@ -67,7 +67,8 @@ const char* wrong(const ft_adapter_logits_args& a, int* code) {
   if (!a.hidden || !a.vocab) return "hidden and vocab must be at least 1";
   if (a.adapters && !a.rank) return "rank must be at least 1";
   *code = FT_E_LIMIT;
-  if (a.adapters > 0x7FFFFFFEu || a.rank > FT_MAX_RANK) return "rank must be at most 256";
+  if (a.rank > FT_MAX_RANK) return "rank must be at most 256";
+  if (a.adapters > 0x7FFFFFFEu) return "too many adapters";
   if (a.vocab > FT_MAX_HEAD_VOCAB) return "vocab must be at most 2^24";
   if (a.hidden > (1u << 24)) return "hidden must be at most 2^24";
   // (the launches: 1024 threads for 16 rows; tiles of 128 tokens by 64 rows

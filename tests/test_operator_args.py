@@ -282,3 +282,8 @@ def test_launch_limits(lib, name, most, more, text):
     if name == "policy_loss":  # without the gradient there is no such launch
         a = CALLS[name](**more, dlogits=None)
         assert getattr(lib, f"ft_{name}_workspace")(C.byref(a)) > 0
+
+
+def test_too_many_adapters(lib):
+    rc, need, message = call(lib, "adapter_logits", logits(adapters=(1 << 31) - 1))
+    assert (rc, need) == (E_LIMIT, 0) and message.endswith("too many adapters")
