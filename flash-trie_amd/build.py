@@ -114,6 +114,9 @@ def build(verbose=False):
         "adapter_logits.hip": os.path.join(OBJ, "adapter_logits.o"),
         "propose.hip": os.path.join(OBJ, "propose.o"),
         "key_loss.hip": os.path.join(OBJ, "key_loss.o"),
+        "cross_entropy.hip": os.path.join(OBJ, "cross_entropy.o"),
+        "packed_logits.hip": os.path.join(OBJ, "packed_logits.o"),
+        "embed.hip": os.path.join(OBJ, "embed.o"),
         "operators.cpp": os.path.join(OBJ, "operators.o"),
     }
     host_objs = {

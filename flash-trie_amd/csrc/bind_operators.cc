@@ -91,7 +91,7 @@ py::object attr(py::handle self, PyObject* name) {
   return py::reinterpret_steal<py::object>(r);
 }
 
-constexpr int kMaxDims = 3;
+constexpr int kMaxDims = 4;
 
 struct Tensor {
   py::object obj;  // kept alive during the call
@@ -241,6 +241,31 @@ void launch(const A& a, int device, const Tensor& like, const char* call,
 
 uint32_t u32(int64_t v) { return v > 0xFFFFFFFFll ? 0xFFFFFFFFu : (uint32_t)v; }
 
+// `out` of a call that writes logits [rows, vocab], or a new tensor for them.
+Tensor logits_out(Reader& in, const Tensor& x, int64_t T, int64_t V, py::handle out_dtype,
+                  py::handle out, int* odt) {
+  const Torch& t = torch();
+  if (!out.is_none()) {
+    const Tensor to = in.rows(out, "out", 2, odt);
+    if (to.size[0] != T || to.size[1] != V) fail_value(in.call, "out must be [rows, vocab]");
+    if (!out_dtype.is_none() && !out_dtype.is(t.dtypes[*odt]))
+      fail_type(in.call, "out is not of out_dtype");
+    // (as torch's own out= do: no gradient passes the call)
+    if (attr(to.obj, t.requires_grad).is(py::bool_(true)) && py::cast<bool>(t.grad_enabled()))
+      fail_value(in.call, "out requires a gradient, which the call does not have");
+    return to;
+  }
+  if (!out_dtype.is_none()) {
+    const int dt = *odt;
+    *odt = -1;
+    for (int i = 0; i < 3; ++i)
+      if (out_dtype.is(t.dtypes[i])) *odt = i;
+    if (*odt != FT_F32 && *odt != dt)
+      fail_type(in.call, "out_dtype must be float32 or the inputs' type");
+  }
+  return make(x, {T, V}, t.dtypes[*odt]);
+}
+
 py::object adapter_logits(py::object x, py::object weight, py::object down, py::object up,
                           py::object adapter, py::object scale, py::object out_dtype,
                           py::object out) {
@@ -261,26 +286,8 @@ py::object adapter_logits(py::object x, py::object weight, py::object down, py::
     fail_value(in.call, "up must be [adapters, vocab, rank] of down and weight");
   const Tensor ta = in.array(adapter, "adapter", t.int32, "int32", {T});
   const Tensor ts = in.array(scale, "scale", t.dtypes[FT_F32], "float32", {G});
-  Tensor to;
   int odt = dt;
-  if (!out.is_none()) {
-    to = in.rows(out, "out", 2, &odt);
-    if (to.size[0] != T || to.size[1] != V) fail_value(in.call, "out must be [rows, vocab]");
-    if (!out_dtype.is_none() && !out_dtype.is(t.dtypes[odt]))
-      fail_type(in.call, "out is not of out_dtype");
-    // (as torch's own out= do: no gradient passes the call)
-    if (attr(to.obj, t.requires_grad).is(py::bool_(true)) && py::cast<bool>(t.grad_enabled()))
-      fail_value(in.call, "out requires a gradient, which the call does not have");
-  } else {
-    if (!out_dtype.is_none()) {
-      odt = -1;
-      for (int i = 0; i < 3; ++i)
-        if (out_dtype.is(t.dtypes[i])) odt = i;
-    }
-    if (odt != FT_F32 && odt != dt)
-      fail_type(in.call, "out_dtype must be float32 or the inputs' type");
-    to = make(tx, {T, V}, t.dtypes[odt]);
-  }
+  const Tensor to = logits_out(in, tx, T, V, out_dtype, out, &odt);
   ft_adapter_logits_args a{};
   a.device = in.device;
   a.dtype = dt;
@@ -422,6 +429,211 @@ py::tuple preference_loss(py::object logits, py::object tokens, py::object lengt
   return results(q, grad);
 }
 
+py::tuple cross_entropy_loss(py::object x, py::object weight, py::object targets,
+                             py::object row_weight, double smoothing, bool grad,
+                             bool weight_grad) {
+  const Torch& t = torch();
+  Reader in{"cross_entropy_loss"};
+  ft_cross_entropy_loss_args a{};
+  int d;
+  const Tensor tx = in.rows(x, "x", 2, &a.dtype), tw = in.rows(weight, "weight", 2, &d);
+  if (d != a.dtype) fail_type(in.call, "weight must be of x's type");
+  if (a.dtype == FT_F32) fail_type(in.call, "x must be float16 or bfloat16");
+  const int64_t T = tx.size[0], H = tx.size[1], V = tw.size[0];
+  if (tw.size[1] != H) fail_value(in.call, "weight and x differ in their hidden size");
+  const Tensor tt = in.array(targets, "targets", t.int32, "int32", {T});
+  const Tensor tr = in.array(row_weight, "row_weight", t.dtypes[FT_F32], "float32", {T});
+  const Tensor loss = make(tx, {}, t.dtypes[FT_F32]), logp = make(tx, {T}, t.dtypes[FT_F32]);
+  Tensor dx, dw;
+  if (grad) dx = make(tx, {T, H}, t.dtypes[a.dtype]);
+  if (grad && weight_grad) dw = make(tx, {V, H}, t.dtypes[a.dtype]);
+  a.device = in.device;
+  a.rows = (uint64_t)T;
+  a.hidden = u32(H);
+  a.vocab = u32(V);
+  a.x = tx.data;
+  a.x_stride = tx.step[0];
+  a.weight = tw.data;
+  a.weight_stride = tw.step[0];
+  a.target = (const int32_t*)tt.data;
+  a.row_weight = (const float*)tr.data;
+  a.smoothing = (float)smoothing;
+  a.loss = (float*)loss.data;
+  a.logp = (float*)logp.data;
+  a.dx = dx.data;
+  a.dx_stride = a.dweight_stride = H;
+  a.dweight = dw.data;
+  launch(a, in.device, tx, "cross_entropy_loss", ft_cross_entropy_loss_workspace,
+         ft_cross_entropy_loss);
+  return py::make_tuple(loss.obj, logp.obj, grad ? dx.obj : py::none(),
+                        grad && weight_grad ? dw.obj : py::none());
+}
+
+py::tuple pack_weight(py::object weight, int64_t group) {
+  const Torch& t = torch();
+  Reader in{"pack_weight"};
+  ft_pack_weight_args a{};
+  const Tensor w = in.rows(weight, "weight", 2, &a.dtype);
+  if (a.dtype == FT_F32) fail_type(in.call, "weight must be float16 or bfloat16");
+  if (group != 32 && group != 64 && group != 128) fail_value(in.call, "group must be 32, 64 or 128");
+  const int64_t tiles = (w.size[0] + 15) / 16, chunks = (w.size[1] + 127) / 128;
+  const Tensor packed = make(w, {tiles, chunks, 64, 16}, t.uint8);
+  const Tensor scales = make(w, {tiles, chunks, 16, 128 / group}, t.dtypes[a.dtype]);
+  a.device = in.device;
+  a.hidden = u32(w.size[1]);
+  a.vocab = u32(w.size[0]);
+  a.group = (uint32_t)group;
+  a.weight = w.data;
+  a.weight_stride = w.step[0];
+  a.packed = packed.data;
+  a.scales = scales.data;
+  launch(a, in.device, w, "pack_weight", ft_pack_weight_workspace, ft_pack_weight);
+  return py::make_tuple(packed.obj, scales.obj);
+}
+
+py::object packed_logits(py::object x, py::object packed, py::object scales, int64_t vocab,
+                         py::object out_dtype, py::object out) {
+  const Torch& t = torch();
+  Reader in{"packed_logits"};
+  ft_packed_logits_args a{};
+  int d;
+  const Tensor tx = in.rows(x, "x", 2, &a.dtype);
+  if (a.dtype == FT_F32) fail_type(in.call, "x must be float16 or bfloat16");
+  const int64_t T = tx.size[0], H = tx.size[1], chunks = (H + 127) / 128;
+  if (vocab < 1) fail_value(in.call, "vocab must be at least 1");
+  const int64_t tiles = vocab / 16 + (vocab % 16 != 0);
+  const Tensor tp = in.array(packed, "packed", t.uint8, "uint8", {tiles, chunks, 64, 16});
+  const int64_t per = in.read(scales, "scales", 4, &d).size[3];
+  if (d != a.dtype) fail_type(in.call, "scales must be of x's type");
+  if (per != 1 && per != 2 && per != 4)
+    fail_value(in.call, "scales must be [tiles, chunks, 16, 128 / group], group 32, 64 or 128");
+  const Tensor ts = in.array(scales, "scales", t.dtypes[a.dtype], "of x's type",
+                             {tiles, chunks, 16, per});
+  a.out_dtype = a.dtype;
+  const Tensor to = logits_out(in, tx, T, vocab, out_dtype, out, &a.out_dtype);
+  a.device = in.device;
+  a.rows = (uint64_t)T;
+  a.hidden = u32(H);
+  a.vocab = u32(vocab);
+  a.group = (uint32_t)(128 / per);
+  a.x = tx.data;
+  a.x_stride = tx.step[0];
+  a.packed = tp.data;
+  a.scales = ts.data;
+  a.out = to.data;
+  a.out_stride = to.step[0];
+  if (!out.is_none()) t.written(to.obj);  // for autograd: its values change
+  launch(a, in.device, tx, "packed_logits", ft_packed_logits_workspace, ft_packed_logits);
+  return to.obj;
+}
+
+// Tokens of one to three dimensions, their steps in the last, and lengths of
+// the others.
+struct Tokens {
+  Tensor tokens, lengths;
+  int64_t groups = 1, steps;
+};
+Tokens read_tokens(Reader& in, py::handle tokens, py::handle lengths) {
+  const Torch& t = torch();
+  Tokens q;
+  const int dims = py::hasattr(tokens, "dim") ? py::cast<int>(tokens.attr("dim")()) : 1;
+  if (dims < 1 || dims > 3) fail_value(in.call, "tokens must have 1 to 3 dimensions");
+  const Tensor shape = in.read(tokens, "tokens", dims);
+  const int64_t* n = shape.size;
+  q.tokens = dims == 1   ? in.array(tokens, "tokens", t.int32, "int32", {n[0]})
+             : dims == 2 ? in.array(tokens, "tokens", t.int32, "int32", {n[0], n[1]})
+                         : in.array(tokens, "tokens", t.int32, "int32", {n[0], n[1], n[2]});
+  for (int i = 0; i + 1 < dims; ++i) q.groups *= n[i];
+  q.steps = n[dims - 1];
+  if (!lengths.is_none()) {
+    if (dims == 1) fail_value(in.call, "lengths need tokens of 2 or 3 dimensions");
+    q.lengths = dims == 2 ? in.array(lengths, "lengths", t.int32, "int32", {n[0]})
+                          : in.array(lengths, "lengths", t.int32, "int32", {n[0], n[1]});
+  }
+  return q;
+}
+
+py::object embed(py::object tokens, py::object table, double scale, py::object lengths) {
+  const Torch& t = torch();
+  Reader in{"embed"};
+  ft_embed_args a{};
+  const Tensor w = in.rows(table, "table", 2, &a.dtype);
+  const Tokens q = read_tokens(in, tokens, lengths);
+  const int64_t H = w.size[1], *n = q.tokens.size;
+  const py::object& dt = t.dtypes[a.dtype];
+  const Tensor out = q.tokens.ndim == 1   ? make(w, {n[0], H}, dt)
+                     : q.tokens.ndim == 2 ? make(w, {n[0], n[1], H}, dt)
+                                          : make(w, {n[0], n[1], n[2], H}, dt);
+  a.device = in.device;
+  a.groups = (uint64_t)q.groups;
+  a.steps = (uint64_t)q.steps;
+  a.hidden = u32(H);
+  a.vocab = u32(w.size[0]);
+  a.tokens = (const int32_t*)q.tokens.data;
+  a.lengths = (const int32_t*)q.lengths.data;
+  a.table = w.data;
+  a.table_stride = w.step[0];
+  a.scale = (float)scale;
+  a.out = out.data;
+  launch(a, in.device, w, "embed", ft_embed_workspace, ft_embed);
+  return out.obj;
+}
+
+py::object embed_grad(py::object grad, py::object tokens, int64_t vocab, double scale,
+                      py::object lengths, py::object out) {
+  const Torch& t = torch();
+  Reader in{"embed_grad"};
+  ft_embed_grad_args a{};
+  const Tokens q = read_tokens(in, tokens, lengths);
+  const int dims = q.tokens.ndim;
+  Tensor g = in.rows(grad, "grad", dims + 1, &a.dtype);
+  for (int i = 0; i < dims; ++i)
+    if (g.size[i] != q.tokens.size[i]) fail_value(in.call, "grad must be [tokens' sizes, hidden]");
+  // one stride from token to token, or a copy that has one
+  int64_t step = 0, want = 0;
+  bool even = true;
+  for (int i = dims - 1; i >= 0; --i) {
+    if (g.size[i] <= 1) continue;
+    if (!step) step = want = g.step[i];
+    even = even && g.step[i] == want;
+    want *= g.size[i];
+  }
+  if (!even) {
+    g.obj = call0(g.obj, t.contiguous);
+    g.data = (void*)PyLong_AsUnsignedLongLong(call0(g.obj, t.data_ptr).ptr());
+    step = g.size[dims];
+  }
+  if (vocab < 1) fail_value(in.call, "vocab must be at least 1");
+  const int64_t H = g.size[dims];
+  Tensor to;
+  if (!out.is_none()) {
+    int d;
+    to = in.rows(out, "out", 2, &d);
+    if (d != a.dtype) fail_type(in.call, "out must be of grad's type");
+    if (to.size[0] != vocab || to.size[1] != H) fail_value(in.call, "out must be [vocab, hidden]");
+    if (attr(to.obj, t.requires_grad).is(py::bool_(true)) && py::cast<bool>(t.grad_enabled()))
+      fail_value(in.call, "out requires a gradient, which the call does not have");
+  } else {
+    to = make(g, {vocab, H}, t.dtypes[a.dtype]);
+  }
+  a.device = in.device;
+  a.groups = (uint64_t)q.groups;
+  a.steps = (uint64_t)q.steps;
+  a.hidden = u32(H);
+  a.vocab = u32(vocab);
+  a.tokens = (const int32_t*)q.tokens.data;
+  a.lengths = (const int32_t*)q.lengths.data;
+  a.grad = g.data;
+  a.grad_stride = step;
+  a.scale = (float)scale;
+  a.add = !out.is_none();
+  a.dtable = to.data;
+  a.dtable_stride = to.step[0];
+  if (!out.is_none()) t.written(to.obj);  // for autograd: its values change
+  launch(a, in.device, g, "embed_grad", ft_embed_grad_workspace, ft_embed_grad);
+  return to.obj;
+}
+
 }  // namespace
 
 void bind_operators(py::module_& m) {
@@ -451,4 +663,28 @@ void bind_operators(py::module_& m) {
         "(loss, logp, dlogits): the loss of pairs [n, 2] (int32 indexes into batch * keys: the "
         "preferred key, the other) on their log-probability ratios to ref_logp [batch, keys]; "
         "weight [n]; the rest as in policy_loss.");
+  m.def("cross_entropy_loss", &cross_entropy_loss, py::arg("x"), py::arg("weight"),
+        py::arg("targets"), py::arg("row_weight"), py::arg("smoothing") = 0.0,
+        py::arg("grad") = true, py::arg("weight_grad") = true,
+        "(loss, logp, dx, dweight): the cross entropy of targets [rows] (int32, negative: none) "
+        "under the softmax of x [rows, hidden] weight^T [vocab, hidden], summed with row_weight "
+        "[rows] and label smoothing; logp [rows] are the targets' log-probabilities, dx and "
+        "dweight the gradients of the inputs' type (None without grad, dweight also without "
+        "weight_grad).  float16 or bfloat16 tensors; the logits are never stored.");
+  m.def("pack_weight", &pack_weight, py::arg("weight"), py::arg("group") = 32,
+        "(packed, scales): weight [vocab, hidden] in 4 bits, a scale of its type for each group "
+        "of 32, 64 or 128 neighbouring columns, laid out for packed_logits.");
+  m.def("packed_logits", &packed_logits, py::arg("x"), py::arg("packed"), py::arg("scales"),
+        py::arg("vocab"), py::arg("out_dtype") = py::none(), py::arg("out") = py::none(),
+        "Logits [rows, vocab] of x [rows, hidden] by a table that pack_weight packed.  float16 or "
+        "bfloat16 x of the scales' type; sums in 32 bits; out_dtype is x's type or float32.");
+  m.def("embed", &embed, py::arg("tokens"), py::arg("table"), py::arg("scale") = 1.0,
+        py::arg("lengths") = py::none(),
+        "scale table[tokens]: rows of table [vocab, hidden] for tokens (int32) of 1 to 3 "
+        "dimensions; 0 for a negative token and, with lengths of the tokens' leading dimensions, "
+        "past a key's length.");
+  m.def("embed_grad", &embed_grad, py::arg("grad"), py::arg("tokens"), py::arg("vocab"),
+        py::arg("scale") = 1.0, py::arg("lengths") = py::none(), py::arg("out") = py::none(),
+        "The gradient [vocab, hidden] of embed's table from grad [tokens' sizes, hidden]: each "
+        "token's rows summed in their order, in 32 bits, times scale; added to `out` if given.");
 }

@@ -159,10 +159,117 @@ const char* wrong(const ft_preference_loss_args& a, int* code) {
   return nullptr;
 }
 
+const char* wrong(const ft_cross_entropy_loss_args& a, int* code) {
+  *code = FT_E_ARG;
+  if (a.dtype != FT_F16 && a.dtype != FT_BF16) return "x must be float16 or bfloat16";
+  if (!a.hidden || !a.vocab) return "hidden and vocab must be at least 1";
+  if (!(a.smoothing >= 0.0f && a.smoothing <= 1.0f)) return "smoothing must be in [0, 1]";
+  *code = FT_E_LIMIT;
+  if (a.vocab > FT_MAX_HEAD_VOCAB) return "vocab must be at most 2^24";
+  if (a.hidden > FT_MAX_TABLE_HIDDEN) return "hidden must be at most 2^16";
+  // (the launches: 256 threads for 4 rows; for tiles of 128 tokens, or hidden
+  // columns, by 64 rows, or tokens)
+  if (a.rows > FT_MAX_TABLE_ROWS ||
+      ceil_div(a.vocab, 128) * ceil_div(a.rows, 64) * 256 > kMaxThreads ||
+      ceil_div(a.hidden, 128) * ceil_div(a.vocab + 256ull, 64) * 256 > kMaxThreads)
+    return "too many rows";
+  *code = FT_E_ARG;
+  if (!a.loss) return "null pointer";
+  if (a.rows && (!a.x || !a.weight || !a.target || !a.row_weight || !a.logp)) return "null pointer";
+  if (a.dx && a.rows > 1 && a.dx_stride < (int64_t)a.hidden) return "rows of dx overlap";
+  if (a.dweight && a.vocab > 1 && a.dweight_stride < (int64_t)a.hidden)
+    return "rows of dweight overlap";
+  return nullptr;
+}
+
+// The packed table's own sizes.
+const char* wrong_table(uint32_t hidden, uint32_t vocab, uint32_t group, int* code) {
+  *code = FT_E_ARG;
+  if (!hidden || !vocab) return "hidden and vocab must be at least 1";
+  if (group != 32 && group != 64 && group != 128) return "group must be 32, 64 or 128";
+  *code = FT_E_LIMIT;
+  if (vocab > FT_MAX_HEAD_VOCAB) return "vocab must be at most 2^24";
+  if (hidden > FT_MAX_TABLE_HIDDEN) return "hidden must be at most 2^16";
+  // (pack_weight: 64 threads for 16 tokens by 128 columns)
+  if (ceil_div(vocab, 16) * ceil_div(hidden, 128) * 64 > kMaxThreads - 1024)
+    return "the table is too large";
+  return nullptr;
+}
+
+const char* wrong(const ft_pack_weight_args& a, int* code) {
+  *code = FT_E_ARG;
+  if (a.dtype != FT_F16 && a.dtype != FT_BF16) return "weight must be float16 or bfloat16";
+  if (const char* w = wrong_table(a.hidden, a.vocab, a.group, code)) return w;
+  *code = FT_E_ARG;
+  if (!a.weight || !a.packed || !a.scales) return "null pointer";
+  if ((uintptr_t)a.packed % 16 || (uintptr_t)a.scales % 8)
+    return "packed must be 16-byte aligned, scales 8-byte";
+  return nullptr;
+}
+
+const char* wrong(const ft_packed_logits_args& a, int* code) {
+  *code = FT_E_ARG;
+  if (a.dtype != FT_F16 && a.dtype != FT_BF16) return "x must be float16 or bfloat16";
+  if (a.out_dtype != FT_F32 && a.out_dtype != a.dtype)
+    return "the logits must be float32 or of x's type";
+  if (const char* w = wrong_table(a.hidden, a.vocab, a.group, code)) return w;
+  *code = FT_E_LIMIT;
+  if (a.rows > FT_MAX_TABLE_ROWS) return "too many rows";
+  *code = FT_E_ARG;
+  if (a.rows) {
+    if (!a.x || !a.packed || !a.scales || !a.out) return "null pointer";
+    if ((uintptr_t)a.packed % 16 || (uintptr_t)a.scales % 8)
+      return "packed must be 16-byte aligned, scales 8-byte";
+    if (a.out_stride < (int64_t)a.vocab && a.rows > 1) return "rows of the logits overlap";
+  }
+  return nullptr;
+}
+
+// Tokens of keys and the table of ft_embed and ft_embed_grad; `threads` for
+// 64 vectors of a token's row.
+const char* wrong_tokens(int dtype, uint64_t groups, uint64_t steps, uint32_t hidden, uint32_t vocab,
+                         uint64_t threads, int* code) {
+  *code = FT_E_ARG;
+  if (dtype != FT_F32 && dtype != FT_F16 && dtype != FT_BF16)
+    return "the table must be float32, float16 or bfloat16";
+  if (!hidden || !vocab) return "hidden and vocab must be at least 1";
+  *code = FT_E_LIMIT;
+  if (vocab > FT_MAX_HEAD_VOCAB) return "vocab must be at most 2^24";
+  if (hidden > FT_MAX_TABLE_HIDDEN) return "hidden must be at most 2^16";
+  if (groups > FT_MAX_TABLE_TOKENS || steps > FT_MAX_TABLE_TOKENS ||
+      groups * steps > FT_MAX_TABLE_TOKENS ||
+      (groups * steps + 32) * ceil_div(hidden, 64 * (dtype == FT_F32 ? 4 : 8)) * threads > kMaxThreads)
+    return "too many tokens";
+  return nullptr;
+}
+
+const char* wrong(const ft_embed_args& a, int* code) {
+  if (const char* w = wrong_tokens(a.dtype, a.groups, a.steps, a.hidden, a.vocab, 16, code)) return w;
+  *code = FT_E_ARG;
+  if (a.groups && a.steps && (!a.tokens || !a.table || !a.out)) return "null pointer";
+  return nullptr;
+}
+
+const char* wrong(const ft_embed_grad_args& a, int* code) {
+  // (a workgroup of 256 joins 32 positions, or 8 of up to 16384)
+  if (const char* w = wrong_tokens(a.dtype, a.groups, a.steps, a.hidden, a.vocab,
+                                   a.groups * a.steps < 16384 ? 32 : 8, code))
+    return w;
+  *code = FT_E_ARG;
+  if (!a.dtable || (a.groups && a.steps && (!a.tokens || !a.grad))) return "null pointer";
+  if (a.vocab > 1 && a.dtable_stride < (int64_t)a.hidden) return "rows of the gradient overlap";
+  return nullptr;
+}
+
 int device_of(const ft_adapter_logits_args& a) { return a.device; }
 int device_of(const ft_propose_args& a) { return a.device; }
 int device_of(const ft_policy_loss_args& a) { return a.k.device; }
 int device_of(const ft_preference_loss_args& a) { return a.k.device; }
+int device_of(const ft_cross_entropy_loss_args& a) { return a.device; }
+int device_of(const ft_pack_weight_args& a) { return a.device; }
+int device_of(const ft_packed_logits_args& a) { return a.device; }
+int device_of(const ft_embed_args& a) { return a.device; }
+int device_of(const ft_embed_grad_args& a) { return a.device; }
 
 template <typename A>
 size_t workspace(const A* a, uint64_t (*size)(const A&)) {
@@ -223,6 +330,46 @@ size_t ft_preference_loss_workspace(const ft_preference_loss_args* a) {
 int ft_preference_loss(const ft_preference_loss_args* a, void* ws, size_t n, void* stream) {
   return run(a, ws, n, stream, "ft_preference_loss", fto::preference_loss_workspace,
              fto::launch_preference_loss);
+}
+
+size_t ft_cross_entropy_loss_workspace(const ft_cross_entropy_loss_args* a) {
+  return workspace(a, fto::cross_entropy_loss_workspace);
+}
+int ft_cross_entropy_loss(const ft_cross_entropy_loss_args* a, void* ws, size_t n, void* stream) {
+  return run(a, ws, n, stream, "ft_cross_entropy_loss", fto::cross_entropy_loss_workspace,
+             fto::launch_cross_entropy_loss);
+}
+
+size_t ft_pack_weight_workspace(const ft_pack_weight_args* a) {
+  return workspace(a, fto::pack_weight_workspace);
+}
+int ft_pack_weight(const ft_pack_weight_args* a, void* ws, size_t n, void* stream) {
+  return run(a, ws, n, stream, "ft_pack_weight", fto::pack_weight_workspace,
+             fto::launch_pack_weight);
+}
+
+size_t ft_packed_logits_workspace(const ft_packed_logits_args* a) {
+  return workspace(a, fto::packed_logits_workspace);
+}
+int ft_packed_logits(const ft_packed_logits_args* a, void* ws, size_t n, void* stream) {
+  return run(a, ws, n, stream, "ft_packed_logits", fto::packed_logits_workspace,
+             fto::launch_packed_logits);
+}
+
+size_t ft_embed_workspace(const ft_embed_args* a) {
+  return workspace(a, fto::embed_workspace);
+}
+int ft_embed(const ft_embed_args* a, void* ws, size_t n, void* stream) {
+  return run(a, ws, n, stream, "ft_embed", fto::embed_workspace,
+             fto::launch_embed);
+}
+
+size_t ft_embed_grad_workspace(const ft_embed_grad_args* a) {
+  return workspace(a, fto::embed_grad_workspace);
+}
+int ft_embed_grad(const ft_embed_grad_args* a, void* ws, size_t n, void* stream) {
+  return run(a, ws, n, stream, "ft_embed_grad", fto::embed_grad_workspace,
+             fto::launch_embed_grad);
 }
 
 }  // extern "C"

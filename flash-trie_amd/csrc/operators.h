@@ -45,6 +45,21 @@ hipError_t launch_policy_loss(const ft_policy_loss_args& a, uint8_t* ws, hipStre
 uint64_t preference_loss_workspace(const ft_preference_loss_args& a);
 hipError_t launch_preference_loss(const ft_preference_loss_args& a, uint8_t* ws, hipStream_t s);
 
+uint64_t cross_entropy_loss_workspace(const ft_cross_entropy_loss_args& a);
+hipError_t launch_cross_entropy_loss(const ft_cross_entropy_loss_args& a, uint8_t* ws, hipStream_t s);
+
+uint64_t pack_weight_workspace(const ft_pack_weight_args& a);
+hipError_t launch_pack_weight(const ft_pack_weight_args& a, uint8_t* ws, hipStream_t s);
+
+uint64_t packed_logits_workspace(const ft_packed_logits_args& a);
+hipError_t launch_packed_logits(const ft_packed_logits_args& a, uint8_t* ws, hipStream_t s);
+
+uint64_t embed_workspace(const ft_embed_args& a);
+hipError_t launch_embed(const ft_embed_args& a, uint8_t* ws, hipStream_t s);
+
+uint64_t embed_grad_workspace(const ft_embed_grad_args& a);
+hipError_t launch_embed_grad(const ft_embed_grad_args& a, uint8_t* ws, hipStream_t s);
+
 }  // namespace fto
 
 namespace ftk {

@@ -287,6 +287,12 @@ int ft_device_info(ft_ctx* ctx, int* num_cus, int* lds_per_block,
  *   ft_policy_loss      a clipped policy loss with a KL term on the keys that
  *                       the search returned, and the logits' gradient
  *   ft_preference_loss  a loss on pairs of such keys, and the gradient
+ *   ft_cross_entropy_loss  hidden states and targets -> the loss of supervised
+ *                       training and its gradients, without the logits
+ *   ft_pack_weight, ft_packed_logits  the vocabulary's table in 4 bits, and
+ *                       logits by it
+ *   ft_embed, ft_embed_grad  keys' tokens -> their rows of the table, and the
+ *                       table's gradient
  *
  * Every pointer is device memory of `device` (or memory mapped for it).  A
  * call checks its arguments, launches on `stream` (a hipStream_t of that
@@ -315,6 +321,9 @@ const void* ft_hip_runtime(void);
 #define FT_MAX_HEAD_VOCAB (1 << 24) /* vocabulary of the head's operators */
 #define FT_MAX_PROPOSALS 4096      /* topk of ft_propose */
 #define FT_MAX_KEYS 4096           /* keys of a request in the losses */
+#define FT_MAX_TABLE_HIDDEN (1 << 16) /* hidden of the table's operators */
+#define FT_MAX_TABLE_ROWS (1 << 22)   /* rows of states of them */
+#define FT_MAX_TABLE_TOKENS (1 << 27) /* tokens of ft_embed, ft_embed_grad */
 
 /* out[t, v] = sum_h x[t, h] weight[v, h]
  *           + scale[g] sum_j up[g, v, j] sum_h down[g, j, h] x[t, h],
@@ -424,6 +433,132 @@ typedef struct ft_preference_loss_args {
 size_t ft_preference_loss_workspace(const ft_preference_loss_args* args);
 int ft_preference_loss(const ft_preference_loss_args* args, void* workspace,
                        size_t workspace_bytes, void* stream);
+
+/* loss = sum over rows with a target of row_weight *
+ *   ((1 - smoothing) (lse - l[target]) + smoothing (lse - mean l)),
+ * l[v] = sum_h x[t, h] weight[v, h], lse = log sum_v exp l[v].  Logits are
+ * made a tile at a time and never stored.  A row whose target is negative
+ * counts nothing and its x may hold anything; so does one of row_weight 0,
+ * but for logp.  A target at or above vocab makes the loss and the row's logp
+ * and dx NaN, and dweight too.  Logits, statistics and sums are held in 32
+ * bits; the logits' slopes are rounded to the inputs' type, of a factor in
+ * [1, 2) for float16 and bfloat16 alike, before the gradients' products. */
+typedef struct ft_cross_entropy_loss_args {
+  int device;
+  int dtype;                  /* of x, weight, dx, dweight: FT_F16 or FT_BF16 */
+  uint64_t rows;
+  uint32_t hidden, vocab;
+  const void* x;              /* [rows, hidden] */
+  int64_t x_stride;
+  const void* weight;         /* [vocab, hidden] */
+  int64_t weight_stride;
+  const int32_t* target;      /* [rows] */
+  const float* row_weight;    /* [rows] */
+  float smoothing;            /* in [0, 1] */
+  float* loss;                /* out [1] */
+  float* logp;                /* out [rows]: l[target] - lse, 0 without one */
+  void* dx;                   /* out [rows, hidden]; null: not wanted */
+  int64_t dx_stride;
+  void* dweight;              /* out [vocab, hidden]; null: not wanted */
+  int64_t dweight_stride;
+} ft_cross_entropy_loss_args;
+
+size_t ft_cross_entropy_loss_workspace(const ft_cross_entropy_loss_args* args);
+int ft_cross_entropy_loss(const ft_cross_entropy_loss_args* args, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* The table in 4 bits: weight[v, h] is about scale * (code - 8), a scale for
+ * `group` neighbouring columns of a token.  Of a group's weights a is the one
+ * of the largest magnitude (the first of equals); scale = a / -8, rounded to
+ * the weights' type, and code = the whole number next to w / scale (ties to
+ * even) + 8, from 0 to 15; codes of a scale of 0 are 8.  A group with a NaN or
+ * an infinity has a scale of NaN.
+ *
+ * Layout: tiles of 16 tokens by chunks of 128 columns; columns and tokens past
+ * the table's are codes of 8 and scales of 0.
+ *   packed [tiles][chunks][64][16 bytes]: of the 16 bytes of lane 16 q + n,
+ *     the 32-bit word i holds token n's columns 32 i + 8 q + j, j = 0 ... 7,
+ *     column j in the four bits from bit 4 ((j >> 1) + 4 (j & 1)) on
+ *   scales [tiles][chunks][16][128 / group] */
+typedef struct ft_pack_weight_args {
+  int device;
+  int dtype;                  /* of weight and scales: FT_F16 or FT_BF16 */
+  uint32_t hidden, vocab;
+  uint32_t group;             /* 32, 64 or 128 */
+  const void* weight;         /* [vocab, hidden] */
+  int64_t weight_stride;
+  void* packed;               /* ceil(vocab / 16) * ceil(hidden / 128) * 1024
+                                 bytes, 16-byte aligned */
+  void* scales;               /* the same * 2048 / group numbers, 8-byte
+                                 aligned */
+} ft_pack_weight_args;
+
+size_t ft_pack_weight_workspace(const ft_pack_weight_args* args);
+int ft_pack_weight(const ft_pack_weight_args* args, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/* out[t, v] = sum over groups of scale[v, g] sum_{h in g} x[t, h] (code[v, h] - 8).
+ * Sums in 32 bits. */
+typedef struct ft_packed_logits_args {
+  int device;
+  int dtype;                  /* of x and scales: FT_F16 or FT_BF16 */
+  int out_dtype;              /* FT_F32, or x's type */
+  uint64_t rows;
+  uint32_t hidden, vocab, group;
+  const void* x;              /* [rows, hidden] */
+  int64_t x_stride;
+  const void* packed;         /* as ft_pack_weight lays them out */
+  const void* scales;
+  void* out;                  /* [rows, vocab] */
+  int64_t out_stride;
+} ft_packed_logits_args;
+
+size_t ft_packed_logits_workspace(const ft_packed_logits_args* args);
+int ft_packed_logits(const ft_packed_logits_args* args, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* out[g, t] = scale * table[tokens[g, t]]: 0 for a negative token and at
+ * t >= lengths[g], NaN for a token at or above vocab. */
+typedef struct ft_embed_args {
+  int device;
+  int dtype;                  /* of table and out: FT_F32, FT_F16 or FT_BF16 */
+  uint64_t groups, steps;     /* groups of steps tokens: keys */
+  uint32_t hidden, vocab;
+  const int32_t* tokens;      /* [groups, steps] */
+  const int32_t* lengths;     /* [groups]; null: all tokens count */
+  const void* table;          /* [vocab, hidden] */
+  int64_t table_stride;
+  float scale;
+  void* out;                  /* [groups, steps, hidden], contiguous */
+} ft_embed_args;
+
+size_t ft_embed_workspace(const ft_embed_args* args);
+int ft_embed(const ft_embed_args* args, void* workspace, size_t workspace_bytes,
+             void* stream);
+
+/* dtable[v] = scale * the sum of grad[g, t] over the tokens that are v, in
+ * their order, in 32 bits, rounded once; 0 for a token that does not occur.
+ * With `add` the sum is added to what dtable holds, and rows of other tokens
+ * are left alone.  Tokens that ft_embed gives no row of the table to count
+ * nothing, and their grad is not read. */
+typedef struct ft_embed_grad_args {
+  int device;
+  int dtype;                  /* of grad and dtable */
+  uint64_t groups, steps;
+  uint32_t hidden, vocab;
+  const int32_t* tokens;      /* [groups, steps] */
+  const int32_t* lengths;     /* [groups]; null: all tokens count */
+  const void* grad;           /* [groups * steps, hidden] */
+  int64_t grad_stride;        /* of a token */
+  float scale;
+  int add;
+  void* dtable;               /* [vocab, hidden] */
+  int64_t dtable_stride;
+} ft_embed_grad_args;
+
+size_t ft_embed_grad_workspace(const ft_embed_grad_args* args);
+int ft_embed_grad(const ft_embed_grad_args* args, void* workspace,
+                  size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
