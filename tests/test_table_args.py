@@ -210,7 +210,7 @@ def test_workspaces_of_the_largest(lib):
                                 weight_stride=4096, dx_stride=4096, dweight_stride=4096))
     assert big > (1 << 22) * 4096 * 6
     assert need_of(lib, "packed_logits", packed(rows=1 << 22, hidden=4096)) >= (1 << 22) * 4096 * 2
-    n = need_of(lib, "embed_grad", embed_grad(groups=1 << 24, steps=8, hidden=256))
+    n = need_of(lib, "embed_grad", embed_grad(groups=1 << 24, steps=8, hidden=256, grad_stride=256, dtable_stride=256))
     assert n >= (1 << 27) * 16 + 2 * (1 << 22) * 256 * 4
 
 
