@@ -74,7 +74,8 @@ struct Args {
   void* slopes;     // [rows64][piece]
   float* dxs;       // [splits][rows64][hidden64]
   // a piece of the vocabulary
-  uint32_t piece, first, splits, split_steps;  // tokens of it; its first; parts of dx and their steps of 64
+  uint32_t piece, first, width;  // most tokens of it; its first; its tokens up to whole 256s
+  uint32_t splits, split_steps;  // parts of dx and their steps of 64
 };
 
 // --- rows -------------------------------------------------------------------
@@ -272,12 +273,14 @@ struct Stage {
   }
 };
 
-// What a product leaves.  The wave's i are i0 ..., 16 kN of them, its j j0 ...;
-// a lane has four neighbouring i of row j.
-template <typename T, Kind kKind, int kN, int kM, int kWaves>
-__device__ __forceinline__ void finish(const Args& a, uint32_t tile, uint32_t i0, uint32_t j0, uint32_t split,
-                                       f32x4 (&acc)[kN][kM], float (*joined)[3][16 * kM], uint32_t wave) {
-  const uint32_t lane = threadIdx.x & 63, col = lane & 15, q = lane >> 4;
+// What a product leaves.  The wave's i are i0 ..., 16 kN of them, its j jb + jw
+// ..., 16 kM of the workgroup's kB; a lane has four neighbouring i of row j.
+// Waves wn = 0 ... kWaves - 1 have other i of the same j.
+template <typename T, Kind kKind, int kN, int kM, int kWaves, int kB>
+__device__ __forceinline__ void finish(const Args& a, uint32_t tid, uint32_t tile, uint32_t i0, uint32_t jb,
+                                       uint32_t jw, uint32_t wn, uint32_t split, f32x4 (&acc)[kN][kM],
+                                       float (*joined)[3][kB]) {
+  const uint32_t lane = tid & 63, col = lane & 15, q = lane >> 4, j0 = jb + jw;
   if constexpr (kKind == kStats) {
 #pragma unroll
     for (int s = 0; s < kM; ++s) {
@@ -303,14 +306,14 @@ __device__ __forceinline__ void finish(const Args& a, uint32_t tile, uint32_t i0
         sum += __shfl_xor(sum, d, 64);
       }
       if (q == 0) {
-        joined[wave][0][s * 16 + col] = p.m;
-        joined[wave][1][s * 16 + col] = p.s;
-        joined[wave][2][s * 16 + col] = sum;
+        joined[wn][0][jw + s * 16 + col] = p.m;
+        joined[wn][1][jw + s * 16 + col] = p.s;
+        joined[wn][2][jw + s * 16 + col] = sum;
       }
     }
     __syncthreads();
     const uint64_t each = (uint64_t)a.tiles * a.rows64;
-    for (uint32_t j = threadIdx.x; j < 16 * kM; j += blockDim.x) {
+    for (uint32_t j = tid; j < kB && jb + j < a.rows64; j += blockDim.x) {
       MaxSum p{joined[0][0][j], joined[0][1][j]};
       float sum = joined[0][2][j];
 #pragma unroll
@@ -318,7 +321,7 @@ __device__ __forceinline__ void finish(const Args& a, uint32_t tile, uint32_t i0
         p = merge(p, MaxSum{joined[w][0][j], joined[w][1][j]});
         sum += joined[w][2][j];
       }
-      const uint64_t at = (uint64_t)tile * a.rows64 + j0 + j;
+      const uint64_t at = (uint64_t)tile * a.rows64 + jb + j;
       a.part[at] = p.m;
       a.part[each + at] = p.s;
       a.part[2 * each + at] = sum;
@@ -328,6 +331,7 @@ __device__ __forceinline__ void finish(const Args& a, uint32_t tile, uint32_t i0
     const float even = a.smoothing / (float)a.vocab, own = 1.0f - a.smoothing;
 #pragma unroll
     for (int s = 0; s < kM; ++s) {
+      if (j0 + s * 16 >= a.rows64) break;
       const uint32_t t = j0 + s * 16 + col;
       const int32_t y = t < a.rows ? a.target[t] : -1;
       const float m = a.mant[t] * kUp<T>, top = a.top[t], ls = a.logsum[t];
@@ -351,7 +355,8 @@ __device__ __forceinline__ void finish(const Args& a, uint32_t tile, uint32_t i0
   }
   if constexpr (kKind == kStates) {
 #pragma unroll
-    for (int s = 0; s < kM; ++s)
+    for (int s = 0; s < kM; ++s) {
+      if (j0 + s * 16 >= a.rows64) break;
 #pragma unroll
       for (int v = 0; v < kN; ++v) {
         const uint32_t h = i0 + v * 16 + q * 4;
@@ -359,6 +364,7 @@ __device__ __forceinline__ void finish(const Args& a, uint32_t tile, uint32_t i0
         f32x4* to = (f32x4*)(a.dxs + ((uint64_t)split * a.rows64 + j0 + s * 16 + col) * a.hidden64 + h);
         *to = a.first ? *to + acc[v][s] : acc[v][s];
       }
+    }
   }
   if constexpr (kKind == kTable) {
     const float f = *a.largest * (1.0f / kUp<T>);
@@ -370,9 +376,18 @@ __device__ __forceinline__ void finish(const Args& a, uint32_t tile, uint32_t i0
 #pragma unroll
       for (int v = 0; v < kN; ++v) {
         const uint32_t h = i0 + v * 16 + q * 4;
+        struct __attribute__((packed, aligned(2))) Four {
+          T e[4];
+        } o;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (h + e < a.hidden) row[h + e] = (T)(acc[v][s][e] * f);
+        for (int e = 0; e < 4; ++e) o.e[e] = (T)(acc[v][s][e] * f);
+        if (h + 4 <= a.hidden) {
+          *(Four*)(row + h) = o;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (h + e < a.hidden) row[h + e] = o.e[e];
+        }
       }
     }
   }
@@ -386,7 +401,7 @@ __global__ void __launch_bounds__(kThreads) xent_product(Args a) {
   __shared__ float joined[4][3][kBM];
   const uint32_t wave = threadIdx.x >> 6;
   // tiles of i, j and, for dx, of k
-  const uint32_t js = kKind == kTable ? a.piece / kBM : a.rows64 / kBM;
+  const uint32_t js = kKind == kTable ? a.width / kBM : a.rows64 / kBM;
   const uint32_t tj = blockIdx.x % js, rest = blockIdx.x / js;
   uint32_t ti = rest, split = 0, k0 = 0, k1;
   Operand po, qo;
@@ -401,7 +416,8 @@ __global__ void __launch_bounds__(kThreads) xent_product(Args a) {
     po = Operand{(const T*)a.weight + (int64_t)a.first * a.weight_stride, a.weight_stride, last + 1, a.hidden};
     qo = Operand{a.slopes, a.piece, a.rows64, a.piece};
     k0 = split * a.split_steps * kBK;
-    k1 = min(k0 + a.split_steps * kBK, a.piece);
+    k1 = min(k0 + a.split_steps * kBK, a.width);
+    if (k0 >= k1) return;  // (a last piece of fewer parts)
   } else {
     po = Operand{a.xs, a.hidden64, a.rows64, a.hidden64};
     qo = Operand{a.slopes, a.piece, a.rows64, a.piece};
@@ -430,7 +446,234 @@ __global__ void __launch_bounds__(kThreads) xent_product(Args a) {
         for (int j = 0; j < kBM / 16; ++j) acc[i][j] = mfma(pf[i], qf[j], acc[i][j], T{});
     }
   }
-  finish<T, kKind, 2, kBM / 16, 4>(a, ti, i0 + wave * 32, j0, split, acc, joined, wave);
+  finish<T, kKind, 2, kBM / 16, 4, kBM>(a, threadIdx.x, ti, i0 + wave * 32, j0, 0, wave, split, acc, joined);
+}
+
+// Operands whose rows are whole lines of 128 bytes: tiles of 256 of i by BM of
+// j, steps of 64 of k copied straight to two LDS stages.  The operands of half
+// a step are read from LDS during the matrix instructions of the half before,
+// so that past a barrier there is work at once.
+//
+// An operand by k is a line of eight 16-byte columns a row, exchanged by the
+// row's number.  One across k has lines of 512 bytes (256 of i) for each k: a
+// copy of a wave brings two, whose 32-byte units are exchanged by the row's
+// lowest bit, and copies lie 64 bytes more than their length apart, every
+// fourth 128 more: a transposed read takes 32 bytes of four rows in 16 lanes,
+// and of eight rows in 32, without bank conflicts.
+constexpr int kTileBN = 256, kTileThreads = 512;
+
+// 16 bytes a lane, from an offset (a lane's and the wave's) of a buffer to
+// the wave's place in LDS.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t whole_buffer(const void* p) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)0xFFFFFFFFu, 0x00027000);
+}
+__device__ __forceinline__ void copy_to_lds(__amdgpu_buffer_rsrc_t from, uint32_t lane, uint32_t wave, void* to) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)to, 16, (int)lane,
+                                           (int)wave, 0, 0);
+}
+// All LDS reads of the wave are done, and all its copies but the last n.
+template <int n>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("" ::: "memory");
+  // vmcnt n, lgkmcnt 0, the third counter free
+  __builtin_amdgcn_s_waitcnt((n & 15) | (n >> 4) << 14 | 7 << 4);
+}
+
+// kWhole: across, rows are whole steps.
+template <typename T, bool kAcross, int kB, bool kWhole>
+struct Lines {
+  static constexpr int kTurns = kB / 64;  // copies of a wave and step
+  static constexpr uint32_t kBytes = kAcross ? 32 * 1088 + 8 * 128 : kB * 128;
+  static constexpr int kOffsets = kAcross ? 1 : kTurns;
+  static_assert(!kAcross || kB == 256, "lines of 512 bytes");
+
+  const char* base;
+  uint32_t line;           // bytes from row to row
+  uint32_t left;           // across: rows from base on
+  uint32_t off[kOffsets];  // of this lane's copies
+  uint32_t at[2];          // this lane's reads: of a step's halves; across: of even and odd subtiles
+
+  // by k: rows i0 ..., from column k0 on; across: columns i0 ..., from row k0 on
+  __device__ __forceinline__ void begin(const Operand& o, uint32_t i0, uint32_t k0, uint32_t sub0, uint32_t tid,
+                                        uint32_t wave) {
+    const uint32_t lane = tid & 63, col = lane & 15, q = lane >> 4;
+    line = (uint32_t)o.stride * 2;
+    if constexpr (kAcross) {
+      const uint32_t row0 = min(k0, o.rows - 1);
+      base = (const char*)((const T*)o.base + (int64_t)row0 * o.stride);
+      left = o.rows - row0;
+      const uint32_t row = 2 * wave + (lane >> 5), piece = (lane & 31) ^ (lane >> 5 << 1);
+      // (columns past the end: the last ones, whose products are not stored)
+      off[0] = row * line + min(i0 / 8 + piece, o.columns / 8 - 1) * 16;
+      const uint32_t r4 = col >> 2, b = r4 & 1;
+      at[0] = q * (4 * 1088 + 128) + (r4 >> 1) * 1088 + b * 512 + sub0 * 32 + (col & 3) * 8;
+      at[1] = at[0] - b * 32;
+      at[0] += b * 32;
+    } else {
+      base = (const char*)((const T*)o.base + (int64_t)i0 * o.stride + k0);
+#pragma unroll
+      for (int c = 0; c < kTurns; ++c) {
+        const uint32_t row = (c * kTileThreads + tid) / 8;
+        off[c] = min(row, o.rows - 1 - i0) * line + ((tid & 7) ^ (row & 7)) * 16;
+      }
+      at[0] = ((sub0 * 16 + col) * 8 + (q ^ (col & 7))) * 16;
+      at[1] = at[0] ^ 64;
+    }
+    asm volatile("" : "+v"(at[0]), "+v"(at[1]));
+  }
+  // step k from the first on
+  __device__ __forceinline__ void copy(char* st, uint32_t k, uint32_t lane, uint32_t wave) const {
+    if constexpr (kAcross) {
+      const uint32_t first = kWhole ? k * 64 : min(k * 64, left - 1);
+      const __amdgpu_buffer_rsrc_t b = whole_buffer(base + (uint64_t)first * line);
+      char* to = st + wave * 1088 + (wave >> 2) * 128;
+      if (kWhole || first + 64 <= left) {
+#pragma unroll
+        for (int c = 0; c < kTurns; ++c) copy_to_lds(b, off[0], c * 16 * line, to + c * (8 * 1088 + 256));
+      } else {  // rows past the end: the last one
+        const uint32_t row = 2 * wave + (lane >> 5), at = off[0] - row * line;
+#pragma unroll
+        for (int c = 0; c < kTurns; ++c)
+          copy_to_lds(b, min(c * 16 + row, left - first - 1) * line + at, 0, to + c * (8 * 1088 + 256));
+      }
+    } else {
+      const __amdgpu_buffer_rsrc_t b = whole_buffer(base);
+#pragma unroll
+      for (int c = 0; c < kTurns; ++c) copy_to_lds(b, off[c], k * 128, st + (c * 8 + wave) * 1024);
+    }
+  }
+  // subtile sub0 + v, half kk of a step
+  __device__ __forceinline__ u32x4 read(const char* st, int v, int kk) const {
+    if constexpr (kAcross) {
+      const char* p = st + at[v & 1] + (v * 32 + kk * (16 * 1088 + 4 * 128));
+      union {
+        s16x4 h[2];
+        u32x4 v;
+      } u;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        u.h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + i * 2 * 1088));
+      return u.v;
+    } else {
+      return *(const u32x4*)(st + at[kk] + v * 2048);
+    }
+  }
+};
+
+// Tile (j, i, split) of a workgroup.  Consecutive workgroups go to the XCDs in
+// turn, so each XCD takes a run of tiles; a run goes over four tiles of j at a
+// time, then over i: what an XCD runs at once shares operands in its L2.
+__device__ __forceinline__ void tile_of(uint32_t js, uint32_t is, uint32_t* tj, uint32_t* ti, uint32_t* split) {
+  const uint32_t n = gridDim.x, run = n / 8;
+  uint32_t t = blockIdx.x < run * 8 ? (blockIdx.x % 8) * run + blockIdx.x / 8 : blockIdx.x;
+  *split = t / (js * is);
+  t -= *split * (js * is);
+  constexpr uint32_t kGroup = 4;
+  const uint32_t g = t / (kGroup * is), in = t - g * kGroup * is;
+  const uint32_t width = min(kGroup, js - g * kGroup);
+  *ti = in / width;
+  *tj = g * kGroup + in % width;
+}
+
+template <int kBMs, int kWM>
+struct TileShape {
+  static constexpr int BM = 16 * kBMs, WM = kWM, WN = 8 / kWM, M = kBMs / WM, N = 16 / WN;
+};
+
+template <typename T, Kind kKind, typename S>
+__global__ void __launch_bounds__(kTileThreads) xent_tile(Args a) {
+  using P = Lines<T, kKind >= kStates, kTileBN, kKind == kTable>;
+  using Q = Lines<T, kKind == kTable, S::BM, true>;
+  __shared__ __attribute__((aligned(1024))) char st0[P::kBytes + Q::kBytes], st1[P::kBytes + Q::kBytes];
+  const uint32_t tid = threadIdx.x, lane = tid & 63;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+  const uint32_t wm = wave % S::WM, wn = wave / S::WM;
+  uint32_t tj, ti, split, k0 = 0, steps;
+  P p;
+  Q x;
+  {
+    const uint32_t js = kKind == kTable ? a.width / S::BM : (a.rows64 + S::BM - 1) / S::BM;
+    const uint32_t is = kKind == kStats ? a.tiles : kKind == kSlopes ? a.width / kTileBN : (a.hidden64 + kTileBN - 1) / kTileBN;
+    tile_of(js, is, &tj, &ti, &split);
+    Operand po, qo;
+    if (kKind == kStats || kKind == kSlopes) {
+      po = Operand{a.weight, a.weight_stride, a.vocab, a.hidden};
+      qo = Operand{a.x, a.x_stride, a.rows, a.hidden};
+      steps = a.hidden64 / 64;
+    } else if (kKind == kStates) {
+      po = Operand{(const T*)a.weight + (int64_t)a.first * a.weight_stride, a.weight_stride, a.vocab - a.first, a.hidden};
+      qo = Operand{a.slopes, a.piece, a.rows64, a.piece};
+      k0 = split * a.split_steps * 64;
+      if (k0 >= a.width) return;  // (a last piece of fewer parts)
+      steps = min(a.split_steps, a.width / 64 - split * a.split_steps);
+    } else {
+      po = Operand{a.xs, a.hidden64, a.rows64, a.hidden64};
+      qo = Operand{a.slopes, a.piece, a.rows64, a.piece};
+      steps = a.rows64 / 64;
+    }
+    const uint32_t first = kKind == kSlopes ? a.first : 0;
+    p.begin(po, ti * kTileBN + first, k0, wn * S::N, tid, wave);
+    x.begin(qo, tj * S::BM, k0, wm * S::M, tid, wave);
+  }
+  const auto copy = [&](char* st, uint32_t i) {
+    const uint32_t k = min(i, steps - 1);  // (past the end: again, unused)
+    p.copy(st, k, lane, wave);
+    x.copy(st + P::kBytes, k, lane, wave);
+  };
+  f32x4 acc[S::N][S::M] = {};
+  constexpr int kCopies = P::kTurns + Q::kTurns;
+  // Half a step: the products of w and x, while w and `ahead` take the next
+  // half's operands, kk of the stage `next`.  A register of w is free when its
+  // products are issued; x has two sets.
+  u32x4 w[S::N], x0[S::M], x1[S::M];
+  const auto half = [&](const u32x4 (&now)[S::M], u32x4 (&ahead)[S::M], const char* next, int kk) {
+#pragma unroll
+    for (int v = 0; v < S::N; ++v) {
+#pragma unroll
+      for (int j = 0; j < S::M; ++j) acc[v][j] = mfma(w[v], now[j], acc[v][j], T{});
+      w[v] = p.read(next, v, kk);
+      constexpr int kEach = (S::M + S::N - 1) / S::N;
+#pragma unroll
+      for (int j = v * kEach; j < (v + 1) * kEach && j < S::M; ++j) ahead[j] = x.read(next + P::kBytes, j, kk);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // Step i: w and x0 hold its first half's operands.  At the barrier all of
+  // the step has been read, and the next is there.
+  const auto step = [&](uint32_t i, char* st, const char* next) {
+    half(x0, x1, st, 1);
+    wait_copies<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    copy(st, i + 2);
+    half(x1, x0, next, 0);
+  };
+  copy(st0, 0);
+  copy(st1, 1);
+  wait_copies<kCopies>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int v = 0; v < S::N; ++v) w[v] = p.read(st0, v, 0);
+#pragma unroll
+  for (int j = 0; j < S::M; ++j) x0[j] = x.read(st0 + P::kBytes, j, 0);
+  for (uint32_t i = 0;;) {
+    step(i, st0, st1);
+    if (++i == steps) break;
+    step(i, st1, st0);
+    if (++i == steps) break;
+  }
+  wait_copies<0>();
+  __syncthreads();
+  // (numbers of the thread anew, so that none of what follows is computed
+  // ahead and takes the loop's registers)
+  uint32_t after = threadIdx.x;
+  asm volatile("" : "+v"(after));
+  const uint32_t wave_after = (uint32_t)__builtin_amdgcn_readfirstlane((int)(after >> 6));
+  const uint32_t wm_after = wave_after % S::WM, wn_after = wave_after / S::WM;
+  finish<T, kKind, S::N, S::M, S::WN, S::BM>(
+      a, after, ti, ti * kTileBN + (kKind == kSlopes ? a.first : 0) + wn_after * S::N * 16, tj * S::BM,
+      wm_after * S::M * 16, wn_after, split, acc, (float(*)[3][S::BM])st0);
 }
 
 // --- plan -------------------------------------------------------------------
@@ -439,15 +682,27 @@ constexpr uint32_t kCUs = 256;
 
 struct Plan {
   uint64_t mant, power, largest, part, picked, top, logsum, terms, xs, slopes, dxs, bytes;
-  uint32_t rows64, hidden64, tiles, piece, splits, split_steps;
+  uint32_t rows64, hidden64, tiles, piece, splits, split_steps, bm, bn;
+  bool lines;
 };
+
+// The states' and the table's rows are whole lines, and 32-bit offsets reach
+// a tile's operands.
+bool whole_lines(const ft_cross_entropy_loss_args& a) {
+  return a.hidden % 64 == 0 && (uintptr_t)a.x % 16 == 0 && (uintptr_t)a.weight % 16 == 0 &&
+         a.x_stride % 8 == 0 && a.weight_stride % 8 == 0 && a.x_stride >= 0 && a.weight_stride >= 0 &&
+         a.x_stride < 1 << 22 && a.weight_stride < 1 << 22;
+}
 
 Plan plan(const ft_cross_entropy_loss_args& a) {
   Plan p{};
   Arena ar;
   p.rows64 = (uint32_t)round_up(a.rows, 64);
   p.hidden64 = (uint32_t)round_up(a.hidden, 64);
-  p.tiles = (a.vocab + kBN - 1) / kBN;
+  p.lines = whole_lines(a);
+  p.bn = p.lines ? kTileBN : kBN;
+  p.bm = !p.lines || p.rows64 <= 64 ? 64 : p.rows64 <= 128 ? 128 : 256;
+  p.tiles = (a.vocab + p.bn - 1) / p.bn;
   const uint64_t r = p.rows64;
   p.mant = ar.take(r * 4);
   p.power = ar.take(r * 4);
@@ -460,15 +715,16 @@ Plan plan(const ft_cross_entropy_loss_args& a) {
   if (a.dx || a.dweight) {
     // a piece's slopes: up to 128 MB, half of the last level's cache
     const uint64_t whole = round_up(a.vocab, 256);
-    p.piece = (uint32_t)std::min(whole, std::max<uint64_t>(256, (128ull << 20) / std::max<uint64_t>(64, r) / 512 * 256));
+    p.piece = (uint32_t)std::min(
+        whole, std::max<uint64_t>(256, (128ull << 20) / std::max<uint64_t>(64, r) / 512 * 256));
     p.slopes = ar.take(r * p.piece * 2);
   }
   if (a.dweight) p.xs = ar.take(r * p.hidden64 * 2);
   if (a.dx) {
     // as many parts of the sum over tokens as fill the chip
-    const uint64_t tiles = std::max<uint64_t>(1, r / kBM * ((p.hidden64 + kBN - 1) / kBN));
+    const uint64_t tiles = std::max<uint64_t>(1, (r + p.bm - 1) / p.bm * ((p.hidden64 + p.bn - 1) / p.bn));
     const uint32_t steps = p.piece / kBK;
-    const uint64_t want = std::max<uint64_t>(1, 2 * kCUs / tiles);
+    const uint64_t want = std::max<uint64_t>(1, (p.lines ? 1 : 2) * kCUs / tiles);
     p.split_steps = (uint32_t)std::max<uint64_t>(4, (steps + want - 1) / want);
     p.splits = (steps + p.split_steps - 1) / p.split_steps;
     p.dxs = ar.take((uint64_t)p.splits * r * p.hidden64 * 4);
@@ -477,31 +733,46 @@ Plan plan(const ft_cross_entropy_loss_args& a) {
   return p;
 }
 
+template <typename T, Kind kKind>
+hipError_t product(const Args& a, const Plan& p, hipStream_t s) {
+  const uint64_t hs = (a.hidden64 + p.bn - 1) / p.bn;
+  const uint64_t js = kKind == kTable ? a.width / (p.lines ? 256 : p.bm) : (a.rows64 + p.bm - 1) / p.bm;
+  const uint64_t blocks = js * (kKind == kStats    ? a.tiles
+                                : kKind == kSlopes ? a.width / p.bn
+                                : kKind == kStates ? hs * a.splits
+                                                   : hs);
+  if (!p.lines) return start(xent_product<T, kKind>, blocks, kThreads, s, a);
+  if constexpr (kKind != kTable) {
+    if (p.bm == 64) return start(xent_tile<T, kKind, TileShape<4, 1>>, blocks, kTileThreads, s, a);
+    if (p.bm == 128) return start(xent_tile<T, kKind, TileShape<8, 2>>, blocks, kTileThreads, s, a);
+  }
+  return start(xent_tile<T, kKind, TileShape<16, 2>>, blocks, kTileThreads, s, a);
+}
+
 template <typename T>
-hipError_t launch(Args a, hipStream_t s) {
+hipError_t launch(Args a, const Plan& p, hipStream_t s) {
   if (a.rows == 0) {
     const hipError_t e = start(xent_loss, 1, 1024, s, a);
     return e == hipSuccess && a.dweight ? start(xent_nothing<T>, a.vocab, 256, s, a) : e;
   }
   hipError_t e = start(xent_rows<T>, a.rows64 / 4, 256, s, a);
   if (e != hipSuccess) return e;
-  const uint64_t js = a.rows64 / kBM;
-  e = start(xent_product<T, kStats>, a.tiles * js, kThreads, s, a);
+  e = product<T, kStats>(a, p, s);
   if (e != hipSuccess) return e;
   e = start(xent_join, a.rows64 / 64, 1024, s, a);
   if (e != hipSuccess) return e;
   e = start(xent_loss, 1, 1024, s, a);
   if (e != hipSuccess || !(a.dx || a.dweight)) return e;
-  const uint64_t hs = (a.hidden64 + kBN - 1) / kBN;
   for (a.first = 0; a.first < a.vocab; a.first += a.piece) {
-    e = start(xent_product<T, kSlopes>, a.piece / kBN * js, kThreads, s, a);
+    a.width = (uint32_t)std::min<uint64_t>(a.piece, round_up(a.vocab - a.first, 256));
+    e = product<T, kSlopes>(a, p, s);
     if (e != hipSuccess) return e;
     if (a.dx) {
-      e = start(xent_product<T, kStates>, hs * js * a.splits, kThreads, s, a);
+      e = product<T, kStates>(a, p, s);
       if (e != hipSuccess) return e;
     }
     if (a.dweight) {
-      e = start(xent_product<T, kTable>, hs * (a.piece / kBM), kThreads, s, a);
+      e = product<T, kTable>(a, p, s);
       if (e != hipSuccess) return e;
     }
   }
@@ -549,7 +820,7 @@ hipError_t launch_cross_entropy_loss(const ft_cross_entropy_loss_args& q, uint8_
   a.piece = p.piece;
   a.splits = p.splits;
   a.split_steps = p.split_steps;
-  return q.dtype == FT_BF16 ? launch<__bf16>(a, s) : launch<_Float16>(a, s);
+  return q.dtype == FT_BF16 ? launch<__bf16>(a, p, s) : launch<_Float16>(a, p, s);
 }
 
 }  // namespace fto
