@@ -65,18 +65,33 @@ struct Args {
   float* mant;      // [rows64]: m, 0 without a target
   float* power;     // [rows64]: 2^e
   float* largest;   // 2^(the largest e)
-  float* part;      // [3][tiles][rows64]: max, sum of exponentials, sum of logits
+  float* part;      // [3][tiles][rows64]: c, s, sum of logits
   float* picked;    // [rows64]: the target's logit
-  float* top;       // [rows64]: max
-  float* logsum;    // [rows64]: lse - max
+  float* top;       // [rows64]: c
+  float* logsum;    // [rows64]: log2 s
   float* terms;     // [rows64]: of the loss
   void* xs;         // [rows64][hidden64]: x times 2^(e - largest)
-  void* slopes;     // [rows64][piece]
+  void* slopes;     // [rows64][slope_stride]
   float* dxs;       // [splits][rows64][hidden64]
   // a piece of the vocabulary
   uint32_t piece, first, width;  // most tokens of it; its first; its tokens up to whole 256s
+  uint32_t slope_stride;  // of the slopes' rows
   uint32_t splits, split_steps;  // parts of dx and their steps of 64
 };
+
+// A part of a row's statistics is (c, s): s = sum of 2^(l log2 e - c), c the
+// part's largest l, times log2 e in 32 bits (0 where that is -infinity).  The
+// product and the difference are one fused step, so a term's exponent is
+// rounded once, relative to itself.  A NaN or +infinity makes s NaN.
+struct Part {
+  float c, s;
+};
+__device__ __forceinline__ float power_of(float l, float c) { return exp2_raw(__builtin_fmaf(l, kLog2e, -c)); }
+__device__ __forceinline__ Part join(Part a, Part b) {
+  // (a part of nothing has s = 0 and takes no part in c)
+  const float c = a.s == 0.0f ? b.c : b.s == 0.0f ? a.c : fmaxf(a.c, b.c);
+  return Part{c, (a.s == 0.0f ? 0.0f : a.s * exp2_raw(a.c - c)) + (b.s == 0.0f ? 0.0f : b.s * exp2_raw(b.c - c))};
+}
 
 // --- rows -------------------------------------------------------------------
 
@@ -132,42 +147,52 @@ __global__ void __launch_bounds__(256) xent_rows(Args a) {
   }
 }
 
-// 64 rows by 16 waves, which take the tiles in turn.
+// 16 rows by 64 parts of the tiles.
 __global__ void __launch_bounds__(1024) xent_join(Args a) {
-  __shared__ float sm[16][64], ss[16][64], sl[16][64];
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = blockIdx.x * 64 + lane;
+  __shared__ float sc[64][16], ss[64][16], sl[64][16];
+  const uint32_t row = threadIdx.x & 15, from = threadIdx.x >> 4, t = blockIdx.x * 16 + row;
   const uint64_t each = (uint64_t)a.tiles * a.rows64;
-  MaxSum p{-INFINITY, 0.0f};
+  Part p{0.0f, 0.0f};
   float l = 0.0f;
 #pragma unroll 4
-  for (uint32_t i = wave; i < a.tiles; i += 16) {
+  for (uint32_t i = from; i < a.tiles; i += 64) {
     const uint64_t at = (uint64_t)i * a.rows64 + t;
-    p = merge(p, MaxSum{a.part[at], a.part[each + at]});
-    l += a.part[2 * each + at];
+    p = join(p, Part{a.part[at], a.part[each + at]});
+    if (a.smoothing != 0.0f) l += a.part[2 * each + at];
   }
-  sm[wave][lane] = p.m;
-  ss[wave][lane] = p.s;
-  sl[wave][lane] = l;
+  sc[from][row] = p.c;
+  ss[from][row] = p.s;
+  sl[from][row] = l;
   __syncthreads();
-  if (wave > 0) return;
+  if (from >= 4) return;  // a wave joins 16 parts a lane, then its lanes'
 #pragma unroll
-  for (int w = 1; w < 16; ++w) {
-    p = merge(p, MaxSum{sm[w][lane], ss[w][lane]});
-    l += sl[w][lane];
+  for (uint32_t w = 4; w < 64; w += 4) {
+    p = join(p, Part{sc[from + w][row], ss[from + w][row]});
+    l += sl[from + w][row];
   }
+#pragma unroll
+  for (int d = 16; d < 64; d *= 2) {
+    const Part other{__shfl_xor(p.c, d, 64), __shfl_xor(p.s, d, 64)};
+    const float more = __shfl_xor(l, d, 64);
+    p = join(p, other);
+    l += more;
+  }
+  if (from > 0) return;
+  constexpr float kLn2 = 0.693147180559945309f;
   const int32_t y = t < a.rows ? a.target[t] : -1;
-  const float base = exp_base(p.m);
-  float ls = logf(p.s);
-  float at = y >= 0 && (uint32_t)y < a.vocab ? a.picked[t] - base : NAN;
-  if (y >= 0 && (uint32_t)y >= a.vocab) ls = NAN;  // and with it the row's slopes
-  a.top[t] = base;
+  const bool there = y >= 0 && (uint32_t)y < a.vocab;
+  // (a target out of range: NaN, and with it the row's slopes)
+  const float ls = y < 0 || there ? __log2f(p.s) : NAN;
+  const float at = there ? (__builtin_fmaf(a.picked[t], kLog2e, -p.c) - ls) * kLn2 : NAN;
+  a.top[t] = p.c;
   a.logsum[t] = ls;
   float term = 0.0f;
   if (y >= 0) {
-    a.logp[t] = at - ls;
+    a.logp[t] = at;
     const float r = a.row_weight[t];
-    term = (1.0f - a.smoothing) * (ls - at);
-    if (a.smoothing != 0.0f) term += a.smoothing * (ls - (l / (float)a.vocab - base));
+    term = (1.0f - a.smoothing) * -at;
+    if (a.smoothing != 0.0f)
+      term += a.smoothing * ((ls - __builtin_fmaf(l / (float)a.vocab, kLog2e, -p.c)) * kLn2);
     term = r == 0.0f ? 0.0f : r * term;
   } else if (t < a.rows) {
     a.logp[t] = 0.0f;
@@ -195,27 +220,31 @@ __global__ void __launch_bounds__(256) xent_nothing(Args a) {
   for (uint32_t h = threadIdx.x; h < a.hidden; h += 256) row[h] = (T)0.0f;
 }
 
-// dx from its parts; a wave a row.
+// dx from its parts: 256 columns of a row a workgroup, whose waves take the
+// parts in turn.
 template <typename T>
-__global__ void __launch_bounds__(256) xent_states(Args a) {
-  const uint32_t lane = threadIdx.x & 63, t = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (t >= a.rows) return;
+__global__ void __launch_bounds__(1024) xent_states(Args a) {
+  __shared__ f32x4 other[15][64];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const uint32_t panels = (a.hidden64 + 255) / 256;
+  const uint32_t t = blockIdx.x / panels, h = (blockIdx.x % panels * 64 + lane) * 4;
+  const uint64_t each = (uint64_t)a.rows64 * a.hidden64;
+  f32x4 y{};
+  if (h < a.hidden64) {
+    const float* p = a.dxs + (uint64_t)t * a.hidden64 + h;
+#pragma unroll 4
+    for (uint32_t s = wave; s < a.splits; s += waves) y += *(const f32x4*)(p + s * each);
+  }
+  if (wave > 0) other[wave - 1][lane] = y;
+  __syncthreads();
+  if (wave > 0) return;
+  for (uint32_t w = 1; w < waves; ++w) y += other[w - 1][lane];
   const bool none = a.mant[t] == 0.0f;
   const float f = a.power[t] * (1.0f / kUp<T>);
-  const uint64_t each = (uint64_t)a.rows64 * a.hidden64;
-  for (uint32_t h = lane * 8; h < a.hidden; h += 512) {
-    float y[8] = {};
-    for (uint32_t s = 0; s < a.splits; ++s) {
-      const float* p = a.dxs + s * each + (uint64_t)t * a.hidden64 + h;
+  T* out = (T*)a.dx + (int64_t)t * a.dx_stride + h;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] += p[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = none ? 0.0f : y[i] * f;
-    T* out = (T*)a.dx + (int64_t)t * a.dx_stride + h;
-    if (h + 8 <= a.hidden) store_vec(out, from_float<T>(y));
-    else store_part(out, (int)(a.hidden - h), from_float<T>(y));
-  }
+  for (int e = 0; e < 4; ++e)
+    if (h + e < a.hidden) out[e] = (T)(none ? 0.0f : y[e] * f);
 }
 
 // --- products ---------------------------------------------------------------
@@ -276,80 +305,149 @@ struct Stage {
 // What a product leaves.  The wave's i are i0 ..., 16 kN of them, its j jb + jw
 // ..., 16 kM of the workgroup's kB; a lane has four neighbouring i of row j.
 // Waves wn = 0 ... kWaves - 1 have other i of the same j.
-template <typename T, Kind kKind, int kN, int kM, int kWaves, int kB>
+// A wave's LDS `mine` (or none) takes 16 rows of numbers of 16 bits, so that
+// they are stored by whole lines.
+template <int kN>
+constexpr int kStored = 16 * (kN * 32 + 16);  // bytes
+
+// Rows r of 16 kN numbers, of which a lane has o[v], numbers 16 v + 4 q ... of
+// row `col`; to(r, c) is where row r's from c on lie, or null.
+template <int kN, typename To>
+__device__ __forceinline__ void store_rows(const uint2 (&o)[kN], char* mine, uint32_t lane, To&& to) {
+  constexpr int kRow = kN * 32 + 16, kPer = kN * 2;  // bytes, pieces of 16
+  const uint32_t col = lane & 15, q = lane >> 4;
+#pragma unroll
+  for (int v = 0; v < kN; ++v) *(uint2*)(mine + col * kRow + v * 32 + q * 8) = o[v];
+  asm volatile("" ::: "memory");  // (a wave's LDS accesses are in order)
+#pragma unroll
+  for (int p = 0; p < 16 * kPer / 64; ++p) {
+    const uint32_t at = p * 64 + lane, r = at / kPer, c = at % kPer * 8;
+    const u32x4 v = *(const u32x4*)(mine + r * kRow + c * 2);
+    to(r, c, v);
+  }
+  asm volatile("" ::: "memory");
+}
+
+template <typename T, Kind kKind, int kN, int kM, int kWaves, int kB, bool kLines>
 __device__ __forceinline__ void finish(const Args& a, uint32_t tid, uint32_t tile, uint32_t i0, uint32_t jb,
                                        uint32_t jw, uint32_t wn, uint32_t split, f32x4 (&acc)[kN][kM],
-                                       float (*joined)[3][kB]) {
+                                       float (*joined)[3][kB], char* mine) {
   const uint32_t lane = tid & 63, col = lane & 15, q = lane >> 4, j0 = jb + jw;
   if constexpr (kKind == kStats) {
+    const bool inside = i0 + 16 * kN <= a.vocab;
 #pragma unroll
     for (int s = 0; s < kM; ++s) {
       const uint32_t t = j0 + s * 16 + col;
-      const int32_t y = t < a.rows ? a.target[t] : -1;
-      MaxSum p{-INFINITY, 0.0f};
-      float sum = 0.0f;
+      float sum = 0.0f, total = 0.0f, big = -INFINITY;
+      // the target, in one tile of many
+      const uint32_t y = (t < a.rows ? (uint32_t)a.target[t] : ~0u) - i0;
+      if (__ballot(y < 16 * kN)) {
 #pragma unroll
-      for (int v = 0; v < kN; ++v) {
-        float l[4];
+        for (int v = 0; v < kN; ++v)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t tok = i0 + v * 16 + q * 4 + e;
-          l[e] = tok < a.vocab ? acc[v][s][e] : -INFINITY;
-          if (tok < a.vocab) sum += l[e];
-          if ((int32_t)tok == y && tok < a.vocab) a.picked[t] = l[e];
-        }
-        add_terms(p, l);
+          for (int e = 0; e < 4; ++e)
+            if (y == v * 16 + q * 4 + e && i0 + y < a.vocab) a.picked[t] = acc[v][s][e];
       }
+      if (!inside) {  // (tokens past the vocabulary add 0 to the sum of logits)
+#pragma unroll
+        for (int v = 0; v < kN; ++v)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (i0 + v * 16 + q * 4 + e >= a.vocab) acc[v][s][e] = 0.0f;
+      }
+      if (a.smoothing != 0.0f) {
+#pragma unroll
+        for (int v = 0; v < kN; ++v) total += (acc[v][s][0] + acc[v][s][1]) + (acc[v][s][2] + acc[v][s][3]);
+      }
+      if (!inside) {
+#pragma unroll
+        for (int v = 0; v < kN; ++v)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (i0 + v * 16 + q * 4 + e >= a.vocab) acc[v][s][e] = -INFINITY;
+      }
+#pragma unroll
+      for (int v = 0; v < kN; ++v)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) big = fmaxf(big, acc[v][s][e]);
+#pragma unroll
+      for (int d = 16; d < 64; d *= 2) big = fmaxf(big, __shfl_xor(big, d, 64));
+      const float c = big == -INFINITY ? 0.0f : big * kLog2e;
+#pragma unroll
+      for (int v = 0; v < kN; ++v)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += power_of(acc[v][s][e], c);
 #pragma unroll
       for (int d = 16; d < 64; d *= 2) {
-        p = merge(p, MaxSum{__shfl_xor(p.m, d, 64), __shfl_xor(p.s, d, 64)});
         sum += __shfl_xor(sum, d, 64);
+        total += __shfl_xor(total, d, 64);
       }
       if (q == 0) {
-        joined[wn][0][jw + s * 16 + col] = p.m;
-        joined[wn][1][jw + s * 16 + col] = p.s;
-        joined[wn][2][jw + s * 16 + col] = sum;
+        joined[wn][0][jw + s * 16 + col] = c;
+        joined[wn][1][jw + s * 16 + col] = sum;
+        joined[wn][2][jw + s * 16 + col] = total;
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
     const uint64_t each = (uint64_t)a.tiles * a.rows64;
     for (uint32_t j = tid; j < kB && jb + j < a.rows64; j += blockDim.x) {
-      MaxSum p{joined[0][0][j], joined[0][1][j]};
+      Part p{joined[0][0][j], joined[0][1][j]};
       float sum = joined[0][2][j];
 #pragma unroll
       for (int w = 1; w < kWaves; ++w) {
-        p = merge(p, MaxSum{joined[w][0][j], joined[w][1][j]});
+        p = join(p, Part{joined[w][0][j], joined[w][1][j]});
         sum += joined[w][2][j];
       }
       const uint64_t at = (uint64_t)tile * a.rows64 + jb + j;
-      a.part[at] = p.m;
+      a.part[at] = p.c;
       a.part[each + at] = p.s;
       a.part[2 * each + at] = sum;
     }
   }
   if constexpr (kKind == kSlopes) {
     const float even = a.smoothing / (float)a.vocab, own = 1.0f - a.smoothing;
+    const bool inside = i0 + 16 * kN <= a.vocab;
 #pragma unroll
     for (int s = 0; s < kM; ++s) {
       if (j0 + s * 16 >= a.rows64) break;
       const uint32_t t = j0 + s * 16 + col;
-      const int32_t y = t < a.rows ? a.target[t] : -1;
-      const float m = a.mant[t] * kUp<T>, top = a.top[t], ls = a.logsum[t];
-      T* row = (T*)a.slopes + (uint64_t)t * a.piece + (i0 - a.first);
+      const uint32_t y = (t < a.rows ? (uint32_t)a.target[t] : ~0u) - i0;
+      const float m = a.mant[t] * kUp<T>, c = a.top[t], ls = a.logsum[t];
+      const bool hit = __ballot(y < 16 * kN) != 0;  // (a target in one tile of many)
+      union {
+        uint2 u;
+        T g[4];
+      } o;
+      uint2 all[kN];
 #pragma unroll
       for (int v = 0; v < kN; ++v) {
-        union {
-          uint2 u;
-          T g[4];
-        } o;
+        float g[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t tok = i0 + v * 16 + q * 4 + e;
-          float g = exp_term(acc[v][s][e] - top, ls) - even;
-          if ((int32_t)tok == y) g -= own;
-          o.g[e] = (T)(m != 0.0f && tok < a.vocab ? g * m : 0.0f);
+        for (int e = 0; e < 4; ++e)
+          g[e] = (exp2_raw(__builtin_fmaf(acc[v][s][e], kLog2e, -c) - ls) - even) * m;
+        if (hit) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (y == v * 16 + q * 4 + e)
+              g[e] = (exp2_raw(__builtin_fmaf(acc[v][s][e], kLog2e, -c) - ls) - even - own) * m;
         }
-        *(uint2*)(row + v * 16 + q * 4) = o.u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (!inside && i0 + v * 16 + q * 4 + e >= a.vocab) g[e] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o.g[e] = (T)g[e];
+        all[v] = m == 0.0f ? uint2{0, 0} : o.u;
+      }
+      T* first = (T*)a.slopes + (i0 - a.first);
+      if constexpr (kLines) {
+        store_rows<kN>(all, mine, lane, [&](uint32_t r, uint32_t c, u32x4 v) {
+          *(u32x4*)(first + (uint64_t)(j0 + s * 16 + r) * a.slope_stride + c) = v;
+        });
+        __builtin_amdgcn_sched_barrier(0);
+      } else {
+#pragma unroll
+        for (int v = 0; v < kN; ++v) *(uint2*)(first + (uint64_t)t * a.slope_stride + v * 16 + q * 4) = all[v];
       }
     }
   }
@@ -370,20 +468,30 @@ __device__ __forceinline__ void finish(const Args& a, uint32_t tid, uint32_t til
     const float f = *a.largest * (1.0f / kUp<T>);
 #pragma unroll
     for (int s = 0; s < kM; ++s) {
-      const uint32_t tok = a.first + j0 + s * 16 + col;
-      if (tok >= a.vocab) continue;
-      T* row = (T*)a.dweight + (int64_t)tok * a.dweight_stride;
+      union {
+        uint2 u;
+        T e[4];
+      } o;
+      uint2 all[kN];
 #pragma unroll
       for (int v = 0; v < kN; ++v) {
-        const uint32_t h = i0 + v * 16 + q * 4;
-        struct __attribute__((packed, aligned(2))) Four {
-          T e[4];
-        } o;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o.e[e] = (T)(acc[v][s][e] * f);
-        if (h + 4 <= a.hidden) {
-          *(Four*)(row + h) = o;
-        } else {
+        all[v] = o.u;
+      }
+      const uint32_t tok = a.first + j0 + s * 16;
+      if constexpr (kLines) {
+        store_rows<kN>(all, mine, lane, [&](uint32_t r, uint32_t c, u32x4 v) {
+          if (tok + r < a.vocab && i0 + c < a.hidden)  // (whole lines of columns)
+            store_vec((T*)a.dweight + (int64_t)(tok + r) * a.dweight_stride + i0 + c, v);
+        });
+        __builtin_amdgcn_sched_barrier(0);
+      } else if (tok + col < a.vocab) {
+        T* row = (T*)a.dweight + (int64_t)(tok + col) * a.dweight_stride;
+#pragma unroll
+        for (int v = 0; v < kN; ++v) {
+          const uint32_t h = i0 + v * 16 + q * 4;
+          o.u = all[v];
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (h + e < a.hidden) row[h + e] = o.e[e];
@@ -414,13 +522,12 @@ __global__ void __launch_bounds__(kThreads) xent_product(Args a) {
     split = rest / ((a.hidden64 + kBN - 1) / kBN);
     const uint32_t last = a.vocab - 1 - a.first;  // (columns of g past the vocabulary are zero)
     po = Operand{(const T*)a.weight + (int64_t)a.first * a.weight_stride, a.weight_stride, last + 1, a.hidden};
-    qo = Operand{a.slopes, a.piece, a.rows64, a.piece};
+    qo = Operand{a.slopes, a.slope_stride, a.rows64, a.piece};
     k0 = split * a.split_steps * kBK;
     k1 = min(k0 + a.split_steps * kBK, a.width);
-    if (k0 >= k1) return;  // (a last piece of fewer parts)
   } else {
     po = Operand{a.xs, a.hidden64, a.rows64, a.hidden64};
-    qo = Operand{a.slopes, a.piece, a.rows64, a.piece};
+    qo = Operand{a.slopes, a.slope_stride, a.rows64, a.piece};
     k1 = a.rows64;
   }
   const uint32_t i0 = ti * kBN + (kKind == kSlopes ? a.first : 0), j0 = tj * kBM;
@@ -446,7 +553,8 @@ __global__ void __launch_bounds__(kThreads) xent_product(Args a) {
         for (int j = 0; j < kBM / 16; ++j) acc[i][j] = mfma(pf[i], qf[j], acc[i][j], T{});
     }
   }
-  finish<T, kKind, 2, kBM / 16, 4, kBM>(a, threadIdx.x, ti, i0 + wave * 32, j0, 0, wave, split, acc, joined);
+  finish<T, kKind, 2, kBM / 16, 4, kBM, false>(a, threadIdx.x, ti, i0 + wave * 32, j0, 0, wave, split, acc, joined,
+                                                nullptr);
 }
 
 // Operands whose rows are whole lines of 128 bytes: tiles of 256 of i by BM of
@@ -560,12 +668,13 @@ struct Lines {
   }
 };
 
-// Tile (j, i, split) of a workgroup.  Consecutive workgroups go to the XCDs in
+// Tile (j, i, split) of n, in turn.  Consecutive workgroups go to the XCDs in
 // turn, so each XCD takes a run of tiles; a run goes over four tiles of j at a
 // time, then over i: what an XCD runs at once shares operands in its L2.
-__device__ __forceinline__ void tile_of(uint32_t js, uint32_t is, uint32_t* tj, uint32_t* ti, uint32_t* split) {
-  const uint32_t n = gridDim.x, run = n / 8;
-  uint32_t t = blockIdx.x < run * 8 ? (blockIdx.x % 8) * run + blockIdx.x / 8 : blockIdx.x;
+__device__ __forceinline__ void tile_of(uint32_t block, uint32_t n, uint32_t js, uint32_t is, uint32_t* tj,
+                                        uint32_t* ti, uint32_t* split) {
+  const uint32_t run = n / 8;
+  uint32_t t = block < run * 8 ? (block % 8) * run + block / 8 : block;
   *split = t / (js * is);
   t -= *split * (js * is);
   constexpr uint32_t kGroup = 4;
@@ -580,109 +689,124 @@ struct TileShape {
   static constexpr int BM = 16 * kBMs, WM = kWM, WN = 8 / kWM, M = kBMs / WM, N = 16 / WN;
 };
 
+// Workgroups take tiles in turn: the next one's first two steps are copied
+// before what this one leaves is worked out.
 template <typename T, Kind kKind, typename S>
 __global__ void __launch_bounds__(kTileThreads) xent_tile(Args a) {
   using P = Lines<T, kKind >= kStates, kTileBN, kKind == kTable>;
   using Q = Lines<T, kKind == kTable, S::BM, true>;
   __shared__ __attribute__((aligned(1024))) char st0[P::kBytes + Q::kBytes], st1[P::kBytes + Q::kBytes];
-  const uint32_t tid = threadIdx.x, lane = tid & 63;
-  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+  __shared__ float joined[kKind == kStats ? S::WN : 1][3][kKind == kStats ? S::BM : 1];
+  __shared__ u32x4 stored[kKind == kSlopes || kKind == kTable ? 8 * kStored<S::N> / 16 : 1];
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t wm = wave % S::WM, wn = wave / S::WM;
-  uint32_t tj, ti, split, k0 = 0, steps;
+  const uint32_t js = kKind == kTable ? a.width / S::BM : (a.rows64 + S::BM - 1) / S::BM;
+  const uint32_t is = kKind == kStats    ? a.tiles
+                      : kKind == kSlopes ? a.width / kTileBN
+                                         : (a.hidden64 + kTileBN - 1) / kTileBN;
+  const uint32_t splits = kKind == kStates ? (a.width / 64 + a.split_steps - 1) / a.split_steps : 1;
+  const uint32_t tiles = js * is * splits;
+  uint32_t tj, ti, split, steps;
   P p;
   Q x;
-  {
-    const uint32_t js = kKind == kTable ? a.width / S::BM : (a.rows64 + S::BM - 1) / S::BM;
-    const uint32_t is = kKind == kStats ? a.tiles : kKind == kSlopes ? a.width / kTileBN : (a.hidden64 + kTileBN - 1) / kTileBN;
-    tile_of(js, is, &tj, &ti, &split);
+  const auto copy = [&](char* st, uint32_t i, uint32_t lane) {
+    const uint32_t k = min(i, steps - 1);  // (past the end: again, unused)
+    p.copy(st, k, lane, wave);
+    x.copy(st + P::kBytes, k, lane, wave);
+  };
+  const auto begin = [&](uint32_t block) {
+    uint32_t tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));  // (nothing of this is kept through a tile)
+    tile_of(block, tiles, js, is, &tj, &ti, &split);
     Operand po, qo;
+    uint32_t k0 = 0;
     if (kKind == kStats || kKind == kSlopes) {
       po = Operand{a.weight, a.weight_stride, a.vocab, a.hidden};
       qo = Operand{a.x, a.x_stride, a.rows, a.hidden};
       steps = a.hidden64 / 64;
     } else if (kKind == kStates) {
       po = Operand{(const T*)a.weight + (int64_t)a.first * a.weight_stride, a.weight_stride, a.vocab - a.first, a.hidden};
-      qo = Operand{a.slopes, a.piece, a.rows64, a.piece};
+      qo = Operand{a.slopes, a.slope_stride, a.rows64, a.piece};
       k0 = split * a.split_steps * 64;
-      if (k0 >= a.width) return;  // (a last piece of fewer parts)
       steps = min(a.split_steps, a.width / 64 - split * a.split_steps);
     } else {
       po = Operand{a.xs, a.hidden64, a.rows64, a.hidden64};
-      qo = Operand{a.slopes, a.piece, a.rows64, a.piece};
+      qo = Operand{a.slopes, a.slope_stride, a.rows64, a.piece};
       steps = a.rows64 / 64;
     }
-    const uint32_t first = kKind == kSlopes ? a.first : 0;
-    p.begin(po, ti * kTileBN + first, k0, wn * S::N, tid, wave);
+    p.begin(po, ti * kTileBN + (kKind == kSlopes ? a.first : 0), k0, wn * S::N, tid, wave);
     x.begin(qo, tj * S::BM, k0, wm * S::M, tid, wave);
-  }
-  const auto copy = [&](char* st, uint32_t i) {
-    const uint32_t k = min(i, steps - 1);  // (past the end: again, unused)
-    p.copy(st, k, lane, wave);
-    x.copy(st + P::kBytes, k, lane, wave);
+    copy(st0, 0, tid & 63);
+    copy(st1, 1, tid & 63);
   };
-  f32x4 acc[S::N][S::M] = {};
-  constexpr int kCopies = P::kTurns + Q::kTurns;
-  // Half a step: the products of w and x, while w and `ahead` take the next
-  // half's operands, kk of the stage `next`.  A register of w is free when its
-  // products are issued; x has two sets.
-  u32x4 w[S::N], x0[S::M], x1[S::M];
-  const auto half = [&](const u32x4 (&now)[S::M], u32x4 (&ahead)[S::M], const char* next, int kk) {
+  begin(blockIdx.x);
+  for (uint32_t block = blockIdx.x;;) {
+    f32x4 acc[S::N][S::M] = {};
+    // Half a step: the products of w and x, while w and `ahead` take the next
+    // half's operands, kk of the stage `next`.  A register of w is free when
+    // its products are issued; x has two sets.
+    u32x4 w[S::N], x0[S::M], x1[S::M];
+    const auto half = [&](const u32x4 (&now)[S::M], u32x4 (&ahead)[S::M], const char* next, int kk) {
 #pragma unroll
-    for (int v = 0; v < S::N; ++v) {
+      for (int v = 0; v < S::N; ++v) {
 #pragma unroll
-      for (int j = 0; j < S::M; ++j) acc[v][j] = mfma(w[v], now[j], acc[v][j], T{});
-      w[v] = p.read(next, v, kk);
-      constexpr int kEach = (S::M + S::N - 1) / S::N;
+        for (int j = 0; j < S::M; ++j) acc[v][j] = mfma(w[v], now[j], acc[v][j], T{});
+        w[v] = p.read(next, v, kk);
+        constexpr int kEach = (S::M + S::N - 1) / S::N;
 #pragma unroll
-      for (int j = v * kEach; j < (v + 1) * kEach && j < S::M; ++j) ahead[j] = x.read(next + P::kBytes, j, kk);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  };
-  // Step i: w and x0 hold its first half's operands.  At the barrier all of
-  // the step has been read, and the next is there.
-  const auto step = [&](uint32_t i, char* st, const char* next) {
-    half(x0, x1, st, 1);
+        for (int j = v * kEach; j < (v + 1) * kEach && j < S::M; ++j) ahead[j] = x.read(next + P::kBytes, j, kk);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    // Step i: w and x0 hold its first half's operands.  At the barrier all of
+    // the step has been read, and the next is there.
+    const auto step = [&](uint32_t i, char* st, const char* next) {
+      half(x0, x1, st, 1);
+      wait_copies<0>();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      copy(st, i + 2, threadIdx.x & 63);
+      half(x1, x0, next, 0);
+    };
     wait_copies<0>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    copy(st, i + 2);
-    half(x1, x0, next, 0);
-  };
-  copy(st0, 0);
-  copy(st1, 1);
-  wait_copies<kCopies>();
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
 #pragma unroll
-  for (int v = 0; v < S::N; ++v) w[v] = p.read(st0, v, 0);
+    for (int v = 0; v < S::N; ++v) w[v] = p.read(st0, v, 0);
 #pragma unroll
-  for (int j = 0; j < S::M; ++j) x0[j] = x.read(st0 + P::kBytes, j, 0);
-  for (uint32_t i = 0;;) {
-    step(i, st0, st1);
-    if (++i == steps) break;
-    step(i, st1, st0);
-    if (++i == steps) break;
+    for (int j = 0; j < S::M; ++j) x0[j] = x.read(st0 + P::kBytes, j, 0);
+    for (uint32_t i = 0;;) {
+      step(i, st0, st1);
+      if (++i == steps) break;
+      step(i, st1, st0);
+      if (++i == steps) break;
+    }
+    wait_copies<0>();
+    __syncthreads();
+    const uint32_t jb = tj * S::BM, tile = ti, part = split;
+    block += gridDim.x;
+    const bool more = block < tiles;
+    if (more) begin(block);
+    uint32_t tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    finish<T, kKind, S::N, S::M, S::WN, S::BM, true>(
+        a, tid, tile, tile * kTileBN + (kKind == kSlopes ? a.first : 0) + wn * S::N * 16, jb, wm * S::M * 16, wn,
+        part, acc, (float(*)[3][S::BM])joined, (char*)stored + wave * kStored<S::N>);
+    if (!more) break;
   }
-  wait_copies<0>();
-  __syncthreads();
-  // (numbers of the thread anew, so that none of what follows is computed
-  // ahead and takes the loop's registers)
-  uint32_t after = threadIdx.x;
-  asm volatile("" : "+v"(after));
-  const uint32_t wave_after = (uint32_t)__builtin_amdgcn_readfirstlane((int)(after >> 6));
-  const uint32_t wm_after = wave_after % S::WM, wn_after = wave_after / S::WM;
-  finish<T, kKind, S::N, S::M, S::WN, S::BM>(
-      a, after, ti, ti * kTileBN + (kKind == kSlopes ? a.first : 0) + wn_after * S::N * 16, tj * S::BM,
-      wm_after * S::M * 16, wn_after, split, acc, (float(*)[3][S::BM])st0);
 }
 
 // --- plan -------------------------------------------------------------------
 
 constexpr uint32_t kCUs = 256;
+#ifndef KP
+#define KP 128
+#endif
+constexpr uint64_t kPieceBytes = (uint64_t)KP << 20;
 
 struct Plan {
   uint64_t mant, power, largest, part, picked, top, logsum, terms, xs, slopes, dxs, bytes;
-  uint32_t rows64, hidden64, tiles, piece, splits, split_steps, bm, bn;
+  uint32_t rows64, hidden64, tiles, piece, slope_stride, splits, split_steps, bm, bn;
   bool lines;
 };
 
@@ -702,6 +826,7 @@ Plan plan(const ft_cross_entropy_loss_args& a) {
   p.lines = whole_lines(a);
   p.bn = p.lines ? kTileBN : kBN;
   p.bm = !p.lines || p.rows64 <= 64 ? 64 : p.rows64 <= 128 ? 128 : 256;
+  if (p.bm == 256 && (p.rows64 + 191) / 192 * 192 < round_up(p.rows64, 256)) p.bm = 192;
   p.tiles = (a.vocab + p.bn - 1) / p.bn;
   const uint64_t r = p.rows64;
   p.mant = ar.take(r * 4);
@@ -714,10 +839,12 @@ Plan plan(const ft_cross_entropy_loss_args& a) {
   p.terms = ar.take(r * 4);
   if (a.dx || a.dweight) {
     // a piece's slopes: up to 128 MB, half of the last level's cache
-    const uint64_t whole = round_up(a.vocab, 256);
-    p.piece = (uint32_t)std::min(
-        whole, std::max<uint64_t>(256, (128ull << 20) / std::max<uint64_t>(64, r) / 512 * 256));
-    p.slopes = ar.take(r * p.piece * 2);
+    const uint64_t most = std::max<uint64_t>(256, kPieceBytes / std::max<uint64_t>(64, r) / 512 * 256);
+    const uint64_t pieces = (a.vocab + most - 1) / most;
+    p.piece = (uint32_t)round_up((a.vocab + pieces - 1) / pieces, 256);
+    // (rows a line more than a piece apart: not all on the same channels)
+    p.slope_stride = p.piece + 64;
+    p.slopes = ar.take(r * p.slope_stride * 2);
   }
   if (a.dweight) p.xs = ar.take(r * p.hidden64 * 2);
   if (a.dx) {
@@ -739,14 +866,18 @@ hipError_t product(const Args& a, const Plan& p, hipStream_t s) {
   const uint64_t js = kKind == kTable ? a.width / (p.lines ? 256 : p.bm) : (a.rows64 + p.bm - 1) / p.bm;
   const uint64_t blocks = js * (kKind == kStats    ? a.tiles
                                 : kKind == kSlopes ? a.width / p.bn
-                                : kKind == kStates ? hs * a.splits
+                                : kKind == kStates ? hs * ((a.width / 64 + a.split_steps - 1) / a.split_steps)
                                                    : hs);
   if (!p.lines) return start(xent_product<T, kKind>, blocks, kThreads, s, a);
   if constexpr (kKind != kTable) {
-    if (p.bm == 64) return start(xent_tile<T, kKind, TileShape<4, 1>>, blocks, kTileThreads, s, a);
-    if (p.bm == 128) return start(xent_tile<T, kKind, TileShape<8, 2>>, blocks, kTileThreads, s, a);
+    if (p.bm == 64)
+      return start(xent_tile<T, kKind, TileShape<4, 1>>, std::min<uint64_t>(blocks, (kKind == kSlopes ? 2 : 1) * kCUs),
+                   kTileThreads, s, a);
+    const uint64_t most = std::min<uint64_t>(blocks, kCUs);
+    if (p.bm == 128) return start(xent_tile<T, kKind, TileShape<8, 2>>, most, kTileThreads, s, a);
+    if (p.bm == 192) return start(xent_tile<T, kKind, TileShape<12, 2>>, most, kTileThreads, s, a);
   }
-  return start(xent_tile<T, kKind, TileShape<16, 2>>, blocks, kTileThreads, s, a);
+  return start(xent_tile<T, kKind, TileShape<16, 2>>, std::min<uint64_t>(blocks, kCUs), kTileThreads, s, a);
 }
 
 template <typename T>
@@ -759,7 +890,7 @@ hipError_t launch(Args a, const Plan& p, hipStream_t s) {
   if (e != hipSuccess) return e;
   e = product<T, kStats>(a, p, s);
   if (e != hipSuccess) return e;
-  e = start(xent_join, a.rows64 / 64, 1024, s, a);
+  e = start(xent_join, a.rows64 / 16, 1024, s, a);
   if (e != hipSuccess) return e;
   e = start(xent_loss, 1, 1024, s, a);
   if (e != hipSuccess || !(a.dx || a.dweight)) return e;
@@ -777,7 +908,7 @@ hipError_t launch(Args a, const Plan& p, hipStream_t s) {
     }
   }
   if (!a.dx) return hipSuccess;
-  return start(xent_states<T>, (a.rows + 3) / 4, 256, s, a);
+  return start(xent_states<T>, (uint64_t)a.rows * ((a.hidden64 + 255) / 256), 64 * std::min(16u, a.splits), s, a);
 }
 
 }  // namespace
@@ -818,6 +949,7 @@ hipError_t launch_cross_entropy_loss(const ft_cross_entropy_loss_args& q, uint8_
   a.slopes = ws + p.slopes;
   a.dxs = (float*)(ws + p.dxs);
   a.piece = p.piece;
+  a.slope_stride = p.slope_stride;
   a.splits = p.splits;
   a.split_steps = p.split_steps;
   return q.dtype == FT_BF16 ? launch<__bf16>(a, p, s) : launch<_Float16>(a, p, s);
