@@ -799,10 +799,6 @@ __global__ void __launch_bounds__(kTileThreads) xent_tile(Args a) {
 // --- plan -------------------------------------------------------------------
 
 constexpr uint32_t kCUs = 256;
-#ifndef KP
-#define KP 128
-#endif
-constexpr uint64_t kPieceBytes = (uint64_t)KP << 20;
 
 struct Plan {
   uint64_t mant, power, largest, part, picked, top, logsum, terms, xs, slopes, dxs, bytes;
@@ -838,8 +834,9 @@ Plan plan(const ft_cross_entropy_loss_args& a) {
   p.logsum = ar.take(r * 4);
   p.terms = ar.take(r * 4);
   if (a.dx || a.dweight) {
-    // a piece's slopes: up to 128 MB, half of the last level's cache
-    const uint64_t most = std::max<uint64_t>(256, kPieceBytes / std::max<uint64_t>(64, r) / 512 * 256);
+    // a piece's slopes: up to 128 MB, half of the last level's cache (512 MB
+    // take the same time within 2%)
+    const uint64_t most = std::max<uint64_t>(256, (128ull << 20) / std::max<uint64_t>(64, r) / 512 * 256);
     const uint64_t pieces = (a.vocab + most - 1) / most;
     p.piece = (uint32_t)round_up((a.vocab + pieces - 1) / pieces, 256);
     // (rows a line more than a piece apart: not all on the same channels)

@@ -147,18 +147,18 @@ struct Args {
   float* xscale;  // [rows to whole 16s]: power of two that x was divided by
 };
 
-// A wave a row: its power of two, then its operands; zero behind the rows.
+// A wave puts a row's operands to `to`, 64 vectors from step to step and 16
+// from quarter to quarter, zero where it is none; returns the power of two
+// that it was divided by.
 template <typename T>
-__global__ void __launch_bounds__(256) packed_rows(Args a) {
-  const uint32_t lane = threadIdx.x & 63, r = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (r >= a.row_tiles * 16) return;
-  const T* row = (const T*)a.x + (int64_t)min(r, a.rows - 1) * a.x_stride;
+__device__ __forceinline__ float put_row(const T* row, uint32_t hidden, uint32_t steps, uint32_t lane, bool any,
+                                         u32x4* to) {
   int e = 0;
-  if (sizeof(T) == 2 && !__is_same(T, _Float16)) {
+  if (!__is_same(T, _Float16)) {
     float big = 0.0f;
-    for (uint32_t k = lane * 8; k < a.hidden; k += 512) {
+    for (uint32_t k = lane * 8; k < hidden; k += 512) {
       float v[8];
-      to_float<T>(load_row_vec(row, k, a.hidden, (T)0.0f), v);
+      to_float<T>(load_row_vec(row, k, hidden, (T)0.0f), v);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (fabsf(v[i]) < INFINITY) big = fmaxf(big, fabsf(v[i]));
@@ -166,10 +166,9 @@ __global__ void __launch_bounds__(256) packed_rows(Args a) {
     big = wave_max(big);
     if (big > 0.0f) (void)frexpf(big, &e), e -= 15;
   }
-  if (lane == 0) a.xscale[r] = ldexpf(1.0f, e);
-  const uint32_t steps = a.chunks * 4;
   for (uint32_t k = lane; k < steps * 4; k += 64) {
-    u32x4 v = load_row_vec(row, k * 8, a.hidden, (T)0.0f);
+    u32x4 v{};
+    if (any) v = load_row_vec(row, k * 8, hidden, (T)0.0f);
     if (!__is_same(T, _Float16)) {
       float f[8];
       to_float<T>(v, f);
@@ -177,17 +176,53 @@ __global__ void __launch_bounds__(256) packed_rows(Args a) {
       for (int i = 0; i < 8; ++i) f[i] = ldexpf(f[i], -e);
       v = from_float<_Float16>(f);
     }
-    if (r >= a.rows) v = u32x4{};
-    a.xs[((uint64_t)(r >> 4) * steps + (k >> 2)) * 64 + (k & 3) * 16 + (r & 15)] = v;
+    to[(k >> 2) * 64 + (k & 3) * 16] = v;
   }
+  return ldexpf(1.0f, e);
 }
 
-// Scale g of a chunk's for this lane's token.
+// A wave a row.
+template <typename T>
+__global__ void __launch_bounds__(256) packed_rows(Args a) {
+  const uint32_t lane = threadIdx.x & 63, r = blockIdx.x * 4 + (threadIdx.x >> 6), steps = a.chunks * 4;
+  if (r >= a.row_tiles * 16) return;
+  const T* row = (const T*)a.x + (int64_t)min(r, a.rows - 1) * a.x_stride;
+  const float down = put_row<T>(row, a.hidden, steps, lane, r < a.rows,
+                                a.xs + (uint64_t)(r >> 4) * steps * 64 + (r & 15));
+  if (lane == 0) a.xscale[r] = down;
+}
+
+// The scales of a chunk's groups for this lane's token.
 template <typename T, int kPer>
 struct alignas(2 * kPer) Scales {
   T s[kPer];
 };
 
+// Adds chunk c's products to the sums of kM row tiles: a group's product in
+// whole numbers, then times its scale.  x(m, i): row tile m's operand of step i.
+template <typename T, int kPer, int kM, typename X>
+__device__ __forceinline__ void add_chunk(u32x4 w, Scales<T, kPer> sc, uint32_t c, uint32_t hidden,
+                                          f32x4 (&acc)[kM], X&& x) {
+  constexpr int kWords = 4 / kPer;
+#pragma unroll
+  for (int g = 0; g < kPer; ++g) {
+    // (a group past the columns: whatever its scale)
+    const float s = c * 128 + g * (128 / kPer) < hidden ? (float)sc.s[g] : 0.0f;
+    f32x4 part[kM] = {};
+#pragma unroll
+    for (int i = g * kWords; i < (g + 1) * kWords; ++i) {
+      const u32x4 wf = unpack(w[i]);
+#pragma unroll
+      for (int m = 0; m < kM; ++m) part[m] = mfma(x(m, i), wf, part[m]);
+    }
+#pragma unroll
+    for (int m = 0; m < kM; ++m)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[m][e] = __builtin_fmaf(part[m][e], s, acc[m][e]);
+  }
+}
+
+// Any number of columns: x's operands from memory (they stay in the caches).
 // A wave a tile of 16 tokens, kM row tiles at a time.
 template <typename T, typename O, int kPer, int kM>
 __global__ void __launch_bounds__(256) packed_direct(Args a) {
@@ -195,31 +230,15 @@ __global__ void __launch_bounds__(256) packed_direct(Args a) {
   const uint32_t tile = blockIdx.x * 4 + (threadIdx.x >> 6), tiles = (a.vocab + 15) / 16;
   if (tile >= tiles) return;
   const uint32_t steps = a.chunks * 4, token = tile * 16 + n;
-  constexpr int kWords = 4 / kPer;
   for (uint32_t m0 = 0; m0 < a.row_tiles; m0 += kM) {
     f32x4 acc[kM] = {};
     for (uint32_t c = 0; c < a.chunks; ++c) {
       const uint64_t at = (uint64_t)tile * a.chunks + c;
       const u32x4 w = a.packed[at * 64 + lane];
       const Scales<T, kPer> sc = ((const Scales<T, kPer>*)a.scales)[at * 16 + n];
-#pragma unroll
-      for (int g = 0; g < kPer; ++g) {
-        // (a group past the columns: whatever its scale)
-        const float s = c * 128 + g * (128 / kPer) < a.hidden ? (float)sc.s[g] : 0.0f;
-        f32x4 part[kM] = {};
-#pragma unroll
-        for (int i = g * kWords; i < (g + 1) * kWords; ++i) {
-          const u32x4 wf = unpack(w[i]);
-#pragma unroll
-          for (int m = 0; m < kM; ++m)
-            part[m] = mfma(a.xs[((uint64_t)min(m0 + m, a.row_tiles - 1) * steps + c * 4 + i) * 64 + lane],
-                           wf, part[m]);
-        }
-#pragma unroll
-        for (int m = 0; m < kM; ++m)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[m][e] = __builtin_fmaf(part[m][e], s, acc[m][e]);
-      }
+      add_chunk<T, kPer, kM>(w, sc, c, a.hidden, acc, [&](int m, int i) {
+        return a.xs[((uint64_t)min(m0 + m, a.row_tiles - 1) * steps + c * 4 + i) * 64 + lane];
+      });
     }
 #pragma unroll
     for (int m = 0; m < kM; ++m)
@@ -232,11 +251,89 @@ __global__ void __launch_bounds__(256) packed_direct(Args a) {
   }
 }
 
+// Up to kHeld vectors of x's operands in LDS, kM row tiles of them: a
+// workgroup a CU, whose waves take tiles of 16 tokens in turn, with the loads
+// of kAhead chunks in flight.  Past the first barrier the waves run by
+// themselves.  More rows than LDS holds go to other workgroups, beside these on
+// the same XCD, whose L2 then has the weights.
+constexpr uint32_t kHeld = 128 * 1024 / 16, kCUs = 256;
+constexpr int kStreamT = 1024, kAhead = 4;
+
+template <typename T, typename O, int kPer, int kM>
+__global__ void __launch_bounds__(kStreamT) packed_stream(Args a) {
+  __shared__ u32x4 xs[kHeld];
+  __shared__ float xscale[kM * 16];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, n = lane & 15, q = lane >> 4;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+  const uint32_t groups = (a.row_tiles + kM - 1) / kM, workers = gridDim.x / groups;
+  // (workgroup b goes to XCD b % 8)
+  const uint32_t eight = blockIdx.x / 8, whole = gridDim.x / (8 * groups) * 8 * groups;
+  const uint32_t group = blockIdx.x < whole ? eight % groups : (blockIdx.x - whole) % groups;
+  const uint32_t worker = blockIdx.x < whole ? eight / groups * 8 + blockIdx.x % 8
+                                             : whole / groups + (blockIdx.x - whole) / groups;
+  const uint32_t r0 = group * kM * 16, rows = min((uint32_t)kM * 16, a.rows - r0);
+  const uint32_t tiles = (a.vocab + 15) / 16, steps = a.chunks * 4;
+  const uint32_t first = worker * 16 + wave, stride = workers * 16;
+
+  // the loads run ahead of the products: chunk ac of tile at
+  uint32_t at = first, ac = 0;
+  u32x4 w[kAhead];
+  Scales<T, kPer> sc[kAhead];
+  const auto load = [&](int u) {
+    const uint64_t place = (uint64_t)min(at, tiles - 1) * a.chunks + ac;
+    w[u] = __builtin_nontemporal_load(a.packed + place * 64 + lane);
+    sc[u] = ((const Scales<T, kPer>*)a.scales)[place * 16 + n];
+    if (++ac == a.chunks) {
+      ac = 0;
+      at += stride;
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) load(u);
+
+  for (uint32_t r = wave; r < kM * 16; r += kStreamT / 64) {
+    const T* row = (const T*)a.x + (int64_t)(r0 + min(r, rows - 1)) * a.x_stride;
+    const float down = put_row<T>(row, a.hidden, steps, lane, r < rows, xs + (r >> 4) * steps * 64 + (r & 15));
+    if (lane == 0) xscale[r] = down;
+  }
+  __syncthreads();
+
+  f32x4 acc[kM] = {};
+  uint32_t tile = first, c = 0;
+  while (tile < tiles) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (tile >= tiles) break;
+      add_chunk<T, kPer, kM>(w[u], sc[u], c, a.hidden, acc,
+                             [&](int m, int i) { return xs[(m * steps + c * 4 + i) * 64 + lane]; });
+      load(u);
+      if (++c < a.chunks) continue;
+      const uint32_t token = tile * 16 + n;
+#pragma unroll
+      for (int m = 0; m < kM; ++m) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t row = m * 16 + q * 4 + e;
+          if (row < rows && token < a.vocab)
+            ((O*)a.out)[(int64_t)(r0 + row) * a.out_stride + token] = (O)(acc[m][e] * xscale[row]);
+        }
+        acc[m] = f32x4{};
+      }
+      c = 0;
+      tile += stride;
+    }
+  }
+}
+
+// Row tiles whose operands LDS holds; 0: not even one's.
+uint32_t held_tiles(uint32_t chunks) { return std::min<uint32_t>(4, kHeld / (chunks * 256)); }
+
 struct Plan {
   uint64_t xs, xscale, bytes;
 };
 Plan plan(const ft_packed_logits_args& a) {
   Plan p{};
+  if (held_tiles((a.hidden + 127) / 128)) return p;
   Arena ar;
   const uint64_t rows = round_up(a.rows, 16);
   p.xs = ar.take(rows * round_up(a.hidden, 128) * 2);
@@ -247,11 +344,19 @@ Plan plan(const ft_packed_logits_args& a) {
 
 template <typename T, typename O, int kPer>
 hipError_t launch(const Args& a, hipStream_t s) {
-  hipError_t e = start(packed_rows<T>, (a.row_tiles * 16 + 3) / 4, 256, s, a);
+  const uint32_t tiles = (a.vocab + 15) / 16;
+  if (const uint32_t held = held_tiles(a.chunks)) {
+    const uint32_t groups = (a.row_tiles + held - 1) / held, each = (a.row_tiles + groups - 1) / groups;
+    const uint32_t used = (a.row_tiles + each - 1) / each;
+    const uint64_t blocks = (uint64_t)used * std::max(1u, std::min(kCUs / used, (tiles + 15) / 16));
+    return each == 1   ? start(packed_stream<T, O, kPer, 1>, blocks, kStreamT, s, a)
+           : each == 2 ? start(packed_stream<T, O, kPer, 2>, blocks, kStreamT, s, a)
+           : each == 3 ? start(packed_stream<T, O, kPer, 3>, blocks, kStreamT, s, a)
+                       : start(packed_stream<T, O, kPer, 4>, blocks, kStreamT, s, a);
+  }
+  const hipError_t e = start(packed_rows<T>, (a.row_tiles * 16 + 3) / 4, 256, s, a);
   if (e != hipSuccess) return e;
-  const uint32_t blocks = ((a.vocab + 15) / 16 + 3) / 4;
-  if (a.row_tiles == 1) return start(packed_direct<T, O, kPer, 1>, blocks, 256, s, a);
-  return start(packed_direct<T, O, kPer, 4>, blocks, 256, s, a);
+  return start(packed_direct<T, O, kPer, 4>, (tiles + 3) / 4, 256, s, a);
 }
 template <typename T, typename O>
 hipError_t launch(const Args& a, uint32_t group, hipStream_t s) {
