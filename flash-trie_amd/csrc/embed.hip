@@ -298,6 +298,40 @@ __device__ __forceinline__ void store_floats(float* to, const float (&v)[kVec<T>
   for (int k = 0; k < kVec<T>; k += 4) *(f32x4*)(to + k) = f32x4{v[k], v[k + 1], v[k + 2], v[k + 3]};
 }
 
+// Adds rows pos(0 ... n - 1) of the gradient, eight loads ahead whatever the
+// runs are: take(i, values) in order.
+constexpr uint32_t kBatch = 8;
+template <typename T, typename Pos, typename Take>
+__device__ __forceinline__ void walk_rows(const GradArgs& a, uint32_t n, uint32_t e, Pos&& pos, Take&& take) {
+  u32x4 v[2][kBatch];
+  const auto load = [&](u32x4 (&to)[kBatch], uint32_t r) {
+#pragma unroll
+    for (uint32_t u = 0; u < kBatch; ++u) {
+      to[u] = u32x4{};
+      if (r + u < n) {
+        const uint32_t row = pos(r + u);
+        if (e < a.hidden) to[u] = load_row_vec((const T*)a.grad + (int64_t)row * a.grad_stride, e, a.hidden, (T)0.0f);
+      }
+    }
+  };
+  const auto add = [&](const u32x4 (&from)[kBatch], uint32_t r) {
+#pragma unroll
+    for (uint32_t u = 0; u < kBatch; ++u) {
+      if (r + u >= n) break;
+      float f[kVec<T>];
+      to_float<T>(from[u], f);
+      take(r + u, f);
+    }
+  };
+  load(v[0], 0);
+  for (uint32_t r = 0; r < n; r += 2 * kBatch) {
+    load(v[1], r + kBatch);
+    add(v[0], r);
+    load(v[0], r + 2 * kBatch);
+    add(v[1], r + kBatch);
+  }
+}
+
 // A wave kRun sorted positions by 64 vectors of their rows.
 template <typename T, int kRun>
 __global__ void __launch_bounds__(256) embed_sums(GradArgs a) {
@@ -310,36 +344,79 @@ __global__ void __launch_bounds__(256) embed_sums(GradArgs a) {
   const uint32_t pos = lane < n ? a.sorted_pos[i0 + lane] : 0u;
   const uint32_t prev = i0 ? a.sorted_key[i0 - 1] : ~0u;
   const uint32_t next = i0 + n < a.count ? a.sorted_key[i0 + n] : ~0u;
-  for (uint32_t i = 0; i < n;) {
-    const uint32_t k = (uint32_t)__builtin_amdgcn_readlane((int)key, (int)i);
-    if (k >= a.vocab) break;  // (so are all behind it)
-    const uint64_t other = __ballot(key != k) & ~((2ull << i) - 1);
-    const uint32_t j = min(n, other ? (uint32_t)__ffsll((unsigned long long)other) - 1u : 64u);
-    float sum[kVec<T>] = {};
-    for (uint32_t r = i; r < j; r += 4) {
-      u32x4 v[4];
-#pragma unroll
-      for (uint32_t u = 0; u < 4; ++u) {
-        const uint32_t row = (uint32_t)__builtin_amdgcn_readlane((int)pos, (int)min(r + u, j - 1));
-        v[u] = u32x4{};
-        if (r + u < j && e < a.hidden)
-          v[u] = load_row_vec((const T*)a.grad + (int64_t)row * a.grad_stride, e, a.hidden, (T)0.0f);
-      }
-#pragma unroll
-      for (uint32_t u = 0; u < 4; ++u) {
-        if (r + u >= j) break;
-        float f[kVec<T>];
-        to_float<T>(v[u], f);
+  // positions with a token (those without are behind them)
+  const uint32_t used = (uint32_t)__popcll(__ballot(key < a.vocab));
+  const auto key_at = [&](uint32_t i) { return (uint32_t)__builtin_amdgcn_readlane((int)key, (int)i); };
+  float sum[kVec<T>] = {};
+  bool starts = used && key_at(0) != prev;
+  walk_rows<T>(
+      a, used, e, [&](uint32_t i) { return (uint32_t)__builtin_amdgcn_readlane((int)pos, (int)i); },
+      [&](uint32_t i, const float (&f)[kVec<T>]) {
 #pragma unroll
         for (int c = 0; c < kVec<T>; ++c) sum[c] += f[c];
-      }
+        const uint32_t k = key_at(i), after = i + 1 < n ? key_at(i + 1) : next;
+        if (after == k && i + 1 < n) return;
+        // the token's last here
+        if (e < a.hidden) {
+          if (starts && after != k) write_row<T>(a, k, e, sum);
+          else store_floats<T>(part_of<T>(a, starts ? 1 : 0, run, e), sum);
+        }
+        starts = true;
+#pragma unroll
+        for (int c = 0; c < kVec<T>; ++c) sum[c] = 0.0f;
+      });
+}
+
+// Few positions of rows that are whole vectors, in one launch: a wave a
+// position and 64 vectors looks for the others of its token (and is done if
+// there is one before it), and the workgroups behind write zeros to the rows
+// of other tokens.
+template <typename T>
+__global__ void __launch_bounds__(256) embed_few(GradArgs a) {
+  __shared__ uint32_t list[4 * kSmall / 2];  // positions of 16 bits, a wave's each
+  const uint32_t tid = threadIdx.x, lane = tid & 63;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+  if (blockIdx.x < a.blocks) {
+    const uint32_t task = blockIdx.x * 4 + wave, p = task / a.panels;
+    const uint32_t e = (task % a.panels * 64 + lane) * kVec<T>;
+    if (p >= a.count) return;
+    const uint32_t k = key_of(a, p);
+    if (k >= a.vocab) return;
+    uint16_t* mine = (uint16_t*)list + wave * kSmall;
+    uint32_t n = 0;
+    for (uint32_t i0 = 0; i0 < a.count; i0 += 64) {
+      const uint32_t i = i0 + lane;
+      const uint64_t same = __ballot(i < a.count && key_of(a, i) == k);
+      if (same && n == 0 && i0 + (uint32_t)__ffsll((unsigned long long)same) - 1 < p) return;
+      if (same >> lane & 1) mine[n + (uint32_t)__popcll(same & ((1ull << lane) - 1))] = (uint16_t)i;
+      n += (uint32_t)__popcll(same);
     }
-    const bool starts = i > 0 || prev != k, ends = j < n || next != k;
-    if (e < a.hidden) {
-      if (starts && ends) write_row<T>(a, k, e, sum);
-      else store_floats<T>(part_of<T>(a, starts ? 1 : 0, run, e), sum);
-    }
-    i = j;
+    asm volatile("" ::: "memory");  // (a wave's LDS accesses are in order)
+    float sum[kVec<T>] = {};
+    walk_rows<T>(
+        a, n, e, [&](uint32_t i) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)mine[i]); },
+        [&](uint32_t, const float (&f)[kVec<T>]) {
+#pragma unroll
+          for (int c = 0; c < kVec<T>; ++c) sum[c] += f[c];
+        });
+    if (e < a.hidden) write_row<T>(a, k, e, sum);
+    return;
+  }
+  // rows r0 ... of the table, which have no gaps
+  const uint32_t per = a.hidden / kVec<T>, rows = a.zero_units, r0 = (blockIdx.x - a.blocks) * rows;
+  const uint32_t n = min(rows, a.vocab - r0);
+  for (uint32_t i = tid; i < (n + 31) / 32; i += 256) list[i] = 0;
+  __syncthreads();
+  for (uint32_t i = tid; i < a.count; i += 256) {
+    const uint32_t k = key_of(a, i) - r0;
+    if (k < n) atomicOr(&list[k / 32], 1u << k % 32);
+  }
+  __syncthreads();
+  T* to = (T*)a.dtable + (uint64_t)r0 * a.hidden;
+#pragma unroll 4
+  for (uint32_t v = tid; v < n * per; v += 256) {
+    const uint32_t row = v / per;
+    if (!(list[row / 32] >> row % 32 & 1)) store_vec(to + (uint64_t)v * kVec<T>, u32x4{});
   }
 }
 
@@ -422,6 +499,13 @@ hipError_t launch_grad(GradArgs a, hipStream_t s) {
   constexpr uint32_t kZeroBlocks = 512;
   const uint64_t units = a.add ? 0 : (uint64_t)a.zero_units * (a.zero_length == a.hidden ? a.vocab : 1);
   hipError_t e;
+  // (the zeros' rows without gaps, 16 to 128 KB a workgroup; a bit for each)
+  const uint32_t per = a.hidden / kVec<T>;
+  if (a.count <= kSmall && a.count > 0 && a.hidden % kVec<T> == 0 && (a.add || a.dtable_stride == (int64_t)a.hidden)) {
+    a.blocks = (a.count * a.panels + 3) / 4;
+    a.zero_units = std::min<uint32_t>(kSmall * 64, std::max(1u, 4096 / per));
+    return start(embed_few<T>, a.blocks + (a.add ? 0 : (a.vocab + a.zero_units - 1) / a.zero_units), 256, s, a);
+  }
   if (a.count <= kSmall) {
     a.zero_last = units;
     e = start(embed_sort_few<T>, 1 + std::min<uint64_t>(units, kZeroBlocks), kSortT, s, a);
