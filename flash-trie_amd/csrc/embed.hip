@@ -245,16 +245,27 @@ __global__ void __launch_bounds__(kSortT) embed_place(GradArgs a) {
     write_zeros<T>(a, blockIdx.x - a.blocks, gridDim.x - a.blocks);
     return;
   }
+  // two threads a digit, half of the workgroups' counts each, all their loads
+  // together
+  const uint32_t bin = tid % kBins, half = tid / kBins;
   uint32_t before = 0, all = 0;
-  if (tid < kBins)
-#pragma unroll 8
-    for (uint32_t b = 0; b < a.blocks; ++b) {
-      const uint32_t c = a.hist[b * kBins + tid];
-      before += b < blockIdx.x ? c : 0u;
-      all += c;
-    }
-  const uint32_t front = exclusive_over_block(all, p.waves);
-  if (tid < kBins) base[tid] = front + before;
+#pragma unroll
+  for (uint32_t i = 0; i < kSortBlocks / 2; ++i) {
+    const uint32_t b = 2 * i + half, c = b < a.blocks ? a.hist[b * kBins + bin] : 0u;
+    before += b < blockIdx.x ? c : 0u;
+    all += c;
+  }
+  if (half) {
+    p.at[bin][0] = before;
+    p.at[bin][1] = all;
+  }
+  __syncthreads();
+  if (!half) {
+    before += p.at[bin][0];
+    all += p.at[bin][1];
+  }
+  const uint32_t front = exclusive_over_block(half ? 0u : all, p.waves);
+  if (!half) base[bin] = front + before;
   __syncthreads();
   const uint32_t i0 = min(blockIdx.x * a.each, a.count), i1 = min(i0 + a.each, a.count);
   const uint32_t* key = a.key[a.from] + i0;
@@ -298,9 +309,9 @@ __device__ __forceinline__ void store_floats(float* to, const float (&v)[kVec<T>
   for (int k = 0; k < kVec<T>; k += 4) *(f32x4*)(to + k) = f32x4{v[k], v[k + 1], v[k + 2], v[k + 3]};
 }
 
-// Adds rows pos(0 ... n - 1) of the gradient, eight loads ahead whatever the
-// runs are: take(i, values) in order.
-constexpr uint32_t kBatch = 8;
+// Walks over rows pos(0 ... n - 1) of the gradient, up to eight loads ahead
+// whatever the runs are: take(i, values) in order.
+constexpr uint32_t kBatch = 4;
 template <typename T, typename Pos, typename Take>
 __device__ __forceinline__ void walk_rows(const GradArgs& a, uint32_t n, uint32_t e, Pos&& pos, Take&& take) {
   u32x4 v[2][kBatch];
