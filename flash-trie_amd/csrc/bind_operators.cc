@@ -136,9 +136,8 @@ struct Reader {
   // a small array of `dt`, made contiguous if it is not
   Tensor array(py::handle h, const char* name, const py::object& dt, const char* dt_name,
                std::initializer_list<int64_t> size) {
-    const Torch& t = torch();
     Tensor r = read(h, name, (int)size.size());
-    if (!attr(r.obj, t.dtype).is(dt)) fail_type(call, std::string(name) + " must be " + dt_name);
+    check_type(r, name, dt, dt_name);
     int i = 0;
     for (int64_t n : size) {
       if (r.size[i] != n)
@@ -146,9 +145,28 @@ struct Reader {
                              " in dimension " + std::to_string(i) + ", not " + std::to_string(n));
       ++i;
     }
+    return make_dense(r);
+  }
+
+  // the same of one to three dimensions of any size
+  Tensor array(py::handle h, const char* name, const py::object& dt, const char* dt_name) {
+    Tensor r = read(h, name, kAnyDims);
+    check_type(r, name, dt, dt_name);
+    return make_dense(r);
+  }
+
+ private:
+  static constexpr int kAnyDims = -3;  // one to three
+
+  void check_type(const Tensor& r, const char* name, const py::object& dt, const char* dt_name) {
+    if (!attr(r.obj, torch().dtype).is(dt)) fail_type(call, std::string(name) + " must be " + dt_name);
+  }
+
+  static Tensor make_dense(Tensor& r) {
+    const Torch& t = torch();
     int64_t want = 1;
     bool dense = true;
-    for (i = r.ndim - 1; i >= 0; --i) {
+    for (int i = r.ndim - 1; i >= 0; --i) {
       dense = dense && (r.size[i] <= 1 || r.step[i] == want);
       want *= r.size[i];
     }
@@ -159,12 +177,13 @@ struct Reader {
     return r;
   }
 
- private:
   void fill(Tensor& r, const char* name, int dims) {
     const Torch& t = torch();
     const py::object shape = attr(r.obj, t.shape);
     r.ndim = (int)PyTuple_GET_SIZE(shape.ptr());
-    if (r.ndim != dims)
+    if (dims < 0 && (r.ndim < 1 || r.ndim > -dims))
+      fail_value(call, std::string(name) + " must have 1 to " + std::to_string(-dims) + " dimensions");
+    if (dims >= 0 && r.ndim != dims)
       fail_value(call, std::string(name) + " must have " + std::to_string(dims) +
                            " dimensions, not " + std::to_string(r.ndim));
     const py::object step = call0(r.obj, t.stride);
@@ -536,13 +555,9 @@ struct Tokens {
 Tokens read_tokens(Reader& in, py::handle tokens, py::handle lengths) {
   const Torch& t = torch();
   Tokens q;
-  const int dims = py::hasattr(tokens, "dim") ? py::cast<int>(tokens.attr("dim")()) : 1;
-  if (dims < 1 || dims > 3) fail_value(in.call, "tokens must have 1 to 3 dimensions");
-  const Tensor shape = in.read(tokens, "tokens", dims);
-  const int64_t* n = shape.size;
-  q.tokens = dims == 1   ? in.array(tokens, "tokens", t.int32, "int32", {n[0]})
-             : dims == 2 ? in.array(tokens, "tokens", t.int32, "int32", {n[0], n[1]})
-                         : in.array(tokens, "tokens", t.int32, "int32", {n[0], n[1], n[2]});
+  q.tokens = in.array(tokens, "tokens", t.int32, "int32");
+  const int dims = q.tokens.ndim;
+  const int64_t* n = q.tokens.size;
   for (int i = 0; i + 1 < dims; ++i) q.groups *= n[i];
   q.steps = n[dims - 1];
   if (!lengths.is_none()) {

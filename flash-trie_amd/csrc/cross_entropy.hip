@@ -77,6 +77,8 @@ struct Args {
   uint32_t piece, first, width;  // most tokens of it; its first; its tokens up to whole 256s
   uint32_t slope_stride;  // of the slopes' rows
   uint32_t splits, split_steps;  // parts of dx and their steps of 64
+  uint64_t split_stride;
+  uint32_t prepare;  // workgroups in front of the statistics' that prepare rows
 };
 
 // A part of a row's statistics is (c, s): s = sum of 2^(l log2 e - c), c the
@@ -104,13 +106,14 @@ __device__ __forceinline__ int exponent_of(const Args& a, uint32_t t, float* m) 
   return e - 1;
 }
 
-// A wave a row.
-template <typename T>
-__global__ void __launch_bounds__(256) xent_rows(Args a) {
-  __shared__ int biggest[4];
+// Rows' weights and, for the table's gradient, their scaled states: a wave of
+// kWaves a row.
+template <typename T, int kWaves>
+__device__ __forceinline__ void prepare_rows(const Args& a, uint32_t block) {
+  __shared__ int biggest[kWaves];
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int big = -1000;
-  for (uint32_t t = tid; t < a.rows; t += 256) {
+  for (uint32_t t = tid; t < a.rows; t += 64 * kWaves) {
     float m;
     big = max(big, exponent_of(a, t, &m));
   }
@@ -118,9 +121,10 @@ __global__ void __launch_bounds__(256) xent_rows(Args a) {
   for (int d = 1; d < 64; d *= 2) big = max(big, __shfl_xor(big, d, 64));
   if (lane == 0) biggest[wave] = big;
   __syncthreads();
-  big = max(max(biggest[0], biggest[1]), max(biggest[2], biggest[3]));
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) big = max(big, biggest[w]);
   if (big == -1000) big = 0;
-  const uint32_t t = blockIdx.x * 4 + wave;
+  const uint32_t t = block * kWaves + wave;
   float m = 0.0f;
   int e = t < a.rows ? exponent_of(a, t, &m) : 0;
   if (e == -1000) e = m == 0.0f ? 0 : big;
@@ -146,11 +150,16 @@ __global__ void __launch_bounds__(256) xent_rows(Args a) {
     ((u32x4*)a.xs)[((uint64_t)t * a.hidden64 + k) / 8] = v;
   }
 }
+template <typename T>
+__global__ void __launch_bounds__(256) xent_rows(Args a) {
+  prepare_rows<T, 4>(a, blockIdx.x);
+}
 
-// 16 rows by 64 parts of the tiles.
-__global__ void __launch_bounds__(1024) xent_join(Args a) {
+// 16 rows by 64 parts of the tiles.  A workgroup that has them all adds up the
+// loss.
+__device__ __forceinline__ void join_rows(const Args& a, uint32_t first) {
   __shared__ float sc[64][16], ss[64][16], sl[64][16];
-  const uint32_t row = threadIdx.x & 15, from = threadIdx.x >> 4, t = blockIdx.x * 16 + row;
+  const uint32_t row = threadIdx.x & 15, from = threadIdx.x >> 4, t = first + row;
   const uint64_t each = (uint64_t)a.tiles * a.rows64;
   Part p{0.0f, 0.0f};
   float l = 0.0f;
@@ -200,7 +209,7 @@ __global__ void __launch_bounds__(1024) xent_join(Args a) {
   a.terms[t] = term;
 }
 
-__global__ void __launch_bounds__(1024) xent_loss(Args a) {
+__device__ __forceinline__ void add_loss(const Args& a) {
   __shared__ float waves[16];
   float sum = 0.0f;
   for (uint32_t t = threadIdx.x; t < a.rows; t += 1024) sum += a.terms[t];
@@ -211,6 +220,14 @@ __global__ void __launch_bounds__(1024) xent_loss(Args a) {
   sum = 0.0f;
   for (int w = 0; w < 16; ++w) sum += waves[w];
   *a.loss = sum;
+}
+__global__ void __launch_bounds__(1024) xent_loss(Args a) { add_loss(a); }
+__global__ void __launch_bounds__(1024) xent_join(Args a) {
+  for (uint32_t t = blockIdx.x * 16; t < a.rows; t += gridDim.x * 16) {
+    join_rows(a, t);
+    __syncthreads();
+  }
+  if (gridDim.x == 1) add_loss(a);
 }
 
 // No rows: a table's gradient of zeros.
@@ -228,12 +245,11 @@ __global__ void __launch_bounds__(1024) xent_states(Args a) {
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const uint32_t panels = (a.hidden64 + 255) / 256;
   const uint32_t t = blockIdx.x / panels, h = (blockIdx.x % panels * 64 + lane) * 4;
-  const uint64_t each = (uint64_t)a.rows64 * a.hidden64;
   f32x4 y{};
   if (h < a.hidden64) {
     const float* p = a.dxs + (uint64_t)t * a.hidden64 + h;
 #pragma unroll 4
-    for (uint32_t s = wave; s < a.splits; s += waves) y += *(const f32x4*)(p + s * each);
+    for (uint32_t s = wave; s < a.splits; s += waves) y += *(const f32x4*)(p + s * a.split_stride);
   }
   if (wave > 0) other[wave - 1][lane] = y;
   __syncthreads();
@@ -459,7 +475,7 @@ __device__ __forceinline__ void finish(const Args& a, uint32_t tid, uint32_t til
       for (int v = 0; v < kN; ++v) {
         const uint32_t h = i0 + v * 16 + q * 4;
         if (h >= a.hidden64) continue;
-        f32x4* to = (f32x4*)(a.dxs + ((uint64_t)split * a.rows64 + j0 + s * 16 + col) * a.hidden64 + h);
+        f32x4* to = (f32x4*)(a.dxs + split * a.split_stride + (uint64_t)(j0 + s * 16 + col) * a.hidden64 + h);
         *to = a.first ? *to + acc[v][s] : acc[v][s];
       }
     }
@@ -698,6 +714,14 @@ __global__ void __launch_bounds__(kTileThreads) xent_tile(Args a) {
   __shared__ __attribute__((aligned(1024))) char st0[P::kBytes + Q::kBytes], st1[P::kBytes + Q::kBytes];
   __shared__ float joined[kKind == kStats ? S::WN : 1][3][kKind == kStats ? S::BM : 1];
   __shared__ u32x4 stored[kKind == kSlopes || kKind == kTable ? 8 * kStored<S::N> / 16 : 1];
+  if constexpr (kKind == kStats && S::BM == 64) {
+    if (blockIdx.x < a.prepare) {
+      prepare_rows<T, 8>(a, blockIdx.x);
+      return;
+    }
+  }
+  const uint32_t own = blockIdx.x - (kKind == kStats ? a.prepare : 0);
+  const uint32_t workers = gridDim.x - (kKind == kStats ? a.prepare : 0);
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t wm = wave % S::WM, wn = wave / S::WM;
   const uint32_t js = kKind == kTable ? a.width / S::BM : (a.rows64 + S::BM - 1) / S::BM;
@@ -739,8 +763,8 @@ __global__ void __launch_bounds__(kTileThreads) xent_tile(Args a) {
     copy(st0, 0, tid & 63);
     copy(st1, 1, tid & 63);
   };
-  begin(blockIdx.x);
-  for (uint32_t block = blockIdx.x;;) {
+  begin(own);
+  for (uint32_t block = own;;) {
     f32x4 acc[S::N][S::M] = {};
     // Half a step: the products of w and x, while w and `ahead` take the next
     // half's operands, kk of the stage `next`.  A register of w is free when
@@ -784,7 +808,7 @@ __global__ void __launch_bounds__(kTileThreads) xent_tile(Args a) {
     wait_copies<0>();
     __syncthreads();
     const uint32_t jb = tj * S::BM, tile = ti, part = split;
-    block += gridDim.x;
+    block += workers;
     const bool more = block < tiles;
     if (more) begin(block);
     uint32_t tid = threadIdx.x;
@@ -796,13 +820,192 @@ __global__ void __launch_bounds__(kTileThreads) xent_tile(Args a) {
   }
 }
 
+// Few rows, whose states fit LDS beside two tiles of the table: one pass over
+// the table leaves both gradients.  A workgroup takes tiles of kTok tokens in
+// turn: their logits (the waves share the hidden columns, or the 16-row
+// subtiles), slopes by way of LDS, then each wave, for its own columns, adds to
+// its sums for dx, which stay in registers to the end, and stores its part of
+// the tokens' dweight rows.  The next tile but one is on its way to registers
+// meanwhile.  A row of the table lies in LDS as it is, its 16-byte columns
+// exchanged by the row's number such that eight rows of a column, and two
+// columns of four rows, are free of bank conflicts: the logits read it by k,
+// dx across.
+constexpr uint32_t kFewBytes = 32768;  // of the states, or of a tile
+
+template <typename T, int kR, int kTok>
+__global__ void __launch_bounds__(512) xent_few(Args a) {
+  constexpr int kTiles = kR * kTok / 16, kSplits = 8 / kTiles;      // 16 x 16 tiles of logits, waves for one
+  constexpr int kSubs = 128 / kTok;  // 16-column subtiles of a wave: 512 or 1024 columns
+  constexpr int kLoads = (int)kFewBytes / 16 / 512, kPitch = 40;
+  __shared__ u32x4 st0[kFewBytes / 16], st1[kFewBytes / 16], xl[kFewBytes / 16];
+  __shared__ f32x4 part[8][64];
+  // the slopes, 32 of k and some space
+  __shared__ __attribute__((aligned(16))) T by_token[kTok][kPitch], by_row[kR * 16][kPitch];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 15, q = lane >> 4;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+  const uint32_t vecs = a.hidden / 8, tiles = (a.vocab + kTok - 1) / kTok, subs = a.hidden / 16;
+  const auto swap = [](uint32_t row) { return 2 * (row & 3) + (row >> 2 & 1); };
+
+  // a tile's vectors, of rows past the vocabulary the last's
+  u32x4 next[kLoads];
+  const auto load = [&](uint32_t tile) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const uint32_t at = i * 512 + tid, row = at / vecs;
+      if (row < (uint32_t)kTok)
+        next[i] = *(const u32x4*)((const T*)a.weight + (int64_t)min(tile * kTok + row, a.vocab - 1) * a.weight_stride +
+                                  (at - row * vecs) * 8);
+    }
+  };
+  const auto keep = [&](u32x4* st) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const uint32_t at = i * 512 + tid, row = at / vecs;
+      if (row < (uint32_t)kTok) st[row * vecs + ((at - row * vecs) ^ swap(row))] = next[i];
+    }
+  };
+  uint32_t tile = blockIdx.x;
+  load(tile);
+  for (uint32_t at = tid; at < kR * 16 * vecs; at += 512) {
+    const uint32_t row = at / vecs, c = at - row * vecs;
+    xl[row * vecs + (c ^ swap(row))] =
+        *(const u32x4*)((const T*)a.x + (int64_t)min(row, a.rows - 1) * a.x_stride + c * 8);
+  }
+  for (uint32_t i = tid; i < kTok * kPitch; i += 512) (&by_token[0][0])[i] = (T)0.0f;
+  for (uint32_t i = tid; i < kR * 16 * kPitch; i += 512) (&by_row[0][0])[i] = (T)0.0f;
+  // this wave's columns of the scaled states, transposed
+  u32x4 xs[kSubs];
+#pragma unroll
+  for (int j = 0; j < kSubs; ++j) {
+    union {
+      T e[8];
+      u32x4 v;
+    } u;
+    const uint32_t sub = wave + 8 * j;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t t = q * 8 + e;
+      u.e[e] = a.dweight && t < kR * 16u && sub < subs ? ((const T*)a.xs)[(uint64_t)t * a.hidden64 + sub * 16 + col]
+                                                       : (T)0.0f;
+    }
+    xs[j] = u.v;
+  }
+  // what a lane of the first waves knows of its row
+  const uint32_t ts = wave % kTiles % (kTok / 16), rs = wave % kTiles / (kTok / 16), t = rs * 16 + col;
+  const int32_t y = t < a.rows ? a.target[t] : -1;
+  const float m = a.mant[t] * kUp<T>, c = a.top[t], ls = a.logsum[t];
+  const float even = a.smoothing / (float)a.vocab, own = 1.0f - a.smoothing;
+  const float f = *a.largest * (1.0f / kUp<T>);
+  keep(st0);
+  f32x4 sum[kSubs][kR] = {};
+  const auto one = [&](const u32x4* st, u32x4* after) {
+    load(min(tile + gridDim.x, tiles - 1));
+    __syncthreads();
+    {
+      const uint32_t steps = a.hidden / 32, each = (steps + kSplits - 1) / kSplits;
+      const uint32_t s0 = wave / kTiles * each, s1 = min(s0 + each, steps);
+      const u32x4* wr = st + (ts * 16 + col) * vecs;
+      const u32x4* xr = xl + (rs * 16 + col) * vecs;
+      f32x4 l{};
+#pragma unroll 4
+      for (uint32_t s = s0; s < s1; ++s) {
+        const uint32_t at = (s * 4 + q) ^ swap(col);
+        l = mfma(wr[at], xr[at], l, T{});
+      }
+      part[wave][lane] = l;
+    }
+    __syncthreads();
+    if (wave < (uint32_t)kTiles) {
+      f32x4 l = part[wave][lane];
+#pragma unroll
+      for (int i = 1; i < kSplits; ++i) l += part[wave + i * kTiles][lane];
+      union {
+        T e[4];
+        uint2 u;
+      } o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t tok = tile * kTok + ts * 16 + q * 4 + e;
+        float g = exp2_raw(__builtin_fmaf(l[e], kLog2e, -c) - ls) - even;
+        if ((int32_t)tok == y) g -= own;
+        o.e[e] = (T)(m != 0.0f && tok < a.vocab ? g * m : 0.0f);
+        by_token[ts * 16 + q * 4 + e][t] = o.e[e];
+      }
+      *(uint2*)&by_row[t][ts * 16 + q * 4] = o.u;
+    }
+    __syncthreads();
+    if (a.dx) {
+      u32x4 gf[kR];
+#pragma unroll
+      for (int r = 0; r < kR; ++r) gf[r] = *(const u32x4*)&by_row[r * 16 + col][q * 8];
+#pragma unroll
+      for (int j = 0; j < kSubs; ++j) {
+        const uint32_t sub = wave + 8 * j;
+        if (sub >= subs) break;
+        union {
+          s16x4 h[2];
+          u32x4 v;
+        } w;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          // (tokens past a tile of 16: its own again, times zero)
+          const uint32_t row = (q * 8 + i * 4 + (col >> 2)) % kTok;
+          const char* p = (const char*)(st + row * vecs + ((sub * 2 + (col >> 1 & 1)) ^ swap(row))) + (col & 1) * 8;
+          w.h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+        }
+#pragma unroll
+        for (int r = 0; r < kR; ++r) sum[j][r] = mfma(w.v, gf[r], sum[j][r], T{});
+      }
+    }
+    keep(after);
+    if (a.dweight) {
+#pragma unroll
+      for (int i = 0; i < kTok / 16; ++i) {
+        const uint32_t tok = tile * kTok + i * 16 + col;
+        const u32x4 gf = *(const u32x4*)&by_token[i * 16 + col][q * 8];
+        T* row = (T*)a.dweight + (int64_t)tok * a.dweight_stride + q * 4;
+#pragma unroll
+        for (int j = 0; j < kSubs; ++j) {
+          const uint32_t sub = wave + 8 * j;
+          if (sub >= subs) break;
+          const f32x4 d = mfma(xs[j], gf, f32x4{}, T{});
+          struct __attribute__((packed, aligned(2))) Four {
+            T e[4];
+          } o;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o.e[e] = (T)(d[e] * f);
+          if (tok < a.vocab) *(Four*)(row + sub * 16) = o;
+        }
+      }
+    }
+    tile += gridDim.x;
+  };
+  while (tile < tiles) {
+    one(st0, st1);
+    if (tile >= tiles) break;
+    one(st1, st0);
+  }
+  if (!a.dx) return;
+#pragma unroll
+  for (int j = 0; j < kSubs; ++j) {
+    const uint32_t sub = wave + 8 * j;
+    if (sub >= subs) break;
+#pragma unroll
+    for (int r = 0; r < kR; ++r)
+      *(f32x4*)(a.dxs + blockIdx.x * a.split_stride + (uint64_t)(r * 16 + col) * a.hidden64 + sub * 16 + q * 4) =
+          sum[j][r];
+  }
+}
+
 // --- plan -------------------------------------------------------------------
 
 constexpr uint32_t kCUs = 256;
 
 struct Plan {
   uint64_t mant, power, largest, part, picked, top, logsum, terms, xs, slopes, dxs, bytes;
+  uint64_t split_stride;
   uint32_t rows64, hidden64, tiles, piece, slope_stride, splits, split_steps, bm, bn;
+  uint32_t few;  // 16-row subtiles of xent_few; 0: other kernels
   bool lines;
 };
 
@@ -825,6 +1028,8 @@ Plan plan(const ft_cross_entropy_loss_args& a) {
   if (p.bm == 256 && (p.rows64 + 191) / 192 * 192 < round_up(p.rows64, 256)) p.bm = 192;
   p.tiles = (a.vocab + p.bn - 1) / p.bn;
   const uint64_t r = p.rows64;
+  if (p.lines && a.rows <= 32 && round_up(a.rows, 16) * a.hidden * 2 <= kFewBytes && (a.dx || a.dweight))
+    p.few = (uint32_t)(a.rows + 15) / 16;
   p.mant = ar.take(r * 4);
   p.power = ar.take(r * 4);
   p.largest = ar.take(4);
@@ -833,7 +1038,7 @@ Plan plan(const ft_cross_entropy_loss_args& a) {
   p.top = ar.take(r * 4);
   p.logsum = ar.take(r * 4);
   p.terms = ar.take(r * 4);
-  if (a.dx || a.dweight) {
+  if ((a.dx || a.dweight) && !p.few) {
     // a piece's slopes: up to 128 MB, half of the last level's cache (512 MB
     // take the same time within 2%)
     const uint64_t most = std::max<uint64_t>(256, (128ull << 20) / std::max<uint64_t>(64, r) / 512 * 256);
@@ -844,14 +1049,20 @@ Plan plan(const ft_cross_entropy_loss_args& a) {
     p.slopes = ar.take(r * p.slope_stride * 2);
   }
   if (a.dweight) p.xs = ar.take(r * p.hidden64 * 2);
-  if (a.dx) {
+  if (p.few) {
+    const uint32_t tok = a.hidden <= 512 ? 32 : 16;
+    p.splits = std::min(kCUs, (a.vocab + tok - 1) / tok);
+    p.split_stride = 16ull * p.few * p.hidden64;
+    if (a.dx) p.dxs = ar.take(p.splits * p.split_stride * 4);
+  } else if (a.dx) {
     // as many parts of the sum over tokens as fill the chip
     const uint64_t tiles = std::max<uint64_t>(1, (r + p.bm - 1) / p.bm * ((p.hidden64 + p.bn - 1) / p.bn));
     const uint32_t steps = p.piece / kBK;
     const uint64_t want = std::max<uint64_t>(1, (p.lines ? 1 : 2) * kCUs / tiles);
     p.split_steps = (uint32_t)std::max<uint64_t>(4, (steps + want - 1) / want);
     p.splits = (steps + p.split_steps - 1) / p.split_steps;
-    p.dxs = ar.take((uint64_t)p.splits * r * p.hidden64 * 4);
+    p.split_stride = r * p.hidden64;
+    p.dxs = ar.take(p.splits * p.split_stride * 4);
   }
   p.bytes = ar.used;
   return p;
@@ -868,8 +1079,8 @@ hipError_t product(const Args& a, const Plan& p, hipStream_t s) {
   if (!p.lines) return start(xent_product<T, kKind>, blocks, kThreads, s, a);
   if constexpr (kKind != kTable) {
     if (p.bm == 64)
-      return start(xent_tile<T, kKind, TileShape<4, 1>>, std::min<uint64_t>(blocks, (kKind == kSlopes ? 2 : 1) * kCUs),
-                   kTileThreads, s, a);
+      return start(xent_tile<T, kKind, TileShape<4, 1>>,
+                   (kKind == kStats ? a.prepare : 0) + std::min<uint64_t>(blocks, kCUs), kTileThreads, s, a);
     const uint64_t most = std::min<uint64_t>(blocks, kCUs);
     if (p.bm == 128) return start(xent_tile<T, kKind, TileShape<8, 2>>, most, kTileThreads, s, a);
     if (p.bm == 192) return start(xent_tile<T, kKind, TileShape<12, 2>>, most, kTileThreads, s, a);
@@ -878,19 +1089,34 @@ hipError_t product(const Args& a, const Plan& p, hipStream_t s) {
 }
 
 template <typename T>
+hipError_t states(const Args& a, hipStream_t s) {
+  return start(xent_states<T>, (uint64_t)a.rows * ((a.hidden64 + 255) / 256), 64 * std::min(16u, a.splits), s, a);
+}
+
+template <typename T>
 hipError_t launch(Args a, const Plan& p, hipStream_t s) {
   if (a.rows == 0) {
     const hipError_t e = start(xent_loss, 1, 1024, s, a);
     return e == hipSuccess && a.dweight ? start(xent_nothing<T>, a.vocab, 256, s, a) : e;
   }
-  hipError_t e = start(xent_rows<T>, a.rows64 / 4, 256, s, a);
+  // few rows are prepared beside the statistics, and joined with the loss
+  hipError_t e = hipSuccess;
+  if (p.lines && p.bm == 64) a.prepare = a.rows64 / 8;
+  else e = start(xent_rows<T>, a.rows64 / 4, 256, s, a);
   if (e != hipSuccess) return e;
   e = product<T, kStats>(a, p, s);
   if (e != hipSuccess) return e;
-  e = start(xent_join, a.rows64 / 16, 1024, s, a);
+  const bool together = a.rows <= 16 || (a.rows <= 64 && a.tiles <= 256);
+  e = start(xent_join, together ? 1 : (a.rows + 15) / 16, 1024, s, a);
   if (e != hipSuccess) return e;
-  e = start(xent_loss, 1, 1024, s, a);
+  if (!together) e = start(xent_loss, 1, 1024, s, a);
   if (e != hipSuccess || !(a.dx || a.dweight)) return e;
+  if (p.few) {
+    e = p.few == 2         ? start(xent_few<T, 2, 32>, a.splits, 512, s, a)
+        : a.hidden <= 512  ? start(xent_few<T, 1, 32>, a.splits, 512, s, a)
+                           : start(xent_few<T, 1, 16>, a.splits, 512, s, a);
+    return e == hipSuccess && a.dx ? states<T>(a, s) : e;
+  }
   for (a.first = 0; a.first < a.vocab; a.first += a.piece) {
     a.width = (uint32_t)std::min<uint64_t>(a.piece, round_up(a.vocab - a.first, 256));
     e = product<T, kSlopes>(a, p, s);
@@ -905,7 +1131,7 @@ hipError_t launch(Args a, const Plan& p, hipStream_t s) {
     }
   }
   if (!a.dx) return hipSuccess;
-  return start(xent_states<T>, (uint64_t)a.rows * ((a.hidden64 + 255) / 256), 64 * std::min(16u, a.splits), s, a);
+  return states<T>(a, s);
 }
 
 }  // namespace
@@ -949,6 +1175,7 @@ hipError_t launch_cross_entropy_loss(const ft_cross_entropy_loss_args& q, uint8_
   a.slope_stride = p.slope_stride;
   a.splits = p.splits;
   a.split_steps = p.split_steps;
+  a.split_stride = p.split_stride;
   return q.dtype == FT_BF16 ? launch<__bf16>(a, p, s) : launch<_Float16>(a, p, s);
 }
 
