@@ -163,11 +163,21 @@ __device__ __forceinline__ void join_rows(const Args& a, uint32_t first) {
   const uint64_t each = (uint64_t)a.tiles * a.rows64;
   Part p{0.0f, 0.0f};
   float l = 0.0f;
-#pragma unroll 4
-  for (uint32_t i = from; i < a.tiles; i += 64) {
-    const uint64_t at = (uint64_t)i * a.rows64 + t;
-    p = join(p, Part{a.part[at], a.part[each + at]});
-    if (a.smoothing != 0.0f) l += a.part[2 * each + at];
+  for (uint32_t i = from; i < a.tiles; i += 64 * 8) {
+    float c[8], s[8], sum[8];  // (their loads together)
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const bool in = i + u * 64 < a.tiles;
+      const uint64_t at = (uint64_t)min(i + u * 64, a.tiles - 1) * a.rows64 + t;
+      c[u] = a.part[at];
+      s[u] = in ? a.part[each + at] : 0.0f;
+      sum[u] = in ? a.part[2 * each + at] : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      p = join(p, Part{c[u], s[u]});
+      l += sum[u];
+    }
   }
   sc[from][row] = p.c;
   ss[from][row] = p.s;
@@ -820,30 +830,34 @@ __global__ void __launch_bounds__(kTileThreads) xent_tile(Args a) {
   }
 }
 
-// Few rows, whose states fit LDS beside two tiles of the table: one pass over
-// the table leaves both gradients.  A workgroup takes tiles of kTok tokens in
-// turn: their logits (the waves share the hidden columns, or the 16-row
-// subtiles), slopes by way of LDS, then each wave, for its own columns, adds to
-// its sums for dx, which stay in registers to the end, and stores its part of
-// the tokens' dweight rows.  The next tile but one is on its way to registers
-// meanwhile.  A row of the table lies in LDS as it is, its 16-byte columns
-// exchanged by the row's number such that eight rows of a column, and two
-// columns of four rows, are free of bank conflicts: the logits read it by k,
-// dx across.
-constexpr uint32_t kFewBytes = 32768;  // of the states, or of a tile
+// Few rows, whose states fit LDS beside a tile of the table: one pass over the
+// table leaves both gradients.  A workgroup takes tiles of kTok tokens in turn:
+// their logits (the waves share the 16 x 16 tiles and the hidden columns),
+// slopes by way of LDS, then each wave, for its own columns, adds to its sums
+// for dx, which stay in registers to the end, and stores its part of the
+// tokens' dweight rows.  The next tile is on its way to registers meanwhile.  A
+// row of the table lies in LDS as it is, its 16-byte columns exchanged by the
+// row's number such that eight rows of a column, and two columns of four rows,
+// are free of bank conflicts: the logits read it by k, dx across.
+constexpr uint32_t kFewStates = 32768, kFewTile = 65536;  // bytes of the states, of a tile
+constexpr int kFewThreads = 1024;
 
 template <typename T, int kR, int kTok>
-__global__ void __launch_bounds__(512) xent_few(Args a) {
-  constexpr int kTiles = kR * kTok / 16, kSplits = 8 / kTiles;      // 16 x 16 tiles of logits, waves for one
-  constexpr int kSubs = 128 / kTok;  // 16-column subtiles of a wave: 512 or 1024 columns
-  constexpr int kLoads = (int)kFewBytes / 16 / 512, kPitch = 40;
-  __shared__ u32x4 st0[kFewBytes / 16], st1[kFewBytes / 16], xl[kFewBytes / 16];
-  __shared__ f32x4 part[8][64];
-  // the slopes, 32 of k and some space
-  __shared__ __attribute__((aligned(16))) T by_token[kTok][kPitch], by_row[kR * 16][kPitch];
+__global__ void __launch_bounds__(kFewThreads) xent_few(Args a) {
+  constexpr int kTiles = kR * kTok / 16, kSplits = 16 / kTiles;  // 16 x 16 tiles of logits, waves for one
+  constexpr int kSubs = 128 / kTok;  // 16-column subtiles of a wave: 1024 or 512 columns
+  constexpr int kLoads = (int)kFewTile / 16 / kFewThreads, kPitch = 40, kRowPitch = kTok + 8;
+  __shared__ u32x4 st[kFewTile / 16], xl[kFewStates / 16];
+  __shared__ f32x4 part[16][64];
+  __shared__ u32x4 lines[16 * kStored<kSubs> / 16];
+  // the slopes (32 rows of k, kTok tokens), and some space
+  __shared__ __attribute__((aligned(16))) T by_token[kTok][kPitch], by_row[kR * 16][kRowPitch];
   const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 15, q = lane >> 4;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
-  const uint32_t vecs = a.hidden / 8, tiles = (a.vocab + kTok - 1) / kTok, subs = a.hidden / 16;
+  const uint32_t vecs = a.hidden / 8, tiles = (a.vocab + kTok - 1) / kTok;
+  // this wave's columns: neighbours, so that it stores by lines
+  const uint32_t subs = a.hidden / 16, each_subs = (subs + 15) / 16, sub0 = wave * each_subs;
+  const uint32_t own_subs = sub0 < subs ? min(each_subs, subs - sub0) : 0;
   const auto swap = [](uint32_t row) { return 2 * (row & 3) + (row >> 2 & 1); };
 
   // a tile's vectors, of rows past the vocabulary the last's
@@ -851,28 +865,27 @@ __global__ void __launch_bounds__(512) xent_few(Args a) {
   const auto load = [&](uint32_t tile) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const uint32_t at = i * 512 + tid, row = at / vecs;
+      const uint32_t at = i * kFewThreads + tid, row = at / vecs;
       if (row < (uint32_t)kTok)
         next[i] = *(const u32x4*)((const T*)a.weight + (int64_t)min(tile * kTok + row, a.vocab - 1) * a.weight_stride +
                                   (at - row * vecs) * 8);
     }
   };
-  const auto keep = [&](u32x4* st) {
+  const auto keep = [&]() {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const uint32_t at = i * 512 + tid, row = at / vecs;
+      const uint32_t at = i * kFewThreads + tid, row = at / vecs;
       if (row < (uint32_t)kTok) st[row * vecs + ((at - row * vecs) ^ swap(row))] = next[i];
     }
   };
   uint32_t tile = blockIdx.x;
   load(tile);
-  for (uint32_t at = tid; at < kR * 16 * vecs; at += 512) {
+  for (uint32_t at = tid; at < kR * 16 * vecs; at += kFewThreads) {
     const uint32_t row = at / vecs, c = at - row * vecs;
     xl[row * vecs + (c ^ swap(row))] =
         *(const u32x4*)((const T*)a.x + (int64_t)min(row, a.rows - 1) * a.x_stride + c * 8);
   }
-  for (uint32_t i = tid; i < kTok * kPitch; i += 512) (&by_token[0][0])[i] = (T)0.0f;
-  for (uint32_t i = tid; i < kR * 16 * kPitch; i += 512) (&by_row[0][0])[i] = (T)0.0f;
+  for (uint32_t i = tid; i < kTok * kPitch; i += kFewThreads) (&by_token[0][0])[i] = (T)0.0f;
   // this wave's columns of the scaled states, transposed
   u32x4 xs[kSubs];
 #pragma unroll
@@ -881,24 +894,24 @@ __global__ void __launch_bounds__(512) xent_few(Args a) {
       T e[8];
       u32x4 v;
     } u;
-    const uint32_t sub = wave + 8 * j;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const uint32_t t = q * 8 + e;
-      u.e[e] = a.dweight && t < kR * 16u && sub < subs ? ((const T*)a.xs)[(uint64_t)t * a.hidden64 + sub * 16 + col]
-                                                       : (T)0.0f;
+      u.e[e] = a.dweight && t < kR * 16u && (uint32_t)j < own_subs
+                   ? ((const T*)a.xs)[(uint64_t)t * a.hidden64 + (sub0 + j) * 16 + col]
+                   : (T)0.0f;
     }
     xs[j] = u.v;
   }
-  // what a lane of the first waves knows of its row
+  // the tile of logits that this wave shares, and what a lane knows of its row
   const uint32_t ts = wave % kTiles % (kTok / 16), rs = wave % kTiles / (kTok / 16), t = rs * 16 + col;
   const int32_t y = t < a.rows ? a.target[t] : -1;
   const float m = a.mant[t] * kUp<T>, c = a.top[t], ls = a.logsum[t];
   const float even = a.smoothing / (float)a.vocab, own = 1.0f - a.smoothing;
   const float f = *a.largest * (1.0f / kUp<T>);
-  keep(st0);
+  keep();
   f32x4 sum[kSubs][kR] = {};
-  const auto one = [&](const u32x4* st, u32x4* after) {
+  for (; tile < tiles; tile += gridDim.x) {
     load(min(tile + gridDim.x, tiles - 1));
     __syncthreads();
     {
@@ -935,64 +948,62 @@ __global__ void __launch_bounds__(512) xent_few(Args a) {
     }
     __syncthreads();
     if (a.dx) {
-      u32x4 gf[kR];
 #pragma unroll
-      for (int r = 0; r < kR; ++r) gf[r] = *(const u32x4*)&by_row[r * 16 + col][q * 8];
+      for (int k = 0; k < kTok / 32; ++k) {
+        u32x4 gf[kR];
 #pragma unroll
-      for (int j = 0; j < kSubs; ++j) {
-        const uint32_t sub = wave + 8 * j;
-        if (sub >= subs) break;
-        union {
-          s16x4 h[2];
-          u32x4 v;
-        } w;
+        for (int r = 0; r < kR; ++r) gf[r] = *(const u32x4*)&by_row[r * 16 + col][k * 32 + q * 8];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          // (tokens past a tile of 16: its own again, times zero)
-          const uint32_t row = (q * 8 + i * 4 + (col >> 2)) % kTok;
-          const char* p = (const char*)(st + row * vecs + ((sub * 2 + (col >> 1 & 1)) ^ swap(row))) + (col & 1) * 8;
-          w.h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+        for (int j = 0; j < kSubs; ++j) {
+          if ((uint32_t)j >= own_subs) break;
+          union {
+            s16x4 h[2];
+            u32x4 v;
+          } w;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t row = k * 32 + q * 8 + i * 4 + (col >> 2);
+            const char* p = (const char*)(st + row * vecs + (((sub0 + j) * 2 + (col >> 1 & 1)) ^ swap(row))) + (col & 1) * 8;
+            w.h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+          }
+#pragma unroll
+          for (int r = 0; r < kR; ++r) sum[j][r] = mfma(w.v, gf[r], sum[j][r], T{});
         }
-#pragma unroll
-        for (int r = 0; r < kR; ++r) sum[j][r] = mfma(w.v, gf[r], sum[j][r], T{});
       }
     }
-    keep(after);
+    __syncthreads();
+    keep();
     if (a.dweight) {
 #pragma unroll
       for (int i = 0; i < kTok / 16; ++i) {
-        const uint32_t tok = tile * kTok + i * 16 + col;
+        const uint32_t tok = tile * kTok + i * 16;
         const u32x4 gf = *(const u32x4*)&by_token[i * 16 + col][q * 8];
-        T* row = (T*)a.dweight + (int64_t)tok * a.dweight_stride + q * 4;
+        uint2 all[kSubs];
 #pragma unroll
         for (int j = 0; j < kSubs; ++j) {
-          const uint32_t sub = wave + 8 * j;
-          if (sub >= subs) break;
           const f32x4 d = mfma(xs[j], gf, f32x4{}, T{});
-          struct __attribute__((packed, aligned(2))) Four {
+          union {
             T e[4];
+            uint2 u;
           } o;
 #pragma unroll
           for (int e = 0; e < 4; ++e) o.e[e] = (T)(d[e] * f);
-          if (tok < a.vocab) *(Four*)(row + sub * 16) = o;
+          all[j] = o.u;
         }
+        store_rows<kSubs>(all, (char*)lines + wave * kStored<kSubs>, lane, [&](uint32_t r, uint32_t c, u32x4 v) {
+          if (tok + r < a.vocab && c < own_subs * 16)
+            store_vec((T*)a.dweight + (int64_t)(tok + r) * a.dweight_stride + sub0 * 16 + c, v);
+        });
       }
     }
-    tile += gridDim.x;
-  };
-  while (tile < tiles) {
-    one(st0, st1);
-    if (tile >= tiles) break;
-    one(st1, st0);
   }
   if (!a.dx) return;
 #pragma unroll
   for (int j = 0; j < kSubs; ++j) {
-    const uint32_t sub = wave + 8 * j;
-    if (sub >= subs) break;
+    if ((uint32_t)j >= own_subs) break;
 #pragma unroll
     for (int r = 0; r < kR; ++r)
-      *(f32x4*)(a.dxs + blockIdx.x * a.split_stride + (uint64_t)(r * 16 + col) * a.hidden64 + sub * 16 + q * 4) =
+      *(f32x4*)(a.dxs + blockIdx.x * a.split_stride + (uint64_t)(r * 16 + col) * a.hidden64 + (sub0 + j) * 16 + q * 4) =
           sum[j][r];
   }
 }
@@ -1028,7 +1039,7 @@ Plan plan(const ft_cross_entropy_loss_args& a) {
   if (p.bm == 256 && (p.rows64 + 191) / 192 * 192 < round_up(p.rows64, 256)) p.bm = 192;
   p.tiles = (a.vocab + p.bn - 1) / p.bn;
   const uint64_t r = p.rows64;
-  if (p.lines && a.rows <= 32 && round_up(a.rows, 16) * a.hidden * 2 <= kFewBytes && (a.dx || a.dweight))
+  if (p.lines && a.rows <= 32 && round_up(a.rows, 16) * a.hidden * 2 <= kFewStates && (a.dx || a.dweight))
     p.few = (uint32_t)(a.rows + 15) / 16;
   p.mant = ar.take(r * 4);
   p.power = ar.take(r * 4);
@@ -1050,7 +1061,7 @@ Plan plan(const ft_cross_entropy_loss_args& a) {
   }
   if (a.dweight) p.xs = ar.take(r * p.hidden64 * 2);
   if (p.few) {
-    const uint32_t tok = a.hidden <= 512 ? 32 : 16;
+    const uint32_t tok = a.hidden <= 512 ? 64 : 32;
     p.splits = std::min(kCUs, (a.vocab + tok - 1) / tok);
     p.split_stride = 16ull * p.few * p.hidden64;
     if (a.dx) p.dxs = ar.take(p.splits * p.split_stride * 4);
@@ -1112,9 +1123,9 @@ hipError_t launch(Args a, const Plan& p, hipStream_t s) {
   if (!together) e = start(xent_loss, 1, 1024, s, a);
   if (e != hipSuccess || !(a.dx || a.dweight)) return e;
   if (p.few) {
-    e = p.few == 2         ? start(xent_few<T, 2, 32>, a.splits, 512, s, a)
-        : a.hidden <= 512  ? start(xent_few<T, 1, 32>, a.splits, 512, s, a)
-                           : start(xent_few<T, 1, 16>, a.splits, 512, s, a);
+    e = p.few == 2        ? start(xent_few<T, 2, 64>, a.splits, kFewThreads, s, a)
+        : a.hidden <= 512 ? start(xent_few<T, 1, 64>, a.splits, kFewThreads, s, a)
+                          : start(xent_few<T, 1, 32>, a.splits, kFewThreads, s, a);
     return e == hipSuccess && a.dx ? states<T>(a, s) : e;
   }
   for (a.first = 0; a.first < a.vocab; a.first += a.piece) {
