@@ -832,26 +832,31 @@ __global__ void __launch_bounds__(kTileThreads) xent_tile(Args a) {
 
 // Few rows, whose states fit LDS beside a tile of the table: one pass over the
 // table leaves both gradients.  A workgroup takes tiles of kTok tokens in turn:
-// their logits (the waves share the 16 x 16 tiles and the hidden columns),
-// slopes by way of LDS, then each wave, for its own columns, adds to its sums
-// for dx, which stay in registers to the end, and stores its part of the
-// tokens' dweight rows.  The next tile is on its way to registers meanwhile.  A
-// row of the table lies in LDS as it is, its 16-byte columns exchanged by the
-// row's number such that eight rows of a column, and two columns of four rows,
-// are free of bank conflicts: the logits read it by k, dx across.
-constexpr uint32_t kFewStates = 32768, kFewTile = 65536;  // bytes of the states, of a tile
+// their logits (the waves share the 16 x 16 tiles and the hidden columns; the
+// states are their registers'), slopes by way of LDS, then each wave, for its
+// own columns, adds to its sums for dx, which stay in registers to the end, and
+// stores its part of the tokens' dweight rows.  The next tile is on its way to
+// registers meanwhile.  Rows of the table and of the scaled states lie in LDS
+// as they are, their 16-byte columns exchanged by the row's number such that
+// eight rows of a column, and two columns of four rows, are free of bank
+// conflicts: the logits read the table by k, the gradients read across.
+constexpr uint32_t kFewBytes = 65536;  // of the states, and of a tile
 constexpr int kFewThreads = 1024;
 
 template <typename T, int kR, int kTok>
 __global__ void __launch_bounds__(kFewThreads) xent_few(Args a) {
   constexpr int kTiles = kR * kTok / 16, kSplits = 16 / kTiles;  // 16 x 16 tiles of logits, waves for one
-  constexpr int kSubs = 128 / kTok;  // 16-column subtiles of a wave: 1024 or 512 columns
-  constexpr int kLoads = (int)kFewTile / 16 / kFewThreads, kPitch = 40, kRowPitch = kTok + 8;
-  __shared__ u32x4 st[kFewTile / 16], xl[kFewStates / 16];
-  __shared__ f32x4 part[16][64];
-  __shared__ u32x4 lines[16 * kStored<kSubs> / 16];
+  constexpr int kColumns = 32768 / kTok;                         // the most
+  constexpr int kSubs = kColumns / 256, kX = kColumns / 32 / kSplits;  // of a wave: 16-column subtiles, steps of 32
+  constexpr int kLoads = (int)kFewBytes / 16 / kFewThreads, kPitch = 40, kRowPitch = (kTok < 32 ? 32 : kTok) + 8;
+  constexpr int kLine = kSubs == 4 && kR == 1 ? 4 : 2;  // subtiles stored at a time: LDS for more where it is left
+  __shared__ u32x4 st[kFewBytes / 16], xl[kR * 16 * kColumns / 8];
+  // of a wave: its part of a tile of logits, then the lines that it stores
+  __shared__ u32x4 own_lds[16][kStored<kLine> / 16];
+  static_assert(kStored<kLine> >= 1024, "a tile's part fits");
   // the slopes (32 rows of k, kTok tokens), and some space
   __shared__ __attribute__((aligned(16))) T by_token[kTok][kPitch], by_row[kR * 16][kRowPitch];
+  __shared__ float known[4][kR * 16];  // of a row: m, c, log2 s, target
   const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 15, q = lane >> 4;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
   const uint32_t vecs = a.hidden / 8, tiles = (a.vocab + kTok - 1) / kTok;
@@ -860,53 +865,65 @@ __global__ void __launch_bounds__(kFewThreads) xent_few(Args a) {
   const uint32_t own_subs = sub0 < subs ? min(each_subs, subs - sub0) : 0;
   const auto swap = [](uint32_t row) { return 2 * (row & 3) + (row >> 2 & 1); };
 
-  // a tile's vectors, of rows past the vocabulary the last's
+  // a tile's vectors, of rows past the vocabulary the last's: bytes from the
+  // tile's first, and their places in LDS
+  const uint32_t line = (uint32_t)a.weight_stride * 2;
+  // (eight columns and more a row: the exchange is of a vector's own number)
+  uint32_t from[kLoads], swaps = 0;
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const uint32_t at = i * kFewThreads + tid, row = at / vecs;
+    from[i] = row < (uint32_t)kTok ? row * line + (at - row * vecs) * 16 : ~0u;
+    swaps |= swap(row) << (3 * i);
+  }
   u32x4 next[kLoads];
   const auto load = [&](uint32_t tile) {
+    const char* base = (const char*)a.weight + (uint64_t)tile * kTok * line;
+    const uint32_t rows = min((uint32_t)kTok, a.vocab - tile * kTok);
+    if (rows == (uint32_t)kTok) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const uint32_t at = i * kFewThreads + tid, row = at / vecs;
-      if (row < (uint32_t)kTok)
-        next[i] = *(const u32x4*)((const T*)a.weight + (int64_t)min(tile * kTok + row, a.vocab - 1) * a.weight_stride +
-                                  (at - row * vecs) * 8);
+      for (int i = 0; i < kLoads; ++i)
+        if (from[i] != ~0u) next[i] = *(const u32x4*)(base + from[i]);
+    } else {
+      uint32_t now = tid;
+      asm volatile("" : "+v"(now));
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const uint32_t at = i * kFewThreads + now, row = at / vecs, c = at - row * vecs;
+        if (from[i] != ~0u) next[i] = *(const u32x4*)(base + (uint64_t)min(row, rows - 1) * line + c * 16);
+      }
     }
   };
   const auto keep = [&]() {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const uint32_t at = i * kFewThreads + tid, row = at / vecs;
-      if (row < (uint32_t)kTok) st[row * vecs + ((at - row * vecs) ^ swap(row))] = next[i];
-    }
+    for (int i = 0; i < kLoads; ++i)
+      if (from[i] != ~0u) st[(i * kFewThreads + tid) ^ (swaps >> (3 * i) & 7)] = next[i];
   };
   uint32_t tile = blockIdx.x;
   load(tile);
-  for (uint32_t at = tid; at < kR * 16 * vecs; at += kFewThreads) {
-    const uint32_t row = at / vecs, c = at - row * vecs;
-    xl[row * vecs + (c ^ swap(row))] =
-        *(const u32x4*)((const T*)a.x + (int64_t)min(row, a.rows - 1) * a.x_stride + c * 8);
-  }
-  for (uint32_t i = tid; i < kTok * kPitch; i += kFewThreads) (&by_token[0][0])[i] = (T)0.0f;
-  // this wave's columns of the scaled states, transposed
-  u32x4 xs[kSubs];
-#pragma unroll
-  for (int j = 0; j < kSubs; ++j) {
-    union {
-      T e[8];
-      u32x4 v;
-    } u;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t t = q * 8 + e;
-      u.e[e] = a.dweight && t < kR * 16u && (uint32_t)j < own_subs
-                   ? ((const T*)a.xs)[(uint64_t)t * a.hidden64 + (sub0 + j) * 16 + col]
-                   : (T)0.0f;
+  if (a.dweight)
+    for (uint32_t at = tid; at < kR * 16 * vecs; at += kFewThreads) {
+      const uint32_t row = at / vecs, c = at - row * vecs;
+      xl[row * vecs + (c ^ swap(row))] = ((const u32x4*)a.xs)[(uint64_t)row * (a.hidden64 / 8) + c];
     }
-    xs[j] = u.v;
-  }
-  // the tile of logits that this wave shares, and what a lane knows of its row
+  for (uint32_t i = tid; i < kTok * kPitch; i += kFewThreads) (&by_token[0][0])[i] = (T)0.0f;
+  for (uint32_t i = tid; i < kR * 16 * kRowPitch; i += kFewThreads) (&by_row[0][0])[i] = (T)0.0f;
+  // the tile of logits that this wave shares, its steps of the hidden columns,
+  // and what a lane knows of its row
   const uint32_t ts = wave % kTiles % (kTok / 16), rs = wave % kTiles / (kTok / 16), t = rs * 16 + col;
-  const int32_t y = t < a.rows ? a.target[t] : -1;
-  const float m = a.mant[t] * kUp<T>, c = a.top[t], ls = a.logsum[t];
+  const uint32_t steps = a.hidden / 32, each = (steps + kSplits - 1) / kSplits;
+  const uint32_t s0 = min(wave / kTiles * each, steps), s1 = min(s0 + each, steps);
+  u32x4 x[kX];
+#pragma unroll
+  for (int s = 0; s < kX; ++s)
+    x[s] = *(const u32x4*)((const T*)a.x + (int64_t)min(t, a.rows - 1) * a.x_stride +
+                           (min(s0 + s, steps - 1) * 4 + q) * 8);
+  if (tid < kR * 16) {
+    known[0][tid] = a.mant[tid] * kUp<T>;
+    known[1][tid] = a.top[tid];
+    known[2][tid] = a.logsum[tid];
+    known[3][tid] = __int_as_float(tid < a.rows ? a.target[tid] : -1);
+  }
   const float even = a.smoothing / (float)a.vocab, own = 1.0f - a.smoothing;
   const float f = *a.largest * (1.0f / kUp<T>);
   keep();
@@ -915,23 +932,25 @@ __global__ void __launch_bounds__(kFewThreads) xent_few(Args a) {
     load(min(tile + gridDim.x, tiles - 1));
     __syncthreads();
     {
-      const uint32_t steps = a.hidden / 32, each = (steps + kSplits - 1) / kSplits;
-      const uint32_t s0 = wave / kTiles * each, s1 = min(s0 + each, steps);
-      const u32x4* wr = st + (ts * 16 + col) * vecs;
-      const u32x4* xr = xl + (rs * 16 + col) * vecs;
+      // (the lane anew here and below, so that addresses are not kept through the
+      // loop: there are 128 registers)
+      uint32_t now = lane;
+      asm volatile("" : "+v"(now));
+      const u32x4* wr = st + (ts * 16 + (now & 15)) * vecs;
+      const uint32_t q = now >> 4, other = swap(now);
       f32x4 l{};
-#pragma unroll 4
-      for (uint32_t s = s0; s < s1; ++s) {
-        const uint32_t at = (s * 4 + q) ^ swap(col);
-        l = mfma(wr[at], xr[at], l, T{});
-      }
-      part[wave][lane] = l;
+#pragma unroll
+      for (int s = 0; s < kX; ++s)
+        if (s0 + s < s1) l = mfma(wr[((s0 + s) * 4 + q) ^ other], x[s], l, T{});
+      *(f32x4*)&own_lds[wave][lane] = l;
     }
     __syncthreads();
     if (wave < (uint32_t)kTiles) {
-      f32x4 l = part[wave][lane];
+      const float m = known[0][t], c = known[1][t], ls = known[2][t];
+      const int32_t y = __float_as_int(known[3][t]);
+      f32x4 l{};
 #pragma unroll
-      for (int i = 1; i < kSplits; ++i) l += part[wave + i * kTiles][lane];
+      for (int i = 0; i < kSplits; ++i) l += *(const f32x4*)&own_lds[wave + i * kTiles][lane];
       union {
         T e[4];
         uint2 u;
@@ -947,53 +966,71 @@ __global__ void __launch_bounds__(kFewThreads) xent_few(Args a) {
       *(uint2*)&by_row[t][ts * 16 + q * 4] = o.u;
     }
     __syncthreads();
+    // columns 16 sub ... of rows k0 + 8 q ... of the table or the states, read
+    // across (rows behind: these again, for slopes of zero)
+    uint32_t now = lane;
+    asm volatile("" : "+v"(now));
+    const auto across = [&](const u32x4* from, uint32_t rows, uint32_t k0, uint32_t sub) {
+      const uint32_t col = now & 15, q = now >> 4;
+      union {
+        s16x4 h[2];
+        u32x4 v;
+      } u;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t row = (k0 + q * 8 + i * 4 + (col >> 2)) % rows;
+        const char* p = (const char*)(from + row * vecs + ((sub * 2 + (col >> 1 & 1)) ^ swap(row))) + (col & 1) * 8;
+        u.h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+      }
+      return u.v;
+    };
     if (a.dx) {
 #pragma unroll
-      for (int k = 0; k < kTok / 32; ++k) {
+      for (int k = 0; k < (kTok + 31) / 32; ++k) {
         u32x4 gf[kR];
 #pragma unroll
         for (int r = 0; r < kR; ++r) gf[r] = *(const u32x4*)&by_row[r * 16 + col][k * 32 + q * 8];
 #pragma unroll
         for (int j = 0; j < kSubs; ++j) {
           if ((uint32_t)j >= own_subs) break;
-          union {
-            s16x4 h[2];
-            u32x4 v;
-          } w;
+          const u32x4 w = across(st, kTok, k * 32, sub0 + j);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t row = k * 32 + q * 8 + i * 4 + (col >> 2);
-            const char* p = (const char*)(st + row * vecs + (((sub0 + j) * 2 + (col >> 1 & 1)) ^ swap(row))) + (col & 1) * 8;
-            w.h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
-          }
-#pragma unroll
-          for (int r = 0; r < kR; ++r) sum[j][r] = mfma(w.v, gf[r], sum[j][r], T{});
+          for (int r = 0; r < kR; ++r) sum[j][r] = mfma(w, gf[r], sum[j][r], T{});
+          if (kSubs > 4 || j % 2) __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
     __syncthreads();
     keep();
     if (a.dweight) {
+#pragma unroll 1
+      for (int j0 = 0; j0 < kSubs; j0 += kLine) {
+        if ((uint32_t)j0 >= own_subs) break;
+        u32x4 xf[kLine];
 #pragma unroll
-      for (int i = 0; i < kTok / 16; ++i) {
-        const uint32_t tok = tile * kTok + i * 16;
-        const u32x4 gf = *(const u32x4*)&by_token[i * 16 + col][q * 8];
-        uint2 all[kSubs];
+        for (int j = 0; j < kLine; ++j) xf[j] = across(xl, kR * 16, 0, min(sub0 + j0 + j, subs - 1));
 #pragma unroll
-        for (int j = 0; j < kSubs; ++j) {
-          const f32x4 d = mfma(xs[j], gf, f32x4{}, T{});
-          union {
-            T e[4];
-            uint2 u;
-          } o;
+        for (int i = 0; i < kTok / 16; ++i) {
+          const uint32_t tok = tile * kTok + i * 16;
+          const u32x4 gf = *(const u32x4*)&by_token[i * 16 + (now & 15)][(now >> 4) * 8];
+          uint2 all[kLine];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o.e[e] = (T)(d[e] * f);
-          all[j] = o.u;
+          for (int j = 0; j < kLine; ++j) {
+            const f32x4 d = mfma(xf[j], gf, f32x4{}, T{});
+            union {
+              T e[4];
+              uint2 u;
+            } o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o.e[e] = (T)(d[e] * f);
+            all[j] = o.u;
+          }
+          store_rows<kLine>(all, (char*)own_lds[wave], now, [&](uint32_t r, uint32_t c, u32x4 v) {
+            if (tok + r < a.vocab && j0 * 16 + c < own_subs * 16)
+              store_vec((T*)a.dweight + (int64_t)(tok + r) * a.dweight_stride + (sub0 + j0) * 16 + c, v);
+          });
+          __builtin_amdgcn_sched_barrier(0);
         }
-        store_rows<kSubs>(all, (char*)lines + wave * kStored<kSubs>, lane, [&](uint32_t r, uint32_t c, u32x4 v) {
-          if (tok + r < a.vocab && c < own_subs * 16)
-            store_vec((T*)a.dweight + (int64_t)(tok + r) * a.dweight_stride + sub0 * 16 + c, v);
-        });
       }
     }
   }
@@ -1039,7 +1076,7 @@ Plan plan(const ft_cross_entropy_loss_args& a) {
   if (p.bm == 256 && (p.rows64 + 191) / 192 * 192 < round_up(p.rows64, 256)) p.bm = 192;
   p.tiles = (a.vocab + p.bn - 1) / p.bn;
   const uint64_t r = p.rows64;
-  if (p.lines && a.rows <= 32 && round_up(a.rows, 16) * a.hidden * 2 <= kFewStates && (a.dx || a.dweight))
+  if (p.lines && a.hidden <= (a.rows <= 16 ? 2048 : a.rows <= 32 ? 512 : 0) && (a.dx || a.dweight))
     p.few = (uint32_t)(a.rows + 15) / 16;
   p.mant = ar.take(r * 4);
   p.power = ar.take(r * 4);
@@ -1061,7 +1098,7 @@ Plan plan(const ft_cross_entropy_loss_args& a) {
   }
   if (a.dweight) p.xs = ar.take(r * p.hidden64 * 2);
   if (p.few) {
-    const uint32_t tok = a.hidden <= 512 ? 64 : 32;
+    const uint32_t tok = a.hidden <= 512 ? 64 : a.hidden <= 1024 ? 32 : 16;
     p.splits = std::min(kCUs, (a.vocab + tok - 1) / tok);
     p.split_stride = 16ull * p.few * p.hidden64;
     if (a.dx) p.dxs = ar.take(p.splits * p.split_stride * 4);
@@ -1123,9 +1160,10 @@ hipError_t launch(Args a, const Plan& p, hipStream_t s) {
   if (!together) e = start(xent_loss, 1, 1024, s, a);
   if (e != hipSuccess || !(a.dx || a.dweight)) return e;
   if (p.few) {
-    e = p.few == 2        ? start(xent_few<T, 2, 64>, a.splits, kFewThreads, s, a)
-        : a.hidden <= 512 ? start(xent_few<T, 1, 64>, a.splits, kFewThreads, s, a)
-                          : start(xent_few<T, 1, 32>, a.splits, kFewThreads, s, a);
+    e = p.few == 2         ? start(xent_few<T, 2, 64>, a.splits, kFewThreads, s, a)
+        : a.hidden <= 512  ? start(xent_few<T, 1, 64>, a.splits, kFewThreads, s, a)
+        : a.hidden <= 1024 ? start(xent_few<T, 1, 32>, a.splits, kFewThreads, s, a)
+                           : start(xent_few<T, 1, 16>, a.splits, kFewThreads, s, a);
     return e == hipSuccess && a.dx ? states<T>(a, s) : e;
   }
   for (a.first = 0; a.first < a.vocab; a.first += a.piece) {

@@ -1,12 +1,15 @@
 """flashtrie.cross_entropy_loss against its definition in 64 bits, within the
 bounds of table_reference.py."""
 
+import ctypes as C
 import math
+import os
 
 import pytest
 import torch
 
 import table_reference as ref
+import test_table_args as args
 
 pytestmark = pytest.mark.gpu
 
@@ -63,6 +66,65 @@ def test_vocabulary_and_hidden(ft, dtype, V, H):
                                          (33, 70001, 64, F16), (300, 5000, 2048, BF16)])
 def test_working_sizes(ft, T, V, H, dtype):
     check(ft, inputs(T, V, H, dtype, T + V), 0.1, "working")
+
+
+# one pass over the table for few rows: its tiles of 64, 32 and 16 tokens, hidden
+# columns that the waves share unevenly, more tiles than workgroups
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,H", [*[(t, h) for t in (1, 9, 16) for h in (64, 448, 512, 576, 960, 1024, 1088, 1600, 2048)],
+                                 *[(t, h) for t in (17, 32) for h in (64, 320, 512)], (17, 576), (3, 2112), (33, 64)])
+def test_few_rows(ft, dtype, T, H):
+    for V in (5, 65, 4113):
+        a = inputs(T, V, H, dtype, T + V + H)
+        whole = check(ft, a, 0.1, "few")
+        some = ft.cross_entropy_loss(**a, smoothing=0.1, weight_grad=False)
+        assert all(torch.equal(p, q) for p, q in zip(whole[:3], some[:3]))
+
+
+@pytest.mark.parametrize("T,V,H", [(10, 70000, 128), (25, 70000, 64)])
+def test_few_rows_many_tokens(ft, T, V, H):
+    check(ft, inputs(T, V, H, BF16, 1), 0.1, "few")
+
+
+def call(ft, a, dx, dweight, smoothing=0.1):
+    """The C call, for what the Python one does not offer."""
+    lib = C.CDLL(os.path.join(args.ROOT, "flash-trie_amd", "libflashtrie_amd.so"))
+    (T, H), V = a["x"].shape, a["weight"].shape[0]
+    loss, logp = torch.empty((), device="cuda"), torch.empty(T, device="cuda")
+    s = args.CrossEntropy(
+        device=0, dtype=args.BF16, rows=T, hidden=H, vocab=V, x=a["x"].data_ptr(), x_stride=a["x"].stride(0),
+        weight=a["weight"].data_ptr(), weight_stride=a["weight"].stride(0), target=a["targets"].data_ptr(),
+        row_weight=a["row_weight"].data_ptr(), smoothing=smoothing, loss=loss.data_ptr(), logp=logp.data_ptr(),
+        dx=dx.data_ptr() if dx is not None else None, dx_stride=dx.stride(0) if dx is not None else 0,
+        dweight=dweight.data_ptr() if dweight is not None else None,
+        dweight_stride=dweight.stride(0) if dweight is not None else 0)
+    lib.ft_cross_entropy_loss_workspace.restype = C.c_size_t
+    n = lib.ft_cross_entropy_loss_workspace(C.byref(s))
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert lib.ft_cross_entropy_loss(C.byref(s), C.c_void_p(ws.data_ptr()), C.c_size_t(n), stream) == 0
+    torch.cuda.synchronize()
+    return loss, logp
+
+
+@pytest.mark.parametrize("T,V,H", [(10, 300, 64), (100, 300, 128), (300, 700, 192), (20, 90, 50), (0, 40, 64)])
+def test_outputs_of_any_stride(ft, T, V, H):
+    """The table's gradient alone; both in rows of wider tensors, whose other
+    columns stay as they were."""
+    a = inputs(T, V, H, BF16, 17)
+    want = ft.cross_entropy_loss(**a, smoothing=0.1)
+    for with_dx in (False, True):
+        dx = torch.full((max(T, 1), H + 9), 5.0, device="cuda").bfloat16()
+        dw = torch.full((V, H + 7), 5.0, device="cuda").bfloat16()
+        loss, logp = call(ft, a, dx[:T, 3:3 + H] if with_dx and T else None, dw[:, 1:1 + H])
+        assert torch.equal(loss, want[0]) and torch.equal(logp, want[1])
+        assert torch.equal(dw[:, 1:1 + H], want[3])
+        assert (dw[:, 0] == 5).all() and (dw[:, 1 + H:] == 5).all()
+        if with_dx and T:
+            assert torch.equal(dx[:, 3:3 + H], want[2])
+            assert (dx[:, :3] == 5).all() and (dx[:, 3 + H:] == 5).all()
+        else:
+            assert (dx == 5).all()
 
 
 @pytest.mark.parametrize("smoothing", [0.0, 1.0, 0.5])

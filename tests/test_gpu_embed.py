@@ -1,12 +1,15 @@
 """flashtrie.embed exactly and embed_grad within the bounds of
 table_reference.py."""
 
+import ctypes as C
 import math
+import os
 
 import pytest
 import torch
 
 import table_reference as ref
+import test_table_args as args
 
 pytestmark = pytest.mark.gpu
 
@@ -177,6 +180,27 @@ def test_grad_strides(ft):
     assert torch.equal(ft.embed_grad(flat, tokens.view(-1), 40), ft.embed_grad(flat.contiguous(), tokens.view(-1), 40))
     one = wide[0, 0, 0, :50].expand(6, 10, 6, 50)
     check(ft, one, tokens, 40, 1.0, None, "one row for all")
+
+
+@pytest.mark.parametrize("n", [0, 50, 5000])
+@pytest.mark.parametrize("H", [40, 41])
+def test_grad_in_wider_rows(ft, n, H):
+    """The C call with a gradient in rows of a wider tensor, whose other columns
+    stay as they were."""
+    lib = C.CDLL(os.path.join(args.ROOT, "flash-trie_amd", "libflashtrie_amd.so"))
+    V, big = 300, torch.full((300, 60), 5.0, dtype=F16, device="cuda")
+    tokens, _ = keys((n,), V, 25, 40)
+    g = normal((n, H), F16, 26)
+    s = args.EmbedGrad(device=0, dtype=args.F16, groups=1, steps=n, hidden=H, vocab=V, tokens=tokens.data_ptr(),
+                       grad=g.data_ptr(), grad_stride=H, scale=2.0, dtable=big.data_ptr() + 6, dtable_stride=60)
+    lib.ft_embed_grad_workspace.restype = C.c_size_t
+    size = lib.ft_embed_grad_workspace(C.byref(s))
+    ws = torch.empty(max(size, 1), dtype=torch.uint8, device="cuda")
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert lib.ft_embed_grad(C.byref(s), C.c_void_p(ws.data_ptr()), C.c_size_t(size), stream) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(big[:, 3:3 + H], ft.embed_grad(g, tokens, V, 2.0))
+    assert (big[:, :3] == 5).all() and (big[:, 3 + H:] == 5).all()
 
 
 def test_grad_repeats(ft):
