@@ -78,6 +78,7 @@ struct Args {
   uint32_t slope_stride;  // of the slopes' rows
   uint32_t splits, split_steps;  // parts of dx and their steps of 64
   uint64_t split_stride;
+  uint32_t tiled;    // rows that the tiles cover
   uint32_t prepare;  // workgroups in front of the statistics' that prepare rows
 };
 
@@ -149,6 +150,9 @@ __device__ __forceinline__ void prepare_rows(const Args& a, uint32_t block) {
     }
     ((u32x4*)a.xs)[((uint64_t)t * a.hidden64 + k) / 8] = v;
   }
+  // rows behind the last tile's, which the table's product reads too
+  if (t >= a.tiled)
+    for (uint32_t k = lane * 8; k < a.piece; k += 512) ((u32x4*)a.slopes)[((uint64_t)t * a.slope_stride + k) / 8] = u32x4{};
 }
 template <typename T>
 __global__ void __launch_bounds__(256) xent_rows(Args a) {
@@ -616,7 +620,7 @@ __device__ __forceinline__ void wait_copies() {
 // kWhole: across, rows are whole steps.
 template <typename T, bool kAcross, int kB, bool kWhole>
 struct Lines {
-  static constexpr int kTurns = kB / 64;  // copies of a wave and step
+  static constexpr int kTurns = (kB + 63) / 64;  // copies of a wave and step (the last: of some waves)
   static constexpr uint32_t kBytes = kAcross ? 32 * 1088 + 8 * 128 : kB * 128;
   static constexpr int kOffsets = kAcross ? 1 : kTurns;
   static_assert(!kAcross || kB == 256, "lines of 512 bytes");
@@ -673,7 +677,8 @@ struct Lines {
     } else {
       const __amdgpu_buffer_rsrc_t b = whole_buffer(base);
 #pragma unroll
-      for (int c = 0; c < kTurns; ++c) copy_to_lds(b, off[c], k * 128, st + (c * 8 + wave) * 1024);
+      for (int c = 0; c < kTurns; ++c)
+        if (kB % 64 == 0 || c * 64 + wave * 8 < (uint32_t)kB) copy_to_lds(b, off[c], k * 128, st + (c * 8 + wave) * 1024);
     }
   }
   // subtile sub0 + v, half kk of a step
@@ -734,7 +739,7 @@ __global__ void __launch_bounds__(kTileThreads) xent_tile(Args a) {
   const uint32_t workers = gridDim.x - (kKind == kStats ? a.prepare : 0);
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t wm = wave % S::WM, wn = wave / S::WM;
-  const uint32_t js = kKind == kTable ? a.width / S::BM : (a.rows64 + S::BM - 1) / S::BM;
+  const uint32_t js = kKind == kTable ? a.width / S::BM : (a.rows + S::BM - 1) / S::BM;
   const uint32_t is = kKind == kStats    ? a.tiles
                       : kKind == kSlopes ? a.width / kTileBN
                                          : (a.hidden64 + kTileBN - 1) / kTileBN;
@@ -1073,7 +1078,22 @@ Plan plan(const ft_cross_entropy_loss_args& a) {
   p.lines = whole_lines(a);
   p.bn = p.lines ? kTileBN : kBN;
   p.bm = !p.lines || p.rows64 <= 64 ? 64 : p.rows64 <= 128 ? 128 : 256;
-  if (p.bm == 256 && (p.rows64 + 191) / 192 * 192 < round_up(p.rows64, 256)) p.bm = 192;
+  // Many rows: the tile that leaves the least of them empty, at what a row costs
+  // in each (6,720 rows x 65,536 x 1,024, whole tiles of each but 256: 2.68 ms by
+  // 224, 2.90 by 192, 2.94 by 160; 4,096 rows x 262,144 x 1,024: 7.91 ms by 256,
+  // 8.39 by 224; 777 rows x 50,021 x 768: 304 us by 160, 315 by 192, 331 by 224,
+  // 337 by 256).
+  if (p.bm == 256) {
+    uint64_t least = ~0ull;
+    constexpr uint32_t kShapes[4][2] = {{256, 100}, {224, 102}, {192, 107}, {160, 109}};
+    for (const auto& shape : kShapes) {
+      const uint64_t cost = round_up(a.rows, shape[0]) * shape[1];
+      if (cost < least) {
+        least = cost;
+        p.bm = shape[0];
+      }
+    }
+  }
   p.tiles = (a.vocab + p.bn - 1) / p.bn;
   const uint64_t r = p.rows64;
   if (p.lines && a.hidden <= (a.rows <= 16 ? 2048 : a.rows <= 32 ? 512 : 0) && (a.dx || a.dweight))
@@ -1104,7 +1124,7 @@ Plan plan(const ft_cross_entropy_loss_args& a) {
     if (a.dx) p.dxs = ar.take(p.splits * p.split_stride * 4);
   } else if (a.dx) {
     // as many parts of the sum over tokens as fill the chip
-    const uint64_t tiles = std::max<uint64_t>(1, (r + p.bm - 1) / p.bm * ((p.hidden64 + p.bn - 1) / p.bn));
+    const uint64_t tiles = std::max<uint64_t>(1, (a.rows + p.bm - 1) / p.bm * ((p.hidden64 + p.bn - 1) / p.bn));
     const uint32_t steps = p.piece / kBK;
     const uint64_t want = std::max<uint64_t>(1, (p.lines ? 1 : 2) * kCUs / tiles);
     p.split_steps = (uint32_t)std::max<uint64_t>(4, (steps + want - 1) / want);
@@ -1119,7 +1139,7 @@ Plan plan(const ft_cross_entropy_loss_args& a) {
 template <typename T, Kind kKind>
 hipError_t product(const Args& a, const Plan& p, hipStream_t s) {
   const uint64_t hs = (a.hidden64 + p.bn - 1) / p.bn;
-  const uint64_t js = kKind == kTable ? a.width / (p.lines ? 256 : p.bm) : (a.rows64 + p.bm - 1) / p.bm;
+  const uint64_t js = kKind == kTable ? a.width / (p.lines ? 256 : p.bm) : (a.rows + p.bm - 1) / p.bm;
   const uint64_t blocks = js * (kKind == kStats    ? a.tiles
                                 : kKind == kSlopes ? a.width / p.bn
                                 : kKind == kStates ? hs * ((a.width / 64 + a.split_steps - 1) / a.split_steps)
@@ -1131,7 +1151,9 @@ hipError_t product(const Args& a, const Plan& p, hipStream_t s) {
                    (kKind == kStats ? a.prepare : 0) + std::min<uint64_t>(blocks, kCUs), kTileThreads, s, a);
     const uint64_t most = std::min<uint64_t>(blocks, kCUs);
     if (p.bm == 128) return start(xent_tile<T, kKind, TileShape<8, 2>>, most, kTileThreads, s, a);
+    if (p.bm == 160) return start(xent_tile<T, kKind, TileShape<10, 2>>, most, kTileThreads, s, a);
     if (p.bm == 192) return start(xent_tile<T, kKind, TileShape<12, 2>>, most, kTileThreads, s, a);
+    if (p.bm == 224) return start(xent_tile<T, kKind, TileShape<14, 2>>, most, kTileThreads, s, a);
   }
   return start(xent_tile<T, kKind, TileShape<16, 2>>, std::min<uint64_t>(blocks, kCUs), kTileThreads, s, a);
 }
@@ -1147,6 +1169,7 @@ hipError_t launch(Args a, const Plan& p, hipStream_t s) {
     const hipError_t e = start(xent_loss, 1, 1024, s, a);
     return e == hipSuccess && a.dweight ? start(xent_nothing<T>, a.vocab, 256, s, a) : e;
   }
+  a.tiled = p.few ? a.rows64 : (uint32_t)std::min<uint64_t>(a.rows64, round_up(a.rows, p.bm));
   // few rows are prepared beside the statistics, and joined with the loss
   hipError_t e = hipSuccess;
   if (p.lines && p.bm == 64) a.prepare = a.rows64 / 8;

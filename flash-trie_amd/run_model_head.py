@@ -17,6 +17,14 @@ Each round of a small training run on seeded data
 6. carries the gradient of the logits to the adapters (plain matrix products)
    and steps them.
 
+With ``--pretrain N`` the head's table is first trained on the wanted keys
+themselves, N supervised steps: a step's hidden state is the request's plus the
+table's row of the token before it (``embed``), the loss and the gradients of
+states and table come without logits (``cross_entropy_loss``), and the lookup's
+gradient is added to the table's (``embed_grad``).  With ``--packed GROUP`` a
+last search takes its logits from the table in 4 bits (``pack_weight``,
+``packed_logits``).
+
 It prints a line per round: the loss, the mean reward of the returned keys,
 and of the key that the search ranks first.  Nothing of it is a trained
 model: hidden states lean towards a wanted key by ``--signal``.
@@ -58,8 +66,14 @@ def parse_args(argv=None):
     p.add_argument("--beta", type=float, default=0.1)
     p.add_argument("--signal", type=float, default=0.35,
                    help="how far the hidden states lean to the wanted key")
+    p.add_argument("--pretrain", type=int, default=0, help="supervised steps on the wanted keys")
+    p.add_argument("--table-lr", type=float, default=0.5)
+    p.add_argument("--packed", type=int, default=0, choices=(0, 32, 64, 128),
+                   help="columns to a scale of the table in 4 bits (0: no such search)")
     p.add_argument("--seed", type=int, default=0)
     args = p.parse_args(argv)
+    if args.pretrain < 0:
+        p.error("--pretrain must be at least 0")
     for name in ("requests", "num_keys", "key_length", "hidden", "adapters", "rank",
                  "topk_tokens", "beam_size", "rounds", "updates"):
         if getattr(args, name) < 1:
@@ -111,6 +125,43 @@ class Head:
         self.optimizer.step()
 
 
+def before(tokens):
+    """The tokens one step earlier, -1 (none) in front of a key."""
+    out = tokens.roll(1, -1)
+    out[..., 0] = -1
+    return out.contiguous()
+
+
+def supervised(ft, x, table, tokens, lengths, scale):
+    """(loss, table's gradient) of keys [R, C, S] whose states are x [R, C, S,
+    hidden] plus scale times the table's row of the token before; a key's tokens
+    share its weight, the keys theirs."""
+    R, C, S = tokens.shape
+    inputs = before(tokens)
+    states = x + ft.embed(inputs, table, scale, lengths)
+    there = tokens.new_tensor(range(S)) < lengths[..., None]
+    targets = tokens.masked_fill(~there, -1).view(-1)
+    share = 1.0 / (lengths.clamp(min=1) * max(1, int((lengths > 0).sum())))
+    weight = share.float()[..., None].expand(R, C, S).reshape(-1)
+    loss, _, dx, dtable = ft.cross_entropy_loss(states.view(R * C * S, -1), table, targets, weight)
+    ft.embed_grad(dx.view(R, C, S, -1), inputs, table.shape[0], scale, lengths, out=dtable)
+    return loss, dtable
+
+
+def pretrain(head, x, wanted, args, log):
+    """Steps of plain gradient descent on the table, held in 32 bits."""
+    torch, (tok, length) = head.torch, key_arrays([[k] for k in wanted], args.key_length)
+    tok, length = torch.from_numpy(tok).cuda(), torch.from_numpy(length).cuda()
+    table, losses = head.weight.float(), []
+    for n in range(args.pretrain):
+        loss, d = supervised(head.ft, x.view(*tok.shape, -1), head.weight, tok, length, 1.0)
+        table -= args.table_lr * d.float()
+        head.weight = table.to(head.dtype)
+        losses.append(loss.item())
+        log(f"pretrain {n}: loss {losses[-1]:.5f}")
+    return losses
+
+
 def key_arrays(sents, steps):
     """The search's keys as (tokens [R, C, steps], lengths [R, C]) int32; a
     request with fewer keys than another has keys of no tokens."""
@@ -157,13 +208,17 @@ def run(args, log=print):
     adapter = adapter.repeat_interleave(S).contiguous()
     base = torch.full_like(adapter, -1)   # the head without its adapters
 
+    def search(logits):
+        ids, logp = ft.propose(logits.view(R, S, -1), args.topk_tokens)
+        return ft.bs_tbs_gpu(trie, R, [[C] * S] * R, list(ids.cpu().numpy()),
+                             list(logp.cpu().numpy()), -1e9, -1e9, 5.0, False)
+
     lines = []
+    if args.pretrain:
+        lines.append({"pretrain": pretrain(head, x, wanted, args, log)})
     for n in range(args.rounds):
         logits = head.logits(x, adapter).view(R, S, -1)
-        ids, logp = ft.propose(logits, args.topk_tokens)
-        sents, _, search_ms, _ = ft.bs_tbs_gpu(
-            trie, R, [[C] * S] * R, list(ids.cpu().numpy()), list(logp.cpu().numpy()),
-            -1e9, -1e9, 5.0, False)
+        sents, _, search_ms, _ = search(logits)
         tok, length = key_arrays(sents, S)
         reward = rewards(tok, length, wanted)
         found = length > 0
@@ -204,6 +259,14 @@ def run(args, log=print):
         log(f"round {n}: {args.loss} loss {losses[0]:+.5f} -> {losses[-1]:+.5f}  "
             f"keys {line['keys']}  reward: mean {line['mean_reward']:.3f}, "
             f"first {line['first_reward']:.3f}  search {search_ms:.3f} ms")
+    if args.packed:
+        packed = ft.packed_logits(x, *ft.pack_weight(head.weight, args.packed), args.vocab_size,
+                                  torch.float32)
+        sents = [search(y)[0] for y in (head.logits(x, base), packed)]
+        same = [len({tuple(k) for k in a} & {tuple(k) for k in b}) / max(len(a), 1)
+                for a, b in zip(*sents)]
+        lines.append({"packed": sum(same) / R, "keys": sum(map(len, sents[1]))})
+        log(f"table in 4 bits: {100 * lines[-1]['packed']:.1f}% of the table's own keys")
     return lines
 
 
