@@ -16,9 +16,11 @@
 //
 // r[t] = m 2^e, m in [1, 2).  g is stored times m, so that its rounding is
 // relative to itself also in float16 (there times 2^14: |g m| < 2, and what is
-// below 2^-28 of it loses digits that no sum keeps); dx is multiplied by 2^e at
-// its end, and dw takes rows of x times 2^(e - the largest e), which is exact
-// but for parts that the largest row's swallow.  A row without a target, or of
+// below 2^-28 of it loses digits that no sum keeps), and times a factor within
+// 2^-8 of 1 by which the target's slope, the largest as a rule, is one of the
+// type's numbers.  dx is multiplied by r over both at its end; dw takes rows of
+// x times that over 2^(the largest e), rounded to x's type.  So dx has about
+// its own rounding alone, and dw that and x's.  A row without a target, or of
 // weight 0, has g = 0 and such an x of 0, whatever its x holds.
 #include <algorithm>
 
@@ -62,8 +64,8 @@ struct Args {
   uint32_t rows, rows64, hidden, hidden64, vocab, tiles;  // (up to whole 64s); token tiles of the statistics
   float smoothing;
   // workspace
-  float* mant;      // [rows64]: m, 0 without a target
-  float* power;     // [rows64]: 2^e
+  float* factor;    // [rows64]: what slopes are stored times, 0 without a target
+  float* power;     // [rows64]: r over it
   float* largest;   // 2^(the largest e)
   float* part;      // [3][tiles][rows64]: c, s, sum of logits
   float* picked;    // [rows64]: the target's logit
@@ -107,9 +109,17 @@ __device__ __forceinline__ int exponent_of(const Args& a, uint32_t t, float* m) 
   return e - 1;
 }
 
-// Rows' weights and, for the table's gradient, their scaled states: a wave of
-// kWaves a row.
-template <typename T, int kWaves>
+// The target's slope over r, as the slopes' product makes it.
+__device__ __forceinline__ float target_slope(const Args& a, uint32_t t) {
+  const float even = a.smoothing / (float)a.vocab, own = 1.0f - a.smoothing;
+  return exp2_raw(__builtin_fmaf(a.picked[t], kLog2e, -a.top[t]) - a.logsum[t]) - even - own;
+}
+
+// Rows' factors and, for the table's gradient, their scaled states: a wave of
+// kWaves a row.  kFit (past the statistics): a row's slopes are stored times a
+// factor next to m for which the target's, the largest as a rule, has no
+// rounding; dx is divided by it in 32 bits, the states in their type.
+template <typename T, int kWaves, bool kFit>
 __device__ __forceinline__ void prepare_rows(const Args& a, uint32_t block) {
   __shared__ int biggest[kWaves];
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -129,9 +139,20 @@ __device__ __forceinline__ void prepare_rows(const Args& a, uint32_t block) {
   float m = 0.0f;
   int e = t < a.rows ? exponent_of(a, t, &m) : 0;
   if (e == -1000) e = m == 0.0f ? 0 : big;
+  float times = m * kUp<T>, back = 1.0f;  // m = times back / kUp
+  if (kFit && m != 0.0f && fabsf(m) < INFINITY) {
+    const float g = (uint32_t)a.target[t] < a.vocab ? target_slope(a, t) : NAN;
+    // (one that is far below the others is left alone; so is NaN)
+    const float fit = (float)(T)(g * times);
+    if (fabsf(fit) > 0x1p-10f && fabsf(fit) < INFINITY) {
+      back = times;
+      times = fit / g;
+      back /= times;
+    }
+  }
   if (lane == 0) {
-    a.mant[t] = m;
-    a.power[t] = ldexpf(1.0f, e);
+    a.factor[t] = times;
+    a.power[t] = ldexpf(back * (1.0f / kUp<T>), e);
     if (t == 0) *a.largest = ldexpf(1.0f, big);
   }
   if (!a.dweight) return;
@@ -140,11 +161,11 @@ __device__ __forceinline__ void prepare_rows(const Args& a, uint32_t block) {
     u32x4 v{};
     if (m != 0.0f) {
       v = load_row_vec(row, k, a.hidden, (T)0.0f);
-      if (e != big) {
+      if (e != big || back != 1.0f) {
         float f[8];
         to_float<T>(v, f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = ldexpf(f[i], e - big);
+        for (int i = 0; i < 8; ++i) f[i] = ldexpf(f[i] * back, e - big);
         v = from_float<T>(f);
       }
     }
@@ -156,7 +177,7 @@ __device__ __forceinline__ void prepare_rows(const Args& a, uint32_t block) {
 }
 template <typename T>
 __global__ void __launch_bounds__(256) xent_rows(Args a) {
-  prepare_rows<T, 4>(a, blockIdx.x);
+  prepare_rows<T, 4, true>(a, blockIdx.x);
 }
 
 // 16 rows by 64 parts of the tiles.  A workgroup that has them all adds up the
@@ -201,21 +222,22 @@ __device__ __forceinline__ void join_rows(const Args& a, uint32_t first) {
     l += more;
   }
   if (from > 0) return;
-  constexpr float kLn2 = 0.693147180559945309f;
+  // (in 64 bits: a score near 0 is a difference of near numbers)
+  constexpr double kLn2 = 0.693147180559945309;
   const int32_t y = t < a.rows ? a.target[t] : -1;
   const bool there = y >= 0 && (uint32_t)y < a.vocab;
   // (a target out of range: NaN, and with it the row's slopes)
-  const float ls = y < 0 || there ? __log2f(p.s) : NAN;
-  const float at = there ? (__builtin_fmaf(a.picked[t], kLog2e, -p.c) - ls) * kLn2 : NAN;
+  const double ls = y < 0 || there ? log2((double)p.s) : (double)NAN;
+  const float at = there ? (float)((((double)a.picked[t] * (double)kLog2e - (double)p.c) - ls) * kLn2) : NAN;
   a.top[t] = p.c;
-  a.logsum[t] = ls;
+  a.logsum[t] = (float)ls;
   float term = 0.0f;
   if (y >= 0) {
     a.logp[t] = at;
     const float r = a.row_weight[t];
     term = (1.0f - a.smoothing) * -at;
     if (a.smoothing != 0.0f)
-      term += a.smoothing * ((ls - __builtin_fmaf(l / (float)a.vocab, kLog2e, -p.c)) * kLn2);
+      term += a.smoothing * (float)((ls - ((double)(l / (float)a.vocab) * (double)kLog2e - (double)p.c)) * kLn2);
     term = r == 0.0f ? 0.0f : r * term;
   } else if (t < a.rows) {
     a.logp[t] = 0.0f;
@@ -269,8 +291,8 @@ __global__ void __launch_bounds__(1024) xent_states(Args a) {
   __syncthreads();
   if (wave > 0) return;
   for (uint32_t w = 1; w < waves; ++w) y += other[w - 1][lane];
-  const bool none = a.mant[t] == 0.0f;
-  const float f = a.power[t] * (1.0f / kUp<T>);
+  const bool none = a.factor[t] == 0.0f;
+  const float f = a.power[t];
   T* out = (T*)a.dx + (int64_t)t * a.dx_stride + h;
 #pragma unroll
   for (int e = 0; e < 4; ++e)
@@ -443,7 +465,7 @@ __device__ __forceinline__ void finish(const Args& a, uint32_t tid, uint32_t til
       if (j0 + s * 16 >= a.rows64) break;
       const uint32_t t = j0 + s * 16 + col;
       const uint32_t y = (t < a.rows ? (uint32_t)a.target[t] : ~0u) - i0;
-      const float m = a.mant[t] * kUp<T>, c = a.top[t], ls = a.logsum[t];
+      const float m = a.factor[t], c = a.top[t], ls = a.logsum[t];
       const bool hit = __ballot(y < 16 * kN) != 0;  // (a target in one tile of many)
       union {
         uint2 u;
@@ -731,7 +753,7 @@ __global__ void __launch_bounds__(kTileThreads) xent_tile(Args a) {
   __shared__ u32x4 stored[kKind == kSlopes || kKind == kTable ? 8 * kStored<S::N> / 16 : 1];
   if constexpr (kKind == kStats && S::BM == 64) {
     if (blockIdx.x < a.prepare) {
-      prepare_rows<T, 8>(a, blockIdx.x);
+      prepare_rows<T, 8, false>(a, blockIdx.x);
       return;
     }
   }
@@ -859,8 +881,11 @@ __global__ void __launch_bounds__(kFewThreads) xent_few(Args a) {
   // of a wave: its part of a tile of logits, then the lines that it stores
   __shared__ u32x4 own_lds[16][kStored<kLine> / 16];
   static_assert(kStored<kLine> >= 1024, "a tile's part fits");
-  // the slopes (32 rows of k, kTok tokens), and some space
-  __shared__ __attribute__((aligned(16))) T by_token[kTok][kPitch], by_row[kR * 16][kRowPitch];
+  // the slopes as a sum of two of the type, which cost nothing here: 16 of a
+  // step's 32 k beside the other 16, or an array each; and some space
+  constexpr int kTokenParts = kR == 1 ? 2 : 1, kRowParts = kTok == 16 ? 2 : 1;  // in a step
+  __shared__ __attribute__((aligned(16))) T by_token[3 - kTokenParts][kTok][kPitch];
+  __shared__ __attribute__((aligned(16))) T by_row[3 - kRowParts][kR * 16][kRowPitch];
   __shared__ float known[4][kR * 16];  // of a row: m, c, log2 s, target
   const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 15, q = lane >> 4;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
@@ -911,8 +936,6 @@ __global__ void __launch_bounds__(kFewThreads) xent_few(Args a) {
       const uint32_t row = at / vecs, c = at - row * vecs;
       xl[row * vecs + (c ^ swap(row))] = ((const u32x4*)a.xs)[(uint64_t)row * (a.hidden64 / 8) + c];
     }
-  for (uint32_t i = tid; i < kTok * kPitch; i += kFewThreads) (&by_token[0][0])[i] = (T)0.0f;
-  for (uint32_t i = tid; i < kR * 16 * kRowPitch; i += kFewThreads) (&by_row[0][0])[i] = (T)0.0f;
   // the tile of logits that this wave shares, its steps of the hidden columns,
   // and what a lane knows of its row
   const uint32_t ts = wave % kTiles % (kTok / 16), rs = wave % kTiles / (kTok / 16), t = rs * 16 + col;
@@ -924,7 +947,7 @@ __global__ void __launch_bounds__(kFewThreads) xent_few(Args a) {
     x[s] = *(const u32x4*)((const T*)a.x + (int64_t)min(t, a.rows - 1) * a.x_stride +
                            (min(s0 + s, steps - 1) * 4 + q) * 8);
   if (tid < kR * 16) {
-    known[0][tid] = a.mant[tid] * kUp<T>;
+    known[0][tid] = a.factor[tid];
     known[1][tid] = a.top[tid];
     known[2][tid] = a.logsum[tid];
     known[3][tid] = __int_as_float(tid < a.rows ? a.target[tid] : -1);
@@ -959,16 +982,24 @@ __global__ void __launch_bounds__(kFewThreads) xent_few(Args a) {
       union {
         T e[4];
         uint2 u;
-      } o;
+      } o, rest;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint32_t tok = tile * kTok + ts * 16 + q * 4 + e;
         float g = exp2_raw(__builtin_fmaf(l[e], kLog2e, -c) - ls) - even;
         if ((int32_t)tok == y) g -= own;
-        o.e[e] = (T)(m != 0.0f && tok < a.vocab ? g * m : 0.0f);
-        by_token[ts * 16 + q * 4 + e][t] = o.e[e];
+        g = m != 0.0f && tok < a.vocab ? g * m : 0.0f;
+        o.e[e] = (T)g;
+        // (an infinity has no rest)
+        rest.e[e] = (T)(fabsf((float)o.e[e]) < INFINITY ? g - (float)o.e[e] : 0.0f);
+        const uint32_t n = ts * 16 + q * 4 + e;
+        by_token[0][n][t] = o.e[e];
+        if (kTokenParts == 2) by_token[0][n][16 + t] = rest.e[e];
+        else by_token[2 - kTokenParts][n][t] = rest.e[e];
       }
-      *(uint2*)&by_row[t][ts * 16 + q * 4] = o.u;
+      *(uint2*)&by_row[0][t][ts * 16 + q * 4] = o.u;
+      if (kRowParts == 2) *(uint2*)&by_row[0][t][16 + q * 4] = rest.u;
+      else *(uint2*)&by_row[2 - kRowParts][t][ts * 16 + q * 4] = rest.u;
     }
     __syncthreads();
     // columns 16 sub ... of rows k0 + 8 q ... of the table or the states, read
@@ -992,15 +1023,19 @@ __global__ void __launch_bounds__(kFewThreads) xent_few(Args a) {
     if (a.dx) {
 #pragma unroll
       for (int k = 0; k < (kTok + 31) / 32; ++k) {
-        u32x4 gf[kR];
+        u32x4 gf[3 - kRowParts][kR];
 #pragma unroll
-        for (int r = 0; r < kR; ++r) gf[r] = *(const u32x4*)&by_row[r * 16 + col][k * 32 + q * 8];
+        for (int i = 0; i < 3 - kRowParts; ++i)
+#pragma unroll
+          for (int r = 0; r < kR; ++r) gf[i][r] = *(const u32x4*)&by_row[i][r * 16 + (now & 15)][k * 32 + (now >> 4) * 8];
 #pragma unroll
         for (int j = 0; j < kSubs; ++j) {
           if ((uint32_t)j >= own_subs) break;
           const u32x4 w = across(st, kTok, k * 32, sub0 + j);
 #pragma unroll
-          for (int r = 0; r < kR; ++r) sum[j][r] = mfma(w, gf[r], sum[j][r], T{});
+          for (int i = 0; i < 3 - kRowParts; ++i)
+#pragma unroll
+            for (int r = 0; r < kR; ++r) sum[j][r] = mfma(w, gf[i][r], sum[j][r], T{});
           if (kSubs > 4 || j % 2) __builtin_amdgcn_sched_barrier(0);
         }
       }
@@ -1017,11 +1052,16 @@ __global__ void __launch_bounds__(kFewThreads) xent_few(Args a) {
 #pragma unroll
         for (int i = 0; i < kTok / 16; ++i) {
           const uint32_t tok = tile * kTok + i * 16;
-          const u32x4 gf = *(const u32x4*)&by_token[i * 16 + (now & 15)][(now >> 4) * 8];
+          u32x4 gf[3 - kTokenParts];
+#pragma unroll
+          for (int p = 0; p < 3 - kTokenParts; ++p)
+            gf[p] = *(const u32x4*)&by_token[p][i * 16 + (now & 15)][(now >> 4) * 8];
           uint2 all[kLine];
 #pragma unroll
           for (int j = 0; j < kLine; ++j) {
-            const f32x4 d = mfma(xf[j], gf, f32x4{}, T{});
+            f32x4 d{};
+#pragma unroll
+            for (int p = 0; p < 3 - kTokenParts; ++p) d = mfma(xf[j], gf[p], d, T{});
             union {
               T e[4];
               uint2 u;
@@ -1055,7 +1095,7 @@ __global__ void __launch_bounds__(kFewThreads) xent_few(Args a) {
 constexpr uint32_t kCUs = 256;
 
 struct Plan {
-  uint64_t mant, power, largest, part, picked, top, logsum, terms, xs, slopes, dxs, bytes;
+  uint64_t factor, power, largest, part, picked, top, logsum, terms, xs, slopes, dxs, bytes;
   uint64_t split_stride;
   uint32_t rows64, hidden64, tiles, piece, slope_stride, splits, split_steps, bm, bn;
   uint32_t few;  // 16-row subtiles of xent_few; 0: other kernels
@@ -1098,7 +1138,7 @@ Plan plan(const ft_cross_entropy_loss_args& a) {
   const uint64_t r = p.rows64;
   if (p.lines && a.hidden <= (a.rows <= 16 ? 2048 : a.rows <= 32 ? 512 : 0) && (a.dx || a.dweight))
     p.few = (uint32_t)(a.rows + 15) / 16;
-  p.mant = ar.take(r * 4);
+  p.factor = ar.take(r * 4);
   p.power = ar.take(r * 4);
   p.largest = ar.take(4);
   p.part = ar.take(3 * r * p.tiles * 4);
@@ -1170,18 +1210,17 @@ hipError_t launch(Args a, const Plan& p, hipStream_t s) {
     return e == hipSuccess && a.dweight ? start(xent_nothing<T>, a.vocab, 256, s, a) : e;
   }
   a.tiled = p.few ? a.rows64 : (uint32_t)std::min<uint64_t>(a.rows64, round_up(a.rows, p.bm));
-  // few rows are prepared beside the statistics, and joined with the loss
-  hipError_t e = hipSuccess;
-  if (p.lines && p.bm == 64) a.prepare = a.rows64 / 8;
-  else e = start(xent_rows<T>, a.rows64 / 4, 256, s, a);
-  if (e != hipSuccess) return e;
-  e = product<T, kStats>(a, p, s);
+  // a few rows are prepared beside the statistics, and joined with the loss
+  if (p.few) a.prepare = a.rows64 / 8;
+  hipError_t e = product<T, kStats>(a, p, s);
   if (e != hipSuccess) return e;
   const bool together = a.rows <= 16 || (a.rows <= 64 && a.tiles <= 256);
   e = start(xent_join, together ? 1 : (a.rows + 15) / 16, 1024, s, a);
   if (e != hipSuccess) return e;
   if (!together) e = start(xent_loss, 1, 1024, s, a);
   if (e != hipSuccess || !(a.dx || a.dweight)) return e;
+  if (!p.few) e = start(xent_rows<T>, a.rows64 / 4, 256, s, a);
+  if (e != hipSuccess) return e;
   if (p.few) {
     e = p.few == 2         ? start(xent_few<T, 2, 64>, a.splits, kFewThreads, s, a)
         : a.hidden <= 512  ? start(xent_few<T, 1, 64>, a.splits, kFewThreads, s, a)
@@ -1232,7 +1271,7 @@ hipError_t launch_cross_entropy_loss(const ft_cross_entropy_loss_args& q, uint8_
   a.vocab = q.vocab;
   a.tiles = p.tiles;
   a.smoothing = q.smoothing;
-  a.mant = (float*)(ws + p.mant);
+  a.factor = (float*)(ws + p.factor);
   a.power = (float*)(ws + p.power);
   a.largest = (float*)(ws + p.largest);
   a.part = (float*)(ws + p.part);

@@ -61,7 +61,10 @@ def cross_entropy(x, weight, targets, row_weight, smoothing):
     rg = rr * g
     dw = rg.t() @ torch.where(used[:, None], xd, 0.0)
     dwe = (rr.abs() * ge).t() @ xa + (T + 8) * U * (rg.abs().t() @ xa)
-    # rows of x are scaled by a power of two to the largest weight's
+    # rows of x are scaled to the largest weight's, by a factor near a power of two
+    # that makes the target's slope one of the type's numbers: a state is rounded
+    # once more, relative to itself, in the products of its row
+    dwe = dwe + HALF_UNIT[dtype] * (rg.abs().t() @ xa)
     if T:
         dwe = dwe + 2 * rr.abs().max() * TINY[dtype] * (g.abs() + ge).sum(0)[:, None]
     zero = torch.zeros((), dtype=torch.float64, device=x.device)
