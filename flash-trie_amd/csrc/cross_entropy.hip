@@ -175,11 +175,6 @@ __device__ __forceinline__ void prepare_rows(const Args& a, uint32_t block) {
   if (t >= a.tiled)
     for (uint32_t k = lane * 8; k < a.piece; k += 512) ((u32x4*)a.slopes)[((uint64_t)t * a.slope_stride + k) / 8] = u32x4{};
 }
-template <typename T>
-__global__ void __launch_bounds__(256) xent_rows(Args a) {
-  prepare_rows<T, 4, true>(a, blockIdx.x);
-}
-
 // 16 rows by 64 parts of the tiles.  A workgroup that has them all adds up the
 // loss.
 __device__ __forceinline__ void join_rows(const Args& a, uint32_t first) {
@@ -245,25 +240,37 @@ __device__ __forceinline__ void join_rows(const Args& a, uint32_t first) {
   a.terms[t] = term;
 }
 
+// In 1024 parts, whatever the workgroup: the same sum from every launch.
 __device__ __forceinline__ void add_loss(const Args& a) {
   __shared__ float waves[16];
-  float sum = 0.0f;
-  for (uint32_t t = threadIdx.x; t < a.rows; t += 1024) sum += a.terms[t];
-  sum = wave_sum(sum);
-  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = sum;
+  const uint32_t lane = threadIdx.x & 63;
+  for (uint32_t w = threadIdx.x >> 6; w < 16; w += blockDim.x >> 6) {
+    float sum = 0.0f;
+    for (uint32_t t = w * 64 + lane; t < a.rows; t += 1024) sum += a.terms[t];
+    sum = wave_sum(sum);
+    if (lane == 0) waves[w] = sum;
+  }
   __syncthreads();
   if (threadIdx.x) return;
-  sum = 0.0f;
+  float sum = 0.0f;
+#pragma unroll
   for (int w = 0; w < 16; ++w) sum += waves[w];
   *a.loss = sum;
 }
 __global__ void __launch_bounds__(1024) xent_loss(Args a) { add_loss(a); }
+// Up to 16 rows: their loss too.
 __global__ void __launch_bounds__(1024) xent_join(Args a) {
-  for (uint32_t t = blockIdx.x * 16; t < a.rows; t += gridDim.x * 16) {
-    join_rows(a, t);
-    __syncthreads();
-  }
-  if (gridDim.x == 1) add_loss(a);
+  join_rows(a, blockIdx.x * 16);
+  if (a.rows > 16) return;
+  __syncthreads();
+  add_loss(a);
+}
+// And the rows' factors and scaled states, of all rows up to whole 64s.
+template <typename T>
+__global__ void __launch_bounds__(1024) xent_rows(Args a) {
+  if (blockIdx.x * 16 < a.rows) join_rows(a, blockIdx.x * 16);
+  __syncthreads();
+  prepare_rows<T, 16, true>(a, blockIdx.x);
 }
 
 // No rows: a table's gradient of zeros.
@@ -280,6 +287,10 @@ __global__ void __launch_bounds__(1024) xent_states(Args a) {
   __shared__ f32x4 other[15][64];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const uint32_t panels = (a.hidden64 + 255) / 256;
+  if (blockIdx.x == a.rows * panels) {  // (the last, where it is there)
+    add_loss(a);
+    return;
+  }
   const uint32_t t = blockIdx.x / panels, h = (blockIdx.x % panels * 64 + lane) * 4;
   f32x4 y{};
   if (h < a.hidden64) {
@@ -1199,8 +1210,9 @@ hipError_t product(const Args& a, const Plan& p, hipStream_t s) {
 }
 
 template <typename T>
-hipError_t states(const Args& a, hipStream_t s) {
-  return start(xent_states<T>, (uint64_t)a.rows * ((a.hidden64 + 255) / 256), 64 * std::min(16u, a.splits), s, a);
+hipError_t states(const Args& a, bool loss, hipStream_t s) {
+  // (with the loss where the rows' launch did not add it up)
+  return start(xent_states<T>, (uint64_t)a.rows * ((a.hidden64 + 255) / 256) + loss, 64 * std::min(16u, a.splits), s, a);
 }
 
 template <typename T>
@@ -1214,19 +1226,19 @@ hipError_t launch(Args a, const Plan& p, hipStream_t s) {
   if (p.few) a.prepare = a.rows64 / 8;
   hipError_t e = product<T, kStats>(a, p, s);
   if (e != hipSuccess) return e;
-  const bool together = a.rows <= 16 || (a.rows <= 64 && a.tiles <= 256);
-  e = start(xent_join, together ? 1 : (a.rows + 15) / 16, 1024, s, a);
+  const bool grads = a.dx || a.dweight;
+  e = grads && !p.few ? start(xent_rows<T>, a.rows64 / 16, 1024, s, a)
+                      : start(xent_join, (a.rows + 15) / 16, 1024, s, a);
   if (e != hipSuccess) return e;
-  if (!together) e = start(xent_loss, 1, 1024, s, a);
-  if (e != hipSuccess || !(a.dx || a.dweight)) return e;
-  if (!p.few) e = start(xent_rows<T>, a.rows64 / 4, 256, s, a);
-  if (e != hipSuccess) return e;
+  // (the loss: with the rows, with dx, or by itself)
+  if (!a.dx && (grads && !p.few || a.rows > 16)) e = start(xent_loss, 1, 1024, s, a);
+  if (e != hipSuccess || !grads) return e;
   if (p.few) {
     e = p.few == 2         ? start(xent_few<T, 2, 64>, a.splits, kFewThreads, s, a)
         : a.hidden <= 512  ? start(xent_few<T, 1, 64>, a.splits, kFewThreads, s, a)
         : a.hidden <= 1024 ? start(xent_few<T, 1, 32>, a.splits, kFewThreads, s, a)
                            : start(xent_few<T, 1, 16>, a.splits, kFewThreads, s, a);
-    return e == hipSuccess && a.dx ? states<T>(a, s) : e;
+    return e == hipSuccess && a.dx ? states<T>(a, a.rows > 16, s) : e;
   }
   for (a.first = 0; a.first < a.vocab; a.first += a.piece) {
     a.width = (uint32_t)std::min<uint64_t>(a.piece, round_up(a.vocab - a.first, 256));
@@ -1242,7 +1254,7 @@ hipError_t launch(Args a, const Plan& p, hipStream_t s) {
     }
   }
   if (!a.dx) return hipSuccess;
-  return states<T>(a, s);
+  return states<T>(a, true, s);
 }
 
 }  // namespace
