@@ -762,14 +762,6 @@ __global__ void __launch_bounds__(kTileThreads) xent_tile(Args a) {
   __shared__ __attribute__((aligned(1024))) char st0[P::kBytes + Q::kBytes], st1[P::kBytes + Q::kBytes];
   __shared__ float joined[kKind == kStats ? S::WN : 1][3][kKind == kStats ? S::BM : 1];
   __shared__ u32x4 stored[kKind == kSlopes || kKind == kTable ? 8 * kStored<S::N> / 16 : 1];
-  if constexpr (kKind == kStats && S::BM == 64) {
-    if (blockIdx.x < a.prepare) {
-      prepare_rows<T, 8, false>(a, blockIdx.x);
-      return;
-    }
-  }
-  const uint32_t own = blockIdx.x - (kKind == kStats ? a.prepare : 0);
-  const uint32_t workers = gridDim.x - (kKind == kStats ? a.prepare : 0);
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t wm = wave % S::WM, wn = wave / S::WM;
   const uint32_t js = kKind == kTable ? a.width / S::BM : (a.rows + S::BM - 1) / S::BM;
@@ -811,8 +803,8 @@ __global__ void __launch_bounds__(kTileThreads) xent_tile(Args a) {
     copy(st0, 0, tid & 63);
     copy(st1, 1, tid & 63);
   };
-  begin(own);
-  for (uint32_t block = own;;) {
+  begin(blockIdx.x);
+  for (uint32_t block = blockIdx.x;;) {
     f32x4 acc[S::N][S::M] = {};
     // Half a step: the products of w and x, while w and `ahead` take the next
     // half's operands, kk of the stage `next`.  A register of w is free when
@@ -856,7 +848,7 @@ __global__ void __launch_bounds__(kTileThreads) xent_tile(Args a) {
     wait_copies<0>();
     __syncthreads();
     const uint32_t jb = tj * S::BM, tile = ti, part = split;
-    block += workers;
+    block += gridDim.x;
     const bool more = block < tiles;
     if (more) begin(block);
     uint32_t tid = threadIdx.x;
@@ -881,14 +873,23 @@ __global__ void __launch_bounds__(kTileThreads) xent_tile(Args a) {
 constexpr uint32_t kFewBytes = 65536;  // of the states, and of a tile
 constexpr int kFewThreads = 1024;
 
-template <typename T, int kR, int kTok>
+// kStats: the pass before it, for the rows' statistics: each workgroup's own,
+// held by lanes (a row, and the tokens 4 q ... of a subtile) to the end.
+template <typename T, int kR, int kTok, bool kStats>
 __global__ void __launch_bounds__(kFewThreads) xent_few(Args a) {
+  if constexpr (kStats) {
+    if (blockIdx.x < a.prepare) {
+      prepare_rows<T, 16, false>(a, blockIdx.x);
+      return;
+    }
+  }
+  const uint32_t block = blockIdx.x - (kStats ? a.prepare : 0), blocks = gridDim.x - (kStats ? a.prepare : 0);
   constexpr int kTiles = kR * kTok / 16, kSplits = 16 / kTiles;  // 16 x 16 tiles of logits, waves for one
   constexpr int kColumns = 32768 / kTok;                         // the most
   constexpr int kSubs = kColumns / 256, kX = kColumns / 32 / kSplits;  // of a wave: 16-column subtiles, steps of 32
   constexpr int kLoads = (int)kFewBytes / 16 / kFewThreads, kPitch = 40, kRowPitch = (kTok < 32 ? 32 : kTok) + 8;
   constexpr int kLine = kSubs == 4 && kR == 1 ? 4 : 2;  // subtiles stored at a time: LDS for more where it is left
-  __shared__ u32x4 st[kFewBytes / 16], xl[kR * 16 * kColumns / 8];
+  __shared__ u32x4 st[kFewBytes / 16], xl[kStats ? 1 : kR * 16 * kColumns / 8];
   // of a wave: its part of a tile of logits, then the lines that it stores
   __shared__ u32x4 own_lds[16][kStored<kLine> / 16];
   static_assert(kStored<kLine> >= 1024, "a tile's part fits");
@@ -940,9 +941,9 @@ __global__ void __launch_bounds__(kFewThreads) xent_few(Args a) {
     for (int i = 0; i < kLoads; ++i)
       if (from[i] != ~0u) st[(i * kFewThreads + tid) ^ (swaps >> (3 * i) & 7)] = next[i];
   };
-  uint32_t tile = blockIdx.x;
+  uint32_t tile = block;
   load(tile);
-  if (a.dweight)
+  if (!kStats && a.dweight)
     for (uint32_t at = tid; at < kR * 16 * vecs; at += kFewThreads) {
       const uint32_t row = at / vecs, c = at - row * vecs;
       xl[row * vecs + (c ^ swap(row))] = ((const u32x4*)a.xs)[(uint64_t)row * (a.hidden64 / 8) + c];
@@ -958,17 +959,21 @@ __global__ void __launch_bounds__(kFewThreads) xent_few(Args a) {
     x[s] = *(const u32x4*)((const T*)a.x + (int64_t)min(t, a.rows - 1) * a.x_stride +
                            (min(s0 + s, steps - 1) * 4 + q) * 8);
   if (tid < kR * 16) {
-    known[0][tid] = a.factor[tid];
-    known[1][tid] = a.top[tid];
-    known[2][tid] = a.logsum[tid];
+    if (!kStats) {
+      known[0][tid] = a.factor[tid];
+      known[1][tid] = a.top[tid];
+      known[2][tid] = a.logsum[tid];
+    }
     known[3][tid] = __int_as_float(tid < a.rows ? a.target[tid] : -1);
   }
   const float even = a.smoothing / (float)a.vocab, own = 1.0f - a.smoothing;
-  const float f = *a.largest * (1.0f / kUp<T>);
+  const float f = kStats ? 0.0f : *a.largest * (1.0f / kUp<T>);
   keep();
   f32x4 sum[kSubs][kR] = {};
-  for (; tile < tiles; tile += gridDim.x) {
-    load(min(tile + gridDim.x, tiles - 1));
+  Part mine{-INFINITY, 0.0f};
+  float total = 0.0f;
+  for (; tile < tiles; tile += blocks) {
+    load(min(tile + blocks, tiles - 1));
     __syncthreads();
     {
       // (the lane anew here and below, so that addresses are not kept through the
@@ -984,6 +989,32 @@ __global__ void __launch_bounds__(kFewThreads) xent_few(Args a) {
       *(f32x4*)&own_lds[wave][lane] = l;
     }
     __syncthreads();
+    if constexpr (kStats) {
+      keep();  // (past the barrier all of the tile has been read)
+      if (wave < (uint32_t)kTiles) {
+        f32x4 l{};
+#pragma unroll
+        for (int i = 0; i < kSplits; ++i) l += *(const f32x4*)&own_lds[wave + i * kTiles][lane];
+        const uint32_t tok = tile * kTok + ts * 16 + q * 4, y = __float_as_uint(known[3][t]) - tok;
+        float big = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool in = tok + e < a.vocab;
+          if (y == (uint32_t)e && in) a.picked[t] = l[e];
+          total += in ? l[e] : 0.0f;
+          if (!in) l[e] = -INFINITY;
+          big = fmaxf(big, l[e]);
+        }
+        if (!(big == -INFINITY)) {
+          const float c = fmaxf(mine.c, big * kLog2e);
+          mine.s = mine.s == 0.0f ? 0.0f : mine.s * exp2_raw(mine.c - c);
+          mine.c = c;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mine.s += power_of(l[e], c);
+        }
+      }
+      continue;
+    }
     if (wave < (uint32_t)kTiles) {
       const float m = known[0][t], c = known[1][t], ls = known[2][t];
       const int32_t y = __float_as_int(known[3][t]);
@@ -1090,13 +1121,45 @@ __global__ void __launch_bounds__(kFewThreads) xent_few(Args a) {
       }
     }
   }
+  if constexpr (kStats) {
+#pragma unroll
+    for (int d = 16; d < 64; d *= 2) {
+      const Part other{__shfl_xor(mine.c, d, 64), __shfl_xor(mine.s, d, 64)};
+      const float more = __shfl_xor(total, d, 64);
+      mine = join(mine, other);
+      total += more;
+    }
+    float* parts = (float*)&by_row[0][0][0];  // [kTiles][3][16]
+    static_assert(sizeof(by_row) >= kTiles * 48 * 4, "the waves' parts fit");
+    if (wave < (uint32_t)kTiles && lane < 16) {
+      parts[wave * 48 + lane] = mine.c;
+      parts[wave * 48 + 16 + lane] = mine.s;
+      parts[wave * 48 + 32 + lane] = total;
+    }
+    __syncthreads();
+    if (tid < kR * 16) {
+      Part p{0.0f, 0.0f};
+      float l = 0.0f;
+      for (uint32_t i = 0; i < kTok / 16; ++i) {
+        const float* from = parts + (tid / 16 * (kTok / 16) + i) * 48 + tid % 16;
+        p = join(p, Part{from[0], from[16]});
+        l += from[32];
+      }
+      const uint64_t each = (uint64_t)a.tiles * a.rows64, at = (uint64_t)block * a.rows64 + tid;
+      // (of nothing but -infinity: c is 0)
+      a.part[at] = p.c == -INFINITY ? 0.0f : p.c;
+      a.part[each + at] = p.s;
+      a.part[2 * each + at] = l;
+    }
+    return;
+  }
   if (!a.dx) return;
 #pragma unroll
   for (int j = 0; j < kSubs; ++j) {
     if ((uint32_t)j >= own_subs) break;
 #pragma unroll
     for (int r = 0; r < kR; ++r)
-      *(f32x4*)(a.dxs + blockIdx.x * a.split_stride + (uint64_t)(r * 16 + col) * a.hidden64 + (sub0 + j) * 16 + q * 4) =
+      *(f32x4*)(a.dxs + block * a.split_stride + (uint64_t)(r * 16 + col) * a.hidden64 + (sub0 + j) * 16 + q * 4) =
           sum[j][r];
   }
 }
@@ -1147,8 +1210,11 @@ Plan plan(const ft_cross_entropy_loss_args& a) {
   }
   p.tiles = (a.vocab + p.bn - 1) / p.bn;
   const uint64_t r = p.rows64;
-  if (p.lines && a.hidden <= (a.rows <= 16 ? 2048 : a.rows <= 32 ? 512 : 0) && (a.dx || a.dweight))
+  if (p.lines && a.rows && a.hidden <= (a.rows <= 16 ? 2048 : a.rows <= 32 ? 512 : 0)) {
+    const uint32_t tok = a.hidden <= 512 ? 64 : a.hidden <= 1024 ? 32 : 16;
     p.few = (uint32_t)(a.rows + 15) / 16;
+    p.tiles = std::min(kCUs, (a.vocab + tok - 1) / tok);  // workgroups
+  }
   p.factor = ar.take(r * 4);
   p.power = ar.take(r * 4);
   p.largest = ar.take(4);
@@ -1169,8 +1235,7 @@ Plan plan(const ft_cross_entropy_loss_args& a) {
   }
   if (a.dweight) p.xs = ar.take(r * p.hidden64 * 2);
   if (p.few) {
-    const uint32_t tok = a.hidden <= 512 ? 64 : a.hidden <= 1024 ? 32 : 16;
-    p.splits = std::min(kCUs, (a.vocab + tok - 1) / tok);
+    p.splits = p.tiles;
     p.split_stride = 16ull * p.few * p.hidden64;
     if (a.dx) p.dxs = ar.take(p.splits * p.split_stride * 4);
   } else if (a.dx) {
@@ -1197,16 +1262,22 @@ hipError_t product(const Args& a, const Plan& p, hipStream_t s) {
                                                    : hs);
   if (!p.lines) return start(xent_product<T, kKind>, blocks, kThreads, s, a);
   if constexpr (kKind != kTable) {
-    if (p.bm == 64)
-      return start(xent_tile<T, kKind, TileShape<4, 1>>,
-                   (kKind == kStats ? a.prepare : 0) + std::min<uint64_t>(blocks, kCUs), kTileThreads, s, a);
     const uint64_t most = std::min<uint64_t>(blocks, kCUs);
+    if (p.bm == 64) return start(xent_tile<T, kKind, TileShape<4, 1>>, most, kTileThreads, s, a);
     if (p.bm == 128) return start(xent_tile<T, kKind, TileShape<8, 2>>, most, kTileThreads, s, a);
     if (p.bm == 160) return start(xent_tile<T, kKind, TileShape<10, 2>>, most, kTileThreads, s, a);
     if (p.bm == 192) return start(xent_tile<T, kKind, TileShape<12, 2>>, most, kTileThreads, s, a);
     if (p.bm == 224) return start(xent_tile<T, kKind, TileShape<14, 2>>, most, kTileThreads, s, a);
   }
   return start(xent_tile<T, kKind, TileShape<16, 2>>, std::min<uint64_t>(blocks, kCUs), kTileThreads, s, a);
+}
+
+template <typename T, bool kStats>
+hipError_t few(const Args& a, const Plan& p, uint64_t blocks, hipStream_t s) {
+  return p.few == 2         ? start(xent_few<T, 2, 64, kStats>, blocks, kFewThreads, s, a)
+         : a.hidden <= 512  ? start(xent_few<T, 1, 64, kStats>, blocks, kFewThreads, s, a)
+         : a.hidden <= 1024 ? start(xent_few<T, 1, 32, kStats>, blocks, kFewThreads, s, a)
+                            : start(xent_few<T, 1, 16, kStats>, blocks, kFewThreads, s, a);
 }
 
 template <typename T>
@@ -1223,10 +1294,10 @@ hipError_t launch(Args a, const Plan& p, hipStream_t s) {
   }
   a.tiled = p.few ? a.rows64 : (uint32_t)std::min<uint64_t>(a.rows64, round_up(a.rows, p.bm));
   // a few rows are prepared beside the statistics, and joined with the loss
-  if (p.few) a.prepare = a.rows64 / 8;
-  hipError_t e = product<T, kStats>(a, p, s);
-  if (e != hipSuccess) return e;
   const bool grads = a.dx || a.dweight;
+  if (p.few && grads) a.prepare = a.rows64 / 16;
+  hipError_t e = p.few ? few<T, true>(a, p, a.prepare + a.tiles, s) : product<T, kStats>(a, p, s);
+  if (e != hipSuccess) return e;
   e = grads && !p.few ? start(xent_rows<T>, a.rows64 / 16, 1024, s, a)
                       : start(xent_join, (a.rows + 15) / 16, 1024, s, a);
   if (e != hipSuccess) return e;
@@ -1234,10 +1305,7 @@ hipError_t launch(Args a, const Plan& p, hipStream_t s) {
   if (!a.dx && (grads && !p.few || a.rows > 16)) e = start(xent_loss, 1, 1024, s, a);
   if (e != hipSuccess || !grads) return e;
   if (p.few) {
-    e = p.few == 2         ? start(xent_few<T, 2, 64>, a.splits, kFewThreads, s, a)
-        : a.hidden <= 512  ? start(xent_few<T, 1, 64>, a.splits, kFewThreads, s, a)
-        : a.hidden <= 1024 ? start(xent_few<T, 1, 32>, a.splits, kFewThreads, s, a)
-                           : start(xent_few<T, 1, 16>, a.splits, kFewThreads, s, a);
+    e = few<T, false>(a, p, a.splits, s);
     return e == hipSuccess && a.dx ? states<T>(a, a.rows > 16, s) : e;
   }
   for (a.first = 0; a.first < a.vocab; a.first += a.piece) {
