@@ -175,10 +175,11 @@ __device__ __forceinline__ void prepare_rows(const Args& a, uint32_t block) {
   if (t >= a.tiled)
     for (uint32_t k = lane * 8; k < a.piece; k += 512) ((u32x4*)a.slopes)[((uint64_t)t * a.slope_stride + k) / 8] = u32x4{};
 }
-// 16 rows by 64 parts of the tiles.  A workgroup that has them all adds up the
-// loss.
-__device__ __forceinline__ void join_rows(const Args& a, uint32_t first) {
-  __shared__ float sc[64][16], ss[64][16], sl[64][16];
+// 16 rows, by 64 parts of the tiles, through 12 KB of LDS: c and log2 s go to
+// `top` and `logsum`, the rows' scores and terms, where `write`, to memory.
+__device__ __forceinline__ void join_rows(const Args& a, uint32_t first, float (*lds)[64][16], float* top,
+                                          float* logsum, bool write) {
+  float(*sc)[16] = lds[0], (*ss)[16] = lds[1], (*sl)[16] = lds[2];
   const uint32_t row = threadIdx.x & 15, from = threadIdx.x >> 4, t = first + row;
   const uint64_t each = (uint64_t)a.tiles * a.rows64;
   Part p{0.0f, 0.0f};
@@ -224,8 +225,9 @@ __device__ __forceinline__ void join_rows(const Args& a, uint32_t first) {
   // (a target out of range: NaN, and with it the row's slopes)
   const double ls = y < 0 || there ? log2((double)p.s) : (double)NAN;
   const float at = there ? (float)((((double)a.picked[t] * (double)kLog2e - (double)p.c) - ls) * kLn2) : NAN;
-  a.top[t] = p.c;
-  a.logsum[t] = (float)ls;
+  top[row] = p.c;
+  logsum[row] = (float)ls;
+  if (!write) return;
   float term = 0.0f;
   if (y >= 0) {
     a.logp[t] = at;
@@ -260,7 +262,8 @@ __device__ __forceinline__ void add_loss(const Args& a) {
 __global__ void __launch_bounds__(1024) xent_loss(Args a) { add_loss(a); }
 // Up to 16 rows: their loss too.
 __global__ void __launch_bounds__(1024) xent_join(Args a) {
-  join_rows(a, blockIdx.x * 16);
+  __shared__ float lds[3][64][16];
+  join_rows(a, blockIdx.x * 16, lds, a.top + blockIdx.x * 16, a.logsum + blockIdx.x * 16, true);
   if (a.rows > 16) return;
   __syncthreads();
   add_loss(a);
@@ -268,7 +271,9 @@ __global__ void __launch_bounds__(1024) xent_join(Args a) {
 // And the rows' factors and scaled states, of all rows up to whole 64s.
 template <typename T>
 __global__ void __launch_bounds__(1024) xent_rows(Args a) {
-  if (blockIdx.x * 16 < a.rows) join_rows(a, blockIdx.x * 16);
+  __shared__ float lds[3][64][16];
+  if (blockIdx.x * 16 < a.rows)
+    join_rows(a, blockIdx.x * 16, lds, a.top + blockIdx.x * 16, a.logsum + blockIdx.x * 16, true);
   __syncthreads();
   prepare_rows<T, 16, true>(a, blockIdx.x);
 }
@@ -280,34 +285,44 @@ __global__ void __launch_bounds__(256) xent_nothing(Args a) {
   for (uint32_t h = threadIdx.x; h < a.hidden; h += 256) row[h] = (T)0.0f;
 }
 
-// dx from its parts: 256 columns of a row a workgroup, whose waves take the
-// parts in turn.
-template <typename T>
+// dx from its parts: 64 columns of a row a wave (kWave, up to 16 parts) or a
+// workgroup, and turn; 16 lanes a part.  The first workgroup adds up the loss
+// where another launch does not.  4 parts of 4,096 rows x 1,024: 22 us by waves,
+// 33 by workgroups of one.
+constexpr uint32_t kStatesGrid = 1 << 20;
+template <typename T, bool kLoss, bool kWave>
 __global__ void __launch_bounds__(1024) xent_states(Args a) {
-  __shared__ f32x4 other[15][64];
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  const uint32_t panels = (a.hidden64 + 255) / 256;
-  if (blockIdx.x == a.rows * panels) {  // (the last, where it is there)
-    add_loss(a);
-    return;
-  }
-  const uint32_t t = blockIdx.x / panels, h = (blockIdx.x % panels * 64 + lane) * 4;
-  f32x4 y{};
-  if (h < a.hidden64) {
+  __shared__ f32x4 waves[16][16];
+  const uint32_t tid = threadIdx.x, lane = tid & 15, wave = tid >> 6;
+  const uint32_t part = kWave ? tid >> 4 & 3 : tid >> 4, parts = kWave ? 4 : blockDim.x / 16;
+  const uint32_t panels = a.hidden64 / 64, each = kWave ? blockDim.x / 64 : 1;
+  if (kLoss && blockIdx.x == 0) add_loss(a);
+  const uint64_t units = (uint64_t)a.rows * panels;
+  for (uint64_t unit = (uint64_t)blockIdx.x * each + (kWave ? wave : 0); unit < units; unit += (uint64_t)gridDim.x * each) {
+    const uint32_t t = (uint32_t)(unit / panels), h = ((uint32_t)(unit % panels) * 16 + lane) * 4;
     const float* p = a.dxs + (uint64_t)t * a.hidden64 + h;
+    f32x4 y{};
 #pragma unroll 4
-    for (uint32_t s = wave; s < a.splits; s += waves) y += *(const f32x4*)(p + s * a.split_stride);
-  }
-  if (wave > 0) other[wave - 1][lane] = y;
-  __syncthreads();
-  if (wave > 0) return;
-  for (uint32_t w = 1; w < waves; ++w) y += other[w - 1][lane];
-  const bool none = a.factor[t] == 0.0f;
-  const float f = a.power[t];
-  T* out = (T*)a.dx + (int64_t)t * a.dx_stride + h;
+    for (uint32_t s = part; s < a.splits; s += parts) y += *(const f32x4*)(p + s * a.split_stride);
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (h + e < a.hidden) out[e] = (T)(none ? 0.0f : y[e] * f);
+    for (int d = 16; d < 64; d *= 2)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] += __shfl_xor(y[e], d, 64);
+    if (!kWave) {
+      __syncthreads();  // (the turn before has read its sums)
+      if ((tid & 63) < 16) waves[wave][lane] = y;
+      __syncthreads();
+      if (wave > 0) continue;
+      for (uint32_t w = 1; w < parts / 4; ++w) y += waves[w][lane];
+    }
+    if ((tid & 63) >= 16) continue;
+    const bool none = a.factor[t] == 0.0f;
+    const float f = a.power[t];
+    T* out = (T*)a.dx + (int64_t)t * a.dx_stride + h;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (h + e < a.hidden) out[e] = (T)(none ? 0.0f : y[e] * f);
+  }
 }
 
 // --- products ---------------------------------------------------------------
@@ -959,15 +974,20 @@ __global__ void __launch_bounds__(kFewThreads) xent_few(Args a) {
     x[s] = *(const u32x4*)((const T*)a.x + (int64_t)min(t, a.rows - 1) * a.x_stride +
                            (min(s0 + s, steps - 1) * 4 + q) * 8);
   if (tid < kR * 16) {
-    if (!kStats) {
-      known[0][tid] = a.factor[tid];
-      known[1][tid] = a.top[tid];
-      known[2][tid] = a.logsum[tid];
-    }
+    if (!kStats) known[0][tid] = a.factor[tid];
     known[3][tid] = __int_as_float(tid < a.rows ? a.target[tid] : -1);
   }
   const float even = a.smoothing / (float)a.vocab, own = 1.0f - a.smoothing;
   const float f = kStats ? 0.0f : *a.largest * (1.0f / kUp<T>);
+  // every workgroup joins the statistics for itself (a launch less); the first
+  // leaves the scores and the loss
+  if (!kStats) {
+    for (uint32_t r = 0; r < kR * 16 && r < a.rows; r += 16) {
+      join_rows(a, r, (float(*)[64][16])st, known[1] + r, known[2] + r, block == 0);
+      __syncthreads();
+    }
+    if (block == 0) add_loss(a);
+  }
   keep();
   f32x4 sum[kSubs][kR] = {};
   Part mine{-INFINITY, 0.0f};
@@ -1282,8 +1302,15 @@ hipError_t few(const Args& a, const Plan& p, uint64_t blocks, hipStream_t s) {
 
 template <typename T>
 hipError_t states(const Args& a, bool loss, hipStream_t s) {
-  // (with the loss where the rows' launch did not add it up)
-  return start(xent_states<T>, (uint64_t)a.rows * ((a.hidden64 + 255) / 256) + loss, 64 * std::min(16u, a.splits), s, a);
+  const uint64_t units = (uint64_t)a.rows * (a.hidden64 / 64);
+  const auto most = [](uint64_t blocks) { return std::min<uint64_t>(kStatesGrid, blocks); };
+  if (a.splits <= 16)
+    return loss ? start(xent_states<T, true, true>, most((units + 3) / 4), 256, s, a)
+                : start(xent_states<T, false, true>, most((units + 3) / 4), 256, s, a);
+  // (few workgroups: as many loads at once as there are parts)
+  const uint32_t threads = (uint32_t)std::min<uint64_t>(units < 1024 ? 1024 : 256, round_up(16 * a.splits, 64));
+  return loss ? start(xent_states<T, true, false>, most(units), threads, s, a)
+              : start(xent_states<T, false, false>, most(units), threads, s, a);
 }
 
 template <typename T>
@@ -1298,16 +1325,15 @@ hipError_t launch(Args a, const Plan& p, hipStream_t s) {
   if (p.few && grads) a.prepare = a.rows64 / 16;
   hipError_t e = p.few ? few<T, true>(a, p, a.prepare + a.tiles, s) : product<T, kStats>(a, p, s);
   if (e != hipSuccess) return e;
-  e = grads && !p.few ? start(xent_rows<T>, a.rows64 / 16, 1024, s, a)
-                      : start(xent_join, (a.rows + 15) / 16, 1024, s, a);
+  if (p.few && grads) {
+    e = few<T, false>(a, p, a.splits, s);
+    return e == hipSuccess && a.dx ? states<T>(a, false, s) : e;
+  }
+  e = grads ? start(xent_rows<T>, a.rows64 / 16, 1024, s, a) : start(xent_join, (a.rows + 15) / 16, 1024, s, a);
   if (e != hipSuccess) return e;
   // (the loss: with the rows, with dx, or by itself)
-  if (!a.dx && (grads && !p.few || a.rows > 16)) e = start(xent_loss, 1, 1024, s, a);
+  if (grads ? !a.dx : a.rows > 16) e = start(xent_loss, 1, 1024, s, a);
   if (e != hipSuccess || !grads) return e;
-  if (p.few) {
-    e = few<T, false>(a, p, a.splits, s);
-    return e == hipSuccess && a.dx ? states<T>(a, a.rows > 16, s) : e;
-  }
   for (a.first = 0; a.first < a.vocab; a.first += a.piece) {
     a.width = (uint32_t)std::min<uint64_t>(a.piece, round_up(a.vocab - a.first, 256));
     e = product<T, kSlopes>(a, p, s);

@@ -167,11 +167,9 @@ const char* wrong(const ft_cross_entropy_loss_args& a, int* code) {
   *code = FT_E_LIMIT;
   if (a.vocab > FT_MAX_HEAD_VOCAB) return "vocab must be at most 2^24";
   if (a.hidden > FT_MAX_TABLE_HIDDEN) return "hidden must be at most 2^16";
-  // (the launches: 1024 threads for 16 rows, or for 256 columns of a row of dx,
-  // 64 where there are many; 256 for tiles of 128 tokens, or hidden columns, by
-  // 64 rows, or tokens)
+  // (the launches: 1024 threads for 16 rows; 256 for tiles of 128 tokens, or
+  // hidden columns, by 64 rows, or tokens)
   if (a.rows > FT_MAX_TABLE_ROWS ||
-      (ceil_div(a.hidden, 256) * a.rows + 1) * (a.rows > 65536 ? 64 : 1024) > kMaxThreads ||
       ceil_div(a.vocab, 128) * ceil_div(a.rows, 64) * 256 > kMaxThreads ||
       ceil_div(a.hidden, 128) * ceil_div(a.vocab + 256ull, 64) * 256 > kMaxThreads)
     return "too many rows";
