@@ -29,8 +29,14 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
 // 16 x 16 tile by 32: lane l gives 8 of row l % 16 of either operand, from
 // column 8 (l / 16) on; it gets rows 4 (l / 16) ... + 3 of column l % 16.
 
-// Eight codes of a word, less 8.
-__device__ __forceinline__ u32x4 unpack(uint32_t w) {
+// Eight codes of a word, less 8.  The masks are registers' (unknown to the
+// compiler), so that a mask and the bits of 1024 are one instruction: nine a
+// word.
+struct Masks {
+  uint32_t low = 0x000F000Fu, high = 0x00F000F0u, base = 0x64006400u;
+  __device__ __forceinline__ Masks() { asm volatile("" : "+v"(low), "+v"(high), "+v"(base)); }
+};
+__device__ __forceinline__ u32x4 unpack(uint32_t w, const Masks& k) {
   const f16x2 low = {(_Float16)1032.0f, (_Float16)1032.0f};
   const f16x2 sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
   const f16x2 high = {(_Float16)-72.0f, (_Float16)-72.0f};
@@ -38,8 +44,8 @@ __device__ __forceinline__ u32x4 unpack(uint32_t w) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const uint32_t v = w >> (8 * i);
-    const f16x2 a = __builtin_bit_cast(f16x2, (v & 0x000F000Fu) | 0x64006400u);
-    const f16x2 b = __builtin_bit_cast(f16x2, (v & 0x00F000F0u) | 0x64006400u);  // 1024 + 16 c
+    const f16x2 a = __builtin_bit_cast(f16x2, (v & k.low) | k.base);
+    const f16x2 b = __builtin_bit_cast(f16x2, (v & k.high) | k.base);  // 1024 + 16 c
     r[2 * i] = __builtin_bit_cast(uint32_t, a - low);
     r[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(b, sixteenth, high));
   }
@@ -201,7 +207,7 @@ struct alignas(2 * kPer) Scales {
 // Adds chunk c's products to the sums of kM row tiles: a group's product in
 // whole numbers, then times its scale.  x(m, i): row tile m's operand of step i.
 template <typename T, int kPer, int kM, typename X>
-__device__ __forceinline__ void add_chunk(u32x4 w, Scales<T, kPer> sc, uint32_t c, uint32_t hidden,
+__device__ __forceinline__ void add_chunk(const Masks& masks, u32x4 w, Scales<T, kPer> sc, uint32_t c, uint32_t hidden,
                                           f32x4 (&acc)[kM], X&& x) {
   constexpr int kWords = 4 / kPer;
 #pragma unroll
@@ -211,7 +217,7 @@ __device__ __forceinline__ void add_chunk(u32x4 w, Scales<T, kPer> sc, uint32_t 
     f32x4 part[kM] = {};
 #pragma unroll
     for (int i = g * kWords; i < (g + 1) * kWords; ++i) {
-      const u32x4 wf = unpack(w[i]);
+      const u32x4 wf = unpack(w[i], masks);
 #pragma unroll
       for (int m = 0; m < kM; ++m) part[m] = mfma(x(m, i), wf, part[m]);
     }
@@ -230,13 +236,14 @@ __global__ void __launch_bounds__(256) packed_direct(Args a) {
   const uint32_t tile = blockIdx.x * 4 + (threadIdx.x >> 6), tiles = (a.vocab + 15) / 16;
   if (tile >= tiles) return;
   const uint32_t steps = a.chunks * 4, token = tile * 16 + n;
+  const Masks masks;
   for (uint32_t m0 = 0; m0 < a.row_tiles; m0 += kM) {
     f32x4 acc[kM] = {};
     for (uint32_t c = 0; c < a.chunks; ++c) {
       const uint64_t at = (uint64_t)tile * a.chunks + c;
       const u32x4 w = a.packed[at * 64 + lane];
       const Scales<T, kPer> sc = ((const Scales<T, kPer>*)a.scales)[at * 16 + n];
-      add_chunk<T, kPer, kM>(w, sc, c, a.hidden, acc, [&](int m, int i) {
+      add_chunk<T, kPer, kM>(masks, w, sc, c, a.hidden, acc, [&](int m, int i) {
         return a.xs[((uint64_t)min(m0 + m, a.row_tiles - 1) * steps + c * 4 + i) * 64 + lane];
       });
     }
@@ -301,13 +308,14 @@ __global__ void __launch_bounds__(kStreamT) packed_stream(Args a) {
   }
   __syncthreads();
 
+  const Masks masks;
   f32x4 acc[kM] = {};
   uint32_t tile = first, c = 0;
   while (tile < tiles) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       if (tile >= tiles) break;
-      add_chunk<T, kPer, kM>(w[u], sc[u], c, a.hidden, acc,
+      add_chunk<T, kPer, kM>(masks, w[u], sc[u], c, a.hidden, acc,
                              [&](int m, int i) { return xs[(m * steps + c * 4 + i) * 64 + lane]; });
       load(u);
       if (++c < a.chunks) continue;
