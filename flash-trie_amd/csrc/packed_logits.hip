@@ -11,6 +11,12 @@
 // holds, no rounding.  x is in float16 too: bfloat16 rows are divided by a
 // power of two that brings their largest to [2^14, 2^15), which leaves
 // everything down to 2^-32 of it exact.
+//
+// Bound by the weights' stream for up to 16 rows (2,200,000 x 512, groups of 64,
+// float32 logits: 134-164 us, 4.5-5.5 TB/s; adapter_logits reads four times as
+// much and takes 481), by the unpacking and the reads of x from LDS for more (84
+// rows x 100,003 x 1,024: 34-37 us, of which the bytes take 14), by its one launch
+// for a single request (8 rows x 32,768 x 512: 7.0 us on the device).
 #include <algorithm>
 
 #include "op_device.h"

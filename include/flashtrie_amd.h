@@ -441,8 +441,9 @@ int ft_preference_loss(const ft_preference_loss_args* args, void* workspace,
  * counts nothing and its x may hold anything; so does one of row_weight 0,
  * but for logp.  A target at or above vocab makes the loss and the row's logp
  * and dx NaN, and dweight too.  Logits, statistics and sums are held in 32
- * bits; the logits' slopes are rounded to the inputs' type, of a factor in
- * [1, 2) for float16 and bfloat16 alike, before the gradients' products. */
+ * bits.  The logits' slopes are rounded to the inputs' type for the gradients'
+ * products, relative to themselves whatever row_weight is; the target's, the
+ * largest as a rule, without error. */
 typedef struct ft_cross_entropy_loss_args {
   int device;
   int dtype;                  /* of x, weight, dx, dweight: FT_F16 or FT_BF16 */

@@ -132,11 +132,14 @@ def test_smoothing(ft, smoothing):
     check(ft, inputs(40, 333, 96, BF16, 3), smoothing, "smoothing")
 
 
-def test_pieces(ft):
+# tiles of 256, 192, 160 and 224 rows, and operands of any alignment
+@pytest.mark.parametrize("T,V,H,dtype", [(20000, 4000, 64, BF16), (1152, 60001, 64, BF16),
+                                         (777, 90001, 64, F16), (2016, 40001, 128, BF16),
+                                         (6000, 30001, 40, F16)])
+def test_pieces(ft, T, V, H, dtype):
     """More tokens than a piece of the vocabulary holds: its size goes with
     the rows."""
-    a = inputs(20000, 4000, 64, BF16, 4)
-    check(ft, a, 0.1, "pieces")
+    check(ft, inputs(T, V, H, dtype, 4), 0.1, "pieces")
 
 
 def test_what_is_asked_for(ft):

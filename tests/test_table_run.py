@@ -77,3 +77,62 @@ def test_tied_gradient(ft, dtype, R, C, S, V, H):
     spread.index_add_(0, inputs[use].long(), 1.5 * dxe.view(R, C, S, H)[use])
     tol = want["dweight"][1] + spread + part + ref.rounding(w.grad, dtype)
     assert ((d.double().cpu() - w.grad).abs() <= tol).all()
+
+
+@pytest.mark.gpu
+def test_calls_side_by_side(ft):
+    """Every operator on two streams at once, with memory of its own each, as
+    one after the other."""
+    g = torch.Generator("cuda").manual_seed(1)
+
+    def normal(*shape):
+        return torch.randn(*shape, device="cuda", generator=g)
+
+    def calls(T, V, H, dtype):
+        w, x = (normal(V, H) * 2 * H ** -0.5).to(dtype), normal(T, H).to(dtype)
+        y = torch.randint(-1, V, (T,), device="cuda", generator=g, dtype=torch.int32)
+        r = torch.rand(T, device="cuda", generator=g)
+        return lambda: (*ft.cross_entropy_loss(x, w, y, r, smoothing=0.1),
+                        ft.packed_logits(x, *ft.pack_weight(w, 64), V), ft.embed(y, w, 2.0),
+                        ft.embed_grad(x, y, V, 3.0))
+
+    work = [calls(300, 20000, 256, torch.bfloat16), calls(10, 30000, 512, torch.float16),
+            calls(5000, 3000, 64, torch.bfloat16), calls(70, 9000, 1024, torch.float16)]
+    want = [c() for c in work]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in work]
+    for _ in range(3):
+        got = []
+        for s, c in zip(streams, work):
+            with torch.cuda.stream(s):
+                got.append([c() for _ in range(3)])
+        torch.cuda.synchronize()
+        for w, three in zip(want, got):
+            for one in three:
+                assert all(torch.equal(p, q) for p, q in zip(one, w))
+
+
+@pytest.mark.gpu
+def test_an_error_of_another_call(ft):
+    """An error that an earlier call of the application left with the HIP
+    runtime is not taken for a launch's."""
+    import ctypes
+    with open("/proc/self/maps") as f:
+        path = next(line.split()[-1] for line in f if "libamdhip64" in line)
+    hip = ctypes.CDLL(path)
+    w = torch.randn(5000, 64, device="cuda").bfloat16()
+    y = torch.arange(3000, device="cuda", dtype=torch.int32)
+    r = torch.ones(3000, device="cuda")
+    packed = ft.pack_weight(w)
+    calls = [lambda: ft.cross_entropy_loss(w[:3000], w, y, r), lambda: ft.cross_entropy_loss(w[:3], w, y[:3], r[:3]),
+             lambda: ft.cross_entropy_loss(w[:30, :50], w[:, :50], y[:30], r[:30]), lambda: ft.pack_weight(w),
+             lambda: (ft.packed_logits(w[:40], *packed, 5000),), lambda: (ft.embed(y, w),),
+             lambda: (ft.embed_grad(w[:3000], y, 5000),), lambda: (ft.embed_grad(w[:30], y[:30], 5000),)]
+    for call in calls:
+        want = call()
+        assert hip.hipSetDevice(1 << 20) != 0  # no such device
+        try:
+            got = call()
+        finally:
+            hip.hipGetLastError()
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
