@@ -19,10 +19,10 @@
 // slopes and the two gradients' products, at last dx from its parts
 // (xent_states).  For few rows: xent_few twice, xent_states.
 //
-// Many rows are bound by the matrix cores (4,096 rows x 262,144 x 1,024 bf16: 7.9
-// ms, 1.11 PFLOP/s over the four products, where the library's four take 8.75),
-// few by the table's way from and to memory (10 rows of these sizes: 335 us for
-// two reads and a write of 512 MB, 4.8 TB/s); one key's 8 rows x 32,768 x 512 take
+// Many rows are bound by the matrix cores (4,096 rows x 262,144 x 1,024 bf16: 7.7
+// ms, 1.14 PFLOP/s over the four products, where the library's four take 8.75),
+// few by the table's way from and to memory (10 rows of these sizes: 303 us for
+// two reads and a write of 537 MB, 5.3 TB/s); one key's 8 rows x 32,768 x 512 take
 // 37 us, three launches.
 //
 // r[t] = m 2^e, m in [1, 2).  g is stored times m, so that its rounding is
@@ -418,7 +418,7 @@ __device__ __forceinline__ void store_rows(const uint2 (&o)[kN], char* mine, uin
   asm volatile("" ::: "memory");
 }
 
-template <typename T, Kind kKind, int kN, int kM, int kWaves, int kB, bool kLines>
+template <typename T, Kind kKind, int kN, int kM, int kWaves, int kB, bool kLines, bool kPast>
 __device__ __forceinline__ void finish(const Args& a, uint32_t tid, uint32_t tile, uint32_t i0, uint32_t jb,
                                        uint32_t jw, uint32_t wn, uint32_t split, f32x4 (&acc)[kN][kM],
                                        float (*joined)[3][kB], char* mine) {
@@ -573,7 +573,7 @@ __device__ __forceinline__ void finish(const Args& a, uint32_t tid, uint32_t til
       if constexpr (kLines) {
         store_rows<kN>(all, mine, lane, [&](uint32_t r, uint32_t c, u32x4 v) {
           if (tok + r < a.vocab && i0 + c < a.hidden)  // (whole lines of columns)
-            store_vec((T*)a.dweight + (int64_t)(tok + r) * a.dweight_stride + i0 + c, v);
+            store_to<kPast>((T*)a.dweight + (int64_t)(tok + r) * a.dweight_stride + i0 + c, v);
         });
         __builtin_amdgcn_sched_barrier(0);
       } else if (tok + col < a.vocab) {
@@ -643,7 +643,7 @@ __global__ void __launch_bounds__(kThreads) xent_product(Args a) {
         for (int j = 0; j < kBM / 16; ++j) acc[i][j] = mfma(pf[i], qf[j], acc[i][j], T{});
     }
   }
-  finish<T, kKind, 2, kBM / 16, 4, kBM, false>(a, threadIdx.x, ti, i0 + wave * 32, j0, 0, wave, split, acc, joined,
+  finish<T, kKind, 2, kBM / 16, 4, kBM, false, false>(a, threadIdx.x, ti, i0 + wave * 32, j0, 0, wave, split, acc, joined,
                                                 nullptr);
 }
 
@@ -782,10 +782,10 @@ struct TileShape {
 
 // Workgroups take tiles in turn: the next one's first two steps are copied
 // before what this one leaves is worked out.  A piece of 16,384 tokens, 4,096
-// rows x 1,024 bf16: slopes 146 us (0.94 PFLOP/s; their exponentials and stores are
-// not hidden), dx 126 (1.09; 67 MB of its parts read and written), the table's
-// gradient 106 (1.29); the statistics of all 262,144 tokens 1.96 ms (1.12).
-template <typename T, Kind kKind, typename S>
+// rows x 1,024 bf16: slopes 142 us (0.97 PFLOP/s; their exponentials and stores are
+// not hidden), dx 117 (1.17; 67 MB of its parts read and written), the table's
+// gradient 100 (1.37); the statistics of all 262,144 tokens 1.94 ms (1.13).
+template <typename T, Kind kKind, typename S, bool kPast = false>
 __global__ void __launch_bounds__(kTileThreads) xent_tile(Args a) {
   using P = Lines<T, kKind >= kStates, kTileBN, kKind == kTable>;
   using Q = Lines<T, kKind == kTable, S::BM, true>;
@@ -883,7 +883,7 @@ __global__ void __launch_bounds__(kTileThreads) xent_tile(Args a) {
     if (more) begin(block);
     uint32_t tid = threadIdx.x;
     asm volatile("" : "+v"(tid));
-    finish<T, kKind, S::N, S::M, S::WN, S::BM, true>(
+    finish<T, kKind, S::N, S::M, S::WN, S::BM, true, kPast>(
         a, tid, tile, tile * kTileBN + (kKind == kSlopes ? a.first : 0) + wn * S::N * 16, jb, wm * S::M * 16, wn,
         part, acc, (float(*)[3][S::BM])joined, (char*)stored + wave * kStored<S::N>);
     if (!more) break;
@@ -900,15 +900,15 @@ __global__ void __launch_bounds__(kTileThreads) xent_tile(Args a) {
 // as they are, their 16-byte columns exchanged by the row's number such that
 // eight rows of a column, and two columns of four rows, are free of bank
 // conflicts: the logits read the table by k, the gradients read across.  10 rows x
-// 262,144 x 1,024 bf16: 216 us for both gradients (5.0 TB/s read and written; 295
-// with dweight stored eight bytes a lane), 100 us for dx alone, 110 for the
+// 262,144 x 1,024 bf16: 208 us for both gradients (5.2 TB/s read and written; 295
+// with dweight stored eight bytes a lane), 112 us for dx alone, 87 for the
 // statistics.
 constexpr uint32_t kFewBytes = 65536;  // of the states, and of a tile
 constexpr int kFewThreads = 1024;
 
 // kStats: the pass before it, for the rows' statistics: each workgroup's own,
 // held by lanes (a row, and the tokens 4 q ... of a subtile) to the end.
-template <typename T, int kR, int kTok, bool kStats>
+template <typename T, int kR, int kTok, bool kStats, bool kPast>
 __global__ void __launch_bounds__(kFewThreads) xent_few(Args a) {
   if constexpr (kStats) {
     if (blockIdx.x < a.prepare) {
@@ -958,7 +958,8 @@ __global__ void __launch_bounds__(kFewThreads) xent_few(Args a) {
     if (rows == (uint32_t)kTok) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i)
-        if (from[i] != ~0u) next[i] = *(const u32x4*)(base + from[i]);
+        if (from[i] != ~0u)
+          next[i] = kPast ? __builtin_nontemporal_load((const u32x4*)(base + from[i])) : *(const u32x4*)(base + from[i]);
     } else {
       uint32_t now = tid;
       asm volatile("" : "+v"(now));
@@ -1152,7 +1153,7 @@ __global__ void __launch_bounds__(kFewThreads) xent_few(Args a) {
           }
           store_rows<kLine>(all, (char*)own_lds[wave], now, [&](uint32_t r, uint32_t c, u32x4 v) {
             if (tok + r < a.vocab && j0 * 16 + c < own_subs * 16)
-              store_vec((T*)a.dweight + (int64_t)(tok + r) * a.dweight_stride + (sub0 + j0) * 16 + c, v);
+              store_to<kPast>((T*)a.dweight + (int64_t)(tok + r) * a.dweight_stride + (sub0 + j0) * 16 + c, v);
           });
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -1211,7 +1212,7 @@ struct Plan {
   uint64_t split_stride;
   uint32_t rows64, hidden64, tiles, piece, slope_stride, splits, split_steps, bm, bn;
   uint32_t few;  // 16-row subtiles of xent_few; 0: other kernels
-  bool lines;
+  bool lines, past;  // past: the caches
 };
 
 // The states' and the table's rows are whole lines, and 32-bit offsets reach
@@ -1228,6 +1229,10 @@ Plan plan(const ft_cross_entropy_loss_args& a) {
   p.rows64 = (uint32_t)round_up(a.rows, 64);
   p.hidden64 = (uint32_t)round_up(a.hidden, 64);
   p.lines = whole_lines(a);
+  // Whether the table is read for the last time, and its gradient written, past the
+  // caches: 10 and 200 rows on H = 1,024 take 74 and 157 us so, 72 and 157 through
+  // them at 100 MB; 95 and 244, 99 and 262 at 150; 169 and 475, 205 and 502 at 300.
+  p.past = 2ull * a.vocab * a.hidden > kPastBytes;
   p.bn = p.lines ? kTileBN : kBN;
   p.bm = !p.lines || p.rows64 <= 64 ? 64 : p.rows64 <= 128 ? 128 : 256;
   // Many rows: the tile that leaves the least of them empty, at what a row costs
@@ -1307,15 +1312,19 @@ hipError_t product(const Args& a, const Plan& p, hipStream_t s) {
     if (p.bm == 192) return start(xent_tile<T, kKind, TileShape<12, 2>>, most, kTileThreads, s, a);
     if (p.bm == 224) return start(xent_tile<T, kKind, TileShape<14, 2>>, most, kTileThreads, s, a);
   }
-  return start(xent_tile<T, kKind, TileShape<16, 2>>, std::min<uint64_t>(blocks, kCUs), kTileThreads, s, a);
+  const uint64_t most = std::min<uint64_t>(blocks, kCUs);
+  if constexpr (kKind == kTable) {
+    if (p.past) return start(xent_tile<T, kKind, TileShape<16, 2>, true>, most, kTileThreads, s, a);
+  }
+  return start(xent_tile<T, kKind, TileShape<16, 2>>, most, kTileThreads, s, a);
 }
 
-template <typename T, bool kStats>
+template <typename T, bool kStats, bool kPast>
 hipError_t few(const Args& a, const Plan& p, uint64_t blocks, hipStream_t s) {
-  return p.few == 2         ? start(xent_few<T, 2, 64, kStats>, blocks, kFewThreads, s, a)
-         : a.hidden <= 512  ? start(xent_few<T, 1, 64, kStats>, blocks, kFewThreads, s, a)
-         : a.hidden <= 1024 ? start(xent_few<T, 1, 32, kStats>, blocks, kFewThreads, s, a)
-                            : start(xent_few<T, 1, 16, kStats>, blocks, kFewThreads, s, a);
+  return p.few == 2         ? start(xent_few<T, 2, 64, kStats, kPast>, blocks, kFewThreads, s, a)
+         : a.hidden <= 512  ? start(xent_few<T, 1, 64, kStats, kPast>, blocks, kFewThreads, s, a)
+         : a.hidden <= 1024 ? start(xent_few<T, 1, 32, kStats, kPast>, blocks, kFewThreads, s, a)
+                            : start(xent_few<T, 1, 16, kStats, kPast>, blocks, kFewThreads, s, a);
 }
 
 template <typename T>
@@ -1341,10 +1350,10 @@ hipError_t launch(Args a, const Plan& p, hipStream_t s) {
   // a few rows are prepared beside the statistics, and joined with the loss
   const bool grads = a.dx || a.dweight;
   if (p.few && grads) a.prepare = a.rows64 / 16;
-  hipError_t e = p.few ? few<T, true>(a, p, a.prepare + a.tiles, s) : product<T, kStats>(a, p, s);
+  hipError_t e = p.few ? few<T, true, false>(a, p, a.prepare + a.tiles, s) : product<T, kStats>(a, p, s);
   if (e != hipSuccess) return e;
   if (p.few && grads) {
-    e = few<T, false>(a, p, a.splits, s);
+    e = p.past ? few<T, false, true>(a, p, a.splits, s) : few<T, false, false>(a, p, a.splits, s);
     return e == hipSuccess && a.dx ? states<T>(a, false, s) : e;
   }
   e = grads ? start(xent_rows<T>, a.rows64 / 16, 1024, s, a) : start(xent_join, (a.rows + 15) / 16, 1024, s, a);

@@ -11,9 +11,10 @@
 // occur get their zeros from workgroups beside those that sort.
 //
 // Bound by memory: 128,000 tokens x 512 bf16 are looked up in 30-38 us (6.2 TB/s
-// counting each row once); their gradient in a table of 262,144 x 1,024 takes 180
-// us: zeros and sorting 95 (537 MB at 5.7 TB/s; sorting alone would take some 60 in
-// its six launches), sums 80, parts 7.
+// counting each row once); their gradient in a table of 262,144 x 1,024 takes 163
+// us, where a trace of one table again and again has 147: zeros and sorting 100 (537
+// MB at 5.4 TB/s; sorting alone would take some 60 in its six launches), sums 41,
+// parts 7.
 #include <algorithm>
 
 #include "op_device.h"
@@ -124,7 +125,7 @@ __device__ __forceinline__ void write_zeros(const GradArgs& a, uint32_t block, u
     for (uint64_t v = at + threadIdx.x; v < at + kZeroUnit; v += kSortT) {
       const uint64_t e = v * kVec<T>;
       if (e >= length) break;
-      if (e + kVec<T> <= length) store_vec(to + e, u32x4{});
+      if (e + kVec<T> <= length) store_to<true>(to + e, u32x4{});
       else store_part(to + e, (int)(length - e), u32x4{});
     }
   }
@@ -292,14 +293,16 @@ __global__ void __launch_bounds__(kSortT) embed_place(GradArgs a) {
           });
 }
 
-template <typename T>
+// Past the caches where positions are many: 19,200 x 1,024 into tables of 50 to 300
+// MB take 49 to 78 us so, 53 to 84 through them.
+template <typename T, bool kPast>
 __device__ __forceinline__ void write_row(const GradArgs& a, uint32_t token, uint32_t e, float (&sum)[kVec<T>]) {
   T* to = (T*)a.dtable + (int64_t)token * a.dtable_stride + e;
   float old[kVec<T>] = {};
   if (a.add) to_float<T>(load_row_vec(to - e, e, a.hidden, (T)0.0f), old);
 #pragma unroll
   for (int k = 0; k < kVec<T>; ++k) sum[k] = __builtin_fmaf(sum[k], a.scale, old[k]);
-  if (e + kVec<T> <= a.hidden) store_vec(to, from_float<T>(sum));
+  if (e + kVec<T> <= a.hidden) store_to<kPast>(to, from_float<T>(sum));
   else store_part(to, (int)(a.hidden - e), from_float<T>(sum));
 }
 
@@ -374,7 +377,7 @@ __global__ void __launch_bounds__(256) embed_sums(GradArgs a) {
         if (after == k && i + 1 < n) return;
         // the token's last here
         if (e < a.hidden) {
-          if (starts && after != k) write_row<T>(a, k, e, sum);
+          if (starts && after != k) write_row<T, true>(a, k, e, sum);
           else store_floats<T>(part_of<T>(a, starts ? 1 : 0, run, e), sum);
         }
         starts = true;
@@ -384,57 +387,92 @@ __global__ void __launch_bounds__(256) embed_sums(GradArgs a) {
 }
 
 // Few positions of rows that are whole vectors, in one launch (80 tokens, 32,768 x
-// 512 f32: 11.4 us where sort, sums and join take 20; 1,664 tokens, 100,003 x 768
-// f16: 24.5, the zeros' 154 MB at 6.3 TB/s): a wave a
-// position and 64 vectors looks for the others of its token (and is done if
-// there is one before it), and the workgroups behind write zeros to the rows
-// of other tokens.
-template <typename T>
-__global__ void __launch_bounds__(256) embed_few(GradArgs a) {
-  __shared__ uint32_t list[4 * kSmall / 2];  // positions of 16 bits, a wave's each
+// 512 f32: 11.5 us where sort, sums and join take 20; 1,664 tokens, 100,003 x 768
+// f16: 28.6, the zeros' 154 MB at 5.4 TB/s): a workgroup a position and 64 vectors
+// looks for the others of its token (and is done if there is one before it), its
+// waves share a long list of them, and other workgroups write zeros to the rows
+// of other tokens.  2,048 positions of one token x 512: 51 us (by a wave each 341).
+constexpr int kFewT = 512, kFewWaves = kFewT / 64;
+template <typename T, bool kPast>
+__global__ void __launch_bounds__(kFewT) embed_few(GradArgs a) {
+  __shared__ uint32_t list[kSmall];  // positions; or the bits of the zeros' rows
+  __shared__ uint32_t found[kFewWaves], earliest[kFewWaves];
+  __shared__ float parts[kFewWaves - 1][64][kVec<T> + 1];
   const uint32_t tid = threadIdx.x, lane = tid & 63;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
-  if (blockIdx.x < a.blocks) {
-    const uint32_t task = blockIdx.x * 4 + wave, p = task / a.panels;
-    const uint32_t e = (task % a.panels * 64 + lane) * kVec<T>;
-    if (p >= a.count) return;
+  // (the two kinds mixed, so that neither waits for the other's end)
+  const uint32_t adds = (uint32_t)((uint64_t)blockIdx.x * a.blocks / gridDim.x);  // of those in front
+  if ((uint32_t)((uint64_t)(blockIdx.x + 1) * a.blocks / gridDim.x) > adds) {
+    const uint32_t p = adds / a.panels, e = (adds % a.panels * 64 + lane) * kVec<T>;
     const uint32_t k = key_of(a, p);
     if (k >= a.vocab) return;
-    uint16_t* mine = (uint16_t*)list + wave * kSmall;
-    uint32_t n = 0;
-    for (uint32_t i0 = 0; i0 < a.count; i0 += 64) {
-      const uint32_t i = i0 + lane;
-      const uint64_t same = __ballot(i < a.count && key_of(a, i) == k);
-      if (same && n == 0 && i0 + (uint32_t)__ffsll((unsigned long long)same) - 1 < p) return;
-      if (same >> lane & 1) mine[n + (uint32_t)__popcll(same & ((1ull << lane) - 1))] = (uint16_t)i;
-      n += (uint32_t)__popcll(same);
+    constexpr uint32_t kMasks = kSmall / 64 / kFewWaves;
+    uint64_t same[kMasks];
+    uint32_t n = 0, first = ~0u;
+#pragma unroll
+    for (uint32_t i = 0; i < kMasks; ++i) {
+      const uint32_t at = (wave * kMasks + i) * 64 + lane;
+      same[i] = __ballot(at < a.count && key_of(a, at) == k);
+      if (same[i] && first == ~0u) first = (wave * kMasks + i) * 64 + (uint32_t)__ffsll((unsigned long long)same[i]) - 1;
+      n += (uint32_t)__popcll(same[i]);
     }
-    asm volatile("" ::: "memory");  // (a wave's LDS accesses are in order)
+    if (lane == 0) {
+      found[wave] = n;
+      earliest[wave] = first;
+    }
+    __syncthreads();
+    uint32_t front = 0, all = 0, least = ~0u;
+#pragma unroll
+    for (uint32_t w = 0; w < (uint32_t)kFewWaves; ++w) {
+      front += w < wave ? found[w] : 0u;
+      all += found[w];
+      least = min(least, earliest[w]);
+    }
+    if (least < p) return;
+#pragma unroll
+    for (uint32_t i = 0; i < kMasks; ++i) {
+      if (same[i] >> lane & 1)
+        list[front + (uint32_t)__popcll(same[i] & ((1ull << lane) - 1))] = (wave * kMasks + i) * 64 + lane;
+      front += (uint32_t)__popcll(same[i]);
+    }
+    __syncthreads();
+    const uint32_t waves = all <= 16 ? 1 : kFewWaves, each = (all + waves - 1) / waves;
+    const uint32_t i0 = min(wave * each, all), i1 = wave < waves ? min(i0 + each, all) : i0;
     float sum[kVec<T>] = {};
     walk_rows<T>(
-        a, n, e, [&](uint32_t i) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)mine[i]); },
+        a, i1 - i0, e, [&](uint32_t i) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)list[i0 + i]); },
         [&](uint32_t, const float (&f)[kVec<T>]) {
 #pragma unroll
           for (int c = 0; c < kVec<T>; ++c) sum[c] += f[c];
         });
-    if (e < a.hidden) write_row<T>(a, k, e, sum);
+    if (waves > 1) {
+      if (wave > 0)
+#pragma unroll
+        for (int c = 0; c < kVec<T>; ++c) parts[wave - 1][lane][c] = sum[c];
+      __syncthreads();
+      if (wave == 0)
+        for (uint32_t w = 1; w < waves; ++w)
+#pragma unroll
+          for (int c = 0; c < kVec<T>; ++c) sum[c] += parts[w - 1][lane][c];
+    }
+    if (wave == 0 && e < a.hidden) write_row<T, kPast>(a, k, e, sum);
     return;
   }
   // rows r0 ... of the table, which have no gaps
-  const uint32_t per = a.hidden / kVec<T>, rows = a.zero_units, r0 = (blockIdx.x - a.blocks) * rows;
+  const uint32_t per = a.hidden / kVec<T>, rows = a.zero_units, r0 = (blockIdx.x - adds) * rows;
   const uint32_t n = min(rows, a.vocab - r0);
-  for (uint32_t i = tid; i < (n + 31) / 32; i += 256) list[i] = 0;
+  for (uint32_t i = tid; i < (n + 31) / 32; i += kFewT) list[i] = 0;
   __syncthreads();
-  for (uint32_t i = tid; i < a.count; i += 256) {
+  for (uint32_t i = tid; i < a.count; i += kFewT) {
     const uint32_t k = key_of(a, i) - r0;
     if (k < n) atomicOr(&list[k / 32], 1u << k % 32);
   }
   __syncthreads();
   T* to = (T*)a.dtable + (uint64_t)r0 * a.hidden;
 #pragma unroll 4
-  for (uint32_t v = tid; v < n * per; v += 256) {
+  for (uint32_t v = tid; v < n * per; v += kFewT) {
     const uint32_t row = v / per;
-    if (!(list[row / 32] >> row % 32 & 1)) store_vec(to + (uint64_t)v * kVec<T>, u32x4{});
+    if (!(list[row / 32] >> row % 32 & 1)) store_to<kPast>(to + (uint64_t)v * kVec<T>, u32x4{});
   }
 }
 
@@ -488,7 +526,7 @@ __global__ void __launch_bounds__(256) embed_join(GradArgs a) {
   for (int w = 0; w < 3; ++w)
 #pragma unroll
     for (int c = 0; c < kVec<T>; ++c) sum[c] += quarter[w][lane][c];
-  write_row<T>(a, k, e, sum);
+  write_row<T, true>(a, k, e, sum);
 }
 
 // Positions of a wave: few where there are few of them.
@@ -517,12 +555,18 @@ hipError_t launch_grad(GradArgs a, hipStream_t s) {
   constexpr uint32_t kZeroBlocks = 512;
   const uint64_t units = a.add ? 0 : (uint64_t)a.zero_units * (a.zero_length == a.hidden ? a.vocab : 1);
   hipError_t e;
-  // (the zeros' rows without gaps, 16 to 128 KB a workgroup; a bit for each)
+  // (the zeros' rows without gaps, 128 KB or a row a workgroup; a bit for each)
+  constexpr uint32_t kZeroVecs = 8192;
+  static_assert(kZeroVecs <= kSmall * 32, "bits for a row of a vector each");
   const uint32_t per = a.hidden / kVec<T>;
   if (a.count <= kSmall && a.count > 0 && a.hidden % kVec<T> == 0 && (a.add || a.dtable_stride == (int64_t)a.hidden)) {
-    a.blocks = (a.count * a.panels + 3) / 4;
-    a.zero_units = std::min<uint32_t>(kSmall * 64, std::max(1u, 4096 / per));
-    return start(embed_few<T>, a.blocks + (a.add ? 0 : (a.vocab + a.zero_units - 1) / a.zero_units), 256, s, a);
+    a.blocks = a.count * a.panels;
+    a.zero_units = std::max(1u, kZeroVecs / per);
+    const uint64_t blocks = a.blocks + (a.add ? 0 : (a.vocab + a.zero_units - 1) / a.zero_units);
+    // (past the caches or through them: 80 tokens x 512 into 67 MB 13.1 us and 11.5;
+    // 1,664 x 768 into 154 MB, another gradient each call, 28.6 and 37)
+    return (uint64_t)a.vocab * a.hidden * sizeof(T) > kPastBytes ? start(embed_few<T, true>, blocks, kFewT, s, a)
+                                                                 : start(embed_few<T, false>, blocks, kFewT, s, a);
   }
   if (a.count <= kSmall) {
     a.zero_last = units;

@@ -30,6 +30,16 @@ template <typename T>
 __device__ __forceinline__ void store_vec(T* p, u32x4 v) {
   ((Vec16<T>*)p)->v = v;
 }
+// store_vec, or past the caches: for what no kernel of the call reads again and
+// is too much for them, which would only drive other memory out.  For a table of
+// kPastBytes or less the last level's cache is left to whoever reads it next.
+constexpr uint64_t kPastBytes = 128ull << 20;
+
+template <bool kPast, typename T>
+__device__ __forceinline__ void store_to(T* p, u32x4 v) {
+  if (kPast) __builtin_nontemporal_store(v, &((Vec16<T>*)p)->v);
+  else store_vec(p, v);
+}
 
 // The first n elements of a vector, the others `fill`; p[0] is there.
 template <typename T>

@@ -86,6 +86,14 @@ def test_few_rows_many_tokens(ft, T, V, H):
     check(ft, inputs(T, V, H, BF16, 1), 0.1, "few")
 
 
+# tables that are read and written past the caches (more than 128 MB), of few rows
+# and more; and just under
+@pytest.mark.parametrize("T,V,H,dtype", [(9, 70001, 1024, BF16), (20, 140000, 512, F16), (3, 33001, 2048, BF16),
+                                         (70, 66000, 1024, F16), (9, 65536, 1024, BF16), (9, 65537, 1024, BF16)])
+def test_large_tables(ft, T, V, H, dtype):
+    check(ft, inputs(T, V, H, dtype, V), 0.1, "large")
+
+
 def call(ft, a, dx, dweight, smoothing=0.1):
     """The C call, for what the Python one does not offer."""
     lib = C.CDLL(os.path.join(args.ROOT, "flash-trie_amd", "libflashtrie_amd.so"))
